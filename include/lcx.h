@@ -51,7 +51,8 @@ typedef enum {
     LCX_ERR_COMM = 5        /* RCCL / the exchange hook failed                */
 } lcx_status;
 
-typedef enum { LCX_F32 = 0, LCX_F64 = 1 } lcx_dtype;
+/* LCX_BF16 / LCX_F16: element types of the lcx_mx4_* operators only; a handle works in LCX_F32 or LCX_F64 */
+typedef enum { LCX_F32 = 0, LCX_F64 = 1, LCX_BF16 = 2, LCX_F16 = 3 } lcx_dtype;
 
 /* scalar slots returned by lcx_read_state() */
 enum {
@@ -418,6 +419,43 @@ int lcx_geometry(lcx_ctx* h, int64_t* n_pad, int64_t* ldx, int* m_pad, int64_t* 
 /* name of the kernel function behind pass `kind` as rocprofv3 prints it (without "void " and the
  * argument list), so that bench.py's roofline line and the committed rocprof summary name the same row */
 int lcx_kernel_name(lcx_ctx* h, int kind, char* buf, int64_t len);
+
+/* ---- matrices in 4 bits per value ("mx4") --------------------------------------------------------------
+ * A value is a 4-bit float (sign, 2 exponent bits, 1 mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6); 32 neighbours along a row share one
+ * power-of-two scale (a byte, 2^(byte - 127); 255: the block is NaN).  An R x C matrix is two device buffers of lcx_mx4_layout's sizes:
+ *   codes  R rows of code_row bytes: two values a byte, the even column in the low half; zeros behind column C
+ *   scales R rows of scale_row bytes: the byte of block 4 s + g of every 16 blocks at place 4 g + s; unused ones 2
+ * What lcx_mx4_quantize writes is defined to the bit: scale = 2^(floor(log2 max|x|) - 2) of the block, at least 2^-125 (also of a block of
+ * zeros); value = x / scale rounded to nearest, ties to the even code, saturating at 6 (largest: 6 * 2^125; float64 beyond float32
+ * saturates too); a block that holds an infinity or a NaN is NaN.
+ *
+ * These entry points have no handle: every pointer is device memory of the current device, the work goes to `stream` (a hipStream_t of
+ * that device, NULL = the default stream) and the call returns without waiting; nothing is kept from one call to the next, so calls on
+ * different streams may overlap.  Codes must be 16-byte aligned, scales 4-byte aligned.  Strides count elements.  rows, cols, M, N, K
+ * may be 0: an empty output is left alone, an empty contraction gives zeros.  Outputs must not overlap inputs. */
+int lcx_mx4_layout(int64_t cols, int64_t* code_row, int64_t* scale_row);
+/* x[r * row_stride + c * col_stride] (any lcx_dtype) -> codes, scales; blocks run along c */
+int lcx_mx4_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, int64_t col_stride, void* codes,
+                     void* scales, void* stream);
+/* codes, scales -> out[r * row_stride + c * col_stride] (any lcx_dtype, rounded to nearest) */
+int lcx_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, void* out, int dtype, int64_t row_stride,
+                       int64_t col_stride, void* stream);
+/* Bytes of device memory that the product of the given sizes wants as work space: op 0 lcx_mx4_matmul, 1 lcx_mx4_linear,
+ * 2 lcx_mx4_linear_grad; dtype as in the call (op 0: of the output).  The same space may serve any number of calls on ONE stream. */
+int lcx_mx4_workspace(int op, int dtype, int64_t M, int64_t N, int64_t K, int64_t* bytes);
+/* out[m * row_stride + n * col_stride] = sum_k A[m][k] B[n][k] of two mx4 matrices (M x K, N x K): products exact, sums in float32, out in
+ * LCX_F32 / LCX_BF16 / LCX_F16, rounded once */
+int lcx_mx4_matmul(const void* a_codes, const void* a_scales, int64_t M, const void* b_codes, const void* b_scales, int64_t N, int64_t K,
+                   void* out, int dtype, int64_t row_stride, int64_t col_stride, void* workspace, int64_t workspace_bytes, void* stream);
+/* out[m * row_stride + n * col_stride] = sum_k x[m][k] W[n][k]: x (M x K, LCX_F32 / LCX_BF16 / LCX_F16, strides x_row / x_col) as it is, W an
+ * mx4 matrix N x K; products exact (x is split into bf16 numbers without loss), sums in float32, out in x's type, rounded once */
+int lcx_mx4_linear(const void* x, int dtype, int64_t M, int64_t x_row, int64_t x_col, const void* codes, const void* scales, int64_t N,
+                   int64_t K, void* out, int64_t row_stride, int64_t col_stride, void* workspace, int64_t workspace_bytes, void* stream);
+/* out[m * row_stride + k * col_stride] = sum_n dy[m][n] W[n][k]: the gradient of lcx_mx4_linear with respect to x (dy M x N), and the product
+ * with W itself where lcx_mx4_linear multiplies with its transpose; same types and rounding */
+int lcx_mx4_linear_grad(const void* dy, int dtype, int64_t M, int64_t dy_row, int64_t dy_col, const void* codes, const void* scales,
+                        int64_t N, int64_t K, void* out, int64_t row_stride, int64_t col_stride, void* workspace, int64_t workspace_bytes,
+                        void* stream);
 
 #ifdef __cplusplus
 }

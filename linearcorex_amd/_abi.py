@@ -14,7 +14,7 @@ import numpy as np
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "liblcx_hip.so")
 
-LCX_F32, LCX_F64 = 0, 1
+LCX_F32, LCX_F64, LCX_BF16, LCX_F16 = 0, 1, 2, 3
 S_TC, S_MAX_UJ, S_INVALID, S_TANGENT, S_SUM_LOG_RJ, S_COUNT = 0, 1, 2, 3, 4, 8
 SB_H = 8                   # offset of H in the scalar exchange buffer (include/lcx.h, lcx_read_sbuf)
 
@@ -97,6 +97,13 @@ SIGNATURES = {
     "lcx_timing_reset": [_vp],
     "lcx_geometry": [_vp, C.POINTER(_i64), C.POINTER(_i64), C.POINTER(_i32), C.POINTER(_i64)],
     "lcx_kernel_name": [_vp, _i32, C.c_char_p, _i64],
+    "lcx_mx4_layout": [_i64, C.POINTER(_i64), C.POINTER(_i64)],
+    "lcx_mx4_quantize": [_vp, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp],
+    "lcx_mx4_dequantize": [_vp, _vp, _i64, _i64, _vp, _i32, _i64, _i64, _vp],
+    "lcx_mx4_workspace": [_i32, _i32, _i64, _i64, _i64, C.POINTER(_i64)],
+    "lcx_mx4_matmul": [_vp, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _i64, _i64, _vp, _i64, _vp],
+    "lcx_mx4_linear": [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp],
+    "lcx_mx4_linear_grad": [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp],
 }
 
 _lib = None

@@ -1,0 +1,229 @@
+"""Matrices in 4 bits per value: quantisation, and the products a fit and a layer make with them.
+
+    from linearcorex_amd import mx4
+
+    q = mx4.quantize(w)                    # w (N, K) on the GPU -> 4.25 bits per value, blocks of 32 along K
+    y = mx4.linear(x, q)                   # x (..., K) . w^T -> (..., N); differentiable with respect to x
+    dx = mx4.linear_grad(dy, q)            # dy (..., N) . w   -> (..., K)
+    y = mx4.matmul(mx4.quantize(x), q)     # both operands in 4 bits: 4-bit matrix instructions
+    w4 = mx4.dequantize(q)                 # the values that the 4 bits stand for
+
+A value is a 4-bit float (0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign); 32 neighbours share one power-of-two scale.  The layout and the
+rounding are defined in include/lcx.h (lcx_mx4_*), which these functions call on torch tensors: on the current stream, without
+waiting, on the device of the tensors.  Wrong arguments raise ValueError or TypeError before anything is launched, a failing call
+`LcxError`; there is no CPU fallback.
+
+`Corex(x_storage="mx4")` keeps the data of a fit in this form.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _abi
+from ._abi import LcxError          # noqa: F401  (what a failing call raises)
+
+_DTYPES = {torch.float32: _abi.LCX_F32, torch.float64: _abi.LCX_F64, torch.bfloat16: _abi.LCX_BF16, torch.float16: _abi.LCX_F16}
+_PRODUCT_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+BLOCK = 32
+
+
+def _rows_bytes(cols):
+    """bytes of a row of codes and of a row of scales (include/lcx.h, lcx_mx4_layout)"""
+    return -(-cols // 256) * 128, -(-cols // 512) * 16
+
+
+class Mx4(object):
+    """A matrix in 4 bits per value, made by `quantize`.
+
+    shape   (rows, columns) of the matrix
+    axis    the axis along which 32 neighbours share a scale: 1 = along a row, 0 = along a column
+    codes, scales   its device buffers (uint8): of the matrix itself for axis 1, of its transpose for axis 0
+    `q.t()` is the transposed matrix on the same buffers."""
+
+    __slots__ = ("shape", "axis", "codes", "scales")
+
+    def __init__(self, shape, axis, codes, scales):
+        self.shape, self.axis, self.codes, self.scales = shape, axis, codes, scales
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @property
+    def nbytes(self):
+        return self.codes.numel() + self.scales.numel()
+
+    def t(self):
+        return Mx4((self.shape[1], self.shape[0]), 1 - self.axis, self.codes, self.scales)
+
+    def _stored(self):
+        """(rows, columns) of the buffers: blocks run along the columns"""
+        return self.shape if self.axis == 1 else (self.shape[1], self.shape[0])
+
+    def __repr__(self):
+        return "Mx4(shape=%r, axis=%d, device=%s)" % (self.shape, self.axis, self.device)
+
+
+def _on_gpu(t, what):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a torch tensor, not %s" % (what, type(t).__name__))
+    if t.layout != torch.strided:
+        raise TypeError("%s must be a dense tensor" % what)
+    if t.device.type != "cuda":
+        raise ValueError("%s must be on the GPU, it is on %s (there is no CPU fallback)" % (what, t.device))
+
+
+def _is_mx4(q, what):
+    if not isinstance(q, Mx4):
+        raise TypeError("%s must be an Mx4 matrix (mx4.quantize), not %s" % (what, type(q).__name__))
+
+
+def _call(device, name, *args):
+    """one entry point on the device's current stream"""
+    fn = getattr(_abi.load(), name)
+    if torch.cuda.current_device() == device.index:
+        status = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if status != 0:
+        _abi.check(status)
+
+
+def _workspace(device, op, dtype, m, n, k):
+    """(tensor or None, pointer, bytes): allocated per call on the current stream, like the outputs"""
+    b = C.c_int64()
+    _abi.check(_abi.load().lcx_mx4_workspace(op, dtype, m, n, k, C.byref(b)))
+    if b.value == 0:
+        return None, None, 0
+    w = torch.empty(b.value, dtype=torch.uint8, device=device)
+    return w, w.data_ptr(), b.value
+
+
+def quantize(x, axis=1):
+    """x (rows, columns) -> `Mx4` of the same shape; blocks of 32 run along `axis`.
+
+    float32, float64, bfloat16 or float16, any strides (a transposed view is read in place).  Per block: scale
+    2^(floor(log2 max|x|) - 2), values rounded to nearest (ties to the even code), those above 6 scales saturate; a block that holds an
+    infinity or a NaN is NaN.  Not differentiable: the result carries no graph."""
+    _on_gpu(x, "x")
+    if x.dim() != 2:
+        raise ValueError("x must have two dimensions, it has %d" % x.dim())
+    if x.dtype not in _DTYPES:
+        raise TypeError("x must be float32, float64, bfloat16 or float16, not %s" % x.dtype)
+    if isinstance(axis, bool) or axis not in (0, 1, -1, -2):
+        raise ValueError("axis must be 0 or 1")
+    axis %= 2
+    x = x.detach()
+    v = x if axis == 1 else x.t()
+    rows, cols = v.shape
+    cb, sb = _rows_bytes(cols)
+    codes = torch.empty((rows, cb), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((rows, sb), dtype=torch.uint8, device=x.device)
+    if rows and cols:
+        _call(x.device, "lcx_mx4_quantize", v.data_ptr(), _DTYPES[x.dtype], rows, cols, v.stride(0), v.stride(1), codes.data_ptr(), scales.data_ptr())
+    return Mx4(tuple(x.shape), axis, codes, scales)
+
+
+def dequantize(q, dtype=torch.float32):
+    """The values that the 4 bits stand for, as a dense tensor of `q.shape` (exact in float32, float64 and bfloat16)."""
+    _is_mx4(q, "q")
+    if dtype not in _DTYPES:
+        raise TypeError("dtype must be float32, float64, bfloat16 or float16, not %s" % dtype)
+    out = torch.empty(q.shape, dtype=dtype, device=q.device)
+    if out.numel():
+        rows, cols = q._stored()
+        v = out if q.axis == 1 else out.t()
+        _call(q.device, "lcx_mx4_dequantize", q.codes.data_ptr(), q.scales.data_ptr(), rows, cols, out.data_ptr(), _DTYPES[dtype], v.stride(0), v.stride(1))
+    return out
+
+
+def matmul(a, b, dtype=torch.float32):
+    """a (M, K) . b (N, K)^T of two `Mx4` matrices -> (M, N) in `dtype` (float32, bfloat16, float16): exact products, float32 sums,
+    rounded once.  Both hold their blocks along K (axis 1)."""
+    _is_mx4(a, "a")
+    _is_mx4(b, "b")
+    if dtype not in _PRODUCT_DTYPES:
+        raise TypeError("dtype must be float32, bfloat16 or float16, not %s" % dtype)
+    if a.axis != 1 or b.axis != 1:
+        raise ValueError("matmul contracts along the blocks: quantize both operands along their columns (axis 1)")
+    if a.shape[1] != b.shape[1]:
+        raise ValueError("a has %d columns, b has %d" % (a.shape[1], b.shape[1]))
+    if a.device != b.device:
+        raise ValueError("a is on %s, b on %s" % (a.device, b.device))
+    (m, k), n = a.shape, b.shape[0]
+    out = torch.empty((m, n), dtype=dtype, device=a.device)
+    if out.numel():
+        dt = _DTYPES[dtype]
+        w, wp, wb = _workspace(a.device, 0, dt, m, n, k)
+        _call(a.device, "lcx_mx4_matmul", a.codes.data_ptr(), a.scales.data_ptr(), m, b.codes.data_ptr(), b.scales.data_ptr(), n, k,
+              out.data_ptr(), dt, n, 1, wp, wb)
+    return out
+
+
+def _product(x, q, along):
+    """x (..., C) . q: along the blocks (contraction over the stored columns) or across them (over the stored rows)"""
+    n, k = q._stored()
+    c, o = (k, n) if along else (n, k)
+    lead = x.shape[:-1]
+    m = 1
+    for d in lead:
+        m *= d
+    x2 = x if x.dim() == 2 else x.reshape(m, c)
+    out = torch.empty((m, o), dtype=x.dtype, device=x.device)
+    if out.numel():
+        dt = _DTYPES[x.dtype]
+        w, wp, wb = _workspace(x.device, 1 if along else 2, dt, m, n, k)
+        _call(x.device, "lcx_mx4_linear" if along else "lcx_mx4_linear_grad", x2.data_ptr(), dt, m, x2.stride(0), x2.stride(1),
+              q.codes.data_ptr(), q.scales.data_ptr(), n, k, out.data_ptr(), o, 1, wp, wb)
+    return out if x.dim() == 2 else out.reshape(lead + (o,))
+
+
+class _Product(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, q, along):
+        ctx.q, ctx.along = q, along
+        return _product(x, q, along)
+
+    @staticmethod
+    def backward(ctx, dy):
+        # the product is linear in x: its gradient is the other product with the same matrix, itself differentiable
+        return _apply(dy, ctx.q, not ctx.along), None, None
+
+
+def _apply(x, q, along):
+    if torch.is_grad_enabled() and x.requires_grad:
+        return _Product.apply(x, q, along)
+    return _product(x, q, along)
+
+
+def _checked(x, q, what, contracted):
+    _on_gpu(x, what)
+    _is_mx4(q, "q")
+    if x.dtype not in _PRODUCT_DTYPES:
+        raise TypeError("%s must be float32, bfloat16 or float16, not %s" % (what, x.dtype))
+    if x.dim() < 1:
+        raise ValueError("%s must have a dimension to contract" % what)
+    if x.shape[-1] != q.shape[contracted]:
+        raise ValueError("%s has %d values to contract, q has shape %r" % (what, x.shape[-1], q.shape))
+    if x.device != q.device:
+        raise ValueError("%s is on %s, q on %s" % (what, x.device, q.device))
+
+
+def linear(x, q):
+    """x (..., K) . q (N, K)^T -> (..., N) in x's type (float32, bfloat16, float16): x as it is, the matrix in 4 bits.
+
+    Every product is exact (x enters as a sum of bfloat16 numbers: three for float32, two for float16), the sums are float32, the
+    result is rounded once.  Any strides of x.  Differentiable with respect to x, any number of times; q is a constant.  Blocks of q
+    along either axis."""
+    _checked(x, q, "x", 1)
+    return _apply(x, q, q.axis == 1)
+
+
+def linear_grad(dy, q):
+    """dy (..., N) . q (N, K) -> (..., K): the gradient of `linear` with respect to x, and the product with the matrix itself where
+    `linear` multiplies with its transpose.  Same types, rounding and differentiability."""
+    _checked(dy, q, "dy", 0)
+    return _apply(dy, q, q.axis == 0)

@@ -1,0 +1,88 @@
+"""Refusals of the 4-bit operators: wrong arguments are turned down before anything reaches a GPU (none is needed here)."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+from linearcorex_amd import _abi, mx4                                   # noqa: E402
+from tests import mx4_reference as R                                     # noqa: E402
+
+
+@pytest.fixture(scope="module")
+def lib():
+    import __graft_entry__ as ge
+    ge.build()
+    return _abi.load()
+
+
+def fake(shape, axis=1):
+    """a matrix on the meta device: what the checks see"""
+    r, c = shape if axis == 1 else shape[::-1]
+    cb, sb = mx4._rows_bytes(c)
+    return mx4.Mx4(shape, axis, torch.empty(r, cb, dtype=torch.uint8, device="meta"), torch.empty(r, sb, dtype=torch.uint8, device="meta"))
+
+
+def test_python_refuses_host_tensors_and_wrong_types():
+    q = fake((4, 64))
+    for call in (lambda: mx4.quantize(torch.zeros(2, 2)), lambda: mx4.linear(torch.zeros(2, 64), q), lambda: mx4.linear_grad(torch.zeros(2, 4), q)):
+        with pytest.raises(ValueError, match="must be on the GPU"):
+            call()
+    for call in (lambda: mx4.quantize(np.zeros((2, 2))), lambda: mx4.linear([1.0], q), lambda: mx4.dequantize(torch.zeros(2, 2)),
+                 lambda: mx4.matmul(q, torch.zeros(2, 2)), lambda: mx4.matmul(q, q, torch.float64), lambda: mx4.dequantize(q, torch.int8)):
+        with pytest.raises(TypeError):
+            call()
+
+
+def test_python_refuses_shapes_that_do_not_fit():
+    with pytest.raises(ValueError, match="columns"):
+        mx4.matmul(fake((4, 64)), fake((4, 65)))
+    with pytest.raises(ValueError, match="along the blocks"):
+        mx4.matmul(fake((4, 64)), fake((4, 64), axis=0))
+    q = fake((4, 64))
+    assert q.t().shape == (64, 4) and q.t().axis == 0 and q.t().t().axis == 1 and q.t()._stored() == (4, 64)
+    assert "Mx4(shape=(4, 64), axis=1" in repr(q)
+
+
+def _call(lib, name, *args):
+    rc = getattr(lib, name)(*args)
+    return rc, (lib.lcx_last_error() or b"").decode()
+
+
+def test_c_entry_points_refuse_bad_arguments(lib):
+    p, odd = 4096, 4097                       # never dereferenced: every call below is refused before a launch
+    bad = [("lcx_mx4_quantize", (p, 9, 4, 64, 64, 1, p, p, None)), ("lcx_mx4_quantize", (p, 0, -1, 64, 64, 1, p, p, None)),
+           ("lcx_mx4_quantize", (p, 0, 4, 1 << 31, 64, 1, p, p, None)), ("lcx_mx4_quantize", (None, 0, 4, 64, 64, 1, p, p, None)),
+           ("lcx_mx4_quantize", (p, 0, 4, 64, 64, 1, odd, p, None)), ("lcx_mx4_quantize", (p, 0, 4, 64, 64, 1, p, odd, None)),
+           ("lcx_mx4_dequantize", (p, p, 4, 64, None, 0, 64, 1, None)), ("lcx_mx4_dequantize", (p, p, 4, 64, p, 4, 64, 1, None)),
+           ("lcx_mx4_dequantize", (odd, p, 4, 64, p, 0, 64, 1, None)),
+           ("lcx_mx4_matmul", (p, p, 4, p, p, 4, 64, p, 1, 4, 1, None, 0, None)), ("lcx_mx4_matmul", (p, p, 4, p, None, 4, 64, p, 0, 4, 1, None, 0, None)),
+           ("lcx_mx4_matmul", (p, p, -4, p, p, 4, 64, p, 0, 4, 1, None, 0, None)), ("lcx_mx4_matmul", (p, p, 4, odd, p, 4, 64, p, 0, 4, 1, None, 0, None)),
+           ("lcx_mx4_linear", (p, 1, 4, 64, 1, p, p, 4, 64, p, 4, 1, None, 0, None)), ("lcx_mx4_linear", (None, 0, 4, 64, 1, p, p, 4, 64, p, 4, 1, None, 0, None)),
+           ("lcx_mx4_linear", (p, 0, 4, 64, 1, p, odd, 4, 64, p, 4, 1, None, 0, None)), ("lcx_mx4_linear", (p, 0, 4, 64, 1, p, p, 4, -1, p, 4, 1, None, 0, None)),
+           ("lcx_mx4_linear_grad", (p, 1, 4, 4, 1, p, p, 4, 64, p, 64, 1, None, 0, None)), ("lcx_mx4_linear_grad", (p, 0, 4, 4, 1, p, p, 4, 64, None, 64, 1, None, 0, None)),
+           ("lcx_mx4_linear_grad", (p, 0, 4, 4, 1, odd, p, 4, 64, p, 64, 1, None, 0, None))]
+    for name, args in bad:
+        rc, msg = _call(lib, name, *args)
+        assert rc == 1 and msg.startswith(name), (name, args, rc, msg)
+    b, n = C.c_int64(), C.c_int64()
+    for args in ((3, 0, 1, 1, 1), (0, 1, 1, 1, 1), (1, 0, -1, 1, 1)):
+        assert _call(lib, "lcx_mx4_workspace", *args, C.byref(b))[0] == 1
+    assert _call(lib, "lcx_mx4_workspace", 1, 0, 1, 1, 1, None)[0] == 1 and _call(lib, "lcx_mx4_layout", -1, None, None)[0] == 1
+    for cols in (0, 1, 31, 256, 257, 512, 513, 5000):
+        assert lib.lcx_mx4_layout(cols, C.byref(b), C.byref(n)) == 0
+        assert (b.value, n.value) == mx4._rows_bytes(cols)
+    # nothing to do: no device is needed either
+    assert lib.lcx_mx4_quantize(None, 0, 0, 64, 64, 1, None, None, None) == 0
+    assert lib.lcx_mx4_linear(None, 0, 0, 64, 1, None, None, 4, 64, None, 4, 1, None, 0, None) == 0
+
+
+def test_reference_format():
+    """the restatement the GPU tests compare with, on values worked out by hand"""
+    x = np.zeros((1, 64))
+    x[0, :9] = [4.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, -7.9]
+    x[0, 32:35] = [1.0, 2.0 ** -4, -2.0 ** -3]
+    code, byte = R.quantize(x)
+    assert byte.tolist() == [[127, 125]]
+    assert code[0, :9].tolist() == [6, 0, 2, 2, 4, 4, 6, 6, 15] and code[0, 32:35].tolist() == [6, 0, 9]
+    assert R.values(code, byte)[0, [0, 8, 32, 34]].tolist() == [4.0, -6.0, 1.0, -0.125]

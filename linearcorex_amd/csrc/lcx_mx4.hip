@@ -82,30 +82,169 @@ static int mx4_matmul(const void* ac, const void* as, int64_t M, const void* bc,
     return LCX_OK;
 }
 
-template <typename T>
-static int mx4_linear(const void* x, int64_t M, int64_t xrs, int64_t xcs, const void* wc, const void* ws, int64_t N, int64_t K, void* out, int64_t rs,
-                      int64_t cs, hipStream_t st) {
-    if (K == 0) return mx4_zero<T>(out, M, N, rs, cs, st);
-    const int64_t mt = cdiv(M, 16);
+// ---- products of x with a 4-bit matrix -------------------------------------------------------------------------------------------------
+// What one call does: sizes of its tiles, its splits of the contraction and its work space [fragments of x | partial sums].
+struct MxPlan {
+    bool row = false;                  // up to 16 rows of x: the row kernels
+    int ct = 1, rt = 1, waves = 8;     // 16-row tiles of x, of W (linear); waves of a row kernel's block
+    int64_t mt = 1, nt = 1;            // tiles over the rows of x / over the output columns
+    int64_t nfrag = 0;                 // fragments of the contraction
+    int split = 1;
+    int64_t frag_bytes = 0, part_bytes = 0;
+};
+constexpr int MX_CUS = 256;            // blocks are sized for a whole MI355X; the choices below only shift speed
+
+static int64_t split_for(int64_t tiles, int64_t steps, int64_t want_blocks, int64_t min_steps) {
+    int64_t s = cdiv(want_blocks, tiles);
+    if (s > steps / min_steps) s = steps / min_steps;
+    return s < 1 ? 1 : s;
+}
+
+// M rows of x, C the contraction, O output columns; along: lcx_mx4_linear, else lcx_mx4_linear_grad
+template <typename T> static MxPlan mx_plan(bool along, int64_t M, int64_t C, int64_t O) {
+    constexpr int TERMS = MxTerms<T>::v;
+    MxPlan p;
+    if (M <= 16) {
+        p.row = true;
+        if (along) {
+            // 2 x 16 rows of W a wave halve the reads of x where there are enough rows to fill the chip; 16 waves split the contraction
+            // where there are few
+            p.rt = M > 4 && O >= 32 * MX_CUS ? 2 : 1;
+            p.waves = cdiv(O, 16 * p.rt) >= 2 * MX_CUS ? 8 : 16;
+        } else {
+            p.waves = 4;
+            p.nt = cdiv(O, 512);
+            p.split = (int)split_for(p.nt, cdiv(C, 32), 2 * MX_CUS, 4);
+        }
+    } else {
+        p.ct = M <= 32 ? 2 : M <= 64 || TERMS > 1 || !along ? 4 : 8;
+        p.rt = 4;
+        p.mt = cdiv(M, 16 * p.ct);
+        p.nt = along ? cdiv(O, 64 * p.rt) : cdiv(O, 512);
+        p.nfrag = along ? cdiv(C, 128) * 4 : cdiv(C, 128) * 4;
+        p.split = (int)split_for(p.mt * p.nt, cdiv(C, 128), 2 * MX_CUS, 8);
+        p.frag_bytes = p.nfrag * TERMS * p.mt * p.ct * 1024;
+    }
+    if (p.split > 1) p.part_bytes = (int64_t)p.split * M * O * 4;
+    return p;
+}
+static int64_t mx_plan_bytes(const MxPlan& p) { return round_up(p.frag_bytes, 256) + p.part_bytes; }
+
+template <typename T> static int64_t mx_workspace(int op, int64_t M, int64_t N, int64_t K) {
+    if (M == 0 || N == 0 || K == 0 || op == 0) return 0;
+    return op == 1 ? mx_plan_bytes(mx_plan<T>(true, M, K, N)) : mx_plan_bytes(mx_plan<T>(false, M, N, K));
+}
+
+// eight neighbours along the contraction can be read at once
+template <typename T> static bool mx_vec(const void* x, int64_t rs, int64_t cs, int64_t C) {
+    return cs == 1 && C % 8 == 0 && ((uintptr_t)x & 15) == 0 && (rs * (int64_t)sizeof(T)) % 16 == 0;
+}
+
+template <typename T, bool ALONG>
+static int mx_fragments(const T* x, int64_t M, int64_t rs, int64_t cs, int64_t C, const MxPlan& p, unsigned short* frag, hipStream_t st) {
+    const int64_t tiles = p.mt * p.ct;
     unsigned g;
-    LCXCHECK(mx_grid(mt, cdiv(N, 16), &g));
-    hipLaunchKernelGGL((mx_linear_kernel<T>), dim3(g), dim3(64), 0, st, (const T*)x, M, xrs, xcs, (const unsigned char*)wc, (const unsigned char*)ws, N, K,
-                       (T*)out, rs, cs, mt);
+    LCXCHECK(mx_grid(tiles, cdiv(p.nfrag * 4, 16), &g));
+    const int rows_first = (rs < 0 ? -rs : rs) < (cs < 0 ? -cs : cs);
+    if (mx_vec<T>(x, rs, cs, C))
+        hipLaunchKernelGGL((mx_fragments_kernel<T, ALONG, true>), dim3(g), dim3(256), 0, st, x, M, rs, cs, C, p.nfrag, tiles, frag, 0);
+    else
+        hipLaunchKernelGGL((mx_fragments_kernel<T, ALONG, false>), dim3(g), dim3(256), 0, st, x, M, rs, cs, C, p.nfrag, tiles, frag, rows_first);
+    KCHECK();
+    return LCX_OK;
+}
+
+template <typename T> static int mx_join(const MxPlan& p, const MxOut<T>& w, hipStream_t st) {
+    if (p.split == 1) return LCX_OK;
+    const int64_t b = cdiv(w.M * w.O, 256);
+    hipLaunchKernelGGL((mx_join_kernel<T>), dim3((unsigned)(b < 8192 ? b : 8192)), dim3(256), 0, st, w.part, p.split, w.M, w.O, w.out, w.rs, w.cs);
+    KCHECK();
+    return LCX_OK;
+}
+
+template <typename T, int CT, int JS>
+static int mx_linear_tiles(const MxPlan& p, const unsigned short* frag, const unsigned char* wc, const unsigned char* ws, int64_t N, int64_t K, const MxOut<T>& w,
+                           hipStream_t st) {
+    unsigned g;
+    LCXCHECK(mx_grid(8, cdiv(p.mt * p.nt * p.split, 8), &g));
+    hipLaunchKernelGGL((mx_linear_tile_kernel<T, CT, 4, JS>), dim3(g), dim3(256), 0, st, frag, p.mt * p.ct, wc, ws, N, K, w, p.mt, p.nt, p.split);
+    KCHECK();
+    return LCX_OK;
+}
+template <typename T, int CT, int JS>
+static int mx_grad_tiles(const MxPlan& p, const unsigned short* frag, const unsigned char* wc, const unsigned char* ws, int64_t N, int64_t K, const MxOut<T>& w,
+                         hipStream_t st) {
+    unsigned g;
+    LCXCHECK(mx_grid(8, cdiv(p.mt * p.nt * p.split, 8), &g));
+    hipLaunchKernelGGL((mx_grad_tile_kernel<T, CT, JS>), dim3(g), dim3(256), 0, st, frag, p.mt * p.ct, wc, ws, N, K, w, p.mt, p.nt, p.split);
+    KCHECK();
+    return LCX_OK;
+}
+
+template <typename T, bool VEC>
+static int mx_linear_rows(const MxPlan& p, const T* x, int64_t rs, int64_t cs, const unsigned char* wc, const unsigned char* ws, int64_t N, int64_t K,
+                          const MxOut<T>& w, hipStream_t st) {
+    unsigned g;
+    LCXCHECK(mx_grid(1, cdiv(N, 16 * p.rt), &g));
+#define MX_ROWS(RT, WV) hipLaunchKernelGGL((mx_linear_row_kernel<T, RT, WV, VEC>), dim3(g), dim3(64 * WV), 0, st, x, w.M, rs, cs, wc, ws, N, K, w)
+    if (p.rt == 2) {
+        if (p.waves == 8) MX_ROWS(2, 8); else MX_ROWS(2, 16);
+    } else {
+        if (p.waves == 8) MX_ROWS(1, 8); else MX_ROWS(1, 16);
+    }
+#undef MX_ROWS
     KCHECK();
     return LCX_OK;
 }
 
 template <typename T>
-static int mx4_linear_grad(const void* dy, int64_t M, int64_t yrs, int64_t ycs, const void* wc, const void* ws, int64_t N, int64_t K, void* out, int64_t rs,
-                           int64_t cs, hipStream_t st) {
+static int mx4_linear(const void* xv, int64_t M, int64_t xrs, int64_t xcs, const void* wcv, const void* wsv, int64_t N, int64_t K, void* out, int64_t rs,
+                      int64_t cs, void* space, int64_t space_bytes, hipStream_t st) {
+    constexpr int TERMS = MxTerms<T>::v;
+    if (K == 0) return mx4_zero<T>(out, M, N, rs, cs, st);
+    const MxPlan p = mx_plan<T>(true, M, K, N);
+    if (space_bytes < mx_plan_bytes(p) || (mx_plan_bytes(p) && !space)) return fail(LCX_ERR_ARG, "lcx_mx4_linear: the work space is smaller than lcx_mx4_workspace says");
+    const T* x = (const T*)xv;
+    const unsigned char *wc = (const unsigned char*)wcv, *ws = (const unsigned char*)wsv;
+    unsigned short* frag = (unsigned short*)space;
+    MxOut<T> w{(T*)out, rs, cs, p.split > 1 ? (float*)((char*)space + round_up(p.frag_bytes, 256)) : nullptr, M, N};
+    if (p.row) return mx_vec<T>(x, xrs, xcs, K) ? mx_linear_rows<T, true>(p, x, xrs, xcs, wc, ws, N, K, w, st)
+                                                : mx_linear_rows<T, false>(p, x, xrs, xcs, wc, ws, N, K, w, st);
+    LCXCHECK((mx_fragments<T, true>(x, M, xrs, xcs, K, p, frag, st)));
+    constexpr int JS = TERMS == 3 ? 2 : 4;
+    if (p.ct == 2) LCXCHECK((mx_linear_tiles<T, 2, 4>(p, frag, wc, ws, N, K, w, st)));
+    else if (p.ct == 4) LCXCHECK((mx_linear_tiles<T, 4, JS>(p, frag, wc, ws, N, K, w, st)));
+    else {
+        if constexpr (TERMS == 1) LCXCHECK((mx_linear_tiles<T, 8, 4>(p, frag, wc, ws, N, K, w, st)));
+    }
+    return mx_join<T>(p, w, st);
+}
+
+template <typename T>
+static int mx4_linear_grad(const void* dyv, int64_t M, int64_t yrs, int64_t ycs, const void* wcv, const void* wsv, int64_t N, int64_t K, void* out, int64_t rs,
+                           int64_t cs, void* space, int64_t space_bytes, hipStream_t st) {
+    constexpr int TERMS = MxTerms<T>::v;
     if (N == 0) return mx4_zero<T>(out, M, K, rs, cs, st);
-    const int64_t mt = cdiv(M, 16);
-    unsigned g;
-    LCXCHECK(mx_grid(mt, cdiv(K, 128), &g));
-    hipLaunchKernelGGL((mx_linear_grad_kernel<T>), dim3(g), dim3(64), 0, st, (const T*)dy, M, yrs, ycs, (const unsigned char*)wc, (const unsigned char*)ws, N,
-                       K, (T*)out, rs, cs, mt);
-    KCHECK();
-    return LCX_OK;
+    const MxPlan p = mx_plan<T>(false, M, N, K);
+    if (space_bytes < mx_plan_bytes(p) || (mx_plan_bytes(p) && !space)) return fail(LCX_ERR_ARG, "lcx_mx4_linear_grad: the work space is smaller than lcx_mx4_workspace says");
+    const T* dy = (const T*)dyv;
+    const unsigned char *wc = (const unsigned char*)wcv, *ws = (const unsigned char*)wsv;
+    unsigned short* frag = (unsigned short*)space;
+    MxOut<T> w{(T*)out, rs, cs, p.split > 1 ? (float*)((char*)space + round_up(p.frag_bytes, 256)) : nullptr, M, K};
+    if (p.row) {
+        const dim3 g((unsigned)p.nt, (unsigned)p.split);
+        if (mx_vec<T>(dy, yrs, ycs, N))
+            hipLaunchKernelGGL((mx_grad_row_kernel<T, 4, true>), g, dim3(256), 0, st, dy, M, yrs, ycs, wc, ws, N, K, w);
+        else
+            hipLaunchKernelGGL((mx_grad_row_kernel<T, 4, false>), g, dim3(256), 0, st, dy, M, yrs, ycs, wc, ws, N, K, w);
+        KCHECK();
+        return mx_join<T>(p, w, st);
+    }
+    LCXCHECK((mx_fragments<T, false>(dy, M, yrs, ycs, N, p, frag, st)));
+    constexpr int JS = TERMS == 3 ? 2 : 4;
+    if (p.ct == 2) LCXCHECK((mx_grad_tiles<T, 2, 4>(p, frag, wc, ws, N, K, w, st)));
+    else LCXCHECK((mx_grad_tiles<T, 4, JS>(p, frag, wc, ws, N, K, w, st)));
+    return mx_join<T>(p, w, st);
 }
 
 extern "C" {
@@ -150,7 +289,7 @@ int lcx_mx4_workspace(int op, int dtype, int64_t M, int64_t N, int64_t K, int64_
     MX_ENTRY({
         if (!bytes || op < 0 || op > 2 || dim_bad(M, N, K)) return fail(LCX_ERR_ARG, "lcx_mx4_workspace: bad argument");
         if (dtype != LCX_F32 && dtype != LCX_BF16 && dtype != LCX_F16) return fail(LCX_ERR_ARG, "lcx_mx4_workspace: bad dtype");
-        *bytes = 0;
+        *bytes = dtype == LCX_F32 ? mx_workspace<float>(op, M, N, K) : dtype == LCX_BF16 ? mx_workspace<__bf16>(op, M, N, K) : mx_workspace<_Float16>(op, M, N, K);
         return LCX_OK;
     })
 }
@@ -177,8 +316,7 @@ int lcx_mx4_linear(const void* x, int dtype, int64_t M, int64_t x_row, int64_t x
         if (M == 0 || N == 0) return LCX_OK;
         if (!out || (K > 0 && (!x || !codes || !scales))) return fail(LCX_ERR_ARG, "lcx_mx4_linear: null pointer");
         if (mx_misaligned(codes, scales)) return fail(LCX_ERR_ARG, "lcx_mx4_linear: codes must be 16-byte and scales 4-byte aligned");
-        (void)workspace; (void)workspace_bytes;
-        MX_FLOATS(dtype, mx4_linear, x, M, x_row, x_col, codes, scales, N, K, out, row_stride, col_stride, (hipStream_t)stream);
+        MX_FLOATS(dtype, mx4_linear, x, M, x_row, x_col, codes, scales, N, K, out, row_stride, col_stride, workspace, workspace_bytes, (hipStream_t)stream);
     })
 }
 
@@ -191,8 +329,7 @@ int lcx_mx4_linear_grad(const void* dy, int dtype, int64_t M, int64_t dy_row, in
         if (M == 0 || K == 0) return LCX_OK;
         if (!out || (N > 0 && (!dy || !codes || !scales))) return fail(LCX_ERR_ARG, "lcx_mx4_linear_grad: null pointer");
         if (mx_misaligned(codes, scales)) return fail(LCX_ERR_ARG, "lcx_mx4_linear_grad: codes must be 16-byte and scales 4-byte aligned");
-        (void)workspace; (void)workspace_bytes;
-        MX_FLOATS(dtype, mx4_linear_grad, dy, M, dy_row, dy_col, codes, scales, N, K, out, row_stride, col_stride, (hipStream_t)stream);
+        MX_FLOATS(dtype, mx4_linear_grad, dy, M, dy_row, dy_col, codes, scales, N, K, out, row_stride, col_stride, workspace, workspace_bytes, (hipStream_t)stream);
     })
 }
 

@@ -193,87 +193,448 @@ __device__ __forceinline__ mx_bf8 mx_unpack8(unsigned int q, float s) {
     return mx_bf8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// x[t * rs + k * cs], eight k from k0 on, as bf16 terms; zeros outside
-template <typename T, int TERMS>
-__device__ __forceinline__ void mx_load_terms(const T* __restrict__ x, int64_t t, int64_t nt, int64_t rs, int64_t k0, int64_t nk, int64_t cs, mx_bf8* f) {
+// x[t * rs + k * cs], eight k from k0 on, as bf16 terms; zeros from nk on.  VEC: cs is 1, the eight values are aligned to 16 bytes and nk is a
+// multiple of 8.  t must be a row.
+template <typename T, int TERMS, bool VEC>
+__device__ __forceinline__ void mx_load_terms(const T* __restrict__ x, int64_t t, int64_t rs, int64_t k0, int64_t nk, int64_t cs, mx_bf8* f) {
+    T v[8];
+    if constexpr (VEC) {
+        if (k0 < nk) {
+            const mx_u4* p = reinterpret_cast<const mx_u4*>(x + t * rs + k0);
+            mx_u4 r[sizeof(T) / 2];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        float p[3] = {0.0f, 0.0f, 0.0f};
-        if (t < nt && k0 + j < nk) mx_split<TERMS>((float)x[t * rs + (k0 + j) * cs], p);
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) r[i] = p[i];
+            __builtin_memcpy(v, r, sizeof(v));
+        } else {
 #pragma unroll
-        for (int u = 0; u < TERMS; ++u) f[u][j] = (__bf16)p[u];
-    }
-}
-
-// out[t][n] = sum_k x[t][k] W[n][k], W in 4 bits with its blocks along k: the codes become bf16 in registers, x is split into bf16 terms
-// (MxTerms), every product is exact, float32 sums.  A wave owns 16 rows of W and 16 of x.
-template <typename T>
-__global__ __launch_bounds__(64) void mx_linear_kernel(const T* __restrict__ x, int64_t M, int64_t xrs, int64_t xcs, const unsigned char* __restrict__ wc,
-                                                       const unsigned char* __restrict__ ws, int64_t N, int64_t K, T* __restrict__ out, int64_t rs,
-                                                       int64_t cs, int64_t mtiles) {
-    constexpr int TERMS = MxTerms<T>::v;
-    const int64_t crow = mx_code_row(K), srow = mx_scale_row(K);
-    const int64_t t0 = (int64_t)(blockIdx.x % mtiles) * 16, n0 = (int64_t)(blockIdx.x / mtiles) * 16;
-    const int l = threadIdx.x & 15, g = threadIdx.x >> 4;
-    const int64_t rn = n0 + l < N ? n0 + l : N - 1;
-    mx_f4 acc = {};
-    for (int64_t s = 0; s * 64 < crow; ++s) {
-        const mx_u4 q = *reinterpret_cast<const mx_u4*>(wc + rn * crow + s * 64 + g * 16);
-        const float sc = __uint_as_float((unsigned int)ws[rn * srow + (s >> 2) * 16 + g * 4 + (s & 3)] << 23);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const mx_bf8 w = mx_unpack8(q[j], sc);
-            mx_bf8 f[TERMS];
-            mx_load_terms<T, TERMS>(x, t0 + l, M, xrs, s * 128 + g * 32 + j * 8, K, xcs, f);
-#pragma unroll
-            for (int u = 0; u < TERMS; ++u) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, f[u], acc, 0, 0, 0);
+            for (int j = 0; j < 8; ++j) v[j] = (T)0.0f;
         }
-    }
+    } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const int64_t n = n0 + 4 * g + e, t = t0 + l;
-        if (n < N && t < M) out[t * rs + n * cs] = mx_from_f32<T>(acc[e]);
+        for (int j = 0; j < 8; ++j) v[j] = k0 + j < nk ? x[t * rs + (k0 + j) * cs] : (T)0.0f;
     }
-}
-
-// dx[t][k] = sum_n dy[t][n] W[n][k]: the contraction runs ACROSS the blocks.  A lane reads the dword of 8 columns from each of 8 rows of W;
-// unpacked, entry m of the eight dwords is what matrix instruction m needs from this lane: column 8 (lane % 16) + m, eight n.  So a
-// wave owns 128 columns as 8 tiles and no value crosses lanes.
-template <typename T>
-__global__ __launch_bounds__(64) void mx_linear_grad_kernel(const T* __restrict__ dy, int64_t M, int64_t yrs, int64_t ycs,
-                                                            const unsigned char* __restrict__ wc, const unsigned char* __restrict__ ws, int64_t N, int64_t K,
-                                                            T* __restrict__ out, int64_t rs, int64_t cs, int64_t mtiles) {
-    constexpr int TERMS = MxTerms<T>::v;
-    const int64_t crow = mx_code_row(K), srow = mx_scale_row(K);
-    const int64_t t0 = (int64_t)(blockIdx.x % mtiles) * 16, k0 = (int64_t)(blockIdx.x / mtiles) * 128;
-    const int l = threadIdx.x & 15, g = threadIdx.x >> 4;
-    const int64_t sat = mx_scale_at((k0 + l * 8) >> 5);
-    mx_f4 acc[8] = {};
-    for (int64_t n0 = 0; n0 < N; n0 += 32) {
-        mx_bf8 w[8];
+    if constexpr (TERMS == 1) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[0][j] = (__bf16)v[j];
+    } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int64_t n = n0 + g * 8 + j;
-            // rows behind the last one contribute zeros (their factor in dy is zero, but a NaN scale must not meet it)
-            const unsigned int q = n < N ? *reinterpret_cast<const unsigned int*>(wc + n * crow + (k0 >> 1) + l * 4) : 0u;
-            const float sc = n < N ? __uint_as_float((unsigned int)ws[n * srow + sat] << 23) : 1.0f;
-            const mx_bf8 v = mx_unpack8(q, sc);
+            float p[3];
+            mx_split<TERMS>((float)v[j], p);
 #pragma unroll
-            for (int m = 0; m < 8; ++m) w[m][j] = v[m];
+            for (int u = 0; u < TERMS; ++u) f[u][j] = (__bf16)p[u];
         }
-        mx_bf8 f[TERMS];
-        mx_load_terms<T, TERMS>(dy, t0 + l, M, yrs, n0 + g * 8, N, ycs, f);
+    }
+}
+
+// where an output goes: split == 1 the result, else float32 partial sums [split][M][O] (mx_join_kernel adds them up in order)
+template <typename T> struct MxOut {
+    T* out;
+    int64_t rs, cs;
+    float* part;
+    int64_t M, O;
+};
+// N consecutive columns o .. of row t
+template <typename T, int N>
+__device__ __forceinline__ void mx_store(const MxOut<T>& w, int64_t z, int64_t t, int64_t o, const float* v) {
+    if (t >= w.M) return;
+    if (w.part) {
+        float* p = w.part + (z * w.M + t) * w.O + o;
 #pragma unroll
-        for (int m = 0; m < 8; ++m)
+        for (int j = 0; j < N; ++j)
+            if (o + j < w.O) p[j] = v[j];
+        return;
+    }
+    T* p = w.out + t * w.rs + o * w.cs;
+    if (w.cs == 1 && o + N <= w.O && ((uintptr_t)p & (N * sizeof(T) - 1)) == 0) {
+        typedef T vec __attribute__((ext_vector_type(N)));
+        vec r;
 #pragma unroll
-            for (int u = 0; u < TERMS; ++u) acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[m], f[u], acc[m], 0, 0, 0);
+        for (int j = 0; j < N; ++j) r[j] = mx_from_f32<T>(v[j]);
+        *reinterpret_cast<vec*>(p) = r;
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (o + j < w.O) p[j * w.cs] = mx_from_f32<T>(v[j]);
+    }
+}
+// out[t][o] = sum over the splits, in order
+template <typename T>
+__global__ __launch_bounds__(256) void mx_join_kernel(const float* __restrict__ part, int split, int64_t M, int64_t O, T* __restrict__ out, int64_t rs,
+                                                      int64_t cs) {
+    const int64_t n = M * O;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        float v = part[i];
+        for (int z = 1; z < split; ++z) v += part[(int64_t)z * n + i];
+        out[(i / O) * rs + (i % O) * cs] = mx_from_f32<T>(v);
+    }
+}
+
+// ---- few rows of x (up to 16: tokens being decoded) -----------------------------------------------------------------------------
+// out[t][n] = sum_k x[t][k] W[n][k], W in 4 bits with its blocks along k: the codes become bf16 in registers, x is split into bf16 terms
+// (MxTerms), every product is exact, float32 sums.  Bound: reading W (4.25 bits a value).  The waves of a block share 16 RT rows of W and
+// split the contraction (128 columns a step), so that a single token still puts every load of W in flight at once; partial sums meet in LDS.
+template <typename T, int RT, int WAVES, bool VEC>
+__global__ __launch_bounds__(64 * WAVES) void mx_linear_row_kernel(const T* __restrict__ x, int64_t M, int64_t xrs, int64_t xcs,
+                                                                   const unsigned char* __restrict__ wc, const unsigned char* __restrict__ ws, int64_t N,
+                                                                   int64_t K, MxOut<T> w) {
+    constexpr int TERMS = MxTerms<T>::v, U = 4;
+    const int64_t crow = mx_code_row(K), srow = mx_scale_row(K);
+    const int64_t n0 = (int64_t)blockIdx.x * 16 * RT;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
+    const int64_t t = l < M ? l : M - 1;                       // rows behind the last one repeat it and are not stored
+    const unsigned char *pc[RT], *ps[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        const int64_t rn = n0 + 16 * i + l < N ? n0 + 16 * i + l : N - 1;
+        pc[i] = wc + rn * crow + g * 16;
+        ps[i] = ws + rn * srow + g * 4;
+    }
+    mx_f4 acc[RT] = {};
+    const int64_t steps = (K + 127) / 128;
+    for (int64_t s0 = wave; s0 < steps; s0 += U * WAVES) {
+        mx_u4 q[U][RT];
+        unsigned int sc[U][RT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t s = s0 + u * WAVES;
+            if (s < steps) {
+#pragma unroll
+                for (int i = 0; i < RT; ++i) {
+                    q[u][i] = *reinterpret_cast<const mx_u4*>(pc[i] + s * 64);
+                    sc[u][i] = ps[i][(s >> 2) * 16 + (s & 3)];
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t s = s0 + u * WAVES;
+            if (s < steps) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    mx_bf8 f[TERMS];
+                    mx_load_terms<T, TERMS, VEC>(x, t, xrs, s * 128 + g * 32 + j * 8, K, xcs, f);
+#pragma unroll
+                    for (int i = 0; i < RT; ++i) {
+                        const mx_bf8 a = mx_unpack8(q[u][i][j], __uint_as_float(sc[u][i] << 23));
+#pragma unroll
+                        for (int e = 0; e < TERMS; ++e) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, f[e], acc[i], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    }
+    __shared__ mx_f4 red[WAVES][RT][64];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) red[wave][i][lane] = acc[i];
+    __syncthreads();
+    for (int i = wave; i < RT; i += WAVES) {
+        mx_f4 v = red[0][i][lane];
+#pragma unroll
+        for (int k = 1; k < WAVES; ++k) v += red[k][i][lane];
+        float o[4] = {v[0], v[1], v[2], v[3]};
+        mx_store<T, 4>(w, 0, l, n0 + 16 * i + 4 * g, o);
+    }
+}
+
+// 8 columns of one row of W as bf16, entry m of dword j -> what matrix instruction m takes from this lane: the transposition of an 8 x 8 piece
+// that the lane holds whole, two values a dword
+__device__ __forceinline__ void mx_unpack_across(const unsigned int* q, const unsigned int* sc, mx_bf8* w) {
+    unsigned int u[8][4];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const mx_bf8 v = mx_unpack8(q[j], __uint_as_float(sc[j] << 23));
+        __builtin_memcpy(u[j], &v, 16);
     }
 #pragma unroll
-    for (int m = 0; m < 8; ++m)
+    for (int m = 0; m < 8; ++m) {
+        unsigned int r[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            r[j] = __builtin_amdgcn_perm(u[2 * j + 1][m >> 1], u[2 * j][m >> 1], (m & 1) ? 0x07060302u : 0x05040100u);
+        __builtin_memcpy(&w[m], r, 16);
+    }
+}
+
+// dx[t][k] = sum_n dy[t][n] W[n][k], up to 16 rows: the contraction runs ACROSS the blocks.  A lane reads 16 bytes (32 columns: one block, one
+// scale) from each of 8 rows of W; entry m of the eight is what matrix instruction m needs from this lane: column 32 (lane % 16) + m,
+// eight n.  So a wave owns 512 columns as 32 tiles and no value crosses lanes.  The waves of a block split the rows, the blocks along
+// y too (partial sums to memory).
+template <typename T, int WAVES, bool VEC>
+__global__ __launch_bounds__(64 * WAVES) void mx_grad_row_kernel(const T* __restrict__ dy, int64_t M, int64_t yrs, int64_t ycs,
+                                                                 const unsigned char* __restrict__ wc, const unsigned char* __restrict__ ws, int64_t N,
+                                                                 int64_t K, MxOut<T> w) {
+    constexpr int TERMS = MxTerms<T>::v;
+    const int64_t crow = mx_code_row(K), srow = mx_scale_row(K);
+    const int64_t k0 = (int64_t)blockIdx.x * 512;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
+    const int64_t t = l < M ? l : M - 1;
+    // (columns behind the row repeat its last 16 bytes and are not stored)
+    const int64_t kb = k0 / 2 + l * 16 < crow ? k0 / 2 + l * 16 : crow - 16;
+    const int64_t sat = mx_scale_at(kb >> 4);
+    mx_f4 acc[32] = {};
+    const int64_t steps = (N + 31) / 32, stride = (int64_t)WAVES * gridDim.y;
+    for (int64_t s = (int64_t)blockIdx.y * WAVES + wave; s < steps; s += stride) {
+        mx_u4 q[8];
+        unsigned int sc[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int64_t n = s * 32 + g * 8 + j;
+            // rows behind the last one are zeros with a finite scale (their factor in dy is zero too, but must not meet a NaN)
+            q[j] = n < N ? *reinterpret_cast<const mx_u4*>(wc + n * crow + kb) : mx_u4{0, 0, 0, 0};
+            sc[j] = n < N ? ws[n * srow + sat] : 127u;
+        }
+        mx_bf8 f[TERMS];
+        mx_load_terms<T, TERMS, VEC>(dy, t, yrs, s * 32 + g * 8, N, ycs, f);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            unsigned int qd[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) qd[j] = q[j][d];
+            mx_bf8 a[8];
+            mx_unpack_across(qd, sc, a);
+#pragma unroll
+            for (int m = 0; m < 8; ++m)
+#pragma unroll
+                for (int e = 0; e < TERMS; ++e) acc[d * 8 + m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[m], f[e], acc[d * 8 + m], 0, 0, 0);
+        }
+    }
+    __shared__ mx_f4 red[WAVES][8][64];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        if (d) __syncthreads();
+#pragma unroll
+        for (int m = 0; m < 8; ++m) red[wave][m][lane] = acc[d * 8 + m];
+        __syncthreads();
+        // lane (l, g) of output row 4 g + e holds columns 32 (4 g + e) + 8 d + m
+        for (int e = wave; e < 4; e += WAVES) {
+            float o[8];
+#pragma unroll
+            for (int m = 0; m < 8; ++m) {
+                o[m] = red[0][m][lane][e];
+#pragma unroll
+                for (int k = 1; k < WAVES; ++k) o[m] += red[k][m][lane][e];
+            }
+            mx_store<T, 8>(w, blockIdx.y, l, k0 + 32 * (4 * g + e) + 8 * d, o);
+        }
+    }
+}
+
+// ---- many rows of x -------------------------------------------------------------------------------------------------------------
+// The rows of x meet the matrix instructions as bf16 fragments: 16 rows, 32 of the contraction, 64 lanes x 16 bytes.  Fragment i of the
+// contraction holds, for lane group g, eight values from
+//   along the blocks   128 (i / 4) + 32 g + 8 (i % 4)      (a lane of W owns one block of each 128 columns, 8 values an instruction)
+//   across the blocks  32 i + 8 g
+// mx_fragments_kernel lays x out that way once per call, split into its bf16 terms: frag[i][term][tile of 16 rows][lane][8].  A tile of the
+// products below is then a contiguous piece of memory, whatever x's type, strides or odd sizes.
+template <bool ALONG> __device__ __forceinline__ int64_t mx_frag_k(int64_t i, int g) {
+    return ALONG ? (i >> 2) * 128 + g * 32 + (i & 3) * 8 : i * 32 + g * 8;
+}
+template <typename T, bool ALONG, bool VEC>
+__global__ __launch_bounds__(256) void mx_fragments_kernel(const T* __restrict__ x, int64_t M, int64_t xrs, int64_t xcs, int64_t K, int64_t nfrag,
+                                                           int64_t tiles, unsigned short* __restrict__ frag, int rows_first) {
+    constexpr int TERMS = MxTerms<T>::v;
+    // a block takes one tile of 16 rows and 16 groups of 8 values; neighbouring threads read neighbouring memory
+    const int64_t tile = blockIdx.x % tiles, c0 = (int64_t)(blockIdx.x / tiles) * 16;
+    const int l = rows_first ? threadIdx.x & 15 : threadIdx.x >> 4;
+    const int64_t c = c0 + (rows_first ? threadIdx.x >> 4 : threadIdx.x & 15);         // group of 8 along the contraction
+    if (c >= nfrag * 4) return;
+    const int64_t i = ALONG ? (c >> 4) * 4 + (c & 3) : c >> 2;
+    const int g = (int)(ALONG ? (c >> 2) & 3 : c & 3);
+    const int64_t t = tile * 16 + l;
+    mx_bf8 f[TERMS] = {};
+    if (t < M) mx_load_terms<T, TERMS, VEC>(x, t, xrs, c * 8, K, xcs, f);
+#pragma unroll
+    for (int u = 0; u < TERMS; ++u) *reinterpret_cast<mx_bf8*>(frag + (((i * TERMS + u) * tiles + tile) * 64 + g * 16 + l) * 8) = f[u];
+}
+
+typedef __attribute__((address_space(1))) const void* mx_gptr;
+typedef __attribute__((address_space(3))) void* mx_lptr;
+
+// block -> (row tile, column tile, split): consecutive blocks go to the 8 XCDs in turn, so each XCD gets a contiguous piece of an order in which
+// eight row tiles share a column tile of W
+struct MxTile { int64_t a, b; int z; };
+__device__ __forceinline__ MxTile mx_tile(int64_t id, int64_t na, int64_t nb, int split) {
+    const int64_t total = na * nb * split, per = (total + 7) / 8;
+    int64_t p = (id & 7) * per + (id >> 3);
+    MxTile r;
+    if (p >= total || (id >> 3) >= per) { r.a = -1; r.b = 0; r.z = 0; return r; }
+    r.z = (int)(p / (na * nb));
+    p -= (int64_t)r.z * na * nb;
+    const int64_t grp = p / (8 * nb), left = na - grp * 8 < 8 ? na - grp * 8 : 8;
+    p -= grp * 8 * nb;
+    r.a = grp * 8 + p % left;
+    r.b = p / left;
+    return r;
+}
+
+// out[t][n] = sum_k x[t][k] W[n][k] for tiles of 16 CT rows of x and 64 RT rows of W.  Bound: the bf16 matrix pipe (TERMS instructions per
+// product).  The four waves own 16 RT rows of W each - codes go from memory to registers and become bf16 there, no LDS - and share the fragments
+// of x through LDS (JS of them a stage, double buffered).
+template <typename T, int CT, int RT, int JS>
+__global__ __launch_bounds__(256) void mx_linear_tile_kernel(const unsigned short* __restrict__ frag, int64_t tiles, const unsigned char* __restrict__ wc,
+                                                             const unsigned char* __restrict__ ws, int64_t N, int64_t K, MxOut<T> w, int64_t mt,
+                                                             int64_t nt, int split) {
+    constexpr int TERMS = MxTerms<T>::v, CH = JS * TERMS * CT;             // 1 KB pieces a stage
+    const int64_t crow = mx_code_row(K), srow = mx_scale_row(K);
+    const MxTile tile = mx_tile(blockIdx.x, mt, nt, split);
+    if (tile.a < 0) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
+    const int64_t n0 = tile.b * 64 * RT + wave * 16 * RT;
+    const int64_t steps = (K + 127) / 128, per = ((steps + split - 1) / split + 3) / 4 * 4;      // (whole dwords of scales)
+    const int64_t s0 = per * tile.z, s1 = s0 + per < steps ? s0 + per : steps;
+    __shared__ __attribute__((aligned(16))) unsigned short lds[2][CH * 512];
+    const unsigned char *pc[RT], *ps[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        const int64_t rn = n0 + 16 * i + l < N ? n0 + 16 * i + l : N - 1;
+        pc[i] = wc + rn * crow + g * 16;
+        ps[i] = ws + rn * srow + g * 4;
+    }
+    auto stage = [&](int64_t f, int b) {                                   // fragments f .. f + JS of the contraction
+#pragma unroll
+        for (int c = 0; c < (CH + 3) / 4; ++c) {
+            const int i = c * 4 + wave;
+            if (CH % 4 == 0 || i < CH) {
+                const int64_t at = ((f * TERMS + i / CT) * tiles + tile.a * CT + i % CT) * 512;
+                __builtin_amdgcn_global_load_lds((mx_gptr)(frag + at + lane * 8), (mx_lptr)(&lds[b][i * 512]), 16, 0, 0);
+            }
+        }
+    };
+    mx_f4 acc[RT][CT] = {};
+    mx_u4 q[RT];
+    unsigned int sd[RT];
+    if (s0 < s1) {
+        stage(s0 * 4, 0);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            q[i] = *reinterpret_cast<const mx_u4*>(pc[i] + s0 * 64);
+            sd[i] = *reinterpret_cast<const unsigned int*>(ps[i] + (s0 >> 2) * 16);
+        }
+    }
+    __syncthreads();
+    int b = 0;
+    for (int64_t s = s0; s < s1; ++s) {
+        mx_u4 qn[RT];
+        unsigned int sn[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) { qn[i] = q[i]; sn[i] = sd[i]; }
+        float sc[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) sc[i] = __uint_as_float(((sd[i] >> (8 * (s & 3))) & 255u) << 23);
+#pragma unroll
+        for (int h = 0; h < 4 / JS; ++h) {
+            if (h + 1 < 4 / JS) stage(s * 4 + (h + 1) * JS, b ^ 1);
+            else if (s + 1 < s1) stage((s + 1) * 4, b ^ 1);
+            if (h == 0 && s + 1 < s1) {
+#pragma unroll
+                for (int i = 0; i < RT; ++i) {
+                    qn[i] = *reinterpret_cast<const mx_u4*>(pc[i] + (s + 1) * 64);
+                    if (((s + 1) & 3) == 0) sn[i] = *reinterpret_cast<const unsigned int*>(ps[i] + ((s + 1) >> 2) * 16);
+                }
+            }
+#pragma unroll
+            for (int jj = 0; jj < JS; ++jj) {
+                mx_bf8 a[RT];
+#pragma unroll
+                for (int i = 0; i < RT; ++i) a[i] = mx_unpack8(q[i][h * JS + jj], sc[i]);
+#pragma unroll
+                for (int u = 0; u < TERMS; ++u)
+#pragma unroll
+                    for (int c = 0; c < CT; ++c) {
+                        const mx_bf8 f = *reinterpret_cast<const mx_bf8*>(&lds[b][((jj * TERMS + u) * CT + c) * 512 + lane * 8]);
+#pragma unroll
+                        for (int i = 0; i < RT; ++i) acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], f, acc[i][c], 0, 0, 0);
+                    }
+            }
+            __syncthreads();
+            b ^= 1;
+        }
+#pragma unroll
+        for (int i = 0; i < RT; ++i) { q[i] = qn[i]; sd[i] = sn[i]; }
+    }
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            float o[4] = {acc[i][c][0], acc[i][c][1], acc[i][c][2], acc[i][c][3]};
+            mx_store<T, 4>(w, tile.z, (tile.a * CT + c) * 16 + l, n0 + 16 * i + 4 * g, o);
+        }
+}
+
+// dx[t][k] = sum_n dy[t][n] W[n][k] for tiles of 16 CT rows of dy and 512 columns of W: as mx_grad_row_kernel, 128 columns a wave (a dword of 8
+// columns from 8 rows, 8 tiles), the fragments of dy shared through LDS.
+template <typename T, int CT, int JS>
+__global__ __launch_bounds__(256) void mx_grad_tile_kernel(const unsigned short* __restrict__ frag, int64_t tiles, const unsigned char* __restrict__ wc,
+                                                           const unsigned char* __restrict__ ws, int64_t N, int64_t K, MxOut<T> w, int64_t mt, int64_t nt,
+                                                           int split) {
+    constexpr int TERMS = MxTerms<T>::v, CH = JS * TERMS * CT;
+    const int64_t crow = mx_code_row(K), srow = mx_scale_row(K);
+    const MxTile tile = mx_tile(blockIdx.x, mt, nt, split);
+    if (tile.a < 0) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
+    const int64_t k0 = tile.b * 512 + wave * 128;
+    const int64_t steps = (N + 31) / 32, per = ((steps + split - 1) / split + JS - 1) / JS * JS;
+    const int64_t s0 = per * tile.z, s1 = s0 + per < steps ? s0 + per : steps;
+    __shared__ __attribute__((aligned(16))) unsigned short lds[2][CH * 512];
+    const int64_t kb = k0 / 2 + l * 4 < crow ? k0 / 2 + l * 4 : crow - 4;  // (columns behind the row are not stored)
+    const unsigned char* pc = wc + kb;
+    const unsigned char* ps = ws + mx_scale_at(kb >> 4);
+    auto stage = [&](int64_t f, int b) {
+#pragma unroll
+        for (int c = 0; c < (CH + 3) / 4; ++c) {
+            const int i = c * 4 + wave;
+            if (CH % 4 == 0 || i < CH) {
+                const int64_t at = ((f * TERMS + i / CT) * tiles + tile.a * CT + i % CT) * 512;
+                __builtin_amdgcn_global_load_lds((mx_gptr)(frag + at + lane * 8), (mx_lptr)(&lds[b][i * 512]), 16, 0, 0);
+            }
+        }
+    };
+    auto load = [&](int64_t s, unsigned int* q, unsigned int* sc) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int64_t n = s * 32 + g * 8 + j;
+            q[j] = n < N ? *reinterpret_cast<const unsigned int*>(pc + n * crow) : 0u;
+            sc[j] = n < N ? ps[n * srow] : 127u;
+        }
+    };
+    mx_f4 acc[8][CT] = {};
+    unsigned int q[8], sc[8];
+    if (s0 < s1) {
+        stage(s0, 0);
+        load(s0, q, sc);
+    }
+    __syncthreads();
+    int b = 0;
+    for (int64_t s = s0; s < s1; s += JS) {
+        if (s + JS < s1) stage(s + JS, b ^ 1);
+#pragma unroll
+        for (int jj = 0; jj < JS; ++jj) {
+            mx_bf8 a[8];
+            mx_unpack_across(q, sc, a);
+            if (s + jj + 1 < s1) load(s + jj + 1, q, sc);
+            if (s + jj < s1) {
+#pragma unroll
+                for (int u = 0; u < TERMS; ++u)
+#pragma unroll
+                    for (int c = 0; c < CT; ++c) {
+                        const mx_bf8 f = *reinterpret_cast<const mx_bf8*>(&lds[b][((jj * TERMS + u) * CT + c) * 512 + lane * 8]);
+#pragma unroll
+                        for (int m = 0; m < 8; ++m) acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[m], f, acc[m][c], 0, 0, 0);
+                    }
+            }
+        }
+        __syncthreads();
+        b ^= 1;
+    }
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int64_t k = k0 + 8 * (4 * g + e) + m, t = t0 + l;
-            if (k < K && t < M) out[t * rs + k * cs] = mx_from_f32<T>(acc[m][e]);
+            float o[8];
+#pragma unroll
+            for (int m = 0; m < 8; ++m) o[m] = acc[m][c][e];
+            mx_store<T, 8>(w, tile.z, (tile.a * CT + c) * 16 + l, k0 + 8 * (4 * g + e), o);
         }
 }
 

@@ -69,19 +69,6 @@ static int mx_grid(int64_t mtiles, int64_t ntiles, unsigned* g) {
     return LCX_OK;
 }
 
-template <typename T>
-static int mx4_matmul(const void* ac, const void* as, int64_t M, const void* bc, const void* bs, int64_t N, int64_t K, void* out, int64_t rs, int64_t cs,
-                      hipStream_t st) {
-    if (K == 0) return mx4_zero<T>(out, M, N, rs, cs, st);
-    const int64_t mt = cdiv(M, 32);
-    unsigned g;
-    LCXCHECK(mx_grid(mt, cdiv(N, 32), &g));
-    hipLaunchKernelGGL((mx_matmul_kernel<T>), dim3(g), dim3(64), 0, st, (const unsigned char*)ac, (const unsigned char*)as, M, (const unsigned char*)bc,
-                       (const unsigned char*)bs, N, K, (T*)out, rs, cs, mt);
-    KCHECK();
-    return LCX_OK;
-}
-
 // ---- products of x with a 4-bit matrix -------------------------------------------------------------------------------------------------
 // What one call does: sizes of its tiles, its splits of the contraction and its work space [fragments of x | partial sums].
 struct MxPlan {
@@ -130,8 +117,10 @@ template <typename T> static MxPlan mx_plan(bool along, int64_t M, int64_t C, in
 }
 static int64_t mx_plan_bytes(const MxPlan& p) { return round_up(p.frag_bytes, 256) + p.part_bytes; }
 
+static int64_t mx_matmul_bytes(int64_t M, int64_t N, int64_t K);
 template <typename T> static int64_t mx_workspace(int op, int64_t M, int64_t N, int64_t K) {
-    if (M == 0 || N == 0 || K == 0 || op == 0) return 0;
+    if (M == 0 || N == 0 || K == 0) return 0;
+    if (op == 0) return mx_matmul_bytes(M, N, K);
     return op == 1 ? mx_plan_bytes(mx_plan<T>(true, M, K, N)) : mx_plan_bytes(mx_plan<T>(false, M, N, K));
 }
 
@@ -154,10 +143,10 @@ static int mx_fragments(const T* x, int64_t M, int64_t rs, int64_t cs, int64_t C
     return LCX_OK;
 }
 
-template <typename T> static int mx_join(const MxPlan& p, const MxOut<T>& w, hipStream_t st) {
-    if (p.split == 1) return LCX_OK;
+template <typename T> static int mx_join(int split, const MxOut<T>& w, hipStream_t st) {
+    if (split == 1) return LCX_OK;
     const int64_t b = cdiv(w.M * w.O, 256);
-    hipLaunchKernelGGL((mx_join_kernel<T>), dim3((unsigned)(b < 8192 ? b : 8192)), dim3(256), 0, st, w.part, p.split, w.M, w.O, w.out, w.rs, w.cs);
+    hipLaunchKernelGGL((mx_join_kernel<T>), dim3((unsigned)(b < 8192 ? b : 8192)), dim3(256), 0, st, w.part, split, w.M, w.O, w.out, w.rs, w.cs);
     KCHECK();
     return LCX_OK;
 }
@@ -217,7 +206,7 @@ static int mx4_linear(const void* xv, int64_t M, int64_t xrs, int64_t xcs, const
     else {
         if constexpr (TERMS == 1) LCXCHECK((mx_linear_tiles<T, 8, 4>(p, frag, wc, ws, N, K, w, st)));
     }
-    return mx_join<T>(p, w, st);
+    return mx_join<T>(p.split, w, st);
 }
 
 template <typename T>
@@ -238,13 +227,76 @@ static int mx4_linear_grad(const void* dyv, int64_t M, int64_t yrs, int64_t ycs,
         else
             hipLaunchKernelGGL((mx_grad_row_kernel<T, 4, false>), g, dim3(256), 0, st, dy, M, yrs, ycs, wc, ws, N, K, w);
         KCHECK();
-        return mx_join<T>(p, w, st);
+        return mx_join<T>(p.split, w, st);
     }
     LCXCHECK((mx_fragments<T, false>(dy, M, yrs, ycs, N, p, frag, st)));
     constexpr int JS = TERMS == 3 ? 2 : 4;
     if (p.ct == 2) LCXCHECK((mx_grad_tiles<T, 2, 4>(p, frag, wc, ws, N, K, w, st)));
     else LCXCHECK((mx_grad_tiles<T, 4, JS>(p, frag, wc, ws, N, K, w, st)));
-    return mx_join<T>(p, w, st);
+    return mx_join<T>(p.split, w, st);
+}
+
+// ---- 4 bits x 4 bits --------------------------------------------------------------------------------------------------------------------
+struct MxMatmulPlan {
+    bool row = false, big = false;
+    int rt = 1, waves = 8, split = 1;
+    int64_t mt = 1, nt = 1, part_bytes = 0;
+};
+static MxMatmulPlan mx_matmul_plan(int64_t M, int64_t N, int64_t K) {
+    MxMatmulPlan p;
+    if (M <= 16) {
+        p.row = true;
+        p.rt = N >= 64 * MX_CUS ? 2 : 1;
+        p.waves = cdiv(N, 16 * p.rt) >= 2 * MX_CUS ? 8 : 16;
+        return p;
+    }
+    // 256 x 256 outputs a block where that fills the chip, else 128 x 128, the contraction split while CUs are left over
+    p.big = cdiv(M, 256) * cdiv(N, 256) >= MX_CUS / 2;
+    p.mt = cdiv(M, p.big ? 256 : 128);
+    p.nt = cdiv(N, p.big ? 256 : 128);
+    p.split = (int)split_for(p.mt * p.nt, cdiv(K, 512), p.big ? MX_CUS : 2 * MX_CUS, 4);
+    if (p.split > 1) p.part_bytes = (int64_t)p.split * M * N * 4;
+    return p;
+}
+
+static int64_t mx_matmul_bytes(int64_t M, int64_t N, int64_t K) { return mx_matmul_plan(M, N, K).part_bytes; }
+
+template <typename T, int WM, int WN, int RM, int RN>
+static int mx_matmul_tiles(const MxMatmulPlan& p, const unsigned char* ac, const unsigned char* as, const unsigned char* bc, const unsigned char* bs, int64_t N,
+                           int64_t K, const MxOut<T>& w, hipStream_t st) {
+    unsigned g;
+    LCXCHECK(mx_grid(8, cdiv(p.mt * p.nt * p.split, 8), &g));
+    constexpr size_t lds = 2 * (WM * 16 * RM + WN * 16 * RN) * 128;
+    LCXCHECK(allow_lds(mx_matmul_tile_kernel<T, WM, WN, RM, RN>, lds));
+    hipLaunchKernelGGL((mx_matmul_tile_kernel<T, WM, WN, RM, RN>), dim3(g), dim3(64 * WM * WN), lds, st, ac, as, bc, bs, N, K, w, p.mt, p.nt, p.split);
+    KCHECK();
+    return LCX_OK;
+}
+
+template <typename T>
+static int mx4_matmul(const void* acv, const void* asv, int64_t M, const void* bcv, const void* bsv, int64_t N, int64_t K, void* out, int64_t rs, int64_t cs,
+                      void* space, int64_t space_bytes, hipStream_t st) {
+    if (K == 0) return mx4_zero<T>(out, M, N, rs, cs, st);
+    const unsigned char *ac = (const unsigned char*)acv, *as = (const unsigned char*)asv, *bc = (const unsigned char*)bcv, *bs = (const unsigned char*)bsv;
+    const MxMatmulPlan p = mx_matmul_plan(M, N, K);
+    if (space_bytes < p.part_bytes || (p.part_bytes && !space)) return fail(LCX_ERR_ARG, "lcx_mx4_matmul: the work space is smaller than lcx_mx4_workspace says");
+    MxOut<T> w{(T*)out, rs, cs, p.split > 1 ? (float*)space : nullptr, M, N};
+    if (p.row) {
+        unsigned g;
+        LCXCHECK(mx_grid(1, cdiv(N, 16 * p.rt), &g));
+#define MX_ROWS(RT, WV) hipLaunchKernelGGL((mx_matmul_row_kernel<T, RT, WV>), dim3(g), dim3(64 * WV), 0, st, ac, as, M, bc, bs, N, K, w)
+        if (p.rt == 2) {
+            if (p.waves == 8) MX_ROWS(2, 8); else MX_ROWS(2, 16);
+        } else {
+            if (p.waves == 8) MX_ROWS(1, 8); else MX_ROWS(1, 16);
+        }
+#undef MX_ROWS
+        KCHECK();
+        return LCX_OK;
+    }
+    if (p.big) LCXCHECK((mx_matmul_tiles<T, 2, 4, 8, 4>(p, ac, as, bc, bs, N, K, w, st)));
+    else LCXCHECK((mx_matmul_tiles<T, 2, 2, 4, 4>(p, ac, as, bc, bs, N, K, w, st)));
+    return mx_join<T>(p.split, w, st);
 }
 
 extern "C" {
@@ -303,8 +355,8 @@ int lcx_mx4_matmul(const void* a_codes, const void* a_scales, int64_t M, const v
         if (!out || (K > 0 && (!a_codes || !a_scales || !b_codes || !b_scales))) return fail(LCX_ERR_ARG, "lcx_mx4_matmul: null pointer");
         if (mx_misaligned(a_codes, a_scales) || mx_misaligned(b_codes, b_scales))
             return fail(LCX_ERR_ARG, "lcx_mx4_matmul: codes must be 16-byte and scales 4-byte aligned");
-        (void)workspace; (void)workspace_bytes;
-        MX_FLOATS(dtype, mx4_matmul, a_codes, a_scales, M, b_codes, b_scales, N, K, out, row_stride, col_stride, (hipStream_t)stream);
+        MX_FLOATS(dtype, mx4_matmul, a_codes, a_scales, M, b_codes, b_scales, N, K, out, row_stride, col_stride, workspace, workspace_bytes,
+                  (hipStream_t)stream);
     })
 }
 

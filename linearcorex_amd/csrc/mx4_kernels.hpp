@@ -138,54 +138,7 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned char*
     }
 }
 
-// ---- products -------------------------------------------------------------------------------------------------------------------
-// 4 bits x 4 bits: out[m][n] = sum_k A[m][k] B[n][k] on v_mfma_scale_f32_16x16x128_f8f6f4: a lane holds one block of 32 of its row (16 bytes)
-// and that block's scale; float32 sums.  Rows behind the last one repeat it and are not stored.
-template <typename TO>
-__global__ __launch_bounds__(64) void mx_matmul_kernel(const unsigned char* __restrict__ ac, const unsigned char* __restrict__ as, int64_t M,
-                                                       const unsigned char* __restrict__ bc, const unsigned char* __restrict__ bs, int64_t N, int64_t K,
-                                                       TO* __restrict__ out, int64_t rs, int64_t cs, int64_t mtiles) {
-    constexpr int RT = 2;                                      // 32 x 32 outputs a wave
-    const int64_t crow = mx_code_row(K), srow = mx_scale_row(K);
-    const int64_t m0 = (int64_t)(blockIdx.x % mtiles) * 16 * RT, n0 = (int64_t)(blockIdx.x / mtiles) * 16 * RT;
-    const int l = threadIdx.x & 15, g = threadIdx.x >> 4;
-    const unsigned char *pa[RT], *pb[RT], *sa[RT], *sb[RT];
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-        const int64_t rm = m0 + 16 * i + l < M ? m0 + 16 * i + l : M - 1, rn = n0 + 16 * i + l < N ? n0 + 16 * i + l : N - 1;
-        pa[i] = ac + rm * crow + g * 16;
-        pb[i] = bc + rn * crow + g * 16;
-        sa[i] = as + rm * srow + g * 4;
-        sb[i] = bs + rn * srow + g * 4;
-    }
-    mx_f4 acc[RT][RT] = {};
-    for (int64_t s = 0; s * 64 < crow; ++s) {                  // 128 columns a step
-        mx_i8 a[RT] = {}, b[RT] = {};
-        int xa[RT], xb[RT];
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-            const mx_u4 ta = *reinterpret_cast<const mx_u4*>(pa[i] + s * 64), tb = *reinterpret_cast<const mx_u4*>(pb[i] + s * 64);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { a[i][j] = (int)ta[j]; b[i][j] = (int)tb[j]; }
-            xa[i] = sa[i][(s >> 2) * 16 + (s & 3)];
-            xb[i] = sb[i][(s >> 2) * 16 + (s & 3)];
-        }
-#pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int j = 0; j < RT; ++j) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[i], b[j], acc[i][j], 4, 4, 0, xa[i], 0, xb[j]);
-    }
-#pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int j = 0; j < RT; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int64_t m = m0 + 16 * i + 4 * g + e, n = n0 + 16 * j + l;
-                if (m < M && n < N) out[m * rs + n * cs] = mx_from_f32<TO>(acc[i][j][e]);
-            }
-}
-
+// ---- products of x (float32, bf16, fp16) with a 4-bit matrix -----------------------------------------------------------------------
 // eight codes of one block -> bf16 (exact: at most 2 significant bits)
 __device__ __forceinline__ mx_bf8 mx_unpack8(unsigned int q, float s) {
     const mx_bf2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, s, 1),
@@ -635,6 +588,161 @@ __global__ __launch_bounds__(256) void mx_grad_tile_kernel(const unsigned short*
 #pragma unroll
             for (int m = 0; m < 8; ++m) o[m] = acc[m][c][e];
             mx_store<T, 8>(w, tile.z, (tile.a * CT + c) * 16 + l, k0 + 8 * (4 * g + e), o);
+        }
+}
+
+// ---- 4 bits x 4 bits -------------------------------------------------------------------------------------------------------------
+// out[m][n] = sum_k A[m][k] B[n][k] on v_mfma_scale_f32_16x16x128_f8f6f4: a lane holds one block of 32 of its row (16 bytes) and that block's
+// scale; the instruction multiplies codes and scales, float32 sums.  Rows behind the last one repeat it and are not stored.
+__device__ __forceinline__ mx_i8 mx_operand(mx_u4 q) { return mx_i8{(int)q[0], (int)q[1], (int)q[2], (int)q[3], 0, 0, 0, 0}; }
+
+// up to 16 rows of A: as mx_linear_row_kernel, bound by reading B
+template <typename T, int RT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void mx_matmul_row_kernel(const unsigned char* __restrict__ ac, const unsigned char* __restrict__ as, int64_t M,
+                                                                   const unsigned char* __restrict__ bc, const unsigned char* __restrict__ bs, int64_t N,
+                                                                   int64_t K, MxOut<T> w) {
+    constexpr int U = 4;
+    const int64_t crow = mx_code_row(K), srow = mx_scale_row(K);
+    const int64_t n0 = (int64_t)blockIdx.x * 16 * RT;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
+    const int64_t t = l < M ? l : M - 1;
+    const unsigned char *pc[RT], *ps[RT], *pa = ac + t * crow + g * 16, *pas = as + t * srow + g * 4;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        const int64_t rn = n0 + 16 * i + l < N ? n0 + 16 * i + l : N - 1;
+        pc[i] = bc + rn * crow + g * 16;
+        ps[i] = bs + rn * srow + g * 4;
+    }
+    mx_f4 acc[RT] = {};
+    const int64_t steps = (K + 127) / 128;
+    for (int64_t s0 = wave; s0 < steps; s0 += U * WAVES) {
+        mx_u4 q[U][RT], qa[U];
+        int sc[U][RT], sa[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t s = s0 + u * WAVES;
+            if (s < steps) {
+                qa[u] = *reinterpret_cast<const mx_u4*>(pa + s * 64);
+                sa[u] = pas[(s >> 2) * 16 + (s & 3)];
+#pragma unroll
+                for (int i = 0; i < RT; ++i) {
+                    q[u][i] = *reinterpret_cast<const mx_u4*>(pc[i] + s * 64);
+                    sc[u][i] = ps[i][(s >> 2) * 16 + (s & 3)];
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (s0 + u * WAVES < steps) {
+#pragma unroll
+                for (int i = 0; i < RT; ++i)
+                    acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(q[u][i]), mx_operand(qa[u]), acc[i], 4, 4, 0, sc[u][i], 0, sa[u]);
+            }
+    }
+    __shared__ mx_f4 red[WAVES][RT][64];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) red[wave][i][lane] = acc[i];
+    __syncthreads();
+    for (int i = wave; i < RT; i += WAVES) {
+        mx_f4 v = red[0][i][lane];
+#pragma unroll
+        for (int k = 1; k < WAVES; ++k) v += red[k][i][lane];
+        float o[4] = {v[0], v[1], v[2], v[3]};
+        mx_store<T, 4>(w, 0, l, n0 + 16 * i + 4 * g, o);
+    }
+}
+
+// Tiles of (WM x 16 RM) rows of A by (WN x 16 RN) rows of B; WM x WN waves of 16 RM x 16 RN outputs.  Bound: the 4-bit matrix pipe (16 cycles an
+// instruction of 64 Kflop).  256 columns a stage: 128 bytes of each row come to LDS without passing registers, double buffered; the
+// 16-byte pieces of a row are stored at piece ^ (row & 7), which spreads a fragment's sixteen rows over all banks.  Scales go from
+// memory to registers, a dword for four steps.
+template <typename T, int WM, int WN, int RM, int RN>
+__global__ __launch_bounds__(64 * WM * WN) void mx_matmul_tile_kernel(const unsigned char* __restrict__ ac, const unsigned char* __restrict__ as,
+                                                                     const unsigned char* __restrict__ bc, const unsigned char* __restrict__ bs, int64_t N,
+                                                                     int64_t K, MxOut<T> w, int64_t mt, int64_t nt, int split) {
+    constexpr int BM = WM * 16 * RM, BN = WN * 16 * RN, NW = WM * WN, CH = (BM + BN) / 8;      // 1 KB pieces (8 rows x 128 bytes) a stage
+    static_assert(CH % NW == 0, "");
+    const int64_t crow = mx_code_row(K), srow = mx_scale_row(K), M = w.M;
+    const MxTile tile = mx_tile(blockIdx.x, mt, nt, split);
+    if (tile.a < 0) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
+    const int64_t m0 = tile.a * BM, n0 = tile.b * BN;
+    const int wm = (wave % WM) * 16 * RM, wn = (wave / WM) * 16 * RN;
+    const int64_t steps = (K + 255) / 256, per = ((steps + split - 1) / split + 1) / 2 * 2;
+    const int64_t s0 = per * tile.z, s1 = s0 + per < steps ? s0 + per : steps;
+    extern __shared__ __attribute__((aligned(16))) unsigned char mlds[];   // [2][BM + BN][128]
+    const unsigned char* src[CH / NW];
+#pragma unroll
+    for (int c = 0; c < CH / NW; ++c) {
+        const int r = (c * NW + wave) * 8 + lane / 8, piece = (lane & 7) ^ (r & 7);
+        if (r < BM) src[c] = ac + (m0 + r < M ? m0 + r : M - 1) * crow + piece * 16;
+        else src[c] = bc + (n0 + r - BM < N ? n0 + r - BM : N - 1) * crow + piece * 16;
+    }
+    const unsigned char *psa[RM], *psb[RN];
+#pragma unroll
+    for (int i = 0; i < RM; ++i) psa[i] = as + (m0 + wm + 16 * i + l < M ? m0 + wm + 16 * i + l : M - 1) * srow + g * 4;
+#pragma unroll
+    for (int i = 0; i < RN; ++i) psb[i] = bs + (n0 + wn + 16 * i + l < N ? n0 + wn + 16 * i + l : N - 1) * srow + g * 4;
+    auto stage = [&](int64_t s, int b) {
+#pragma unroll
+        for (int c = 0; c < CH / NW; ++c)
+            __builtin_amdgcn_global_load_lds((mx_gptr)(src[c] + s * 128), (mx_lptr)(mlds + b * (BM + BN) * 128 + (c * NW + wave) * 1024), 16, 0, 0);
+    };
+    mx_f4 acc[RM][RN] = {};
+    int sa[RM], sb[RN], san[RM], sbn[RN];
+    if (s0 < s1) {
+        stage(s0, 0);
+#pragma unroll
+        for (int i = 0; i < RM; ++i) sa[i] = *reinterpret_cast<const int*>(psa[i] + (s0 >> 1) * 16);
+#pragma unroll
+        for (int i = 0; i < RN; ++i) sb[i] = *reinterpret_cast<const int*>(psb[i] + (s0 >> 1) * 16);
+    }
+    __syncthreads();
+    int b = 0;
+    // two stages (512 columns: one dword of scales) a turn
+    for (int64_t s = s0; s < s1; s += 2) {
+        const int64_t sn = s + 2 < s1 ? s + 2 : s;
+#pragma unroll
+        for (int i = 0; i < RM; ++i) san[i] = *reinterpret_cast<const int*>(psa[i] + (sn >> 1) * 16);
+#pragma unroll
+        for (int i = 0; i < RN; ++i) sbn[i] = *reinterpret_cast<const int*>(psb[i] + (sn >> 1) * 16);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (s + h >= s1) break;
+            if (s + h + 1 < s1) stage(s + h + 1, b ^ 1);
+            const unsigned char* base = mlds + b * (BM + BN) * 128;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                mx_u4 fa[RM], fb[RN];
+#pragma unroll
+                for (int i = 0; i < RM; ++i) fa[i] = *reinterpret_cast<const mx_u4*>(base + (wm + 16 * i + l) * 128 + (((j * 4 + g) ^ (l & 7)) * 16));
+#pragma unroll
+                for (int i = 0; i < RN; ++i) fb[i] = *reinterpret_cast<const mx_u4*>(base + (BM + wn + 16 * i + l) * 128 + (((j * 4 + g) ^ (l & 7)) * 16));
+#pragma unroll
+                for (int i = 0; i < RM; ++i)
+#pragma unroll
+                    for (int k = 0; k < RN; ++k) {
+                        // outputs transposed (B's rows along the instruction's rows): a lane ends up with four neighbours of one output row
+                        if (h == 0 && j == 0) acc[i][k] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(fb[k]), mx_operand(fa[i]), acc[i][k], 4, 4, 0, sb[k], 0, sa[i]);
+                        else if (h == 0) acc[i][k] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(fb[k]), mx_operand(fa[i]), acc[i][k], 4, 4, 1, sb[k], 1, sa[i]);
+                        else if (j == 0) acc[i][k] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(fb[k]), mx_operand(fa[i]), acc[i][k], 4, 4, 2, sb[k], 2, sa[i]);
+                        else acc[i][k] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(fb[k]), mx_operand(fa[i]), acc[i][k], 4, 4, 3, sb[k], 3, sa[i]);
+                    }
+            }
+            __syncthreads();
+            b ^= 1;
+        }
+#pragma unroll
+        for (int i = 0; i < RM; ++i) sa[i] = san[i];
+#pragma unroll
+        for (int i = 0; i < RN; ++i) sb[i] = sbn[i];
+    }
+#pragma unroll
+    for (int i = 0; i < RM; ++i)
+#pragma unroll
+        for (int k = 0; k < RN; ++k) {
+            float o[4] = {acc[i][k][0], acc[i][k][1], acc[i][k][2], acc[i][k][3]};
+            mx_store<T, 4>(w, tile.z, m0 + wm + 16 * i + l, n0 + wn + 16 * k + 4 * g, o);
         }
 }
 

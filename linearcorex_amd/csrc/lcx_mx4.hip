@@ -23,6 +23,8 @@ static constexpr int64_t MX_MAX_DIM = (int64_t)1 << 31;
         default: return fail(LCX_ERR_ARG, std::string(#fn) + ": dtype must be LCX_F32, LCX_BF16 or LCX_F16"); \
     }
 
+constexpr int MX_CUS = 256;            // blocks are sized for a whole MI355X; the choices below only shift speed
+
 static int64_t dim_bad(int64_t a, int64_t b, int64_t c = 0) { return a < 0 || b < 0 || c < 0 || a >= MX_MAX_DIM || b >= MX_MAX_DIM || c >= MX_MAX_DIM; }
 static bool mx_misaligned(const void* codes, const void* scales) { return ((uintptr_t)codes & 15) != 0 || ((uintptr_t)scales & 3) != 0; }
 
@@ -33,25 +35,56 @@ static int mx_tpr_log2(int64_t cols) {
     return lg;
 }
 static dim3 mx_row_grid(int64_t rows, int64_t cols, int lg) {
+    // a thread takes up to four groups of a long row where there are rows enough to fill the chip
     int64_t gy = cdiv(cdiv(cols, 8), (int64_t)1 << lg);
-    if (gy > 64) gy = 64;
+    if (rows * gy > 8 * MX_CUS * (256 >> lg)) gy = cdiv(gy, 4);
+    if (gy > 4096) gy = 4096;
     return dim3((unsigned)cdiv(rows, 256 >> lg), (unsigned)(gy < 1 ? 1 : gy));
+}
+
+static int mx_grid(int64_t mtiles, int64_t ntiles, unsigned* g) {
+    if (mtiles * ntiles > 0x7fffffffll) return fail(LCX_ERR_ARG, "lcx_mx4: the output is too large for one call");
+    *g = (unsigned)(mtiles * ntiles);
+    return LCX_OK;
+}
+
+// rows that can be read or written 16 bytes at a time
+template <typename T> static bool mx_row_vec(const void* x, int64_t rs, int64_t cs) {
+    return cs == 1 && ((uintptr_t)x & 15) == 0 && (rs * (int64_t)sizeof(T)) % 16 == 0;
 }
 
 template <typename T>
 static int mx4_quantize(const void* x, int64_t rows, int64_t cols, int64_t rs, int64_t cs, void* codes, void* scales, hipStream_t st) {
-    const int lg = mx_tpr_log2(cols);
-    hipLaunchKernelGGL((mx_quantize_kernel<T>), mx_row_grid(rows, cols, lg), dim3(256), 0, st, (const T*)x, rows, cols, rs, cs, (unsigned char*)codes,
-                       (unsigned char*)scales, lg);
+    unsigned char *qc = (unsigned char*)codes, *qs = (unsigned char*)scales;
+    if (rs == 1 && cs != 1) {
+        const int64_t rt = cdiv(rows, 64);
+        unsigned g;
+        LCXCHECK(mx_grid(rt, cdiv(cols, 512), &g));
+        hipLaunchKernelGGL((mx_quantize_across_kernel<T>), dim3(g), dim3(512), 0, st, (const T*)x, rows, cols, cs, qc, qs, rt);
+    } else {
+        const int lg = mx_tpr_log2(cols);
+        const dim3 g = mx_row_grid(rows, cols, lg);
+        if (mx_row_vec<T>(x, rs, cs)) hipLaunchKernelGGL((mx_quantize_kernel<T, true>), g, dim3(256), 0, st, (const T*)x, rows, cols, rs, cs, qc, qs, lg);
+        else hipLaunchKernelGGL((mx_quantize_kernel<T, false>), g, dim3(256), 0, st, (const T*)x, rows, cols, rs, cs, qc, qs, lg);
+    }
     KCHECK();
     return LCX_OK;
 }
 
 template <typename T>
 static int mx4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, void* out, int64_t rs, int64_t cs, hipStream_t st) {
-    const int lg = mx_tpr_log2(cols);
-    hipLaunchKernelGGL((mx_dequantize_kernel<T>), mx_row_grid(rows, cols, lg), dim3(256), 0, st, (const unsigned char*)codes, (const unsigned char*)scales,
-                       rows, cols, (T*)out, rs, cs, lg);
+    const unsigned char *qc = (const unsigned char*)codes, *qs = (const unsigned char*)scales;
+    if (rs == 1 && cs != 1) {
+        const int64_t rt = cdiv(rows, 64);
+        unsigned g;
+        LCXCHECK(mx_grid(rt, cdiv(cols, 512), &g));
+        hipLaunchKernelGGL((mx_dequantize_across_kernel<T>), dim3(g), dim3(512), 0, st, qc, qs, rows, cols, (T*)out, cs, rt);
+    } else {
+        const int lg = mx_tpr_log2(cols);
+        const dim3 g = mx_row_grid(rows, cols, lg);
+        if (mx_row_vec<T>(out, rs, cs)) hipLaunchKernelGGL((mx_dequantize_kernel<T, true>), g, dim3(256), 0, st, qc, qs, rows, cols, (T*)out, rs, cs, lg);
+        else hipLaunchKernelGGL((mx_dequantize_kernel<T, false>), g, dim3(256), 0, st, qc, qs, rows, cols, (T*)out, rs, cs, lg);
+    }
     KCHECK();
     return LCX_OK;
 }
@@ -63,11 +96,6 @@ template <typename T> static int mx4_zero(void* out, int64_t rows, int64_t cols,
     return LCX_OK;
 }
 
-static int mx_grid(int64_t mtiles, int64_t ntiles, unsigned* g) {
-    if (mtiles * ntiles > 0x7fffffffll) return fail(LCX_ERR_ARG, "lcx_mx4: the output is too large for one call");
-    *g = (unsigned)(mtiles * ntiles);
-    return LCX_OK;
-}
 
 // ---- products of x with a 4-bit matrix -------------------------------------------------------------------------------------------------
 // What one call does: sizes of its tiles, its splits of the contraction and its work space [fragments of x | partial sums].
@@ -79,7 +107,6 @@ struct MxPlan {
     int split = 1;
     int64_t frag_bytes = 0, part_bytes = 0;
 };
-constexpr int MX_CUS = 256;            // blocks are sized for a whole MI355X; the choices below only shift speed
 
 static int64_t split_for(int64_t tiles, int64_t steps, int64_t want_blocks, int64_t min_steps) {
     int64_t s = cdiv(want_blocks, tiles);

@@ -85,38 +85,123 @@ __device__ __forceinline__ unsigned int mx_pack8(const float* v, int sc) {
     return q;
 }
 
-// x[r * rs + c * cs] -> codes, scales.  Four lanes share a block, each takes 8 columns.  grid (row groups, column chunks)
-template <typename T>
+// largest of the four lanes that share a block (quad permutations: no LDS)
+__device__ __forceinline__ unsigned int mx_quad_max(unsigned int v) {
+    unsigned int o = (unsigned int)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true);        // lanes 1 0 3 2
+    v = o > v ? o : v;
+    o = (unsigned int)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true);                     // lanes 2 3 0 1
+    return o > v ? o : v;
+}
+template <typename T> struct MxRaw8 { T v[8]; };
+// eight neighbours of a row; zeros behind the last column
+template <typename T, bool VEC>
+__device__ __forceinline__ MxRaw8<T> mx_load8(const T* __restrict__ x, int64_t c0, int64_t cols, int64_t cs) {
+    MxRaw8<T> r;
+    if (VEC && c0 + 8 <= cols) {
+        const mx_u4* p = reinterpret_cast<const mx_u4*>(x + c0);
+        mx_u4 t[sizeof(T) / 2];
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) t[i] = p[i];
+        __builtin_memcpy(&r, t, sizeof(r));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r.v[j] = c0 + j < cols ? x[(c0 + j) * cs] : (T)0.0f;
+    }
+    return r;
+}
+
+// x[r * rs + c * cs] -> codes, scales.  Bound: reading x.  Four lanes share a block, each takes 8 columns (16 bytes of a 16-bit type: VEC, when
+// rows are contiguous and aligned), a few of them in flight per thread.  grid (row groups, column chunks)
+template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t rs, int64_t cs,
                                                           unsigned char* __restrict__ codes, unsigned char* __restrict__ scales, int tpr_log2) {
+    constexpr int U = sizeof(T) == 8 ? 1 : 2;
     const int64_t crow = mx_code_row(cols), srow = mx_scale_row(cols);
     const int tpr = 1 << tpr_log2;
     const int64_t r = (int64_t)blockIdx.x * (256 >> tpr_log2) + (threadIdx.x >> tpr_log2);
     if (r >= rows) return;                                     // (whole groups of 4 lanes: tpr >= 32)
-    for (int64_t c8 = (int64_t)blockIdx.y * tpr + (threadIdx.x & (tpr - 1)); c8 < srow * 4; c8 += (int64_t)gridDim.y * tpr) {
-        const int64_t c0 = c8 * 8;
-        float v[8];
+    const int64_t stride = (int64_t)gridDim.y * tpr;
+    for (int64_t c8 = (int64_t)blockIdx.y * tpr + (threadIdx.x & (tpr - 1)); c8 < srow * 4; c8 += U * stride) {
+        MxRaw8<T> raw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u] = mx_load8<T, VEC>(x + r * rs, (c8 + u * stride) * 8, cols, cs);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t c = c8 + u * stride;
+            float v[8];
+            unsigned int am = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] = mx_to_f32(raw[u].v[j]);
+                const unsigned int b = __float_as_uint(v[j]) & 0x7fffffffu;
+                am = b > am ? b : am;
+            }
+            const int sc = mx_scale_of(mx_quad_max(am));
+            if (c * 4 < crow) *reinterpret_cast<unsigned int*>(codes + r * crow + c * 4) = mx_pack8(v, sc);
+            if ((threadIdx.x & 3) == 0 && c < srow * 4) scales[r * srow + mx_scale_at(c >> 2)] = (unsigned char)sc;
+        }
+    }
+}
+
+// the same for a matrix whose ROWS are neighbours in memory (rs == 1: a transposed view).  A block of 8 waves takes 64 rows x 512 columns; lane =
+// row, so that every load of a wave is contiguous; a thread holds whole blocks of 32 columns.  Codes cross through LDS (16-byte pieces at piece ^
+// (row & 15): a wave writes one piece of 64 rows, then stores whole rows).
+template <typename T>
+__global__ __launch_bounds__(512) void mx_quantize_across_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t cs,
+                                                                 unsigned char* __restrict__ codes, unsigned char* __restrict__ scales, int64_t rtiles) {
+    const int64_t crow = mx_code_row(cols), srow = mx_scale_row(cols);
+    __shared__ mx_u4 lc[64][16];
+    __shared__ __attribute__((aligned(16))) unsigned char ls[64][16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t r0 = (int64_t)(blockIdx.x % rtiles) * 64, c0 = (int64_t)(blockIdx.x / rtiles) * 512;
+    const T* p = x + (r0 + lane < rows ? r0 + lane : rows - 1);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int b = wave * 2 + h;
+        const int64_t c = c0 + b * 32;
+        T raw[32];
+        if (c + 32 <= cols) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) raw[j] = p[(c + j) * cs];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) raw[j] = c + j < cols ? p[(c + j) * cs] : (T)0.0f;
+        }
+        float v[32];
         unsigned int am = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[j] = c0 + j < cols ? mx_to_f32(x[r * rs + (c0 + j) * cs]) : 0.0f;
+        for (int j = 0; j < 32; ++j) {
+            v[j] = mx_to_f32(raw[j]);
             const unsigned int u = __float_as_uint(v[j]) & 0x7fffffffu;
             am = u > am ? u : am;
         }
-        unsigned int o = (unsigned int)__shfl_xor((int)am, 1);
-        am = o > am ? o : am;
-        o = (unsigned int)__shfl_xor((int)am, 2);
-        am = o > am ? o : am;
         const int sc = mx_scale_of(am);
-        if (c8 * 4 < crow) *reinterpret_cast<unsigned int*>(codes + r * crow + c8 * 4) = mx_pack8(v, sc);
-        if ((threadIdx.x & 3) == 0) scales[r * srow + mx_scale_at(c8 >> 2)] = (unsigned char)sc;
+        lc[lane][b ^ (lane & 15)] = mx_u4{mx_pack8(v, sc), mx_pack8(v + 8, sc), mx_pack8(v + 16, sc), mx_pack8(v + 24, sc)};
+        ls[lane][mx_scale_at(b)] = (unsigned char)sc;
     }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int r = (threadIdx.x >> 4) + h * 32, piece = threadIdx.x & 15;
+        if (r0 + r < rows && c0 / 2 + piece * 16 < crow) *reinterpret_cast<mx_u4*>(codes + (r0 + r) * crow + c0 / 2 + piece * 16) = lc[r][piece ^ (r & 15)];
+    }
+    if (threadIdx.x < 256 && r0 + (threadIdx.x >> 2) < rows)
+        *reinterpret_cast<unsigned int*>(scales + (r0 + (threadIdx.x >> 2)) * srow + c0 / 32 + (threadIdx.x & 3) * 4) =
+            *reinterpret_cast<const unsigned int*>(&ls[threadIdx.x >> 2][(threadIdx.x & 3) * 4]);
 }
 
 template <typename T> __device__ __forceinline__ T mx_from_f32(float v) { return (T)v; }
 
-// codes, scales -> out[r * rs + c * cs]
-template <typename T>
+__device__ __forceinline__ void mx_values8(unsigned int q, float s, float* v) {
+    mx_f2 p;
+    p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, s, 0); v[0] = p[0]; v[1] = p[1];
+    p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, s, 1); v[2] = p[0]; v[3] = p[1];
+    p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, s, 2); v[4] = p[0]; v[5] = p[1];
+    p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, s, 3); v[6] = p[0]; v[7] = p[1];
+}
+
+// codes, scales -> out[r * rs + c * cs].  Bound: writing out.  VEC: rows of out are contiguous and aligned to 16 bytes
+template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
                                                             int64_t rows, int64_t cols, T* __restrict__ out, int64_t rs, int64_t cs, int tpr_log2) {
     const int64_t crow = mx_code_row(cols), srow = mx_scale_row(cols);
@@ -127,14 +212,61 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned char*
         const unsigned int q = *reinterpret_cast<const unsigned int*>(codes + r * crow + c8 * 4);
         const float s = __uint_as_float((unsigned int)scales[r * srow + mx_scale_at(c8 >> 2)] << 23);
         float v[8];
-        mx_f2 p;
-        p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, s, 0); v[0] = p[0]; v[1] = p[1];
-        p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, s, 1); v[2] = p[0]; v[3] = p[1];
-        p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, s, 2); v[4] = p[0]; v[5] = p[1];
-        p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, s, 3); v[6] = p[0]; v[7] = p[1];
+        mx_values8(q, s, v);
+        T* p = out + r * rs + c8 * 8 * cs;
+        if (VEC && c8 * 8 + 8 <= cols) {
+            MxRaw8<T> o;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (c8 * 8 + j < cols) out[r * rs + (c8 * 8 + j) * cs] = mx_from_f32<T>(v[j]);
+            for (int j = 0; j < 8; ++j) o.v[j] = mx_from_f32<T>(v[j]);
+            mx_u4 t[sizeof(T) / 2];
+            __builtin_memcpy(t, &o, sizeof(o));
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<mx_u4*>(p)[i] = t[i];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c8 * 8 + j < cols) p[j * cs] = mx_from_f32<T>(v[j]);
+        }
+    }
+}
+
+// the same into a matrix whose rows are neighbours in memory (rs == 1): the mirror image of mx_quantize_across_kernel
+template <typename T>
+__global__ __launch_bounds__(512) void mx_dequantize_across_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
+                                                                   int64_t rows, int64_t cols, T* __restrict__ out, int64_t cs, int64_t rtiles) {
+    const int64_t crow = mx_code_row(cols), srow = mx_scale_row(cols);
+    __shared__ mx_u4 lc[64][16];
+    __shared__ __attribute__((aligned(16))) unsigned char ls[64][16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t r0 = (int64_t)(blockIdx.x % rtiles) * 64, c0 = (int64_t)(blockIdx.x / rtiles) * 512;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int r = (threadIdx.x >> 4) + h * 32, piece = threadIdx.x & 15;
+        mx_u4 q = {0, 0, 0, 0};
+        if (r0 + r < rows && c0 / 2 + piece * 16 < crow) q = *reinterpret_cast<const mx_u4*>(codes + (r0 + r) * crow + c0 / 2 + piece * 16);
+        lc[r][piece ^ (r & 15)] = q;
+    }
+    if (threadIdx.x < 256 && r0 + (threadIdx.x >> 2) < rows)
+        *reinterpret_cast<unsigned int*>(&ls[threadIdx.x >> 2][(threadIdx.x & 3) * 4]) =
+            *reinterpret_cast<const unsigned int*>(scales + (r0 + (threadIdx.x >> 2)) * srow + c0 / 32 + (threadIdx.x & 3) * 4);
+    __syncthreads();
+    if (r0 + lane >= rows) return;
+    T* p = out + r0 + lane;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int b = wave * 2 + h;
+        const int64_t c = c0 + b * 32;
+        if (c >= cols) break;
+        const mx_u4 q = lc[lane][b ^ (lane & 15)];
+        const float s = __uint_as_float((unsigned int)ls[lane][mx_scale_at(b)] << 23);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            float v[8];
+            mx_values8(q[d], s, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c + 8 * d + j < cols) p[(c + 8 * d + j) * cs] = mx_from_f32<T>(v[j]);
+        }
     }
 }
 

@@ -18,6 +18,7 @@ waiting, on the device of the tensors.  Wrong arguments raise ValueError or Type
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -40,23 +41,52 @@ class Mx4(object):
     shape   (rows, columns) of the matrix
     axis    the axis along which 32 neighbours share a scale: 1 = along a row, 0 = along a column
     codes, scales   its device buffers (uint8): of the matrix itself for axis 1, of its transpose for axis 0
-    `q.t()` is the transposed matrix on the same buffers."""
+    `q.t()` is the transposed matrix on the same buffers.  Like any tensor, a matrix that is used on another stream than the one it was
+    made on must outlive that use."""
 
-    __slots__ = ("shape", "axis", "codes", "scales")
+    __slots__ = ("shape", "axis", "index", "_buf", "_codes", "_scales", "_cp", "_sp")
 
     def __init__(self, shape, axis, codes, scales):
-        self.shape, self.axis, self.codes, self.scales = shape, axis, codes, scales
+        self.shape, self.axis, self._buf, self._codes, self._scales = shape, axis, None, codes, scales
+        self.index, self._cp, self._sp = codes.get_device(), codes.data_ptr(), scales.data_ptr()
+
+    @classmethod
+    def _over(cls, shape, axis, index, buf, cp, sp):
+        """on one buffer that holds the codes and, behind them, the scales"""
+        q = cls.__new__(cls)
+        q.shape, q.axis, q.index, q._buf, q._codes, q._scales, q._cp, q._sp = shape, axis, index, buf, None, None, cp, sp
+        return q
+
+    @property
+    def codes(self):
+        if self._codes is None:
+            rows, cols = self._stored()
+            cb = _rows_bytes(cols)[0]
+            self._codes = self._buf[:rows * cb].view(rows, cb)
+        return self._codes
+
+    @property
+    def scales(self):
+        if self._scales is None:
+            rows, cols = self._stored()
+            cb, sb = _rows_bytes(cols)
+            self._scales = self._buf[rows * cb:].view(rows, sb)
+        return self._scales
 
     @property
     def device(self):
-        return self.codes.device
+        return (self._codes if self._buf is None else self._buf).device
 
     @property
     def nbytes(self):
-        return self.codes.numel() + self.scales.numel()
+        rows, cols = self._stored()
+        return rows * sum(_rows_bytes(cols))
 
     def t(self):
-        return Mx4((self.shape[1], self.shape[0]), 1 - self.axis, self.codes, self.scales)
+        q = Mx4.__new__(Mx4)
+        q.shape, q.axis, q.index = (self.shape[1], self.shape[0]), 1 - self.axis, self.index
+        q._buf, q._codes, q._scales, q._cp, q._sp = self._buf, self._codes, self._scales, self._cp, self._sp
+        return q
 
     def _stored(self):
         """(rows, columns) of the buffers: blocks run along the columns"""
@@ -69,9 +99,9 @@ class Mx4(object):
 def _on_gpu(t, what):
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s must be a torch tensor, not %s" % (what, type(t).__name__))
-    if t.layout != torch.strided:
+    if t.layout is not torch.strided:
         raise TypeError("%s must be a dense tensor" % what)
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError("%s must be on the GPU, it is on %s (there is no CPU fallback)" % (what, t.device))
 
 
@@ -80,26 +110,28 @@ def _is_mx4(q, what):
         raise TypeError("%s must be an Mx4 matrix (mx4.quantize), not %s" % (what, type(q).__name__))
 
 
-def _call(device, name, *args):
-    """one entry point on the device's current stream"""
-    fn = getattr(_abi.load(), name)
-    if torch.cuda.current_device() == device.index:
-        status = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+_entry = {}
+
+
+def _call(index, name, *args):
+    """one entry point on the current stream of device `index`"""
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = getattr(_abi.load(), name)
+    if torch.cuda.current_device() == index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            status = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if status != 0:
         _abi.check(status)
 
 
-def _workspace(device, op, dtype, m, n, k):
-    """(tensor or None, pointer, bytes): allocated per call on the current stream, like the outputs"""
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(op, dtype, m, n, k):
     b = C.c_int64()
     _abi.check(_abi.load().lcx_mx4_workspace(op, dtype, m, n, k, C.byref(b)))
-    if b.value == 0:
-        return None, None, 0
-    w = torch.empty(b.value, dtype=torch.uint8, device=device)
-    return w, w.data_ptr(), b.value
+    return b.value
 
 
 def quantize(x, axis=1):
@@ -116,15 +148,17 @@ def quantize(x, axis=1):
     if isinstance(axis, bool) or axis not in (0, 1, -1, -2):
         raise ValueError("axis must be 0 or 1")
     axis %= 2
-    x = x.detach()
-    v = x if axis == 1 else x.t()
-    rows, cols = v.shape
+    (rows, cols), (rs, cs) = x.shape, x.stride()
+    shape = (rows, cols)
+    if axis == 0:
+        rows, cols, rs, cs = cols, rows, cs, rs
     cb, sb = _rows_bytes(cols)
-    codes = torch.empty((rows, cb), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((rows, sb), dtype=torch.uint8, device=x.device)
+    buf = torch.empty(rows * (cb + sb), dtype=torch.uint8, device=x.device)
+    index, cp = x.get_device(), buf.data_ptr()
+    sp = cp + rows * cb
     if rows and cols:
-        _call(x.device, "lcx_mx4_quantize", v.data_ptr(), _DTYPES[x.dtype], rows, cols, v.stride(0), v.stride(1), codes.data_ptr(), scales.data_ptr())
-    return Mx4(tuple(x.shape), axis, codes, scales)
+        _call(index, "lcx_mx4_quantize", x.data_ptr(), _DTYPES[x.dtype], rows, cols, rs, cs, cp, sp)
+    return Mx4._over(shape, axis, index, buf, cp, sp)
 
 
 def dequantize(q, dtype=torch.float32):
@@ -134,9 +168,9 @@ def dequantize(q, dtype=torch.float32):
         raise TypeError("dtype must be float32, float64, bfloat16 or float16, not %s" % dtype)
     out = torch.empty(q.shape, dtype=dtype, device=q.device)
     if out.numel():
-        rows, cols = q._stored()
-        v = out if q.axis == 1 else out.t()
-        _call(q.device, "lcx_mx4_dequantize", q.codes.data_ptr(), q.scales.data_ptr(), rows, cols, out.data_ptr(), _DTYPES[dtype], v.stride(0), v.stride(1))
+        (rows, cols), ld = q._stored(), q.shape[1]
+        rs, cs = (ld, 1) if q.axis == 1 else (1, ld)
+        _call(q.index, "lcx_mx4_dequantize", q._cp, q._sp, rows, cols, out.data_ptr(), _DTYPES[dtype], rs, cs)
     return out
 
 
@@ -151,15 +185,15 @@ def matmul(a, b, dtype=torch.float32):
         raise ValueError("matmul contracts along the blocks: quantize both operands along their columns (axis 1)")
     if a.shape[1] != b.shape[1]:
         raise ValueError("a has %d columns, b has %d" % (a.shape[1], b.shape[1]))
-    if a.device != b.device:
+    if a.index != b.index:
         raise ValueError("a is on %s, b on %s" % (a.device, b.device))
     (m, k), n = a.shape, b.shape[0]
     out = torch.empty((m, n), dtype=dtype, device=a.device)
-    if out.numel():
+    if m and n:
         dt = _DTYPES[dtype]
-        w, wp, wb = _workspace(a.device, 0, dt, m, n, k)
-        _call(a.device, "lcx_mx4_matmul", a.codes.data_ptr(), a.scales.data_ptr(), m, b.codes.data_ptr(), b.scales.data_ptr(), n, k,
-              out.data_ptr(), dt, n, 1, wp, wb)
+        wb = _workspace_bytes(0, dt, m, n, k)
+        w = torch.empty(wb, dtype=torch.uint8, device=a.device) if wb else None
+        _call(a.index, "lcx_mx4_matmul", a._cp, a._sp, m, b._cp, b._sp, n, k, out.data_ptr(), dt, n, 1, w.data_ptr() if wb else None, wb)
     return out
 
 
@@ -168,16 +202,21 @@ def _product(x, q, along):
     n, k = q._stored()
     c, o = (k, n) if along else (n, k)
     lead = x.shape[:-1]
-    m = 1
-    for d in lead:
-        m *= d
-    x2 = x if x.dim() == 2 else x.reshape(m, c)
+    if x.dim() == 2:
+        m, x2 = lead[0], x
+    else:
+        m = 1
+        for d in lead:
+            m *= d
+        x2 = x.reshape(m, c)
     out = torch.empty((m, o), dtype=x.dtype, device=x.device)
-    if out.numel():
+    if m and o:
         dt = _DTYPES[x.dtype]
-        w, wp, wb = _workspace(x.device, 1 if along else 2, dt, m, n, k)
-        _call(x.device, "lcx_mx4_linear" if along else "lcx_mx4_linear_grad", x2.data_ptr(), dt, m, x2.stride(0), x2.stride(1),
-              q.codes.data_ptr(), q.scales.data_ptr(), n, k, out.data_ptr(), o, 1, wp, wb)
+        wb = _workspace_bytes(1 if along else 2, dt, m, n, k)
+        w = torch.empty(wb, dtype=torch.uint8, device=x.device) if wb else None
+        rs, cs = x2.stride()
+        _call(q.index, "lcx_mx4_linear" if along else "lcx_mx4_linear_grad", x2.data_ptr(), dt, m, rs, cs, q._cp, q._sp, n, k,
+              out.data_ptr(), o, 1, w.data_ptr() if wb else None, wb)
     return out if x.dim() == 2 else out.reshape(lead + (o,))
 
 
@@ -208,7 +247,7 @@ def _checked(x, q, what, contracted):
         raise ValueError("%s must have a dimension to contract" % what)
     if x.shape[-1] != q.shape[contracted]:
         raise ValueError("%s has %d values to contract, q has shape %r" % (what, x.shape[-1], q.shape))
-    if x.device != q.device:
+    if x.get_device() != q.index:
         raise ValueError("%s is on %s, q on %s" % (what, x.device, q.device))
 
 

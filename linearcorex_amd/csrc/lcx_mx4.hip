@@ -192,7 +192,9 @@ static int mx_grad_tiles(const MxPlan& p, const unsigned short* frag, const unsi
                          hipStream_t st) {
     unsigned g;
     LCXCHECK(mx_grid(8, cdiv(p.mt * p.nt * p.split, 8), &g));
-    hipLaunchKernelGGL((mx_grad_tile_kernel<T, CT, JS>), dim3(g), dim3(256), 0, st, frag, p.mt * p.ct, wc, ws, N, K, w, p.mt, p.nt, p.split);
+    constexpr size_t lds = 2 * MxGradLds<CT, JS, MxTerms<T>::v>::stage;
+    LCXCHECK(allow_lds(mx_grad_tile_kernel<T, CT, JS>, lds));
+    hipLaunchKernelGGL((mx_grad_tile_kernel<T, CT, JS>), dim3(g), dim3(256), lds, st, frag, p.mt * p.ct, wc, ws, N, K, w, p.mt, p.nt, p.split);
     KCHECK();
     return LCX_OK;
 }
@@ -257,8 +259,8 @@ static int mx4_linear_grad(const void* dyv, int64_t M, int64_t yrs, int64_t ycs,
         return mx_join<T>(p.split, w, st);
     }
     LCXCHECK((mx_fragments<T, false>(dy, M, yrs, ycs, N, p, frag, st)));
-    constexpr int JS = TERMS == 3 ? 2 : 4;
-    if (p.ct == 2) LCXCHECK((mx_grad_tiles<T, 2, 4>(p, frag, wc, ws, N, K, w, st)));
+    constexpr int JS = TERMS == 3 ? 1 : 2;
+    if (p.ct == 2) LCXCHECK((mx_grad_tiles<T, 2, JS>(p, frag, wc, ws, N, K, w, st)));
     else LCXCHECK((mx_grad_tiles<T, 4, JS>(p, frag, wc, ws, N, K, w, st)));
     return mx_join<T>(p.split, w, st);
 }

@@ -325,9 +325,14 @@ __device__ __forceinline__ void mx_store(const MxOut<T>& w, int64_t z, int64_t t
     if (t >= w.M) return;
     if (w.part) {
         float* p = w.part + (z * w.M + t) * w.O + o;
+        if (o + N <= w.O && ((uintptr_t)p & 15) == 0) {
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (o + j < w.O) p[j] = v[j];
+            for (int j = 0; j < N; j += 4) *reinterpret_cast<mx_f4*>(p + j) = mx_f4{v[j], v[j + 1], v[j + 2], v[j + 3]};
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (o + j < w.O) p[j] = v[j];
+        }
         return;
     }
     T* p = w.out + t * w.rs + o * w.cs;
@@ -557,7 +562,7 @@ __device__ __forceinline__ MxTile mx_tile(int64_t id, int64_t na, int64_t nb, in
 // product).  The four waves own 16 RT rows of W each - codes go from memory to registers and become bf16 there, no LDS - and share the fragments
 // of x through LDS (JS of them a stage, double buffered).
 template <typename T, int CT, int RT, int JS>
-__global__ __launch_bounds__(256) void mx_linear_tile_kernel(const unsigned short* __restrict__ frag, int64_t tiles, const unsigned char* __restrict__ wc,
+__global__ __launch_bounds__(256, 2) void mx_linear_tile_kernel(const unsigned short* __restrict__ frag, int64_t tiles, const unsigned char* __restrict__ wc,
                                                              const unsigned char* __restrict__ ws, int64_t N, int64_t K, MxOut<T> w, int64_t mt,
                                                              int64_t nt, int split) {
     constexpr int TERMS = MxTerms<T>::v, CH = JS * TERMS * CT;             // 1 KB pieces a stage
@@ -648,66 +653,82 @@ __global__ __launch_bounds__(256) void mx_linear_tile_kernel(const unsigned shor
 }
 
 // dx[t][k] = sum_n dy[t][n] W[n][k] for tiles of 16 CT rows of dy and 512 columns of W: as mx_grad_row_kernel, 128 columns a wave (a dword of 8
-// columns from 8 rows, 8 tiles), the fragments of dy shared through LDS.
+// columns from each of 8 rows, 8 tiles).  Bound: the bf16 matrix pipe; unpacking costs a cycle of the vector pipe per value of W and tile of
+// rows, so a tile takes as many rows as the registers hold.  32 JS rows of W (codes, scales) and their fragments of dy a stage, all of them to
+// LDS without passing registers, double buffered: the loads of W are 64-byte pieces whose latency nothing else would hide.  The 16-byte
+// pieces of a row of codes are stored at piece ^ 4 ((row / 8) % 4): the four lane groups read different banks.
+template <int CT, int JS, int TERMS> struct MxGradLds {
+    static constexpr int frag = JS * TERMS * CT * 1024, codes = JS * 32 * 256, scales = JS * 32 * 16, stage = frag + codes + scales;
+};
 template <typename T, int CT, int JS>
-__global__ __launch_bounds__(256) void mx_grad_tile_kernel(const unsigned short* __restrict__ frag, int64_t tiles, const unsigned char* __restrict__ wc,
-                                                           const unsigned char* __restrict__ ws, int64_t N, int64_t K, MxOut<T> w, int64_t mt, int64_t nt,
-                                                           int split) {
+__global__ __launch_bounds__(256, 2) void mx_grad_tile_kernel(const unsigned short* __restrict__ frag, int64_t tiles, const unsigned char* __restrict__ wc,
+                                                                             const unsigned char* __restrict__ ws, int64_t N, int64_t K, MxOut<T> w, int64_t mt,
+                                                                             int64_t nt, int split) {
     constexpr int TERMS = MxTerms<T>::v, CH = JS * TERMS * CT;
+    typedef MxGradLds<CT, JS, TERMS> L;
     const int64_t crow = mx_code_row(K), srow = mx_scale_row(K);
     const MxTile tile = mx_tile(blockIdx.x, mt, nt, split);
     if (tile.a < 0) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
-    const int64_t k0 = tile.b * 512 + wave * 128;
+    const int64_t kblk = tile.b * 512, k0 = kblk + wave * 128;
     const int64_t steps = (N + 31) / 32, per = ((steps + split - 1) / split + JS - 1) / JS * JS;
     const int64_t s0 = per * tile.z, s1 = s0 + per < steps ? s0 + per : steps;
-    __shared__ __attribute__((aligned(16))) unsigned short lds[2][CH * 512];
-    const int64_t kb = k0 / 2 + l * 4 < crow ? k0 / 2 + l * 4 : crow - 4;  // (columns behind the row are not stored)
-    const unsigned char* pc = wc + kb;
-    const unsigned char* ps = ws + mx_scale_at(kb >> 4);
-    auto stage = [&](int64_t f, int b) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char glds[];
+    auto stage = [&](int64_t s, int b) {
+        unsigned char* at = glds + b * L::stage;
 #pragma unroll
         for (int c = 0; c < (CH + 3) / 4; ++c) {
             const int i = c * 4 + wave;
-            if (CH % 4 == 0 || i < CH) {
-                const int64_t at = ((f * TERMS + i / CT) * tiles + tile.a * CT + i % CT) * 512;
-                __builtin_amdgcn_global_load_lds((mx_gptr)(frag + at + lane * 8), (mx_lptr)(&lds[b][i * 512]), 16, 0, 0);
-            }
+            if (CH % 4 == 0 || i < CH)
+                __builtin_amdgcn_global_load_lds((mx_gptr)(frag + ((s * TERMS + i / CT) * tiles + tile.a * CT + i % CT) * 512 + lane * 8),
+                                                 (mx_lptr)(at + i * 1024), 16, 0, 0);
         }
-    };
-    auto load = [&](int64_t s, unsigned int* q, unsigned int* sc) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int64_t n = s * 32 + g * 8 + j;
-            q[j] = n < N ? *reinterpret_cast<const unsigned int*>(pc + n * crow) : 0u;
-            sc[j] = n < N ? ps[n * srow] : 127u;
+        for (int c = 0; c < JS * 2; ++c) {                     // 4 rows of codes a piece
+            const int r = (c * 4 + wave) * 4 + lane / 16, piece = (lane & 15) ^ (((r >> 3) & 3) * 4);
+            const int64_t n = s * 32 + r < N ? s * 32 + r : N - 1, kb = kblk / 2 + piece * 16 < crow ? kblk / 2 + piece * 16 : crow - 16;
+            __builtin_amdgcn_global_load_lds((mx_gptr)(wc + n * crow + kb), (mx_lptr)(at + L::frag + (c * 4 + wave) * 1024), 16, 0, 0);
+        }
+        if (lane < 32 && wave < JS) {                          // 32 rows of scales a piece
+            const int64_t n = s * 32 + wave * 32 + lane < N ? s * 32 + wave * 32 + lane : N - 1;
+            __builtin_amdgcn_global_load_lds((mx_gptr)(ws + n * srow + kblk / 32), (mx_lptr)(at + L::frag + L::codes + wave * 512), 16, 0, 0);
         }
     };
     mx_f4 acc[8][CT] = {};
-    unsigned int q[8], sc[8];
-    if (s0 < s1) {
-        stage(s0, 0);
-        load(s0, q, sc);
-    }
+    if (s0 < s1) stage(s0, 0);
     __syncthreads();
     int b = 0;
+    // a lane's dword of row 8 g + j, and the byte of its block's scale
+    const int qat = L::frag + g * 8 * 256 + (((wave * 4 + (l >> 2)) ^ (g * 4)) * 16) + (l & 3) * 4;
+    const int sat = L::frag + L::codes + g * 8 * 16 + (l >> 2) * 4 + wave;
     for (int64_t s = s0; s < s1; s += JS) {
         if (s + JS < s1) stage(s + JS, b ^ 1);
+        const unsigned char* at = glds + b * L::stage;
 #pragma unroll
         for (int jj = 0; jj < JS; ++jj) {
+            if (JS > 1 && s + jj >= s1) break;
+            unsigned int q[8], sc[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                q[j] = *reinterpret_cast<const unsigned int*>(at + qat + jj * 32 * 256 + j * 256);
+                sc[j] = at[sat + jj * 32 * 16 + j * 16];
+            }
+            if ((s + jj) * 32 + 32 > N) {
+                // rows behind the last one are zeros with a finite scale (their factor in dy is zero too, but must not meet a NaN)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if ((s + jj) * 32 + g * 8 + j >= N) { q[j] = 0; sc[j] = 127; }
+            }
             mx_bf8 a[8];
             mx_unpack_across(q, sc, a);
-            if (s + jj + 1 < s1) load(s + jj + 1, q, sc);
-            if (s + jj < s1) {
 #pragma unroll
-                for (int u = 0; u < TERMS; ++u)
+            for (int u = 0; u < TERMS; ++u)
 #pragma unroll
-                    for (int c = 0; c < CT; ++c) {
-                        const mx_bf8 f = *reinterpret_cast<const mx_bf8*>(&lds[b][((jj * TERMS + u) * CT + c) * 512 + lane * 8]);
+                for (int c = 0; c < CT; ++c) {
+                    const mx_bf8 f = *reinterpret_cast<const mx_bf8*>(at + ((jj * TERMS + u) * CT + c) * 1024 + lane * 16);
 #pragma unroll
-                        for (int m = 0; m < 8; ++m) acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[m], f, acc[m][c], 0, 0, 0);
-                    }
-            }
+                    for (int m = 0; m < 8; ++m) acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[m], f, acc[m][c], 0, 0, 0);
+                }
         }
         __syncthreads();
         b ^= 1;
@@ -789,7 +810,7 @@ __global__ __launch_bounds__(64 * WAVES) void mx_matmul_row_kernel(const unsigne
 // 16-byte pieces of a row are stored at piece ^ (row & 7), which spreads a fragment's sixteen rows over all banks.  Scales go from
 // memory to registers, a dword for four steps.
 template <typename T, int WM, int WN, int RM, int RN>
-__global__ __launch_bounds__(64 * WM * WN) void mx_matmul_tile_kernel(const unsigned char* __restrict__ ac, const unsigned char* __restrict__ as,
+__global__ __launch_bounds__(64 * WM * WN, 2) void mx_matmul_tile_kernel(const unsigned char* __restrict__ ac, const unsigned char* __restrict__ as,
                                                                      const unsigned char* __restrict__ bc, const unsigned char* __restrict__ bs, int64_t N,
                                                                      int64_t K, MxOut<T> w, int64_t mt, int64_t nt, int split) {
     constexpr int BM = WM * 16 * RM, BN = WN * 16 * RN, NW = WM * WN, CH = (BM + BN) / 8;      // 1 KB pieces (8 rows x 128 bytes) a stage

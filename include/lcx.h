@@ -422,18 +422,21 @@ int lcx_kernel_name(lcx_ctx* h, int kind, char* buf, int64_t len);
 
 /* ---- matrices in 4 bits per value ("mx4") --------------------------------------------------------------
  * A value is a 4-bit float (sign, 2 exponent bits, 1 mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6); 32 neighbours along a row share one
- * power-of-two scale (a byte, 2^(byte - 127); 255: the block is NaN).  An R x C matrix is two device buffers of lcx_mx4_layout's sizes:
- *   codes  R rows of code_row bytes: two values a byte, the even column in the low half; zeros behind column C
- *   scales R rows of scale_row bytes: the byte of block 4 s + g of every 16 blocks at place 4 g + s; unused ones 2
+ * power-of-two scale (a byte, 2^(byte - 127); 255: the block is NaN).  An R x C matrix is two device buffers of lcx_mx4_layout's sizes, in
+ * the order in which the matrix instructions take their operands: tiles of 16 rows x 128 columns (a step), 64 lanes each, lane 16 g + l
+ * holds block 4 s + g of row l:
+ *   codes  [row tiles][steps, an even number][64 lanes][16 bytes]: two values a byte, the even column in the low half
+ *   scales [row tiles][steps / 4, rounded up][64 lanes][4 bytes]: the lane's blocks of four steps
+ * Rows and columns behind the matrix are zeros with the scale byte 2.
  * What lcx_mx4_quantize writes is defined to the bit: scale = 2^(floor(log2 max|x|) - 2) of the block, at least 2^-125 (also of a block of
  * zeros); value = x / scale rounded to nearest, ties to the even code, saturating at 6 (largest: 6 * 2^125; float64 beyond float32
  * saturates too); a block that holds an infinity or a NaN is NaN.
  *
  * These entry points have no handle: every pointer is device memory of the current device, the work goes to `stream` (a hipStream_t of
  * that device, NULL = the default stream) and the call returns without waiting; nothing is kept from one call to the next, so calls on
- * different streams may overlap.  Codes must be 16-byte aligned, scales 4-byte aligned.  Strides count elements.  rows, cols, M, N, K
+ * different streams may overlap.  Codes, scales and work space must be 16-byte aligned.  Strides count elements.  rows, cols, M, N, K
  * may be 0: an empty output is left alone, an empty contraction gives zeros.  Outputs must not overlap inputs. */
-int lcx_mx4_layout(int64_t cols, int64_t* code_row, int64_t* scale_row);
+int lcx_mx4_layout(int64_t rows, int64_t cols, int64_t* code_bytes, int64_t* scale_bytes);
 /* x[r * row_stride + c * col_stride] (any lcx_dtype) -> codes, scales; blocks run along c */
 int lcx_mx4_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, int64_t col_stride, void* codes,
                      void* scales, void* stream);

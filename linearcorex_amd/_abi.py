@@ -97,7 +97,7 @@ SIGNATURES = {
     "lcx_timing_reset": [_vp],
     "lcx_geometry": [_vp, C.POINTER(_i64), C.POINTER(_i64), C.POINTER(_i32), C.POINTER(_i64)],
     "lcx_kernel_name": [_vp, _i32, C.c_char_p, _i64],
-    "lcx_mx4_layout": [_i64, C.POINTER(_i64), C.POINTER(_i64)],
+    "lcx_mx4_layout": [_i64, _i64, C.POINTER(_i64), C.POINTER(_i64)],
     "lcx_mx4_quantize": [_vp, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp],
     "lcx_mx4_dequantize": [_vp, _vp, _i64, _i64, _vp, _i32, _i64, _i64, _vp],
     "lcx_mx4_workspace": [_i32, _i32, _i64, _i64, _i64, C.POINTER(_i64)],

@@ -26,21 +26,7 @@ static constexpr int64_t MX_MAX_DIM = (int64_t)1 << 31;
 constexpr int MX_CUS = 256;            // blocks are sized for a whole MI355X; the choices below only shift speed
 
 static int64_t dim_bad(int64_t a, int64_t b, int64_t c = 0) { return a < 0 || b < 0 || c < 0 || a >= MX_MAX_DIM || b >= MX_MAX_DIM || c >= MX_MAX_DIM; }
-static bool mx_misaligned(const void* codes, const void* scales) { return ((uintptr_t)codes & 15) != 0 || ((uintptr_t)scales & 3) != 0; }
-
-// threads per row of the element-wise kernels: a power of two in [32, 256] that covers the row's groups of 8 columns
-static int mx_tpr_log2(int64_t cols) {
-    int lg = 5;
-    while (lg < 8 && ((int64_t)8 << lg) < cols) ++lg;
-    return lg;
-}
-static dim3 mx_row_grid(int64_t rows, int64_t cols, int lg) {
-    // a thread takes up to four groups of a long row where there are rows enough to fill the chip
-    int64_t gy = cdiv(cdiv(cols, 8), (int64_t)1 << lg);
-    if (rows * gy > 8 * MX_CUS * (256 >> lg)) gy = cdiv(gy, 4);
-    if (gy > 4096) gy = 4096;
-    return dim3((unsigned)cdiv(rows, 256 >> lg), (unsigned)(gy < 1 ? 1 : gy));
-}
+static bool mx_misaligned(const void* codes, const void* scales) { return (((uintptr_t)codes | (uintptr_t)scales) & 15) != 0; }
 
 static int mx_grid(int64_t mtiles, int64_t ntiles, unsigned* g) {
     if (mtiles * ntiles > 0x7fffffffll) return fail(LCX_ERR_ARG, "lcx_mx4: the output is too large for one call");
@@ -56,16 +42,14 @@ template <typename T> static bool mx_row_vec(const void* x, int64_t rs, int64_t 
 template <typename T>
 static int mx4_quantize(const void* x, int64_t rows, int64_t cols, int64_t rs, int64_t cs, void* codes, void* scales, hipStream_t st) {
     unsigned char *qc = (unsigned char*)codes, *qs = (unsigned char*)scales;
+    unsigned g;
     if (rs == 1 && cs != 1) {
-        const int64_t rt = cdiv(rows, 64);
-        unsigned g;
-        LCXCHECK(mx_grid(rt, cdiv(cols, 512), &g));
-        hipLaunchKernelGGL((mx_quantize_across_kernel<T>), dim3(g), dim3(512), 0, st, (const T*)x, rows, cols, cs, qc, qs, rt);
+        LCXCHECK(mx_grid(cdiv(rows, 64), mx_quads(cols), &g));
+        hipLaunchKernelGGL((mx_quantize_across_kernel<T>), dim3(g), dim3(512), 0, st, (const T*)x, rows, cols, cs, qc, qs);
     } else {
-        const int lg = mx_tpr_log2(cols);
-        const dim3 g = mx_row_grid(rows, cols, lg);
-        if (mx_row_vec<T>(x, rs, cs)) hipLaunchKernelGGL((mx_quantize_kernel<T, true>), g, dim3(256), 0, st, (const T*)x, rows, cols, rs, cs, qc, qs, lg);
-        else hipLaunchKernelGGL((mx_quantize_kernel<T, false>), g, dim3(256), 0, st, (const T*)x, rows, cols, rs, cs, qc, qs, lg);
+        LCXCHECK(mx_grid(mx_row_tiles(rows), mx_quads(cols), &g));
+        if (mx_row_vec<T>(x, rs, cs)) hipLaunchKernelGGL((mx_quantize_kernel<T, true>), dim3(g), dim3(256), 0, st, (const T*)x, rows, cols, rs, cs, qc, qs);
+        else hipLaunchKernelGGL((mx_quantize_kernel<T, false>), dim3(g), dim3(256), 0, st, (const T*)x, rows, cols, rs, cs, qc, qs);
     }
     KCHECK();
     return LCX_OK;
@@ -74,16 +58,14 @@ static int mx4_quantize(const void* x, int64_t rows, int64_t cols, int64_t rs, i
 template <typename T>
 static int mx4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, void* out, int64_t rs, int64_t cs, hipStream_t st) {
     const unsigned char *qc = (const unsigned char*)codes, *qs = (const unsigned char*)scales;
+    unsigned g;
     if (rs == 1 && cs != 1) {
-        const int64_t rt = cdiv(rows, 64);
-        unsigned g;
-        LCXCHECK(mx_grid(rt, cdiv(cols, 512), &g));
-        hipLaunchKernelGGL((mx_dequantize_across_kernel<T>), dim3(g), dim3(512), 0, st, qc, qs, rows, cols, (T*)out, cs, rt);
+        LCXCHECK(mx_grid(cdiv(rows, 64), mx_quads(cols), &g));
+        hipLaunchKernelGGL((mx_dequantize_across_kernel<T>), dim3(g), dim3(512), 0, st, qc, qs, rows, cols, (T*)out, cs);
     } else {
-        const int lg = mx_tpr_log2(cols);
-        const dim3 g = mx_row_grid(rows, cols, lg);
-        if (mx_row_vec<T>(out, rs, cs)) hipLaunchKernelGGL((mx_dequantize_kernel<T, true>), g, dim3(256), 0, st, qc, qs, rows, cols, (T*)out, rs, cs, lg);
-        else hipLaunchKernelGGL((mx_dequantize_kernel<T, false>), g, dim3(256), 0, st, qc, qs, rows, cols, (T*)out, rs, cs, lg);
+        LCXCHECK(mx_grid(mx_row_tiles(rows), mx_quads(cols), &g));
+        if (mx_row_vec<T>(out, rs, cs)) hipLaunchKernelGGL((mx_dequantize_kernel<T, true>), dim3(g), dim3(256), 0, st, qc, qs, rows, cols, (T*)out, rs, cs);
+        else hipLaunchKernelGGL((mx_dequantize_kernel<T, false>), dim3(g), dim3(256), 0, st, qc, qs, rows, cols, (T*)out, rs, cs);
     }
     KCHECK();
     return LCX_OK;
@@ -118,25 +100,19 @@ static int64_t split_for(int64_t tiles, int64_t steps, int64_t want_blocks, int6
 template <typename T> static MxPlan mx_plan(bool along, int64_t M, int64_t C, int64_t O) {
     constexpr int TERMS = MxTerms<T>::v;
     MxPlan p;
-    if (M <= 16) {
+    if (M <= 16 && along) {
         p.row = true;
-        if (along) {
-            // 2 x 16 rows of W a wave halve the reads of x where there are enough rows to fill the chip; 16 waves split the contraction
-            // where there are few
-            p.rt = M > 4 && O >= 32 * MX_CUS ? 2 : 1;
-            p.waves = cdiv(O, 16 * p.rt) >= 2 * MX_CUS ? 8 : 16;
-        } else {
-            p.waves = 4;
-            p.nt = cdiv(O, 512);
-            p.split = (int)split_for(p.nt, cdiv(C, 32), 2 * MX_CUS, 4);
-        }
+        // 2 x 16 rows of W a wave halve the reads of x where there are enough rows to fill the chip; 16 waves split the contraction
+        // where there are few
+        p.rt = M > 4 && O >= 32 * MX_CUS ? 2 : 1;
+        p.waves = cdiv(O, 16 * p.rt) >= 2 * MX_CUS ? 8 : 16;
     } else {
-        p.ct = M <= 32 ? 2 : M <= 64 || TERMS > 1 || !along ? 4 : 8;
+        p.ct = M <= 16 ? 1 : M <= 32 ? 2 : M <= 64 || TERMS > 1 || !along ? 4 : 8;
         p.rt = 4;
         p.mt = cdiv(M, 16 * p.ct);
         p.nt = along ? cdiv(O, 64 * p.rt) : cdiv(O, 512);
-        p.nfrag = along ? cdiv(C, 128) * 4 : cdiv(C, 128) * 4;
-        p.split = (int)split_for(p.mt * p.nt, cdiv(C, 128), 2 * MX_CUS, 8);
+        p.nfrag = cdiv(C, 128) * 4;
+        p.split = (int)split_for(p.mt * p.nt, cdiv(C, 128), 2 * MX_CUS, p.ct == 1 ? 2 : 8);
         p.frag_bytes = p.nfrag * TERMS * p.mt * p.ct * 1024;
     }
     if (p.split > 1) p.part_bytes = (int64_t)p.split * M * O * 4;
@@ -221,7 +197,7 @@ static int mx4_linear(const void* xv, int64_t M, int64_t xrs, int64_t xcs, const
     constexpr int TERMS = MxTerms<T>::v;
     if (K == 0) return mx4_zero<T>(out, M, N, rs, cs, st);
     const MxPlan p = mx_plan<T>(true, M, K, N);
-    if (space_bytes < mx_plan_bytes(p) || (mx_plan_bytes(p) && !space)) return fail(LCX_ERR_ARG, "lcx_mx4_linear: the work space is smaller than lcx_mx4_workspace says");
+    if (space_bytes < mx_plan_bytes(p) || (mx_plan_bytes(p) && (!space || ((uintptr_t)space & 15)))) return fail(LCX_ERR_ARG, "lcx_mx4_linear: the work space is smaller than lcx_mx4_workspace says or not 16-byte aligned");
     const T* x = (const T*)xv;
     const unsigned char *wc = (const unsigned char*)wcv, *ws = (const unsigned char*)wsv;
     unsigned short* frag = (unsigned short*)space;
@@ -244,31 +220,23 @@ static int mx4_linear_grad(const void* dyv, int64_t M, int64_t yrs, int64_t ycs,
     constexpr int TERMS = MxTerms<T>::v;
     if (N == 0) return mx4_zero<T>(out, M, K, rs, cs, st);
     const MxPlan p = mx_plan<T>(false, M, N, K);
-    if (space_bytes < mx_plan_bytes(p) || (mx_plan_bytes(p) && !space)) return fail(LCX_ERR_ARG, "lcx_mx4_linear_grad: the work space is smaller than lcx_mx4_workspace says");
+    if (space_bytes < mx_plan_bytes(p) || (mx_plan_bytes(p) && (!space || ((uintptr_t)space & 15)))) return fail(LCX_ERR_ARG, "lcx_mx4_linear_grad: the work space is smaller than lcx_mx4_workspace says or not 16-byte aligned");
     const T* dy = (const T*)dyv;
     const unsigned char *wc = (const unsigned char*)wcv, *ws = (const unsigned char*)wsv;
     unsigned short* frag = (unsigned short*)space;
     MxOut<T> w{(T*)out, rs, cs, p.split > 1 ? (float*)((char*)space + round_up(p.frag_bytes, 256)) : nullptr, M, K};
-    if (p.row) {
-        const dim3 g((unsigned)p.nt, (unsigned)p.split);
-        if (mx_vec<T>(dy, yrs, ycs, N))
-            hipLaunchKernelGGL((mx_grad_row_kernel<T, 4, true>), g, dim3(256), 0, st, dy, M, yrs, ycs, wc, ws, N, K, w);
-        else
-            hipLaunchKernelGGL((mx_grad_row_kernel<T, 4, false>), g, dim3(256), 0, st, dy, M, yrs, ycs, wc, ws, N, K, w);
-        KCHECK();
-        return mx_join<T>(p.split, w, st);
-    }
     LCXCHECK((mx_fragments<T, false>(dy, M, yrs, ycs, N, p, frag, st)));
     constexpr int JS = TERMS == 3 ? 1 : 2;
-    if (p.ct == 2) LCXCHECK((mx_grad_tiles<T, 2, JS>(p, frag, wc, ws, N, K, w, st)));
+    if (p.ct == 1) LCXCHECK((mx_grad_tiles<T, 1, JS>(p, frag, wc, ws, N, K, w, st)));
+    else if (p.ct == 2) LCXCHECK((mx_grad_tiles<T, 2, JS>(p, frag, wc, ws, N, K, w, st)));
     else LCXCHECK((mx_grad_tiles<T, 4, JS>(p, frag, wc, ws, N, K, w, st)));
     return mx_join<T>(p.split, w, st);
 }
 
 // ---- 4 bits x 4 bits --------------------------------------------------------------------------------------------------------------------
 struct MxMatmulPlan {
-    bool row = false, big = false;
-    int rt = 1, waves = 8, split = 1;
+    bool row = false;
+    int ct = 1, rt = 1, waves = 8, split = 1;
     int64_t mt = 1, nt = 1, part_bytes = 0;
 };
 static MxMatmulPlan mx_matmul_plan(int64_t M, int64_t N, int64_t K) {
@@ -279,25 +247,23 @@ static MxMatmulPlan mx_matmul_plan(int64_t M, int64_t N, int64_t K) {
         p.waves = cdiv(N, 16 * p.rt) >= 2 * MX_CUS ? 8 : 16;
         return p;
     }
-    // 256 x 256 outputs a block where that fills the chip, else 128 x 128, the contraction split while CUs are left over
-    p.big = cdiv(M, 256) * cdiv(N, 256) >= MX_CUS / 2;
-    p.mt = cdiv(M, p.big ? 256 : 128);
-    p.nt = cdiv(N, p.big ? 256 : 128);
-    p.split = (int)split_for(p.mt * p.nt, cdiv(K, 512), p.big ? MX_CUS : 2 * MX_CUS, 4);
+    // tiles of 128 rows of A where there are so many, the contraction split while CUs are left over
+    p.ct = M <= 32 ? 2 : M <= 64 ? 4 : 8;
+    p.mt = cdiv(M, 16 * p.ct);
+    p.nt = cdiv(N, 256);
+    p.split = (int)split_for(p.mt * p.nt, cdiv(K, 512), 2 * MX_CUS, 2);
     if (p.split > 1) p.part_bytes = (int64_t)p.split * M * N * 4;
     return p;
 }
 
 static int64_t mx_matmul_bytes(int64_t M, int64_t N, int64_t K) { return mx_matmul_plan(M, N, K).part_bytes; }
 
-template <typename T, int WM, int WN, int RM, int RN>
+template <typename T, int CT, int RT>
 static int mx_matmul_tiles(const MxMatmulPlan& p, const unsigned char* ac, const unsigned char* as, const unsigned char* bc, const unsigned char* bs, int64_t N,
                            int64_t K, const MxOut<T>& w, hipStream_t st) {
     unsigned g;
     LCXCHECK(mx_grid(8, cdiv(p.mt * p.nt * p.split, 8), &g));
-    constexpr size_t lds = 2 * (WM * 16 * RM + WN * 16 * RN) * 128;
-    LCXCHECK(allow_lds(mx_matmul_tile_kernel<T, WM, WN, RM, RN>, lds));
-    hipLaunchKernelGGL((mx_matmul_tile_kernel<T, WM, WN, RM, RN>), dim3(g), dim3(64 * WM * WN), lds, st, ac, as, bc, bs, N, K, w, p.mt, p.nt, p.split);
+    hipLaunchKernelGGL((mx_matmul_tile_kernel<T, CT, RT>), dim3(g), dim3(256), 0, st, ac, as, bc, bs, N, K, w, p.mt, p.nt, p.split);
     KCHECK();
     return LCX_OK;
 }
@@ -308,7 +274,7 @@ static int mx4_matmul(const void* acv, const void* asv, int64_t M, const void* b
     if (K == 0) return mx4_zero<T>(out, M, N, rs, cs, st);
     const unsigned char *ac = (const unsigned char*)acv, *as = (const unsigned char*)asv, *bc = (const unsigned char*)bcv, *bs = (const unsigned char*)bsv;
     const MxMatmulPlan p = mx_matmul_plan(M, N, K);
-    if (space_bytes < p.part_bytes || (p.part_bytes && !space)) return fail(LCX_ERR_ARG, "lcx_mx4_matmul: the work space is smaller than lcx_mx4_workspace says");
+    if (space_bytes < p.part_bytes || (p.part_bytes && (!space || ((uintptr_t)space & 15)))) return fail(LCX_ERR_ARG, "lcx_mx4_matmul: the work space is smaller than lcx_mx4_workspace says or not 16-byte aligned");
     MxOut<T> w{(T*)out, rs, cs, p.split > 1 ? (float*)space : nullptr, M, N};
     if (p.row) {
         unsigned g;
@@ -323,18 +289,19 @@ static int mx4_matmul(const void* acv, const void* asv, int64_t M, const void* b
         KCHECK();
         return LCX_OK;
     }
-    if (p.big) LCXCHECK((mx_matmul_tiles<T, 2, 4, 8, 4>(p, ac, as, bc, bs, N, K, w, st)));
-    else LCXCHECK((mx_matmul_tiles<T, 2, 2, 4, 4>(p, ac, as, bc, bs, N, K, w, st)));
+    if (p.ct == 8) LCXCHECK((mx_matmul_tiles<T, 8, 4>(p, ac, as, bc, bs, N, K, w, st)));
+    else if (p.ct == 4) LCXCHECK((mx_matmul_tiles<T, 4, 4>(p, ac, as, bc, bs, N, K, w, st)));
+    else LCXCHECK((mx_matmul_tiles<T, 2, 4>(p, ac, as, bc, bs, N, K, w, st)));
     return mx_join<T>(p.split, w, st);
 }
 
 extern "C" {
 
-int lcx_mx4_layout(int64_t cols, int64_t* code_row, int64_t* scale_row) {
+int lcx_mx4_layout(int64_t rows, int64_t cols, int64_t* code_bytes, int64_t* scale_bytes) {
     MX_ENTRY({
-        if (cols < 0 || cols >= MX_MAX_DIM) return fail(LCX_ERR_ARG, "lcx_mx4_layout: bad size");
-        if (code_row) *code_row = mx_code_row(cols);
-        if (scale_row) *scale_row = mx_scale_row(cols);
+        if (dim_bad(rows, cols)) return fail(LCX_ERR_ARG, "lcx_mx4_layout: bad sizes");
+        if (code_bytes) *code_bytes = mx_row_tiles(rows) * mx_steps(cols) * 1024;
+        if (scale_bytes) *scale_bytes = mx_row_tiles(rows) * mx_quads(cols) * 256;
         return LCX_OK;
     })
 }
@@ -345,7 +312,7 @@ int lcx_mx4_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64
         if (dtype < LCX_F32 || dtype > LCX_F16) return fail(LCX_ERR_ARG, "lcx_mx4_quantize: bad dtype");
         if (rows == 0 || cols == 0) return LCX_OK;
         if (!x || !codes || !scales) return fail(LCX_ERR_ARG, "lcx_mx4_quantize: null pointer");
-        if (mx_misaligned(codes, scales)) return fail(LCX_ERR_ARG, "lcx_mx4_quantize: codes must be 16-byte and scales 4-byte aligned");
+        if (mx_misaligned(codes, scales)) return fail(LCX_ERR_ARG, "lcx_mx4_quantize: codes and scales must be 16-byte aligned");
         hipStream_t st = (hipStream_t)stream;
         if (dtype == LCX_F64) return mx4_quantize<double>(x, rows, cols, row_stride, col_stride, codes, scales, st);
         MX_FLOATS(dtype, mx4_quantize, x, rows, cols, row_stride, col_stride, codes, scales, st);
@@ -359,7 +326,7 @@ int lcx_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int6
         if (dtype < LCX_F32 || dtype > LCX_F16) return fail(LCX_ERR_ARG, "lcx_mx4_dequantize: bad dtype");
         if (rows == 0 || cols == 0) return LCX_OK;
         if (!out || !codes || !scales) return fail(LCX_ERR_ARG, "lcx_mx4_dequantize: null pointer");
-        if (mx_misaligned(codes, scales)) return fail(LCX_ERR_ARG, "lcx_mx4_dequantize: codes must be 16-byte and scales 4-byte aligned");
+        if (mx_misaligned(codes, scales)) return fail(LCX_ERR_ARG, "lcx_mx4_dequantize: codes and scales must be 16-byte aligned");
         hipStream_t st = (hipStream_t)stream;
         if (dtype == LCX_F64) return mx4_dequantize<double>(codes, scales, rows, cols, out, row_stride, col_stride, st);
         MX_FLOATS(dtype, mx4_dequantize, codes, scales, rows, cols, out, row_stride, col_stride, st);
@@ -383,7 +350,7 @@ int lcx_mx4_matmul(const void* a_codes, const void* a_scales, int64_t M, const v
         if (M == 0 || N == 0) return LCX_OK;
         if (!out || (K > 0 && (!a_codes || !a_scales || !b_codes || !b_scales))) return fail(LCX_ERR_ARG, "lcx_mx4_matmul: null pointer");
         if (mx_misaligned(a_codes, a_scales) || mx_misaligned(b_codes, b_scales))
-            return fail(LCX_ERR_ARG, "lcx_mx4_matmul: codes must be 16-byte and scales 4-byte aligned");
+            return fail(LCX_ERR_ARG, "lcx_mx4_matmul: codes and scales must be 16-byte aligned");
         MX_FLOATS(dtype, mx4_matmul, a_codes, a_scales, M, b_codes, b_scales, N, K, out, row_stride, col_stride, workspace, workspace_bytes,
                   (hipStream_t)stream);
     })
@@ -396,7 +363,7 @@ int lcx_mx4_linear(const void* x, int dtype, int64_t M, int64_t x_row, int64_t x
         if (dtype != LCX_F32 && dtype != LCX_BF16 && dtype != LCX_F16) return fail(LCX_ERR_ARG, "lcx_mx4_linear: dtype must be LCX_F32, LCX_BF16 or LCX_F16");
         if (M == 0 || N == 0) return LCX_OK;
         if (!out || (K > 0 && (!x || !codes || !scales))) return fail(LCX_ERR_ARG, "lcx_mx4_linear: null pointer");
-        if (mx_misaligned(codes, scales)) return fail(LCX_ERR_ARG, "lcx_mx4_linear: codes must be 16-byte and scales 4-byte aligned");
+        if (mx_misaligned(codes, scales)) return fail(LCX_ERR_ARG, "lcx_mx4_linear: codes and scales must be 16-byte aligned");
         MX_FLOATS(dtype, mx4_linear, x, M, x_row, x_col, codes, scales, N, K, out, row_stride, col_stride, workspace, workspace_bytes, (hipStream_t)stream);
     })
 }
@@ -409,7 +376,7 @@ int lcx_mx4_linear_grad(const void* dy, int dtype, int64_t M, int64_t dy_row, in
             return fail(LCX_ERR_ARG, "lcx_mx4_linear_grad: dtype must be LCX_F32, LCX_BF16 or LCX_F16");
         if (M == 0 || K == 0) return LCX_OK;
         if (!out || (N > 0 && (!dy || !codes || !scales))) return fail(LCX_ERR_ARG, "lcx_mx4_linear_grad: null pointer");
-        if (mx_misaligned(codes, scales)) return fail(LCX_ERR_ARG, "lcx_mx4_linear_grad: codes must be 16-byte and scales 4-byte aligned");
+        if (mx_misaligned(codes, scales)) return fail(LCX_ERR_ARG, "lcx_mx4_linear_grad: codes and scales must be 16-byte aligned");
         MX_FLOATS(dtype, mx4_linear_grad, dy, M, dy_row, dy_col, codes, scales, N, K, out, row_stride, col_stride, workspace, workspace_bytes, (hipStream_t)stream);
     })
 }

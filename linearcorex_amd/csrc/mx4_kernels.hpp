@@ -3,11 +3,13 @@
 // A value is a 4-bit float (sign, 2 exponent bits, 1 mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6); 32 neighbours along a row share one
 // power-of-two scale, held as its biased exponent (a byte: 2^(byte - 127); 255 = the whole block is NaN).  4.25 bits per value.
 //
-// Layout of an R x C matrix:
-//   codes  [R][code_row_bytes(C)]   two values a byte, the even column in the low half; rows padded with zeros to 256 columns (128 B)
-//   scales [R][scale_row_bytes(C)]  one byte per 32 columns, rows padded to 512 columns (16 B); inside every 16 blocks the byte of
-//                                   block 4 s + g sits at 4 g + s.  A lane of the matrix instructions below owns block g = lane / 16 of
-//                                   each 128-column step s: one dword holds its scales of four steps, and the instruction picks a byte.
+// Layout of an R x C matrix: that of the matrix instructions' operands, so that every kernel reads it in whole lines and a fragment needs no
+// shuffling.  A fragment is 16 rows x 128 columns (a step): lane 16 g + l of a wave holds the 16 bytes of block 4 s + g (32 columns) of row
+// l, two values a byte, the even column in the low half.
+//   codes  [row tiles of 16][steps][64 lanes][16 bytes]          steps = columns / 128, rounded up to an even number
+//   scales [row tiles of 16][steps / 4][64 lanes][4 bytes]       the lane's scales of four steps: one dword, of which the instructions (or a
+//                                                                shift) pick a byte
+// Padding rows and columns are zeros with the scale byte 2.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -15,10 +17,9 @@
 namespace lcx {
 
 constexpr int MX_BLOCK = 32;
-__host__ __device__ inline int64_t mx_code_row(int64_t cols) { return (cols + 255) / 256 * 128; }
-__host__ __device__ inline int64_t mx_scale_row(int64_t cols) { return (cols + 511) / 512 * 16; }
-// place of block b (of 32 columns) in its row of scales
-__host__ __device__ inline int64_t mx_scale_at(int64_t b) { return (b & ~(int64_t)15) + (b & 3) * 4 + ((b >> 2) & 3); }
+__host__ __device__ inline int64_t mx_steps(int64_t cols) { return (cols + 255) / 256 * 2; }           // 128 columns each
+__host__ __device__ inline int64_t mx_quads(int64_t cols) { return (cols + 511) / 512; }               // groups of four steps
+__host__ __device__ inline int64_t mx_row_tiles(int64_t rows) { return (rows + 15) / 16; }
 
 typedef __attribute__((ext_vector_type(2))) __bf16 mx_bf2;
 typedef __attribute__((ext_vector_type(8))) __bf16 mx_bf8;
@@ -110,55 +111,57 @@ __device__ __forceinline__ MxRaw8<T> mx_load8(const T* __restrict__ x, int64_t c
     return r;
 }
 
-// x[r * rs + c * cs] -> codes, scales.  Bound: reading x.  Four lanes share a block, each takes 8 columns (16 bytes of a 16-bit type: VEC, when
-// rows are contiguous and aligned), a few of them in flight per thread.  grid (row groups, column chunks)
+// x[r * rs + c * cs] -> codes, scales.  Bound: reading x.  A block takes 16 rows x 512 columns: a thread 8 columns of each of four steps (16 bytes
+// of a 16-bit type each: VEC, where rows are contiguous and aligned), so that it ends up with a whole dword of scales; four lanes share a
+// block of 32.  grid (row tile, quad of steps)
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t rs, int64_t cs,
-                                                          unsigned char* __restrict__ codes, unsigned char* __restrict__ scales, int tpr_log2) {
-    constexpr int U = sizeof(T) == 8 ? 1 : 2;
-    const int64_t crow = mx_code_row(cols), srow = mx_scale_row(cols);
-    const int tpr = 1 << tpr_log2;
-    const int64_t r = (int64_t)blockIdx.x * (256 >> tpr_log2) + (threadIdx.x >> tpr_log2);
-    if (r >= rows) return;                                     // (whole groups of 4 lanes: tpr >= 32)
-    const int64_t stride = (int64_t)gridDim.y * tpr;
-    for (int64_t c8 = (int64_t)blockIdx.y * tpr + (threadIdx.x & (tpr - 1)); c8 < srow * 4; c8 += U * stride) {
-        MxRaw8<T> raw[U];
+                                                          unsigned char* __restrict__ codes, unsigned char* __restrict__ scales) {
+    const int64_t steps = mx_steps(cols), quads = mx_quads(cols);
+    const int64_t rt = blockIdx.x / quads, quad = blockIdx.x % quads;
+    const int l = threadIdx.x >> 4, c = threadIdx.x & 15;                  // row of the tile, 8 columns of the step
+    const int64_t r = rt * 16 + l;
+    MxRaw8<T> raw[4];
 #pragma unroll
-        for (int u = 0; u < U; ++u) raw[u] = mx_load8<T, VEC>(x + r * rs, (c8 + u * stride) * 8, cols, cs);
+    for (int u = 0; u < 4; ++u) {
+        if (r < rows) raw[u] = mx_load8<T, VEC>(x + r * rs, quad * 512 + u * 128 + c * 8, cols, cs);
+        else
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t c = c8 + u * stride;
-            float v[8];
-            unsigned int am = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[j] = mx_to_f32(raw[u].v[j]);
-                const unsigned int b = __float_as_uint(v[j]) & 0x7fffffffu;
-                am = b > am ? b : am;
-            }
-            const int sc = mx_scale_of(mx_quad_max(am));
-            if (c * 4 < crow) *reinterpret_cast<unsigned int*>(codes + r * crow + c * 4) = mx_pack8(v, sc);
-            if ((threadIdx.x & 3) == 0 && c < srow * 4) scales[r * srow + mx_scale_at(c >> 2)] = (unsigned char)sc;
-        }
+            for (int j = 0; j < 8; ++j) raw[u].v[j] = (T)0.0f;
     }
+    unsigned int sd = 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        float v[8];
+        unsigned int am = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[j] = mx_to_f32(raw[u].v[j]);
+            const unsigned int b = __float_as_uint(v[j]) & 0x7fffffffu;
+            am = b > am ? b : am;
+        }
+        const int sc = mx_scale_of(mx_quad_max(am));
+        sd |= (unsigned int)sc << (8 * u);
+        const int64_t s = quad * 4 + u;
+        if (s < steps) *reinterpret_cast<unsigned int*>(codes + (rt * steps + s) * 1024 + (c >> 2) * 256 + l * 16 + (c & 3) * 4) = mx_pack8(v, sc);
+    }
+    if ((c & 3) == 0) *reinterpret_cast<unsigned int*>(scales + (rt * quads + quad) * 256 + (c >> 2) * 64 + l * 4) = sd;
 }
 
 // the same for a matrix whose ROWS are neighbours in memory (rs == 1: a transposed view).  A block of 8 waves takes 64 rows x 512 columns; lane =
-// row, so that every load of a wave is contiguous; a thread holds whole blocks of 32 columns.  Codes cross through LDS (16-byte pieces at piece ^
-// (row & 15): a wave writes one piece of 64 rows, then stores whole rows).
+// row, so that every load of a wave is contiguous; a thread holds whole blocks of 32 columns and writes its 16 bytes of the fragment.
 template <typename T>
 __global__ __launch_bounds__(512) void mx_quantize_across_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t cs,
-                                                                 unsigned char* __restrict__ codes, unsigned char* __restrict__ scales, int64_t rtiles) {
-    const int64_t crow = mx_code_row(cols), srow = mx_scale_row(cols);
-    __shared__ mx_u4 lc[64][16];
-    __shared__ __attribute__((aligned(16))) unsigned char ls[64][16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t r0 = (int64_t)(blockIdx.x % rtiles) * 64, c0 = (int64_t)(blockIdx.x / rtiles) * 512;
-    const T* p = x + (r0 + lane < rows ? r0 + lane : rows - 1);
+                                                                 unsigned char* __restrict__ codes, unsigned char* __restrict__ scales) {
+    const int64_t steps = mx_steps(cols), quads = mx_quads(cols);
+    __shared__ __attribute__((aligned(16))) unsigned char ls[4][256];      // [row tile][lane][step]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tile = lane >> 4, l = lane & 15;
+    const int64_t quad = blockIdx.x % quads, rt = blockIdx.x / quads * 4 + tile, r = rt * 16 + l, rts = mx_row_tiles(rows);
+    const T* p = x + (r < rows ? r : rows - 1);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const int b = wave * 2 + h;
-        const int64_t c = c0 + b * 32;
+        const int b = wave * 2 + h, s = b >> 2, g = b & 3;
+        const int64_t c = quad * 512 + b * 32;
         T raw[32];
         if (c + 32 <= cols) {
 #pragma unroll
@@ -171,23 +174,20 @@ __global__ __launch_bounds__(512) void mx_quantize_across_kernel(const T* __rest
         unsigned int am = 0;
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
-            v[j] = mx_to_f32(raw[j]);
+            v[j] = r < rows ? mx_to_f32(raw[j]) : 0.0f;
             const unsigned int u = __float_as_uint(v[j]) & 0x7fffffffu;
             am = u > am ? u : am;
         }
         const int sc = mx_scale_of(am);
-        lc[lane][b ^ (lane & 15)] = mx_u4{mx_pack8(v, sc), mx_pack8(v + 8, sc), mx_pack8(v + 16, sc), mx_pack8(v + 24, sc)};
-        ls[lane][mx_scale_at(b)] = (unsigned char)sc;
+        if (rt < rts && quad * 4 + s < steps)
+            *reinterpret_cast<mx_u4*>(codes + (rt * steps + quad * 4 + s) * 1024 + (g * 16 + l) * 16) =
+                mx_u4{mx_pack8(v, sc), mx_pack8(v + 8, sc), mx_pack8(v + 16, sc), mx_pack8(v + 24, sc)};
+        ls[tile][(g * 16 + l) * 4 + s] = (unsigned char)sc;
     }
     __syncthreads();
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int r = (threadIdx.x >> 4) + h * 32, piece = threadIdx.x & 15;
-        if (r0 + r < rows && c0 / 2 + piece * 16 < crow) *reinterpret_cast<mx_u4*>(codes + (r0 + r) * crow + c0 / 2 + piece * 16) = lc[r][piece ^ (r & 15)];
-    }
-    if (threadIdx.x < 256 && r0 + (threadIdx.x >> 2) < rows)
-        *reinterpret_cast<unsigned int*>(scales + (r0 + (threadIdx.x >> 2)) * srow + c0 / 32 + (threadIdx.x & 3) * 4) =
-            *reinterpret_cast<const unsigned int*>(&ls[threadIdx.x >> 2][(threadIdx.x & 3) * 4]);
+    const int64_t wt = blockIdx.x / quads * 4 + (threadIdx.x >> 6);
+    if (threadIdx.x < 256 && wt < rts)
+        *reinterpret_cast<unsigned int*>(scales + (wt * quads + quad) * 256 + lane * 4) = *reinterpret_cast<const unsigned int*>(&ls[threadIdx.x >> 6][lane * 4]);
 }
 
 template <typename T> __device__ __forceinline__ T mx_from_f32(float v) { return (T)v; }
@@ -200,21 +200,27 @@ __device__ __forceinline__ void mx_values8(unsigned int q, float s, float* v) {
     p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, s, 3); v[6] = p[0]; v[7] = p[1];
 }
 
-// codes, scales -> out[r * rs + c * cs].  Bound: writing out.  VEC: rows of out are contiguous and aligned to 16 bytes
+// codes, scales -> out[r * rs + c * cs].  Bound: writing out.  Threads as in mx_quantize_kernel; VEC: rows of out are contiguous and aligned
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
-                                                            int64_t rows, int64_t cols, T* __restrict__ out, int64_t rs, int64_t cs, int tpr_log2) {
-    const int64_t crow = mx_code_row(cols), srow = mx_scale_row(cols);
-    const int tpr = 1 << tpr_log2;
-    const int64_t r = (int64_t)blockIdx.x * (256 >> tpr_log2) + (threadIdx.x >> tpr_log2);
+                                                            int64_t rows, int64_t cols, T* __restrict__ out, int64_t rs, int64_t cs) {
+    const int64_t steps = mx_steps(cols), quads = mx_quads(cols);
+    const int64_t rt = blockIdx.x / quads, quad = blockIdx.x % quads;
+    const int l = threadIdx.x >> 4, c = threadIdx.x & 15;
+    const int64_t r = rt * 16 + l;
     if (r >= rows) return;
-    for (int64_t c8 = (int64_t)blockIdx.y * tpr + (threadIdx.x & (tpr - 1)); c8 * 8 < cols; c8 += (int64_t)gridDim.y * tpr) {
-        const unsigned int q = *reinterpret_cast<const unsigned int*>(codes + r * crow + c8 * 4);
-        const float s = __uint_as_float((unsigned int)scales[r * srow + mx_scale_at(c8 >> 2)] << 23);
+    const unsigned int sd = *reinterpret_cast<const unsigned int*>(scales + (rt * quads + quad) * 256 + (c >> 2) * 64 + l * 4);
+    unsigned int q[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+        q[u] = quad * 4 + u < steps ? *reinterpret_cast<const unsigned int*>(codes + (rt * steps + quad * 4 + u) * 1024 + (c >> 2) * 256 + l * 16 + (c & 3) * 4) : 0u;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int64_t c0 = quad * 512 + u * 128 + c * 8;
         float v[8];
-        mx_values8(q, s, v);
-        T* p = out + r * rs + c8 * 8 * cs;
-        if (VEC && c8 * 8 + 8 <= cols) {
+        mx_values8(q[u], __uint_as_float(((sd >> (8 * u)) & 255u) << 23), v);
+        T* p = out + r * rs + c0 * cs;
+        if (VEC && c0 + 8 <= cols) {
             MxRaw8<T> o;
 #pragma unroll
             for (int j = 0; j < 8; ++j) o.v[j] = mx_from_f32<T>(v[j]);
@@ -225,7 +231,7 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned char*
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (c8 * 8 + j < cols) p[j * cs] = mx_from_f32<T>(v[j]);
+                if (c0 + j < cols) p[j * cs] = mx_from_f32<T>(v[j]);
         }
     }
 }
@@ -233,39 +239,25 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned char*
 // the same into a matrix whose rows are neighbours in memory (rs == 1): the mirror image of mx_quantize_across_kernel
 template <typename T>
 __global__ __launch_bounds__(512) void mx_dequantize_across_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
-                                                                   int64_t rows, int64_t cols, T* __restrict__ out, int64_t cs, int64_t rtiles) {
-    const int64_t crow = mx_code_row(cols), srow = mx_scale_row(cols);
-    __shared__ mx_u4 lc[64][16];
-    __shared__ __attribute__((aligned(16))) unsigned char ls[64][16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t r0 = (int64_t)(blockIdx.x % rtiles) * 64, c0 = (int64_t)(blockIdx.x / rtiles) * 512;
+                                                                   int64_t rows, int64_t cols, T* __restrict__ out, int64_t cs) {
+    const int64_t steps = mx_steps(cols), quads = mx_quads(cols);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15;
+    const int64_t quad = blockIdx.x % quads, rt = blockIdx.x / quads * 4 + (lane >> 4), r = rt * 16 + l;
+    if (r >= rows) return;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const int r = (threadIdx.x >> 4) + h * 32, piece = threadIdx.x & 15;
-        mx_u4 q = {0, 0, 0, 0};
-        if (r0 + r < rows && c0 / 2 + piece * 16 < crow) q = *reinterpret_cast<const mx_u4*>(codes + (r0 + r) * crow + c0 / 2 + piece * 16);
-        lc[r][piece ^ (r & 15)] = q;
-    }
-    if (threadIdx.x < 256 && r0 + (threadIdx.x >> 2) < rows)
-        *reinterpret_cast<unsigned int*>(&ls[threadIdx.x >> 2][(threadIdx.x & 3) * 4]) =
-            *reinterpret_cast<const unsigned int*>(scales + (r0 + (threadIdx.x >> 2)) * srow + c0 / 32 + (threadIdx.x & 3) * 4);
-    __syncthreads();
-    if (r0 + lane >= rows) return;
-    T* p = out + r0 + lane;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int b = wave * 2 + h;
-        const int64_t c = c0 + b * 32;
+        const int b = wave * 2 + h, s = b >> 2, g = b & 3;
+        const int64_t c = quad * 512 + b * 32;
         if (c >= cols) break;
-        const mx_u4 q = lc[lane][b ^ (lane & 15)];
-        const float s = __uint_as_float((unsigned int)ls[lane][mx_scale_at(b)] << 23);
+        const mx_u4 q = *reinterpret_cast<const mx_u4*>(codes + (rt * steps + quad * 4 + s) * 1024 + (g * 16 + l) * 16);
+        const float sc = __uint_as_float((unsigned int)scales[(rt * quads + quad) * 256 + (g * 16 + l) * 4 + s] << 23);
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
             float v[8];
-            mx_values8(q[d], s, v);
+            mx_values8(q[d], sc, v);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (c + 8 * d + j < cols) p[(c + 8 * d + j) * cs] = mx_from_f32<T>(v[j]);
+                if (c + 8 * d + j < cols) out[r + (c + 8 * d + j) * cs] = mx_from_f32<T>(v[j]);
         }
     }
 }
@@ -369,16 +361,16 @@ __global__ __launch_bounds__(64 * WAVES) void mx_linear_row_kernel(const T* __re
                                                                    const unsigned char* __restrict__ wc, const unsigned char* __restrict__ ws, int64_t N,
                                                                    int64_t K, MxOut<T> w) {
     constexpr int TERMS = MxTerms<T>::v, U = 4;
-    const int64_t crow = mx_code_row(K), srow = mx_scale_row(K);
+    const int64_t ksteps = mx_steps(K), quads = mx_quads(K), rts = mx_row_tiles(N);
     const int64_t n0 = (int64_t)blockIdx.x * 16 * RT;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
     const int64_t t = l < M ? l : M - 1;                       // rows behind the last one repeat it and are not stored
     const unsigned char *pc[RT], *ps[RT];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-        const int64_t rn = n0 + 16 * i + l < N ? n0 + 16 * i + l : N - 1;
-        pc[i] = wc + rn * crow + g * 16;
-        ps[i] = ws + rn * srow + g * 4;
+        const int64_t rt = (int64_t)blockIdx.x * RT + i < rts ? (int64_t)blockIdx.x * RT + i : rts - 1;
+        pc[i] = wc + rt * ksteps * 1024 + lane * 16;
+        ps[i] = ws + rt * quads * 256 + lane * 4;
     }
     mx_f4 acc[RT] = {};
     const int64_t steps = (K + 127) / 128;
@@ -391,8 +383,8 @@ __global__ __launch_bounds__(64 * WAVES) void mx_linear_row_kernel(const T* __re
             if (s < steps) {
 #pragma unroll
                 for (int i = 0; i < RT; ++i) {
-                    q[u][i] = *reinterpret_cast<const mx_u4*>(pc[i] + s * 64);
-                    sc[u][i] = ps[i][(s >> 2) * 16 + (s & 3)];
+                    q[u][i] = *reinterpret_cast<const mx_u4*>(pc[i] + s * 1024);
+                    sc[u][i] = ps[i][(s >> 2) * 256 + (s & 3)];
                 }
             }
         }
@@ -443,70 +435,6 @@ __device__ __forceinline__ void mx_unpack_across(const unsigned int* q, const un
         for (int j = 0; j < 4; ++j)
             r[j] = __builtin_amdgcn_perm(u[2 * j + 1][m >> 1], u[2 * j][m >> 1], (m & 1) ? 0x07060302u : 0x05040100u);
         __builtin_memcpy(&w[m], r, 16);
-    }
-}
-
-// dx[t][k] = sum_n dy[t][n] W[n][k], up to 16 rows: the contraction runs ACROSS the blocks.  A lane reads 16 bytes (32 columns: one block, one
-// scale) from each of 8 rows of W; entry m of the eight is what matrix instruction m needs from this lane: column 32 (lane % 16) + m,
-// eight n.  So a wave owns 512 columns as 32 tiles and no value crosses lanes.  The waves of a block split the rows, the blocks along
-// y too (partial sums to memory).
-template <typename T, int WAVES, bool VEC>
-__global__ __launch_bounds__(64 * WAVES) void mx_grad_row_kernel(const T* __restrict__ dy, int64_t M, int64_t yrs, int64_t ycs,
-                                                                 const unsigned char* __restrict__ wc, const unsigned char* __restrict__ ws, int64_t N,
-                                                                 int64_t K, MxOut<T> w) {
-    constexpr int TERMS = MxTerms<T>::v;
-    const int64_t crow = mx_code_row(K), srow = mx_scale_row(K);
-    const int64_t k0 = (int64_t)blockIdx.x * 512;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
-    const int64_t t = l < M ? l : M - 1;
-    // (columns behind the row repeat its last 16 bytes and are not stored)
-    const int64_t kb = k0 / 2 + l * 16 < crow ? k0 / 2 + l * 16 : crow - 16;
-    const int64_t sat = mx_scale_at(kb >> 4);
-    mx_f4 acc[32] = {};
-    const int64_t steps = (N + 31) / 32, stride = (int64_t)WAVES * gridDim.y;
-    for (int64_t s = (int64_t)blockIdx.y * WAVES + wave; s < steps; s += stride) {
-        mx_u4 q[8];
-        unsigned int sc[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int64_t n = s * 32 + g * 8 + j;
-            // rows behind the last one are zeros with a finite scale (their factor in dy is zero too, but must not meet a NaN)
-            q[j] = n < N ? *reinterpret_cast<const mx_u4*>(wc + n * crow + kb) : mx_u4{0, 0, 0, 0};
-            sc[j] = n < N ? ws[n * srow + sat] : 127u;
-        }
-        mx_bf8 f[TERMS];
-        mx_load_terms<T, TERMS, VEC>(dy, t, yrs, s * 32 + g * 8, N, ycs, f);
-#pragma unroll
-        for (int d = 0; d < 4; ++d) {
-            unsigned int qd[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) qd[j] = q[j][d];
-            mx_bf8 a[8];
-            mx_unpack_across(qd, sc, a);
-#pragma unroll
-            for (int m = 0; m < 8; ++m)
-#pragma unroll
-                for (int e = 0; e < TERMS; ++e) acc[d * 8 + m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[m], f[e], acc[d * 8 + m], 0, 0, 0);
-        }
-    }
-    __shared__ mx_f4 red[WAVES][8][64];
-#pragma unroll
-    for (int d = 0; d < 4; ++d) {
-        if (d) __syncthreads();
-#pragma unroll
-        for (int m = 0; m < 8; ++m) red[wave][m][lane] = acc[d * 8 + m];
-        __syncthreads();
-        // lane (l, g) of output row 4 g + e holds columns 32 (4 g + e) + 8 d + m
-        for (int e = wave; e < 4; e += WAVES) {
-            float o[8];
-#pragma unroll
-            for (int m = 0; m < 8; ++m) {
-                o[m] = red[0][m][lane][e];
-#pragma unroll
-                for (int k = 1; k < WAVES; ++k) o[m] += red[k][m][lane][e];
-            }
-            mx_store<T, 8>(w, blockIdx.y, l, k0 + 32 * (4 * g + e) + 8 * d, o);
-        }
     }
 }
 
@@ -566,7 +494,7 @@ __global__ __launch_bounds__(256, 2) void mx_linear_tile_kernel(const unsigned s
                                                              const unsigned char* __restrict__ ws, int64_t N, int64_t K, MxOut<T> w, int64_t mt,
                                                              int64_t nt, int split) {
     constexpr int TERMS = MxTerms<T>::v, CH = JS * TERMS * CT;             // 1 KB pieces a stage
-    const int64_t crow = mx_code_row(K), srow = mx_scale_row(K);
+    const int64_t ksteps = mx_steps(K), quads = mx_quads(K), rts = mx_row_tiles(N);
     const MxTile tile = mx_tile(blockIdx.x, mt, nt, split);
     if (tile.a < 0) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
@@ -577,9 +505,9 @@ __global__ __launch_bounds__(256, 2) void mx_linear_tile_kernel(const unsigned s
     const unsigned char *pc[RT], *ps[RT];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-        const int64_t rn = n0 + 16 * i + l < N ? n0 + 16 * i + l : N - 1;
-        pc[i] = wc + rn * crow + g * 16;
-        ps[i] = ws + rn * srow + g * 4;
+        const int64_t rt = n0 / 16 + i < rts ? n0 / 16 + i : rts - 1;      // (tiles behind the last one repeat it and are not stored)
+        pc[i] = wc + rt * ksteps * 1024;
+        ps[i] = ws + rt * quads * 256;
     }
     auto stage = [&](int64_t f, int b) {                                   // fragments f .. f + JS of the contraction
 #pragma unroll
@@ -598,8 +526,8 @@ __global__ __launch_bounds__(256, 2) void mx_linear_tile_kernel(const unsigned s
         stage(s0 * 4, 0);
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
-            q[i] = *reinterpret_cast<const mx_u4*>(pc[i] + s0 * 64);
-            sd[i] = *reinterpret_cast<const unsigned int*>(ps[i] + (s0 >> 2) * 16);
+            q[i] = *reinterpret_cast<const mx_u4*>(pc[i] + s0 * 1024 + lane * 16);
+            sd[i] = *reinterpret_cast<const unsigned int*>(ps[i] + (s0 >> 2) * 256 + lane * 4);
         }
     }
     __syncthreads();
@@ -619,8 +547,8 @@ __global__ __launch_bounds__(256, 2) void mx_linear_tile_kernel(const unsigned s
             if (h == 0 && s + 1 < s1) {
 #pragma unroll
                 for (int i = 0; i < RT; ++i) {
-                    qn[i] = *reinterpret_cast<const mx_u4*>(pc[i] + (s + 1) * 64);
-                    if (((s + 1) & 3) == 0) sn[i] = *reinterpret_cast<const unsigned int*>(ps[i] + ((s + 1) >> 2) * 16);
+                    qn[i] = *reinterpret_cast<const mx_u4*>(pc[i] + (s + 1) * 1024 + lane * 16);
+                    if (((s + 1) & 3) == 0) sn[i] = *reinterpret_cast<const unsigned int*>(ps[i] + ((s + 1) >> 2) * 256 + lane * 4);
                 }
             }
 #pragma unroll
@@ -652,25 +580,26 @@ __global__ __launch_bounds__(256, 2) void mx_linear_tile_kernel(const unsigned s
         }
 }
 
-// dx[t][k] = sum_n dy[t][n] W[n][k] for tiles of 16 CT rows of dy and 512 columns of W: as mx_grad_row_kernel, 128 columns a wave (a dword of 8
-// columns from each of 8 rows, 8 tiles).  Bound: the bf16 matrix pipe; unpacking costs a cycle of the vector pipe per value of W and tile of
-// rows, so a tile takes as many rows as the registers hold.  32 JS rows of W (codes, scales) and their fragments of dy a stage, all of them to
-// LDS without passing registers, double buffered: the loads of W are 64-byte pieces whose latency nothing else would hide.  The 16-byte
-// pieces of a row of codes are stored at piece ^ 4 ((row / 8) % 4): the four lane groups read different banks.
+// dx[t][k] = sum_n dy[t][n] W[n][k] for tiles of 16 CT rows of dy and 512 columns of W: the contraction runs ACROSS the blocks.  A lane reads the
+// dword of 8 columns from each of 8 rows; unpacked, entry m of the eight dwords is what matrix instruction m needs from this lane: column 8
+// (lane % 16) + m, eight n.  So a wave owns 128 columns as 8 tiles and no value crosses lanes.  Bound: the bf16 matrix pipe; unpacking
+// costs the vector pipe a cycle per value of W and tile of rows.  32 JS rows of W (codes, scales) and their fragments of dy a stage, all of
+// them to LDS without passing registers, double buffered.  Row r of block b in row tile p is stored at row r ^ (b | 4 (p % 2)) of its
+// block: the sixteen (block, lane group) that a wave reads at once lie in different banks.
 template <int CT, int JS, int TERMS> struct MxGradLds {
-    static constexpr int frag = JS * TERMS * CT * 1024, codes = JS * 32 * 256, scales = JS * 32 * 16, stage = frag + codes + scales;
+    static constexpr int frag = JS * TERMS * CT * 1024, codes = JS * 8 * 1024, scales = JS * 2 * 256, stage = frag + codes + scales;
 };
 template <typename T, int CT, int JS>
 __global__ __launch_bounds__(256, 2) void mx_grad_tile_kernel(const unsigned short* __restrict__ frag, int64_t tiles, const unsigned char* __restrict__ wc,
-                                                                             const unsigned char* __restrict__ ws, int64_t N, int64_t K, MxOut<T> w, int64_t mt,
-                                                                             int64_t nt, int split) {
+                                                             const unsigned char* __restrict__ ws, int64_t N, int64_t K, MxOut<T> w, int64_t mt,
+                                                             int64_t nt, int split) {
     constexpr int TERMS = MxTerms<T>::v, CH = JS * TERMS * CT;
     typedef MxGradLds<CT, JS, TERMS> L;
-    const int64_t crow = mx_code_row(K), srow = mx_scale_row(K);
+    const int64_t ksteps = mx_steps(K), quads = mx_quads(K), rts = mx_row_tiles(N);
     const MxTile tile = mx_tile(blockIdx.x, mt, nt, split);
     if (tile.a < 0) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
-    const int64_t kblk = tile.b * 512, k0 = kblk + wave * 128;
+    const int64_t k0 = tile.b * 512 + wave * 128;
     const int64_t steps = (N + 31) / 32, per = ((steps + split - 1) / split + JS - 1) / JS * JS;
     const int64_t s0 = per * tile.z, s1 = s0 + per < steps ? s0 + per : steps;
     extern __shared__ __attribute__((aligned(16))) unsigned char glds[];
@@ -684,23 +613,24 @@ __global__ __launch_bounds__(256, 2) void mx_grad_tile_kernel(const unsigned sho
                                                  (mx_lptr)(at + i * 1024), 16, 0, 0);
         }
 #pragma unroll
-        for (int c = 0; c < JS * 2; ++c) {                     // 4 rows of codes a piece
-            const int r = (c * 4 + wave) * 4 + lane / 16, piece = (lane & 15) ^ (((r >> 3) & 3) * 4);
-            const int64_t n = s * 32 + r < N ? s * 32 + r : N - 1, kb = kblk / 2 + piece * 16 < crow ? kblk / 2 + piece * 16 : crow - 16;
-            __builtin_amdgcn_global_load_lds((mx_gptr)(wc + n * crow + kb), (mx_lptr)(at + L::frag + (c * 4 + wave) * 1024), 16, 0, 0);
+        for (int p = 0; p < JS * 2; ++p) {                     // the wave's step of each row tile (tiles and steps behind the last repeat it)
+            const int64_t rt = s * 2 + p < rts ? s * 2 + p : rts - 1, st = tile.b * 4 + wave < ksteps ? tile.b * 4 + wave : ksteps - 1;
+            __builtin_amdgcn_global_load_lds((mx_gptr)(wc + (rt * ksteps + st) * 1024 + g * 256 + ((l ^ (g | 4 * (p & 1))) * 16)),
+                                             (mx_lptr)(at + L::frag + (p * 4 + wave) * 1024), 16, 0, 0);
         }
-        if (lane < 32 && wave < JS) {                          // 32 rows of scales a piece
-            const int64_t n = s * 32 + wave * 32 + lane < N ? s * 32 + wave * 32 + lane : N - 1;
-            __builtin_amdgcn_global_load_lds((mx_gptr)(ws + n * srow + kblk / 32), (mx_lptr)(at + L::frag + L::codes + wave * 512), 16, 0, 0);
+        if (wave < JS * 2 && lane < 16) {
+            const int64_t rt = s * 2 + wave < rts ? s * 2 + wave : rts - 1;
+            __builtin_amdgcn_global_load_lds((mx_gptr)(ws + (rt * quads + tile.b) * 256 + lane * 16), (mx_lptr)(at + L::frag + L::codes + wave * 256), 16, 0, 0);
         }
     };
     mx_f4 acc[8][CT] = {};
     if (s0 < s1) stage(s0, 0);
     __syncthreads();
     int b = 0;
-    // a lane's dword of row 8 g + j, and the byte of its block's scale
-    const int qat = L::frag + g * 8 * 256 + (((wave * 4 + (l >> 2)) ^ (g * 4)) * 16) + (l & 3) * 4;
-    const int sat = L::frag + L::codes + g * 8 * 16 + (l >> 2) * 4 + wave;
+    // row 8 g + j of a step is row 8 (g % 2) + j of row tile g / 2
+    const int blk = l >> 2, mask = blk | 4 * (g >> 1);
+    const int qat = L::frag + ((g >> 1) * 4 + wave) * 1024 + blk * 256 + (g & 1) * 128 + (l & 3) * 4;
+    const int sat = L::frag + L::codes + (g >> 1) * 256 + blk * 64 + (g & 1) * 32 + wave;
     for (int64_t s = s0; s < s1; s += JS) {
         if (s + JS < s1) stage(s + JS, b ^ 1);
         const unsigned char* at = glds + b * L::stage;
@@ -710,8 +640,8 @@ __global__ __launch_bounds__(256, 2) void mx_grad_tile_kernel(const unsigned sho
             unsigned int q[8], sc[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                q[j] = *reinterpret_cast<const unsigned int*>(at + qat + jj * 32 * 256 + j * 256);
-                sc[j] = at[sat + jj * 32 * 16 + j * 16];
+                q[j] = *reinterpret_cast<const unsigned int*>(at + qat + jj * 8192 + ((j ^ mask) * 16));
+                sc[j] = at[sat + jj * 512 + j * 4];
             }
             if ((s + jj) * 32 + 32 > N) {
                 // rows behind the last one are zeros with a finite scale (their factor in dy is zero too, but must not meet a NaN)
@@ -755,16 +685,15 @@ __global__ __launch_bounds__(64 * WAVES) void mx_matmul_row_kernel(const unsigne
                                                                    const unsigned char* __restrict__ bc, const unsigned char* __restrict__ bs, int64_t N,
                                                                    int64_t K, MxOut<T> w) {
     constexpr int U = 4;
-    const int64_t crow = mx_code_row(K), srow = mx_scale_row(K);
+    const int64_t ksteps = mx_steps(K), quads = mx_quads(K), rts = mx_row_tiles(N);
     const int64_t n0 = (int64_t)blockIdx.x * 16 * RT;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
-    const int64_t t = l < M ? l : M - 1;
-    const unsigned char *pc[RT], *ps[RT], *pa = ac + t * crow + g * 16, *pas = as + t * srow + g * 4;
+    const unsigned char *pc[RT], *ps[RT], *pa = ac + lane * 16, *pas = as + lane * 4;      // (one row tile)
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-        const int64_t rn = n0 + 16 * i + l < N ? n0 + 16 * i + l : N - 1;
-        pc[i] = bc + rn * crow + g * 16;
-        ps[i] = bs + rn * srow + g * 4;
+        const int64_t rt = (int64_t)blockIdx.x * RT + i < rts ? (int64_t)blockIdx.x * RT + i : rts - 1;
+        pc[i] = bc + rt * ksteps * 1024 + lane * 16;
+        ps[i] = bs + rt * quads * 256 + lane * 4;
     }
     mx_f4 acc[RT] = {};
     const int64_t steps = (K + 127) / 128;
@@ -775,12 +704,12 @@ __global__ __launch_bounds__(64 * WAVES) void mx_matmul_row_kernel(const unsigne
         for (int u = 0; u < U; ++u) {
             const int64_t s = s0 + u * WAVES;
             if (s < steps) {
-                qa[u] = *reinterpret_cast<const mx_u4*>(pa + s * 64);
-                sa[u] = pas[(s >> 2) * 16 + (s & 3)];
+                qa[u] = *reinterpret_cast<const mx_u4*>(pa + s * 1024);
+                sa[u] = pas[(s >> 2) * 256 + (s & 3)];
 #pragma unroll
                 for (int i = 0; i < RT; ++i) {
-                    q[u][i] = *reinterpret_cast<const mx_u4*>(pc[i] + s * 64);
-                    sc[u][i] = ps[i][(s >> 2) * 16 + (s & 3)];
+                    q[u][i] = *reinterpret_cast<const mx_u4*>(pc[i] + s * 1024);
+                    sc[u][i] = ps[i][(s >> 2) * 256 + (s & 3)];
                 }
             }
         }
@@ -805,97 +734,109 @@ __global__ __launch_bounds__(64 * WAVES) void mx_matmul_row_kernel(const unsigne
     }
 }
 
-// Tiles of (WM x 16 RM) rows of A by (WN x 16 RN) rows of B; WM x WN waves of 16 RM x 16 RN outputs.  Bound: the 4-bit matrix pipe (16 cycles an
-// instruction of 64 Kflop).  256 columns a stage: 128 bytes of each row come to LDS without passing registers, double buffered; the
-// 16-byte pieces of a row are stored at piece ^ (row & 7), which spreads a fragment's sixteen rows over all banks.  Scales go from
-// memory to registers, a dword for four steps.
-template <typename T, int WM, int WN, int RM, int RN>
-__global__ __launch_bounds__(64 * WM * WN, 2) void mx_matmul_tile_kernel(const unsigned char* __restrict__ ac, const unsigned char* __restrict__ as,
-                                                                     const unsigned char* __restrict__ bc, const unsigned char* __restrict__ bs, int64_t N,
-                                                                     int64_t K, MxOut<T> w, int64_t mt, int64_t nt, int split) {
-    constexpr int BM = WM * 16 * RM, BN = WN * 16 * RN, NW = WM * WN, CH = (BM + BN) / 8;      // 1 KB pieces (8 rows x 128 bytes) a stage
-    static_assert(CH % NW == 0, "");
-    const int64_t crow = mx_code_row(K), srow = mx_scale_row(K), M = w.M;
+// Tiles of 16 CT rows of A by 64 RT rows of B.  Bound: the 4-bit matrix pipe (16 cycles an instruction of 64 Kflop) and what feeds it: as in
+// mx_linear_tile_kernel the four waves own 16 RT rows of B each, whose fragments and scales go from memory to registers (an instruction's
+// operands are 2 KB, and both through LDS would take all of its bandwidth), and share the fragments of A through LDS, two steps a stage,
+// double buffered.  A dword of scales serves four steps.
+template <typename T, int CT, int RT>
+__global__ __launch_bounds__(256, 2) void mx_matmul_tile_kernel(const unsigned char* __restrict__ ac, const unsigned char* __restrict__ as,
+                                                               const unsigned char* __restrict__ bc, const unsigned char* __restrict__ bs, int64_t N,
+                                                               int64_t K, MxOut<T> w, int64_t mt, int64_t nt, int split) {
+    constexpr int CH = CT * 2 / 4;                                         // fragments a wave and stage
+    const int64_t ksteps = mx_steps(K), quads = mx_quads(K), mts = mx_row_tiles(w.M), nts = mx_row_tiles(N);
     const MxTile tile = mx_tile(blockIdx.x, mt, nt, split);
     if (tile.a < 0) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
-    const int64_t m0 = tile.a * BM, n0 = tile.b * BN;
-    const int wm = (wave % WM) * 16 * RM, wn = (wave / WM) * 16 * RN;
-    const int64_t steps = (K + 255) / 256, per = ((steps + split - 1) / split + 1) / 2 * 2;
+    const int64_t steps = ksteps / 2, per = ((steps + split - 1) / split + 1) / 2 * 2;     // stages
     const int64_t s0 = per * tile.z, s1 = s0 + per < steps ? s0 + per : steps;
-    extern __shared__ __attribute__((aligned(16))) unsigned char mlds[];   // [2][BM + BN][128]
-    const unsigned char* src[CH / NW];
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2][CT * 2 * 1024];           // [step][row tile][lane]
+    // (row tiles behind the last one repeat it and are not stored)
+    const unsigned char *xb[CH], *xsb[CT], *qb[RT], *sb[RT];
 #pragma unroll
-    for (int c = 0; c < CH / NW; ++c) {
-        const int r = (c * NW + wave) * 8 + lane / 8, piece = (lane & 7) ^ (r & 7);
-        if (r < BM) src[c] = ac + (m0 + r < M ? m0 + r : M - 1) * crow + piece * 16;
-        else src[c] = bc + (n0 + r - BM < N ? n0 + r - BM : N - 1) * crow + piece * 16;
+    for (int c = 0; c < CH; ++c) {
+        const int i = c * 4 + wave;
+        const int64_t rt = tile.a * CT + i % CT < mts ? tile.a * CT + i % CT : mts - 1;
+        xb[c] = ac + (rt * ksteps + i / CT) * 1024;
     }
-    const unsigned char *psa[RM], *psb[RN];
 #pragma unroll
-    for (int i = 0; i < RM; ++i) psa[i] = as + (m0 + wm + 16 * i + l < M ? m0 + wm + 16 * i + l : M - 1) * srow + g * 4;
+    for (int c = 0; c < CT; ++c) xsb[c] = as + (tile.a * CT + c < mts ? tile.a * CT + c : mts - 1) * quads * 256;
 #pragma unroll
-    for (int i = 0; i < RN; ++i) psb[i] = bs + (n0 + wn + 16 * i + l < N ? n0 + wn + 16 * i + l : N - 1) * srow + g * 4;
+    for (int i = 0; i < RT; ++i) {
+        int64_t rt = (tile.b * 4 + wave) * RT + i;
+        rt = rt < nts ? rt : nts - 1;
+        qb[i] = bc + rt * ksteps * 1024;
+        sb[i] = bs + rt * quads * 256;
+    }
     auto stage = [&](int64_t s, int b) {
 #pragma unroll
-        for (int c = 0; c < CH / NW; ++c)
-            __builtin_amdgcn_global_load_lds((mx_gptr)(src[c] + s * 128), (mx_lptr)(mlds + b * (BM + BN) * 128 + (c * NW + wave) * 1024), 16, 0, 0);
+        for (int c = 0; c < CH; ++c)
+            __builtin_amdgcn_global_load_lds((mx_gptr)(xb[c] + s * 2048 + lane * 16), (mx_lptr)(&lds[b][(c * 4 + wave) * 1024]), 16, 0, 0);
     };
-    mx_f4 acc[RM][RN] = {};
-    int sa[RM], sb[RN], san[RM], sbn[RN];
+    mx_f4 acc[RT][CT] = {};
+    mx_u4 q[RT][2];
+    int sd[RT], sx[CT];
     if (s0 < s1) {
         stage(s0, 0);
 #pragma unroll
-        for (int i = 0; i < RM; ++i) sa[i] = *reinterpret_cast<const int*>(psa[i] + (s0 >> 1) * 16);
+        for (int i = 0; i < RT; ++i) {
+            q[i][0] = *reinterpret_cast<const mx_u4*>(qb[i] + s0 * 2048 + lane * 16);
+            q[i][1] = *reinterpret_cast<const mx_u4*>(qb[i] + s0 * 2048 + 1024 + lane * 16);
+            sd[i] = *reinterpret_cast<const int*>(sb[i] + (s0 >> 1) * 256 + lane * 4);
+        }
 #pragma unroll
-        for (int i = 0; i < RN; ++i) sb[i] = *reinterpret_cast<const int*>(psb[i] + (s0 >> 1) * 16);
+        for (int c = 0; c < CT; ++c) sx[c] = *reinterpret_cast<const int*>(xsb[c] + (s0 >> 1) * 256 + lane * 4);
     }
     __syncthreads();
-    int b = 0;
-    // two stages (512 columns: one dword of scales) a turn
+    // two stages (four steps: one dword of scales) a turn
     for (int64_t s = s0; s < s1; s += 2) {
+        int sdn[RT], sxn[CT];
         const int64_t sn = s + 2 < s1 ? s + 2 : s;
-#pragma unroll
-        for (int i = 0; i < RM; ++i) san[i] = *reinterpret_cast<const int*>(psa[i] + (sn >> 1) * 16);
-#pragma unroll
-        for (int i = 0; i < RN; ++i) sbn[i] = *reinterpret_cast<const int*>(psb[i] + (sn >> 1) * 16);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             if (s + h >= s1) break;
-            if (s + h + 1 < s1) stage(s + h + 1, b ^ 1);
-            const unsigned char* base = mlds + b * (BM + BN) * 128;
+            const int64_t nx = s + h + 1 < s1 ? s + h + 1 : s;             // (the last stage loads something it does not use)
+            mx_u4 qn[RT][2];
+            stage(nx, h ^ 1);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                mx_u4 fa[RM], fb[RN];
-#pragma unroll
-                for (int i = 0; i < RM; ++i) fa[i] = *reinterpret_cast<const mx_u4*>(base + (wm + 16 * i + l) * 128 + (((j * 4 + g) ^ (l & 7)) * 16));
-#pragma unroll
-                for (int i = 0; i < RN; ++i) fb[i] = *reinterpret_cast<const mx_u4*>(base + (BM + wn + 16 * i + l) * 128 + (((j * 4 + g) ^ (l & 7)) * 16));
-#pragma unroll
-                for (int i = 0; i < RM; ++i)
-#pragma unroll
-                    for (int k = 0; k < RN; ++k) {
-                        // outputs transposed (B's rows along the instruction's rows): a lane ends up with four neighbours of one output row
-                        if (h == 0 && j == 0) acc[i][k] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(fb[k]), mx_operand(fa[i]), acc[i][k], 4, 4, 0, sb[k], 0, sa[i]);
-                        else if (h == 0) acc[i][k] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(fb[k]), mx_operand(fa[i]), acc[i][k], 4, 4, 1, sb[k], 1, sa[i]);
-                        else if (j == 0) acc[i][k] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(fb[k]), mx_operand(fa[i]), acc[i][k], 4, 4, 2, sb[k], 2, sa[i]);
-                        else acc[i][k] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(fb[k]), mx_operand(fa[i]), acc[i][k], 4, 4, 3, sb[k], 3, sa[i]);
-                    }
+            for (int i = 0; i < RT; ++i) {
+                qn[i][0] = *reinterpret_cast<const mx_u4*>(qb[i] + nx * 2048 + lane * 16);
+                qn[i][1] = *reinterpret_cast<const mx_u4*>(qb[i] + nx * 2048 + 1024 + lane * 16);
             }
+            if (h == 0) {
+#pragma unroll
+                for (int i = 0; i < RT; ++i) sdn[i] = *reinterpret_cast<const int*>(sb[i] + (sn >> 1) * 256 + lane * 4);
+#pragma unroll
+                for (int c = 0; c < CT; ++c) sxn[c] = *reinterpret_cast<const int*>(xsb[c] + (sn >> 1) * 256 + lane * 4);
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int c = 0; c < CT; ++c) {
+                    const mx_u4 f = *reinterpret_cast<const mx_u4*>(&lds[h][(j * CT + c) * 1024 + lane * 16]);
+#pragma unroll
+                    for (int i = 0; i < RT; ++i) {
+                        // (the byte of the scales is part of the instruction)
+                        if (h == 0 && j == 0) acc[i][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(q[i][j]), mx_operand(f), acc[i][c], 4, 4, 0, sd[i], 0, sx[c]);
+                        else if (h == 0) acc[i][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(q[i][j]), mx_operand(f), acc[i][c], 4, 4, 1, sd[i], 1, sx[c]);
+                        else if (j == 0) acc[i][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(q[i][j]), mx_operand(f), acc[i][c], 4, 4, 2, sd[i], 2, sx[c]);
+                        else acc[i][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(q[i][j]), mx_operand(f), acc[i][c], 4, 4, 3, sd[i], 3, sx[c]);
+                    }
+                }
             __syncthreads();
-            b ^= 1;
+#pragma unroll
+            for (int i = 0; i < RT; ++i) { q[i][0] = qn[i][0]; q[i][1] = qn[i][1]; }
         }
 #pragma unroll
-        for (int i = 0; i < RM; ++i) sa[i] = san[i];
+        for (int i = 0; i < RT; ++i) sd[i] = sdn[i];
 #pragma unroll
-        for (int i = 0; i < RN; ++i) sb[i] = sbn[i];
+        for (int c = 0; c < CT; ++c) sx[c] = sxn[c];
     }
 #pragma unroll
-    for (int i = 0; i < RM; ++i)
+    for (int c = 0; c < CT; ++c)
 #pragma unroll
-        for (int k = 0; k < RN; ++k) {
-            float o[4] = {acc[i][k][0], acc[i][k][1], acc[i][k][2], acc[i][k][3]};
-            mx_store<T, 4>(w, tile.z, m0 + wm + 16 * i + l, n0 + wn + 16 * k + 4 * g, o);
+        for (int i = 0; i < RT; ++i) {
+            float o[4] = {acc[i][c][0], acc[i][c][1], acc[i][c][2], acc[i][c][3]};
+            mx_store<T, 4>(w, tile.z, (tile.a * CT + c) * 16 + l, ((tile.b * 4 + wave) * RT + i) * 16 + 4 * g, o);
         }
 }
 

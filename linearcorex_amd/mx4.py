@@ -30,9 +30,10 @@ _PRODUCT_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 BLOCK = 32
 
 
-def _rows_bytes(cols):
-    """bytes of a row of codes and of a row of scales (include/lcx.h, lcx_mx4_layout)"""
-    return -(-cols // 256) * 128, -(-cols // 512) * 16
+def _sizes(rows, cols):
+    """bytes of the codes and of the scales (include/lcx.h, lcx_mx4_layout)"""
+    tiles = (rows + 15) >> 4
+    return tiles * ((cols + 255) >> 8) * 2048, tiles * ((cols + 511) >> 9) * 256
 
 
 class Mx4(object):
@@ -60,17 +61,13 @@ class Mx4(object):
     @property
     def codes(self):
         if self._codes is None:
-            rows, cols = self._stored()
-            cb = _rows_bytes(cols)[0]
-            self._codes = self._buf[:rows * cb].view(rows, cb)
+            self._codes = self._buf[:_sizes(*self._stored())[0]]
         return self._codes
 
     @property
     def scales(self):
         if self._scales is None:
-            rows, cols = self._stored()
-            cb, sb = _rows_bytes(cols)
-            self._scales = self._buf[rows * cb:].view(rows, sb)
+            self._scales = self._buf[_sizes(*self._stored())[0]:]
         return self._scales
 
     @property
@@ -79,8 +76,7 @@ class Mx4(object):
 
     @property
     def nbytes(self):
-        rows, cols = self._stored()
-        return rows * sum(_rows_bytes(cols))
+        return sum(_sizes(*self._stored()))
 
     def t(self):
         q = Mx4.__new__(Mx4)
@@ -152,10 +148,10 @@ def quantize(x, axis=1):
     shape = (rows, cols)
     if axis == 0:
         rows, cols, rs, cs = cols, rows, cs, rs
-    cb, sb = _rows_bytes(cols)
-    buf = torch.empty(rows * (cb + sb), dtype=torch.uint8, device=x.device)
+    cb, sb = _sizes(rows, cols)
+    buf = torch.empty(cb + sb, dtype=torch.uint8, device=x.device)
     index, cp = x.get_device(), buf.data_ptr()
-    sp = cp + rows * cb
+    sp = cp + cb
     if rows and cols:
         _call(index, "lcx_mx4_quantize", x.data_ptr(), _DTYPES[x.dtype], rows, cols, rs, cs, cp, sp)
     return Mx4._over(shape, axis, index, buf, cp, sp)

@@ -36,10 +36,11 @@ def round4(x):
     return values(*quantize(np.asarray(x, np.float64)))
 
 
-def unpack(codes, scales, shape):
-    """device buffers of lcx_mx4_layout's form -> codes (R, C), scale bytes (R, ceil(C / 32))"""
-    r, c = shape
-    code = np.empty((r, codes.shape[1] * 2), np.int64)
-    code[:, 0::2], code[:, 1::2] = codes & 15, codes >> 4
-    b = np.arange(-(-c // 32))
-    return code[:, :c], scales[:, (b & ~15) + (b & 3) * 4 + ((b >> 2) & 3)].astype(np.int64)
+def unpack(codes, scales, rows, cols):
+    """device buffers of lcx_mx4_layout's form -> codes (R', C'), scale bytes (R', C' / 32) of the padded matrix: 16-row tiles, 256 columns"""
+    tiles, steps, quads = -(-rows // 16), -(-cols // 256) * 2, -(-cols // 512)
+    c = codes.reshape(tiles, steps, 4, 16, 16).transpose(0, 3, 1, 2, 4).reshape(tiles * 16, steps * 64)       # [row][step, group, byte]
+    code = np.empty((tiles * 16, steps * 128), np.int64)
+    code[:, 0::2], code[:, 1::2] = c & 15, c >> 4
+    b = scales.reshape(tiles, quads, 4, 16, 4).transpose(0, 3, 1, 4, 2).reshape(tiles * 16, quads * 16)       # [row][quad, step, group]
+    return code, b.astype(np.int64)

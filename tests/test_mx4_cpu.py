@@ -19,8 +19,8 @@ def lib():
 def fake(shape, axis=1):
     """a matrix on the meta device: what the checks see"""
     r, c = shape if axis == 1 else shape[::-1]
-    cb, sb = mx4._rows_bytes(c)
-    return mx4.Mx4(shape, axis, torch.empty(r, cb, dtype=torch.uint8, device="meta"), torch.empty(r, sb, dtype=torch.uint8, device="meta"))
+    cb, sb = mx4._sizes(r, c)
+    return mx4.Mx4(shape, axis, torch.empty(cb, dtype=torch.uint8, device="meta"), torch.empty(sb, dtype=torch.uint8, device="meta"))
 
 
 def test_python_refuses_host_tensors_and_wrong_types():
@@ -68,10 +68,11 @@ def test_c_entry_points_refuse_bad_arguments(lib):
     b, n = C.c_int64(), C.c_int64()
     for args in ((3, 0, 1, 1, 1), (0, 1, 1, 1, 1), (1, 0, -1, 1, 1)):
         assert _call(lib, "lcx_mx4_workspace", *args, C.byref(b))[0] == 1
-    assert _call(lib, "lcx_mx4_workspace", 1, 0, 1, 1, 1, None)[0] == 1 and _call(lib, "lcx_mx4_layout", -1, None, None)[0] == 1
-    for cols in (0, 1, 31, 256, 257, 512, 513, 5000):
-        assert lib.lcx_mx4_layout(cols, C.byref(b), C.byref(n)) == 0
-        assert (b.value, n.value) == mx4._rows_bytes(cols)
+    assert _call(lib, "lcx_mx4_workspace", 1, 0, 1, 1, 1, None)[0] == 1 and _call(lib, "lcx_mx4_layout", 4, -1, None, None)[0] == 1
+    for rows in (0, 1, 16, 17, 5000):
+        for cols in (0, 1, 31, 256, 257, 512, 513, 5000):
+            assert lib.lcx_mx4_layout(rows, cols, C.byref(b), C.byref(n)) == 0
+            assert (b.value, n.value) == mx4._sizes(rows, cols)
     # nothing to do: no device is needed either
     assert lib.lcx_mx4_quantize(None, 0, 0, 64, 64, 1, None, None, None) == 0
     assert lib.lcx_mx4_linear(None, 0, 0, 64, 1, None, None, 4, 64, None, 4, 1, None, 0, None) == 0

@@ -51,16 +51,13 @@ def test_quantize_to_the_bit(mx4, dt, shape, axis):
     q = mx4.quantize(x, axis=axis)
     want = f64(x) if axis == 1 else f64(x).T
     code, byte = R.quantize(want)
-    got_code, got_byte = R.unpack(q.codes.cpu().numpy(), q.scales.cpu().numpy(), want.shape)
-    assert np.array_equal(got_byte, byte)
-    assert np.array_equal(got_code, code)
-    # what lies behind the last column is defined: zeros and the scale byte 2
-    pad = q.codes.cpu().numpy()
-    assert pad.shape[1] % 128 == 0 and not pad[:, (want.shape[1] + 1) // 2:].any()
-    if want.shape[1] % 2:
-        assert not (pad[:, want.shape[1] // 2] >> 4).any()
-    allb = R.unpack(pad, q.scales.cpu().numpy(), (want.shape[0], q.scales.shape[1] * 32))[1]
-    assert (allb[:, byte.shape[1]:] == 2).all()
+    got_code, got_byte = R.unpack(q.codes.cpu().numpy(), q.scales.cpu().numpy(), *want.shape)
+    r, c = want.shape
+    assert np.array_equal(got_byte[:r, :byte.shape[1]], byte)
+    assert np.array_equal(got_code[:r, :c], code)
+    # what lies behind the last row and column is defined: zeros and the scale byte 2
+    assert not got_code[r:].any() and not got_code[:, c:].any()
+    assert (got_byte[r:] == 2).all() and (got_byte[:, byte.shape[1]:] == 2).all()
     val = R.values(code, byte)
     for out in (torch.float32, torch.float64, torch.bfloat16):
         v = mx4.dequantize(q, out)
@@ -96,7 +93,8 @@ def test_quantize_ties_extremes_and_non_finite(mx4, dt):
     x = torch.cat([x, torch.ones_like(x)], dim=1)                       # a clean block beside each
     q = mx4.quantize(x.cuda())
     code, byte = R.quantize(f64(x))
-    got_code, got_byte = R.unpack(q.codes.cpu().numpy(), q.scales.cpu().numpy(), x.shape)
+    got_code, got_byte = R.unpack(q.codes.cpu().numpy(), q.scales.cpu().numpy(), *x.shape)
+    got_code, got_byte = got_code[:code.shape[0], :code.shape[1]], got_byte[:byte.shape[0], :byte.shape[1]]
     assert np.array_equal(got_byte, byte)
     ok = np.repeat(byte != 255, 32, axis=1)
     assert np.array_equal(got_code[ok], code[ok])
@@ -336,8 +334,9 @@ def test_offsets_beyond_32_bits(mx4):
     w = torch.zeros(64, k, device="cuda")
     w[torch.arange(64), torch.arange(64) * 1000] = 4.0
     q = mx4.quantize(w)
-    big = mx4.Mx4((n, k), 1, torch.zeros(n, q.codes.shape[1], dtype=torch.uint8, device="cuda"), torch.full((n, q.scales.shape[1]), 2, dtype=torch.uint8, device="cuda"))
-    big.codes[-64:], big.scales[-64:] = q.codes, q.scales
+    z = torch.zeros(n // 16 * (k // 128) * 1024, dtype=torch.uint8, device="cuda")
+    big = mx4.Mx4((n, k), 1, z, torch.full((z.numel() // 16,), 2, dtype=torch.uint8, device="cuda"))
+    big.codes[-q.codes.numel():], big.scales[-q.scales.numel():] = q.codes, q.scales       # (whole tiles of 16 rows)
     for m in (1, 33):
         x = ints((m, k), 1, torch.bfloat16)
         y = mx4.linear(x, big)
@@ -345,6 +344,7 @@ def test_offsets_beyond_32_bits(mx4):
         dy = ints((m, n), 2, torch.bfloat16)
         assert torch.equal(mx4.linear_grad(dy, big), mx4.linear_grad(dy[:, -64:], q))
         assert torch.equal(mx4.matmul(mx4.quantize(x), big)[:, -64:], mx4.matmul(mx4.quantize(x), q))
-    x = torch.randn(3, k, device="cuda", dtype=torch.bfloat16).expand(n // 3, 3, k).reshape(-1, k)[: n // 3 * 3]
+    x = torch.randn(16, k, device="cuda", dtype=torch.bfloat16).expand(n // 16, 16, k).reshape(-1, k)
     z = mx4.quantize(x)
-    assert torch.equal(z.codes[-3:], z.codes[:3]) and torch.equal(z.scales[-3:], z.scales[:3])
+    one = k // 128 * 1024
+    assert torch.equal(z.codes[-one:], z.codes[:one]) and torch.equal(z.scales[-one // 16:], z.scales[:one // 16])

@@ -34,11 +34,6 @@ static int mx_grid(int64_t mtiles, int64_t ntiles, unsigned* g) {
     return LCX_OK;
 }
 
-// rows that can be read or written 16 bytes at a time
-template <typename T> static bool mx_row_vec(const void* x, int64_t rs, int64_t cs) {
-    return cs == 1 && ((uintptr_t)x & 15) == 0 && (rs * (int64_t)sizeof(T)) % 16 == 0;
-}
-
 template <typename T>
 static int mx4_quantize(const void* x, int64_t rows, int64_t cols, int64_t rs, int64_t cs, void* codes, void* scales, hipStream_t st) {
     unsigned char *qc = (unsigned char*)codes, *qs = (unsigned char*)scales;
@@ -48,7 +43,7 @@ static int mx4_quantize(const void* x, int64_t rows, int64_t cols, int64_t rs, i
         hipLaunchKernelGGL((mx_quantize_across_kernel<T>), dim3(g), dim3(512), 0, st, (const T*)x, rows, cols, cs, qc, qs);
     } else {
         LCXCHECK(mx_grid(mx_row_tiles(rows), mx_quads(cols), &g));
-        if (mx_row_vec<T>(x, rs, cs)) hipLaunchKernelGGL((mx_quantize_kernel<T, true>), dim3(g), dim3(256), 0, st, (const T*)x, rows, cols, rs, cs, qc, qs);
+        if (cs == 1) hipLaunchKernelGGL((mx_quantize_kernel<T, true>), dim3(g), dim3(256), 0, st, (const T*)x, rows, cols, rs, cs, qc, qs);
         else hipLaunchKernelGGL((mx_quantize_kernel<T, false>), dim3(g), dim3(256), 0, st, (const T*)x, rows, cols, rs, cs, qc, qs);
     }
     KCHECK();
@@ -64,7 +59,7 @@ static int mx4_dequantize(const void* codes, const void* scales, int64_t rows, i
         hipLaunchKernelGGL((mx_dequantize_across_kernel<T>), dim3(g), dim3(512), 0, st, qc, qs, rows, cols, (T*)out, cs);
     } else {
         LCXCHECK(mx_grid(mx_row_tiles(rows), mx_quads(cols), &g));
-        if (mx_row_vec<T>(out, rs, cs)) hipLaunchKernelGGL((mx_dequantize_kernel<T, true>), dim3(g), dim3(256), 0, st, qc, qs, rows, cols, (T*)out, rs, cs);
+        if (cs == 1) hipLaunchKernelGGL((mx_dequantize_kernel<T, true>), dim3(g), dim3(256), 0, st, qc, qs, rows, cols, (T*)out, rs, cs);
         else hipLaunchKernelGGL((mx_dequantize_kernel<T, false>), dim3(g), dim3(256), 0, st, qc, qs, rows, cols, (T*)out, rs, cs);
     }
     KCHECK();
@@ -90,10 +85,16 @@ struct MxPlan {
     int64_t frag_bytes = 0, part_bytes = 0;
 };
 
-static int64_t split_for(int64_t tiles, int64_t steps, int64_t want_blocks, int64_t min_steps) {
-    int64_t s = cdiv(want_blocks, tiles);
-    if (s > steps / min_steps) s = steps / min_steps;
-    return s < 1 ? 1 : s;
+// Parts a contraction of `steps` is cut into for `tiles` output tiles on `slots` resident blocks: time of the rounds (a block's steps and,
+// worth `fixed` of them, its start and its outputs) and of writing and adding up the partial sums (`join` steps a part)
+static int64_t split_for(int64_t tiles, int64_t steps, int64_t slots, double fixed, double join) {
+    int64_t best = 1;
+    double best_t = 1e300;
+    for (int64_t s = 1; s <= 64 && s <= steps; ++s) {
+        const double t = (double)cdiv(tiles * s, slots) * ((double)cdiv(steps, s) + fixed) + (s > 1 ? join * (double)s + fixed : 0.0);
+        if (t < best_t * 0.98) { best_t = t; best = s; }
+    }
+    return best;
 }
 
 // M rows of x, C the contraction, O output columns; along: lcx_mx4_linear, else lcx_mx4_linear_grad
@@ -104,15 +105,17 @@ template <typename T> static MxPlan mx_plan(bool along, int64_t M, int64_t C, in
         p.row = true;
         // 2 x 16 rows of W a wave halve the reads of x where there are enough rows to fill the chip; 16 waves split the contraction
         // where there are few
-        p.rt = M > 4 && O >= 32 * MX_CUS ? 2 : 1;
-        p.waves = cdiv(O, 16 * p.rt) >= 2 * MX_CUS ? 8 : 16;
+        p.rt = M <= 4 || O < 32 * MX_CUS ? 1 : 2;
+        p.waves = p.rt == 2 || cdiv(O, 16) >= 2 * MX_CUS ? 8 : 16;
     } else {
         p.ct = M <= 16 ? 1 : M <= 32 ? 2 : M <= 64 || TERMS > 1 || !along ? 4 : 8;
         p.rt = 4;
         p.mt = cdiv(M, 16 * p.ct);
         p.nt = along ? cdiv(O, 64 * p.rt) : cdiv(O, 512);
         p.nfrag = cdiv(C, 128) * 4;
-        p.split = (int)split_for(p.mt * p.nt, cdiv(C, 128), 2 * MX_CUS, p.ct == 1 ? 2 : 8);
+        // a step of 128 takes two blocks of a CU about 0.4 us per tile of 16 rows and bf16 term; partial sums move at about 4 TB/s
+        const double step_us = 0.4 * p.ct * TERMS;
+        p.split = (int)split_for(p.mt * p.nt, cdiv(C, 128), 2 * MX_CUS, 3.0 / step_us, (double)M * O * 8 / 4e6 / step_us);
         p.frag_bytes = p.nfrag * TERMS * p.mt * p.ct * 1024;
     }
     if (p.split > 1) p.part_bytes = (int64_t)p.split * M * O * 4;
@@ -127,18 +130,13 @@ template <typename T> static int64_t mx_workspace(int op, int64_t M, int64_t N, 
     return op == 1 ? mx_plan_bytes(mx_plan<T>(true, M, K, N)) : mx_plan_bytes(mx_plan<T>(false, M, N, K));
 }
 
-// eight neighbours along the contraction can be read at once
-template <typename T> static bool mx_vec(const void* x, int64_t rs, int64_t cs, int64_t C) {
-    return cs == 1 && C % 8 == 0 && ((uintptr_t)x & 15) == 0 && (rs * (int64_t)sizeof(T)) % 16 == 0;
-}
-
 template <typename T, bool ALONG>
 static int mx_fragments(const T* x, int64_t M, int64_t rs, int64_t cs, int64_t C, const MxPlan& p, unsigned short* frag, hipStream_t st) {
     const int64_t tiles = p.mt * p.ct;
     unsigned g;
     LCXCHECK(mx_grid(tiles, cdiv(p.nfrag * 4, 16), &g));
     const int rows_first = (rs < 0 ? -rs : rs) < (cs < 0 ? -cs : cs);
-    if (mx_vec<T>(x, rs, cs, C))
+    if (cs == 1)
         hipLaunchKernelGGL((mx_fragments_kernel<T, ALONG, true>), dim3(g), dim3(256), 0, st, x, M, rs, cs, C, p.nfrag, tiles, frag, 0);
     else
         hipLaunchKernelGGL((mx_fragments_kernel<T, ALONG, false>), dim3(g), dim3(256), 0, st, x, M, rs, cs, C, p.nfrag, tiles, frag, rows_first);
@@ -148,8 +146,8 @@ static int mx_fragments(const T* x, int64_t M, int64_t rs, int64_t cs, int64_t C
 
 template <typename T> static int mx_join(int split, const MxOut<T>& w, hipStream_t st) {
     if (split == 1) return LCX_OK;
-    const int64_t b = cdiv(w.M * w.O, 256);
-    hipLaunchKernelGGL((mx_join_kernel<T>), dim3((unsigned)(b < 8192 ? b : 8192)), dim3(256), 0, st, w.part, split, w.M, w.O, w.out, w.rs, w.cs);
+    hipLaunchKernelGGL((mx_join_kernel<T>), dim3((unsigned)cdiv(w.O, 1024), (unsigned)(w.M < 32768 ? w.M : 32768)), dim3(256), 0, st, w.part, split, w.M, w.O,
+                       w.out, w.rs, w.cs);
     KCHECK();
     return LCX_OK;
 }
@@ -159,7 +157,7 @@ static int mx_linear_tiles(const MxPlan& p, const unsigned short* frag, const un
                            hipStream_t st) {
     unsigned g;
     LCXCHECK(mx_grid(8, cdiv(p.mt * p.nt * p.split, 8), &g));
-    hipLaunchKernelGGL((mx_linear_tile_kernel<T, CT, 4, JS>), dim3(g), dim3(256), 0, st, frag, p.mt * p.ct, wc, ws, N, K, w, p.mt, p.nt, p.split);
+    hipLaunchKernelGGL((mx_linear_tile_kernel<T, CT, 4, JS>), dim3(g), dim3(256), 0, st, frag, p.mt * p.ct, wc, ws, N, K, w, (int)p.mt, (int)p.nt, p.split);
     KCHECK();
     return LCX_OK;
 }
@@ -168,9 +166,9 @@ static int mx_grad_tiles(const MxPlan& p, const unsigned short* frag, const unsi
                          hipStream_t st) {
     unsigned g;
     LCXCHECK(mx_grid(8, cdiv(p.mt * p.nt * p.split, 8), &g));
-    constexpr size_t lds = 2 * MxGradLds<CT, JS, MxTerms<T>::v>::stage;
+    constexpr size_t lds = MxGradLds<CT, JS, MxTerms<T>::v>::total;
     LCXCHECK(allow_lds(mx_grad_tile_kernel<T, CT, JS>, lds));
-    hipLaunchKernelGGL((mx_grad_tile_kernel<T, CT, JS>), dim3(g), dim3(256), lds, st, frag, p.mt * p.ct, wc, ws, N, K, w, p.mt, p.nt, p.split);
+    hipLaunchKernelGGL((mx_grad_tile_kernel<T, CT, JS>), dim3(g), dim3(256), lds, st, frag, p.mt * p.ct, wc, ws, N, K, w, (int)p.mt, (int)p.nt, p.split);
     KCHECK();
     return LCX_OK;
 }
@@ -181,11 +179,9 @@ static int mx_linear_rows(const MxPlan& p, const T* x, int64_t rs, int64_t cs, c
     unsigned g;
     LCXCHECK(mx_grid(1, cdiv(N, 16 * p.rt), &g));
 #define MX_ROWS(RT, WV) hipLaunchKernelGGL((mx_linear_row_kernel<T, RT, WV, VEC>), dim3(g), dim3(64 * WV), 0, st, x, w.M, rs, cs, wc, ws, N, K, w)
-    if (p.rt == 2) {
-        if (p.waves == 8) MX_ROWS(2, 8); else MX_ROWS(2, 16);
-    } else {
-        if (p.waves == 8) MX_ROWS(1, 8); else MX_ROWS(1, 16);
-    }
+    if (p.rt == 2) MX_ROWS(2, 8);
+    else if (p.waves == 8) MX_ROWS(1, 8);
+    else MX_ROWS(1, 16);
 #undef MX_ROWS
     KCHECK();
     return LCX_OK;
@@ -202,7 +198,7 @@ static int mx4_linear(const void* xv, int64_t M, int64_t xrs, int64_t xcs, const
     const unsigned char *wc = (const unsigned char*)wcv, *ws = (const unsigned char*)wsv;
     unsigned short* frag = (unsigned short*)space;
     MxOut<T> w{(T*)out, rs, cs, p.split > 1 ? (float*)((char*)space + round_up(p.frag_bytes, 256)) : nullptr, M, N};
-    if (p.row) return mx_vec<T>(x, xrs, xcs, K) ? mx_linear_rows<T, true>(p, x, xrs, xcs, wc, ws, N, K, w, st)
+    if (p.row) return xcs == 1 ? mx_linear_rows<T, true>(p, x, xrs, xcs, wc, ws, N, K, w, st)
                                                 : mx_linear_rows<T, false>(p, x, xrs, xcs, wc, ws, N, K, w, st);
     LCXCHECK((mx_fragments<T, true>(x, M, xrs, xcs, K, p, frag, st)));
     constexpr int JS = TERMS == 3 ? 2 : 4;
@@ -226,7 +222,7 @@ static int mx4_linear_grad(const void* dyv, int64_t M, int64_t yrs, int64_t ycs,
     unsigned short* frag = (unsigned short*)space;
     MxOut<T> w{(T*)out, rs, cs, p.split > 1 ? (float*)((char*)space + round_up(p.frag_bytes, 256)) : nullptr, M, K};
     LCXCHECK((mx_fragments<T, false>(dy, M, yrs, ycs, N, p, frag, st)));
-    constexpr int JS = TERMS == 3 ? 1 : 2;
+    constexpr int JS = TERMS > 1 ? 1 : 2;
     if (p.ct == 1) LCXCHECK((mx_grad_tiles<T, 1, JS>(p, frag, wc, ws, N, K, w, st)));
     else if (p.ct == 2) LCXCHECK((mx_grad_tiles<T, 2, JS>(p, frag, wc, ws, N, K, w, st)));
     else LCXCHECK((mx_grad_tiles<T, 4, JS>(p, frag, wc, ws, N, K, w, st)));
@@ -251,7 +247,8 @@ static MxMatmulPlan mx_matmul_plan(int64_t M, int64_t N, int64_t K) {
     p.ct = M <= 32 ? 2 : M <= 64 ? 4 : 8;
     p.mt = cdiv(M, 16 * p.ct);
     p.nt = cdiv(N, 256);
-    p.split = (int)split_for(p.mt * p.nt, cdiv(K, 512), 2 * MX_CUS, 2);
+    const double quad_us = 0.25 * p.ct;
+    p.split = (int)split_for(p.mt * p.nt, cdiv(K, 512), 2 * MX_CUS, 3.0 / quad_us, (double)M * N * 8 / 4e6 / quad_us);
     if (p.split > 1) p.part_bytes = (int64_t)p.split * M * N * 4;
     return p;
 }
@@ -263,7 +260,7 @@ static int mx_matmul_tiles(const MxMatmulPlan& p, const unsigned char* ac, const
                            int64_t K, const MxOut<T>& w, hipStream_t st) {
     unsigned g;
     LCXCHECK(mx_grid(8, cdiv(p.mt * p.nt * p.split, 8), &g));
-    hipLaunchKernelGGL((mx_matmul_tile_kernel<T, CT, RT>), dim3(g), dim3(256), 0, st, ac, as, bc, bs, N, K, w, p.mt, p.nt, p.split);
+    hipLaunchKernelGGL((mx_matmul_tile_kernel<T, CT, RT>), dim3(g), dim3(256), 0, st, ac, as, bc, bs, N, K, w, (int)p.mt, (int)p.nt, p.split);
     KCHECK();
     return LCX_OK;
 }

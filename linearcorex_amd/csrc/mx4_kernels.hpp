@@ -28,6 +28,9 @@ typedef __attribute__((ext_vector_type(4))) float mx_f4;
 typedef __attribute__((ext_vector_type(4))) unsigned int mx_u4;
 typedef __attribute__((ext_vector_type(8))) int mx_i8;
 
+// the wave's number in its block, known to be the same for all lanes (addresses that depend on it then live in scalar registers)
+__device__ __forceinline__ int mx_wave() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
+
 template <typename T> struct MxTerms;                              // bf16 numbers that add up to a T exactly
 template <> struct MxTerms<float> { static constexpr int v = 3; };     // 24 significant bits = 8 + 8 + 8
 template <> struct MxTerms<_Float16> { static constexpr int v = 2; };  // 11 = 8 + 3
@@ -35,15 +38,14 @@ template <> struct MxTerms<__bf16> { static constexpr int v = 1; };
 
 __device__ __forceinline__ float mx_trunc_bf16(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 // x = term 0 + term 1 + term 2, each a bf16 number: the leading 8 significant bits are cut off twice, what remains has at most 8.  Every
-// term takes part in the products below, so cutting (rather than rounding) leaves no bias.  An infinity or NaN stays in term 0
-// (the remainder would be NaN: zeros instead, the sum is the same).
+// term takes part in the products below, so cutting (rather than rounding) leaves no bias.  An infinity stays in term 0 alone (its
+// remainder would be a NaN); a NaN leaves one in the remainder, whatever the cut makes of its payload.
 template <int TERMS> __device__ __forceinline__ void mx_split(float x, float* t) {
-    t[0] = TERMS > 1 ? mx_trunc_bf16(x) : x;
-    if constexpr (TERMS > 1) {
-        const bool finite = (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u;
-        // (cutting a NaN's payload could leave an infinity)
-        if (!finite) t[0] = x;
-        const float r = finite ? x - t[0] : 0.0f;
+    if constexpr (TERMS == 1) {
+        t[0] = x;
+    } else {
+        t[0] = mx_trunc_bf16(x);
+        const float r = __builtin_isinf(x) ? 0.0f : x - t[0];
         t[1] = TERMS > 2 ? mx_trunc_bf16(r) : r;
         if constexpr (TERMS > 2) t[2] = r - t[1];
     }
@@ -93,16 +95,33 @@ __device__ __forceinline__ unsigned int mx_quad_max(unsigned int v) {
     o = (unsigned int)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true);                     // lanes 2 3 0 1
     return o > v ? o : v;
 }
+// 16 bytes at an address that only the element type aligns
+typedef unsigned int mx_u4u __attribute__((ext_vector_type(4), aligned(2)));
+typedef float mx_f4u __attribute__((ext_vector_type(4), aligned(4)));
+template <typename T, int N> __device__ __forceinline__ void mx_put(T* p, const T* v) {
+    if constexpr (N * sizeof(T) % 16 == 0) {
+        mx_u4 t[N * sizeof(T) / 16];
+        __builtin_memcpy(t, v, sizeof(t));
+#pragma unroll
+        for (int i = 0; i < (int)(N * sizeof(T) / 16); ++i) reinterpret_cast<mx_u4u*>(p)[i] = t[i];
+    } else {
+        typedef unsigned int u2u __attribute__((ext_vector_type(2), aligned(2)));
+        static_assert(N * sizeof(T) == 8, "");
+        u2u t;
+        __builtin_memcpy(&t, v, 8);
+        *reinterpret_cast<u2u*>(p) = t;
+    }
+}
+// eight neighbours of a row, read or written 16 bytes at a time from any address the element type allows (global memory takes it)
 template <typename T> struct MxRaw8 { T v[8]; };
-// eight neighbours of a row; zeros behind the last column
+// zeros behind the last column; VEC: the columns are neighbours (cs == 1)
 template <typename T, bool VEC>
 __device__ __forceinline__ MxRaw8<T> mx_load8(const T* __restrict__ x, int64_t c0, int64_t cols, int64_t cs) {
     MxRaw8<T> r;
     if (VEC && c0 + 8 <= cols) {
-        const mx_u4* p = reinterpret_cast<const mx_u4*>(x + c0);
         mx_u4 t[sizeof(T) / 2];
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) t[i] = p[i];
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) t[i] = reinterpret_cast<const mx_u4u*>(x + c0)[i];
         __builtin_memcpy(&r, t, sizeof(r));
     } else {
 #pragma unroll
@@ -112,13 +131,14 @@ __device__ __forceinline__ MxRaw8<T> mx_load8(const T* __restrict__ x, int64_t c
 }
 
 // x[r * rs + c * cs] -> codes, scales.  Bound: reading x.  A block takes 16 rows x 512 columns: a thread 8 columns of each of four steps (16 bytes
-// of a 16-bit type each: VEC, where rows are contiguous and aligned), so that it ends up with a whole dword of scales; four lanes share a
+// of a 16-bit type each: VEC, where the columns are neighbours), so that it ends up with a whole dword of scales; four lanes share a
 // block of 32.  grid (row tile, quad of steps)
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t rs, int64_t cs,
                                                           unsigned char* __restrict__ codes, unsigned char* __restrict__ scales) {
     const int64_t steps = mx_steps(cols), quads = mx_quads(cols);
-    const int64_t rt = blockIdx.x / quads, quad = blockIdx.x % quads;
+    const unsigned int rt32 = blockIdx.x / (unsigned int)quads;
+    const int64_t rt = rt32, quad = blockIdx.x - rt32 * (unsigned int)quads;
     const int l = threadIdx.x >> 4, c = threadIdx.x & 15;                  // row of the tile, 8 columns of the step
     const int64_t r = rt * 16 + l;
     MxRaw8<T> raw[4];
@@ -155,8 +175,9 @@ __global__ __launch_bounds__(512) void mx_quantize_across_kernel(const T* __rest
                                                                  unsigned char* __restrict__ codes, unsigned char* __restrict__ scales) {
     const int64_t steps = mx_steps(cols), quads = mx_quads(cols);
     __shared__ __attribute__((aligned(16))) unsigned char ls[4][256];      // [row tile][lane][step]
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tile = lane >> 4, l = lane & 15;
-    const int64_t quad = blockIdx.x % quads, rt = blockIdx.x / quads * 4 + tile, r = rt * 16 + l, rts = mx_row_tiles(rows);
+    const int lane = threadIdx.x & 63, wave = mx_wave(), tile = lane >> 4, l = lane & 15;
+    const unsigned int rt32 = blockIdx.x / (unsigned int)quads;
+    const int64_t quad = blockIdx.x - rt32 * (unsigned int)quads, rt = (int64_t)rt32 * 4 + tile, r = rt * 16 + l, rts = mx_row_tiles(rows);
     const T* p = x + (r < rows ? r : rows - 1);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -185,7 +206,7 @@ __global__ __launch_bounds__(512) void mx_quantize_across_kernel(const T* __rest
         ls[tile][(g * 16 + l) * 4 + s] = (unsigned char)sc;
     }
     __syncthreads();
-    const int64_t wt = blockIdx.x / quads * 4 + (threadIdx.x >> 6);
+    const int64_t wt = (int64_t)rt32 * 4 + (threadIdx.x >> 6);
     if (threadIdx.x < 256 && wt < rts)
         *reinterpret_cast<unsigned int*>(scales + (wt * quads + quad) * 256 + lane * 4) = *reinterpret_cast<const unsigned int*>(&ls[threadIdx.x >> 6][lane * 4]);
 }
@@ -200,12 +221,13 @@ __device__ __forceinline__ void mx_values8(unsigned int q, float s, float* v) {
     p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, s, 3); v[6] = p[0]; v[7] = p[1];
 }
 
-// codes, scales -> out[r * rs + c * cs].  Bound: writing out.  Threads as in mx_quantize_kernel; VEC: rows of out are contiguous and aligned
+// codes, scales -> out[r * rs + c * cs].  Bound: writing out.  Threads as in mx_quantize_kernel; VEC: the columns of out are neighbours
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
                                                             int64_t rows, int64_t cols, T* __restrict__ out, int64_t rs, int64_t cs) {
     const int64_t steps = mx_steps(cols), quads = mx_quads(cols);
-    const int64_t rt = blockIdx.x / quads, quad = blockIdx.x % quads;
+    const unsigned int rt32 = blockIdx.x / (unsigned int)quads;
+    const int64_t rt = rt32, quad = blockIdx.x - rt32 * (unsigned int)quads;
     const int l = threadIdx.x >> 4, c = threadIdx.x & 15;
     const int64_t r = rt * 16 + l;
     if (r >= rows) return;
@@ -224,10 +246,7 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned char*
             MxRaw8<T> o;
 #pragma unroll
             for (int j = 0; j < 8; ++j) o.v[j] = mx_from_f32<T>(v[j]);
-            mx_u4 t[sizeof(T) / 2];
-            __builtin_memcpy(t, &o, sizeof(o));
-#pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<mx_u4*>(p)[i] = t[i];
+            mx_put<T, 8>(p, o.v);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -241,8 +260,9 @@ template <typename T>
 __global__ __launch_bounds__(512) void mx_dequantize_across_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
                                                                    int64_t rows, int64_t cols, T* __restrict__ out, int64_t cs) {
     const int64_t steps = mx_steps(cols), quads = mx_quads(cols);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15;
-    const int64_t quad = blockIdx.x % quads, rt = blockIdx.x / quads * 4 + (lane >> 4), r = rt * 16 + l;
+    const int lane = threadIdx.x & 63, wave = mx_wave(), l = lane & 15;
+    const unsigned int rt32 = blockIdx.x / (unsigned int)quads;
+    const int64_t quad = blockIdx.x - rt32 * (unsigned int)quads, rt = (int64_t)rt32 * 4 + (lane >> 4), r = rt * 16 + l;
     if (r >= rows) return;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -263,6 +283,10 @@ __global__ __launch_bounds__(512) void mx_dequantize_across_kernel(const unsigne
 }
 
 // ---- products of x (float32, bf16, fp16) with a 4-bit matrix -----------------------------------------------------------------------
+// The scale operand of the conversions: only the exponent field of the dword counts (sign and mantissa are ignored: checked for every byte
+// and exponent), so the byte i of a dword of scales takes one rotation.
+__device__ __forceinline__ float mx_scale_operand(unsigned int dword, int i) { return __uint_as_float(__builtin_amdgcn_alignbit(dword, dword, (9 + 8 * i) & 31)); }
+
 // eight codes of one block -> bf16 (exact: at most 2 significant bits)
 __device__ __forceinline__ mx_bf8 mx_unpack8(unsigned int q, float s) {
     const mx_bf2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, s, 1),
@@ -270,40 +294,27 @@ __device__ __forceinline__ mx_bf8 mx_unpack8(unsigned int q, float s) {
     return mx_bf8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// x[t * rs + k * cs], eight k from k0 on, as bf16 terms; zeros from nk on.  VEC: cs is 1, the eight values are aligned to 16 bytes and nk is a
-// multiple of 8.  t must be a row.
-template <typename T, int TERMS, bool VEC>
-__device__ __forceinline__ void mx_load_terms(const T* __restrict__ x, int64_t t, int64_t rs, int64_t k0, int64_t nk, int64_t cs, mx_bf8* f) {
-    T v[8];
-    if constexpr (VEC) {
-        if (k0 < nk) {
-            const mx_u4* p = reinterpret_cast<const mx_u4*>(x + t * rs + k0);
-            mx_u4 r[sizeof(T) / 2];
-#pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; ++i) r[i] = p[i];
-            __builtin_memcpy(v, r, sizeof(v));
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = (T)0.0f;
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = k0 + j < nk ? x[t * rs + (k0 + j) * cs] : (T)0.0f;
-    }
+// eight values as bf16 terms
+template <typename T, int TERMS> __device__ __forceinline__ void mx_terms(const MxRaw8<T>& r, mx_bf8* f) {
     if constexpr (TERMS == 1) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[0][j] = (__bf16)v[j];
+        for (int j = 0; j < 8; ++j) f[0][j] = (__bf16)r.v[j];
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             float p[3];
-            mx_split<TERMS>((float)v[j], p);
+            mx_split<TERMS>((float)r.v[j], p);
 #pragma unroll
             for (int u = 0; u < TERMS; ++u) f[u][j] = (__bf16)p[u];
         }
     }
 }
 
+// x[t * rs + k * cs], eight k from k0 on, as bf16 terms; zeros from nk on.  t must be a row.
+template <typename T, int TERMS, bool VEC>
+__device__ __forceinline__ void mx_load_terms(const T* __restrict__ x, int64_t t, int64_t rs, int64_t k0, int64_t nk, int64_t cs, mx_bf8* f) {
+    mx_terms<T, TERMS>(mx_load8<T, VEC>(x + t * rs, k0, nk, cs), f);
+}
 // where an output goes: split == 1 the result, else float32 partial sums [split][M][O] (mx_join_kernel adds them up in order)
 template <typename T> struct MxOut {
     T* out;
@@ -317,9 +328,8 @@ __device__ __forceinline__ void mx_store(const MxOut<T>& w, int64_t z, int64_t t
     if (t >= w.M) return;
     if (w.part) {
         float* p = w.part + (z * w.M + t) * w.O + o;
-        if (o + N <= w.O && ((uintptr_t)p & 15) == 0) {
-#pragma unroll
-            for (int j = 0; j < N; j += 4) *reinterpret_cast<mx_f4*>(p + j) = mx_f4{v[j], v[j + 1], v[j + 2], v[j + 3]};
+        if (o + N <= w.O) {
+            mx_put<float, N>(p, v);
         } else {
 #pragma unroll
             for (int j = 0; j < N; ++j)
@@ -328,27 +338,45 @@ __device__ __forceinline__ void mx_store(const MxOut<T>& w, int64_t z, int64_t t
         return;
     }
     T* p = w.out + t * w.rs + o * w.cs;
-    if (w.cs == 1 && o + N <= w.O && ((uintptr_t)p & (N * sizeof(T) - 1)) == 0) {
-        typedef T vec __attribute__((ext_vector_type(N)));
-        vec r;
+    if (w.cs == 1 && o + N <= w.O) {
+        T r[N];
 #pragma unroll
         for (int j = 0; j < N; ++j) r[j] = mx_from_f32<T>(v[j]);
-        *reinterpret_cast<vec*>(p) = r;
+        mx_put<T, N>(p, r);
     } else {
 #pragma unroll
         for (int j = 0; j < N; ++j)
             if (o + j < w.O) p[j * w.cs] = mx_from_f32<T>(v[j]);
     }
 }
-// out[t][o] = sum over the splits, in order
+// out[t][o] = sum over the splits, in order; four columns a thread.  grid (columns, rows)
 template <typename T>
 __global__ __launch_bounds__(256) void mx_join_kernel(const float* __restrict__ part, int split, int64_t M, int64_t O, T* __restrict__ out, int64_t rs,
                                                       int64_t cs) {
-    const int64_t n = M * O;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        float v = part[i];
-        for (int z = 1; z < split; ++z) v += part[(int64_t)z * n + i];
-        out[(i / O) * rs + (i % O) * cs] = mx_from_f32<T>(v);
+    const int64_t o = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, n = M * O;
+    if (o >= O) return;
+    for (int64_t t = blockIdx.y; t < M; t += gridDim.y) {
+        const float* p = part + t * O + o;
+        if (o + 4 <= O) {
+            mx_f4 v = *reinterpret_cast<const mx_f4u*>(p);
+            for (int z = 1; z < split; ++z) v += *reinterpret_cast<const mx_f4u*>(p + z * n);
+            T* q = out + t * rs + o * cs;
+            if (cs == 1) {
+                T r[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) r[j] = mx_from_f32<T>(v[j]);
+                mx_put<T, 4>(q, r);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) q[j * cs] = mx_from_f32<T>(v[j]);
+            }
+        } else {
+            for (int j = 0; o + j < O; ++j) {
+                float v = p[j];
+                for (int z = 1; z < split; ++z) v += p[z * n + j];
+                out[t * rs + (o + j) * cs] = mx_from_f32<T>(v);
+            }
+        }
     }
 }
 
@@ -363,7 +391,7 @@ __global__ __launch_bounds__(64 * WAVES) void mx_linear_row_kernel(const T* __re
     constexpr int TERMS = MxTerms<T>::v, U = 4;
     const int64_t ksteps = mx_steps(K), quads = mx_quads(K), rts = mx_row_tiles(N);
     const int64_t n0 = (int64_t)blockIdx.x * 16 * RT;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = mx_wave(), l = lane & 15, g = lane >> 4;
     const int64_t t = l < M ? l : M - 1;                       // rows behind the last one repeat it and are not stored
     const unsigned char *pc[RT], *ps[RT];
 #pragma unroll
@@ -392,10 +420,13 @@ __global__ __launch_bounds__(64 * WAVES) void mx_linear_row_kernel(const T* __re
         for (int u = 0; u < U; ++u) {
             const int64_t s = s0 + u * WAVES;
             if (s < steps) {
+                MxRaw8<T> raw[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) raw[j] = mx_load8<T, VEC>(x + t * xrs, s * 128 + g * 32 + j * 8, K, xcs);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     mx_bf8 f[TERMS];
-                    mx_load_terms<T, TERMS, VEC>(x, t, xrs, s * 128 + g * 32 + j * 8, K, xcs, f);
+                    mx_terms<T, TERMS>(raw[j], f);
 #pragma unroll
                     for (int i = 0; i < RT; ++i) {
                         const mx_bf8 a = mx_unpack8(q[u][i][j], __uint_as_float(sc[u][i] << 23));
@@ -421,11 +452,11 @@ __global__ __launch_bounds__(64 * WAVES) void mx_linear_row_kernel(const T* __re
 
 // 8 columns of one row of W as bf16, entry m of dword j -> what matrix instruction m takes from this lane: the transposition of an 8 x 8 piece
 // that the lane holds whole, two values a dword
-__device__ __forceinline__ void mx_unpack_across(const unsigned int* q, const unsigned int* sc, mx_bf8* w) {
+__device__ __forceinline__ void mx_unpack_across(const unsigned int* q, const float* sc, mx_bf8* w) {
     unsigned int u[8][4];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const mx_bf8 v = mx_unpack8(q[j], __uint_as_float(sc[j] << 23));
+        const mx_bf8 v = mx_unpack8(q[j], sc[j]);
         __builtin_memcpy(u[j], &v, 16);
     }
 #pragma unroll
@@ -453,7 +484,8 @@ __global__ __launch_bounds__(256) void mx_fragments_kernel(const T* __restrict__
                                                            int64_t tiles, unsigned short* __restrict__ frag, int rows_first) {
     constexpr int TERMS = MxTerms<T>::v;
     // a block takes one tile of 16 rows and 16 groups of 8 values; neighbouring threads read neighbouring memory
-    const int64_t tile = blockIdx.x % tiles, c0 = (int64_t)(blockIdx.x / tiles) * 16;
+    const unsigned int grp = blockIdx.x / (unsigned int)tiles;
+    const int64_t tile = blockIdx.x - grp * (unsigned int)tiles, c0 = (int64_t)grp * 16;
     const int l = rows_first ? threadIdx.x & 15 : threadIdx.x >> 4;
     const int64_t c = c0 + (rows_first ? threadIdx.x >> 4 : threadIdx.x & 15);         // group of 8 along the contraction
     if (c >= nfrag * 4) return;
@@ -466,23 +498,43 @@ __global__ __launch_bounds__(256) void mx_fragments_kernel(const T* __restrict__
     for (int u = 0; u < TERMS; ++u) *reinterpret_cast<mx_bf8*>(frag + (((i * TERMS + u) * tiles + tile) * 64 + g * 16 + l) * 8) = f[u];
 }
 
+// Order of the instructions around READS fragments from LDS of MFMA matrix instructions each.  Left alone, a wave reads a fragment, waits, uses
+// it, and unpacks in one piece; two waves of a SIMD then fall into step and neither pipe is fed while they do.  So: the fragments two ahead
+// (EXTRA reads of other data with the first of them), and VALU vector instructions behind every matrix instruction.
+template <int N, int VALU> __device__ __forceinline__ void mx_schedule_mfma() {
+    if constexpr (N > 0) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if constexpr (VALU > 0) __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
+        mx_schedule_mfma<N - 1, VALU>();
+    }
+}
+template <int READS, int MFMA, int EXTRA, int VALU, bool FIRST = true> __device__ __forceinline__ void mx_schedule() {
+    constexpr int G = READS > 1 ? 2 : 1, REST = READS - G, NEXT = REST < 2 ? REST : 2;
+    if constexpr (FIRST) __builtin_amdgcn_sched_group_barrier(0x100, G + EXTRA, 0);
+    mx_schedule_mfma<1, VALU>();
+    if constexpr (NEXT > 0) __builtin_amdgcn_sched_group_barrier(0x100, NEXT, 0);
+    mx_schedule_mfma<G * MFMA - 1, VALU>();
+    if constexpr (NEXT > 0) mx_schedule<REST, MFMA, 0, VALU, false>();
+}
+
 typedef __attribute__((address_space(1))) const void* mx_gptr;
 typedef __attribute__((address_space(3))) void* mx_lptr;
 
 // block -> (row tile, column tile, split): consecutive blocks go to the 8 XCDs in turn, so each XCD gets a contiguous piece of an order in which
 // eight row tiles share a column tile of W
-struct MxTile { int64_t a, b; int z; };
-__device__ __forceinline__ MxTile mx_tile(int64_t id, int64_t na, int64_t nb, int split) {
-    const int64_t total = na * nb * split, per = (total + 7) / 8;
-    int64_t p = (id & 7) * per + (id >> 3);
-    MxTile r;
-    if (p >= total || (id >> 3) >= per) { r.a = -1; r.b = 0; r.z = 0; return r; }
-    r.z = (int)(p / (na * nb));
-    p -= (int64_t)r.z * na * nb;
-    const int64_t grp = p / (8 * nb), left = na - grp * 8 < 8 ? na - grp * 8 : 8;
+struct MxTile { int a, b, z; };
+__device__ __forceinline__ MxTile mx_tile(unsigned int id, unsigned int na, unsigned int nb, unsigned int split) {
+    const unsigned int area = na * nb, total = area * split, per = (total + 7) / 8;       // (all below 2^31)
+    unsigned int p = (id & 7) * per + (id >> 3);
+    MxTile r = {-1, 0, 0};
+    if (p >= total || (id >> 3) >= per) return r;
+    const unsigned int z = p / area;
+    p -= z * area;
+    const unsigned int grp = p / (8 * nb), left = na - grp * 8 < 8 ? na - grp * 8 : 8;
     p -= grp * 8 * nb;
-    r.a = grp * 8 + p % left;
-    r.b = p / left;
+    r.z = (int)z;
+    r.b = (int)(p / left);
+    r.a = (int)(grp * 8 + (p - (unsigned int)r.b * left));
     return r;
 }
 
@@ -491,15 +543,14 @@ __device__ __forceinline__ MxTile mx_tile(int64_t id, int64_t na, int64_t nb, in
 // of x through LDS (JS of them a stage, double buffered).
 template <typename T, int CT, int RT, int JS>
 __global__ __launch_bounds__(256, 2) void mx_linear_tile_kernel(const unsigned short* __restrict__ frag, int64_t tiles, const unsigned char* __restrict__ wc,
-                                                             const unsigned char* __restrict__ ws, int64_t N, int64_t K, MxOut<T> w, int64_t mt,
-                                                             int64_t nt, int split) {
+                                                             const unsigned char* __restrict__ ws, int64_t N, int64_t K, MxOut<T> w, int mt, int nt, int split) {
     constexpr int TERMS = MxTerms<T>::v, CH = JS * TERMS * CT;             // 1 KB pieces a stage
     const int64_t ksteps = mx_steps(K), quads = mx_quads(K), rts = mx_row_tiles(N);
     const MxTile tile = mx_tile(blockIdx.x, mt, nt, split);
     if (tile.a < 0) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
-    const int64_t n0 = tile.b * 64 * RT + wave * 16 * RT;
-    const int64_t steps = (K + 127) / 128, per = ((steps + split - 1) / split + 3) / 4 * 4;      // (whole dwords of scales)
+    const int lane = threadIdx.x & 63, wave = mx_wave(), l = lane & 15, g = lane >> 4;
+    const int64_t n0 = (int64_t)tile.b * 64 * RT + wave * 16 * RT;
+    const int64_t steps = (K + 127) / 128, per = (steps + split - 1) / split;
     const int64_t s0 = per * tile.z, s1 = s0 + per < steps ? s0 + per : steps;
     __shared__ __attribute__((aligned(16))) unsigned short lds[2][CH * 512];
     const unsigned char *pc[RT], *ps[RT];
@@ -509,21 +560,23 @@ __global__ __launch_bounds__(256, 2) void mx_linear_tile_kernel(const unsigned s
         pc[i] = wc + rt * ksteps * 1024;
         ps[i] = ws + rt * quads * 256;
     }
-    auto stage = [&](int64_t f, int b) {                                   // fragments f .. f + JS of the contraction
+    // running address of the next stage: scalar, advanced by a constant
+    const unsigned char* fp = (const unsigned char*)frag + (s0 * 4 * TERMS * tiles + (int64_t)tile.a * CT) * 1024;
+    const int64_t fterm = tiles * 1024;
+    auto stage = [&](int b) {                                              // the next JS fragments of the contraction
 #pragma unroll
         for (int c = 0; c < (CH + 3) / 4; ++c) {
             const int i = c * 4 + wave;
-            if (CH % 4 == 0 || i < CH) {
-                const int64_t at = ((f * TERMS + i / CT) * tiles + tile.a * CT + i % CT) * 512;
-                __builtin_amdgcn_global_load_lds((mx_gptr)(frag + at + lane * 8), (mx_lptr)(&lds[b][i * 512]), 16, 0, 0);
-            }
+            if (CH % 4 == 0 || i < CH)
+                __builtin_amdgcn_global_load_lds((mx_gptr)(fp + (i / CT) * fterm + (i % CT) * 1024 + lane * 16), (mx_lptr)(&lds[b][i * 512]), 16, 0, 0);
         }
+        fp += JS * TERMS * fterm;
     };
     mx_f4 acc[RT][CT] = {};
     mx_u4 q[RT];
     unsigned int sd[RT];
     if (s0 < s1) {
-        stage(s0 * 4, 0);
+        stage(0);
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
             q[i] = *reinterpret_cast<const mx_u4*>(pc[i] + s0 * 1024 + lane * 16);
@@ -539,11 +592,10 @@ __global__ __launch_bounds__(256, 2) void mx_linear_tile_kernel(const unsigned s
         for (int i = 0; i < RT; ++i) { qn[i] = q[i]; sn[i] = sd[i]; }
         float sc[RT];
 #pragma unroll
-        for (int i = 0; i < RT; ++i) sc[i] = __uint_as_float(((sd[i] >> (8 * (s & 3))) & 255u) << 23);
+        for (int i = 0; i < RT; ++i) sc[i] = mx_scale_operand(sd[i], (int)(s & 3));
 #pragma unroll
         for (int h = 0; h < 4 / JS; ++h) {
-            if (h + 1 < 4 / JS) stage(s * 4 + (h + 1) * JS, b ^ 1);
-            else if (s + 1 < s1) stage((s + 1) * 4, b ^ 1);
+            if (h + 1 < 4 / JS || s + 1 < s1) stage(b ^ 1);
             if (h == 0 && s + 1 < s1) {
 #pragma unroll
                 for (int i = 0; i < RT; ++i) {
@@ -565,6 +617,7 @@ __global__ __launch_bounds__(256, 2) void mx_linear_tile_kernel(const unsigned s
                         for (int i = 0; i < RT; ++i) acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], f, acc[i][c], 0, 0, 0);
                     }
             }
+            mx_schedule<JS * TERMS * CT, RT, 0, 1>();
             __syncthreads();
             b ^= 1;
         }
@@ -576,92 +629,117 @@ __global__ __launch_bounds__(256, 2) void mx_linear_tile_kernel(const unsigned s
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
             float o[4] = {acc[i][c][0], acc[i][c][1], acc[i][c][2], acc[i][c][3]};
-            mx_store<T, 4>(w, tile.z, (tile.a * CT + c) * 16 + l, n0 + 16 * i + 4 * g, o);
+            mx_store<T, 4>(w, tile.z, ((int64_t)tile.a * CT + c) * 16 + l, n0 + 16 * i + 4 * g, o);
         }
 }
 
 // dx[t][k] = sum_n dy[t][n] W[n][k] for tiles of 16 CT rows of dy and 512 columns of W: the contraction runs ACROSS the blocks.  A lane reads the
 // dword of 8 columns from each of 8 rows; unpacked, entry m of the eight dwords is what matrix instruction m needs from this lane: column 8
 // (lane % 16) + m, eight n.  So a wave owns 128 columns as 8 tiles and no value crosses lanes.  Bound: the bf16 matrix pipe; unpacking
-// costs the vector pipe a cycle per value of W and tile of rows.  32 JS rows of W (codes, scales) and their fragments of dy a stage, all of
-// them to LDS without passing registers, double buffered.  Row r of block b in row tile p is stored at row r ^ (b | 4 (p % 2)) of its
-// block: the sixteen (block, lane group) that a wave reads at once lie in different banks.
+// costs three vector instructions per matrix instruction at CT 4, one step ahead and in between them.  32 JS rows of W (codes, scales) and
+// their fragments of dy a stage, all of them to LDS without passing registers: the fragments double buffered, W in three buffers, since it is
+// unpacked a step early.  Row r of block b in row tile p is stored at row r ^ (b | 4 (p % 2)) of its block: the sixteen (block, lane group)
+// that a wave reads at once lie in different banks.
 template <int CT, int JS, int TERMS> struct MxGradLds {
-    static constexpr int frag = JS * TERMS * CT * 1024, codes = JS * 8 * 1024, scales = JS * 2 * 256, stage = frag + codes + scales;
+    static constexpr int frag = JS * TERMS * CT * 1024, codes = JS * 8 * 1024, scales = JS * 2 * 256, wstage = codes + scales, total = 2 * frag + 3 * wstage;
 };
 template <typename T, int CT, int JS>
 __global__ __launch_bounds__(256, 2) void mx_grad_tile_kernel(const unsigned short* __restrict__ frag, int64_t tiles, const unsigned char* __restrict__ wc,
-                                                             const unsigned char* __restrict__ ws, int64_t N, int64_t K, MxOut<T> w, int64_t mt,
-                                                             int64_t nt, int split) {
+                                                             const unsigned char* __restrict__ ws, int64_t N, int64_t K, MxOut<T> w, int mt, int nt, int split) {
     constexpr int TERMS = MxTerms<T>::v, CH = JS * TERMS * CT;
+    constexpr bool AHEAD = TERMS == 1 && JS % 2 == 0;
     typedef MxGradLds<CT, JS, TERMS> L;
     const int64_t ksteps = mx_steps(K), quads = mx_quads(K), rts = mx_row_tiles(N);
     const MxTile tile = mx_tile(blockIdx.x, mt, nt, split);
     if (tile.a < 0) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
-    const int64_t k0 = tile.b * 512 + wave * 128;
+    const int lane = threadIdx.x & 63, wave = mx_wave(), l = lane & 15, g = lane >> 4;
+    const int64_t k0 = (int64_t)tile.b * 512 + wave * 128;
     const int64_t steps = (N + 31) / 32, per = ((steps + split - 1) / split + JS - 1) / JS * JS;
     const int64_t s0 = per * tile.z, s1 = s0 + per < steps ? s0 + per : steps;
     extern __shared__ __attribute__((aligned(16))) unsigned char glds[];
-    auto stage = [&](int64_t s, int b) {
-        unsigned char* at = glds + b * L::stage;
+    // running addresses of the next stage: scalar, advanced by a constant
+    const unsigned char* fp = (const unsigned char*)frag + (s0 * TERMS * tiles + (int64_t)tile.a * CT) * 1024;
+    const int64_t fterm = tiles * 1024, wtile = ksteps * 1024, stile = quads * 256;
+    const unsigned char* wp = wc + (s0 * 2 * ksteps + ((int64_t)tile.b * 4 + wave < ksteps ? (int64_t)tile.b * 4 + wave : ksteps - 1)) * 1024;
+    const unsigned char* sp = ws + ((s0 * 2 + (wave < JS * 2 ? wave : 0)) * quads + tile.b) * 256;
+    // row tiles from the next stage on.  Those behind the last one: its codes again, whose factors in dy are zero; their scales must not be a
+    // NaN, so they are taken from those very zeros, the half fragments of dy
+    int64_t left = rts - s0 * 2;
+    const unsigned char* zp = (const unsigned char*)frag + ((s0 + (wave >> 1)) * TERMS * tiles + (int64_t)tile.a * CT) * 1024 + (wave & 1) * 512;
+    const int wlane[2] = {g * 256 + (l ^ g) * 16, g * 256 + (l ^ (g | 4)) * 16};
+    auto stage_frag = [&](int at) {
 #pragma unroll
         for (int c = 0; c < (CH + 3) / 4; ++c) {
             const int i = c * 4 + wave;
             if (CH % 4 == 0 || i < CH)
-                __builtin_amdgcn_global_load_lds((mx_gptr)(frag + ((s * TERMS + i / CT) * tiles + tile.a * CT + i % CT) * 512 + lane * 8),
-                                                 (mx_lptr)(at + i * 1024), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((mx_gptr)(fp + (i / CT) * fterm + (i % CT) * 1024 + lane * 16), (mx_lptr)(glds + at + i * 1024), 16, 0, 0);
         }
-#pragma unroll
-        for (int p = 0; p < JS * 2; ++p) {                     // the wave's step of each row tile (tiles and steps behind the last repeat it)
-            const int64_t rt = s * 2 + p < rts ? s * 2 + p : rts - 1, st = tile.b * 4 + wave < ksteps ? tile.b * 4 + wave : ksteps - 1;
-            __builtin_amdgcn_global_load_lds((mx_gptr)(wc + (rt * ksteps + st) * 1024 + g * 256 + ((l ^ (g | 4 * (p & 1))) * 16)),
-                                             (mx_lptr)(at + L::frag + (p * 4 + wave) * 1024), 16, 0, 0);
-        }
-        if (wave < JS * 2 && lane < 16) {
-            const int64_t rt = s * 2 + wave < rts ? s * 2 + wave : rts - 1;
-            __builtin_amdgcn_global_load_lds((mx_gptr)(ws + (rt * quads + tile.b) * 256 + lane * 16), (mx_lptr)(at + L::frag + L::codes + wave * 256), 16, 0, 0);
-        }
+        fp += JS * TERMS * fterm;
     };
-    mx_f4 acc[8][CT] = {};
-    if (s0 < s1) stage(s0, 0);
-    __syncthreads();
-    int b = 0;
+    auto stage_w = [&](int at) {
+#pragma unroll
+        for (int p = 0; p < JS * 2; ++p)                       // the wave's step of each row tile
+            __builtin_amdgcn_global_load_lds((mx_gptr)(wp + (p < left ? p : left - 1) * wtile + wlane[p & 1]), (mx_lptr)(glds + at + (p * 4 + wave) * 1024), 16,
+                                             0, 0);
+        if (wave < JS * 2 && lane < 16)
+            __builtin_amdgcn_global_load_lds((mx_gptr)((wave < left ? sp : zp) + lane * 16), (mx_lptr)(glds + at + L::codes + wave * 256), 16, 0, 0);
+        wp += JS * 2 * wtile;
+        sp += JS * 2 * stile;
+        zp += JS * TERMS * fterm;
+        left -= JS * 2;
+    };
     // row 8 g + j of a step is row 8 (g % 2) + j of row tile g / 2
     const int blk = l >> 2, mask = blk | 4 * (g >> 1);
-    const int qat = L::frag + ((g >> 1) * 4 + wave) * 1024 + blk * 256 + (g & 1) * 128 + (l & 3) * 4;
-    const int sat = L::frag + L::codes + (g >> 1) * 256 + blk * 64 + (g & 1) * 32 + wave;
+    int qat[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) qat[j] = ((g >> 1) * 4 + wave) * 1024 + blk * 256 + (g & 1) * 128 + (l & 3) * 4 + ((j ^ mask) * 16);
+    const int sat = L::codes + (g >> 1) * 256 + blk * 64 + (g & 1) * 32;
+    mx_f4 acc[8][CT] = {};
+    int f0 = 0, f1 = L::frag, w0 = 2 * L::frag, w1 = w0 + L::wstage, w2 = w1 + L::wstage;
+    mx_bf8 a[2][8];
+    auto unpack_step = [&](int at, int jj, mx_bf8* to) {                    // the jj-th step of the stage at LDS offset at
+        unsigned int q[8];
+        mx_u4 d[2];
+        float sc[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = *reinterpret_cast<const unsigned int*>(glds + at + jj * 8192 + qat[j]);
+        d[0] = *reinterpret_cast<const mx_u4*>(glds + at + jj * 512 + sat);
+        d[1] = *reinterpret_cast<const mx_u4*>(glds + at + jj * 512 + sat + 16);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sc[j] = mx_scale_operand(d[j >> 2][j & 3], wave);
+        mx_unpack_across(q, sc, to);
+    };
+    if (s0 < s1) {
+        stage_frag(f0);
+        stage_w(w0);
+        if (left > 0) stage_w(w1);
+    }
+    __syncthreads();
+    if (AHEAD && s0 < s1) unpack_step(w0, 0, a[0]);
     for (int64_t s = s0; s < s1; s += JS) {
-        if (s + JS < s1) stage(s + JS, b ^ 1);
-        const unsigned char* at = glds + b * L::stage;
+        if (s + JS < s1) {
+            stage_frag(f1);
+            if (left > 0) stage_w(w2);
+        }
 #pragma unroll
-        for (int jj = 0; jj < JS; ++jj) {
-            if (JS > 1 && s + jj >= s1) break;
-            unsigned int q[8], sc[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                q[j] = *reinterpret_cast<const unsigned int*>(at + qat + jj * 8192 + ((j ^ mask) * 16));
-                sc[j] = at[sat + jj * 512 + j * 4];
-            }
-            if ((s + jj) * 32 + 32 > N) {
-                // rows behind the last one are zeros with a finite scale (their factor in dy is zero too, but must not meet a NaN)
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if ((s + jj) * 32 + g * 8 + j >= N) { q[j] = 0; sc[j] = 127; }
-            }
-            mx_bf8 a[8];
-            mx_unpack_across(q, sc, a);
+        for (int jj = 0; jj < JS; ++jj) {                      // (a step behind the last one: the fragments of dy are zeros)
+            const int cur = AHEAD ? jj & 1 : 0, nxt = cur ^ 1;
+            if (!AHEAD) unpack_step(w0, jj, a[0]);
+            else if (jj + 1 < JS) unpack_step(w0, jj + 1, a[nxt]);
+            else unpack_step(w1, 0, a[nxt]);
 #pragma unroll
             for (int u = 0; u < TERMS; ++u)
 #pragma unroll
                 for (int c = 0; c < CT; ++c) {
-                    const mx_bf8 f = *reinterpret_cast<const mx_bf8*>(at + ((jj * TERMS + u) * CT + c) * 1024 + lane * 16);
+                    const mx_bf8 f = *reinterpret_cast<const mx_bf8*>(glds + f0 + ((jj * TERMS + u) * CT + c) * 1024 + lane * 16);
 #pragma unroll
-                    for (int m = 0; m < 8; ++m) acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[m], f, acc[m][c], 0, 0, 0);
+                    for (int m = 0; m < 8; ++m) acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[cur][m], f, acc[m][c], 0, 0, 0);
                 }
+            if (AHEAD) mx_schedule<TERMS * CT, 8, 10, (80 + TERMS * CT * 8 - 1) / (TERMS * CT * 8)>();
         }
         __syncthreads();
-        b ^= 1;
+        { const int t = f0; f0 = f1; f1 = t; }
+        { const int t = w0; w0 = w1; w1 = w2; w2 = t; }
     }
 #pragma unroll
     for (int c = 0; c < CT; ++c)
@@ -670,7 +748,7 @@ __global__ __launch_bounds__(256, 2) void mx_grad_tile_kernel(const unsigned sho
             float o[8];
 #pragma unroll
             for (int m = 0; m < 8; ++m) o[m] = acc[m][c][e];
-            mx_store<T, 8>(w, tile.z, (tile.a * CT + c) * 16 + l, k0 + 8 * (4 * g + e), o);
+            mx_store<T, 8>(w, tile.z, ((int64_t)tile.a * CT + c) * 16 + l, k0 + 8 * (4 * g + e), o);
         }
 }
 
@@ -687,7 +765,7 @@ __global__ __launch_bounds__(64 * WAVES) void mx_matmul_row_kernel(const unsigne
     constexpr int U = 4;
     const int64_t ksteps = mx_steps(K), quads = mx_quads(K), rts = mx_row_tiles(N);
     const int64_t n0 = (int64_t)blockIdx.x * 16 * RT;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = mx_wave(), l = lane & 15, g = lane >> 4;
     const unsigned char *pc[RT], *ps[RT], *pa = ac + lane * 16, *pas = as + lane * 4;      // (one row tile)
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
@@ -741,12 +819,12 @@ __global__ __launch_bounds__(64 * WAVES) void mx_matmul_row_kernel(const unsigne
 template <typename T, int CT, int RT>
 __global__ __launch_bounds__(256, 2) void mx_matmul_tile_kernel(const unsigned char* __restrict__ ac, const unsigned char* __restrict__ as,
                                                                const unsigned char* __restrict__ bc, const unsigned char* __restrict__ bs, int64_t N,
-                                                               int64_t K, MxOut<T> w, int64_t mt, int64_t nt, int split) {
+                                                               int64_t K, MxOut<T> w, int mt, int nt, int split) {
     constexpr int CH = CT * 2 / 4;                                         // fragments a wave and stage
     const int64_t ksteps = mx_steps(K), quads = mx_quads(K), mts = mx_row_tiles(w.M), nts = mx_row_tiles(N);
     const MxTile tile = mx_tile(blockIdx.x, mt, nt, split);
     if (tile.a < 0) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = mx_wave(), l = lane & 15, g = lane >> 4;
     const int64_t steps = ksteps / 2, per = ((steps + split - 1) / split + 1) / 2 * 2;     // stages
     const int64_t s0 = per * tile.z, s1 = s0 + per < steps ? s0 + per : steps;
     __shared__ __attribute__((aligned(16))) unsigned char lds[2][CT * 2 * 1024];           // [step][row tile][lane]
@@ -755,14 +833,14 @@ __global__ __launch_bounds__(256, 2) void mx_matmul_tile_kernel(const unsigned c
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int i = c * 4 + wave;
-        const int64_t rt = tile.a * CT + i % CT < mts ? tile.a * CT + i % CT : mts - 1;
+        const int64_t rt = (int64_t)tile.a * CT + i % CT < mts ? (int64_t)tile.a * CT + i % CT : mts - 1;
         xb[c] = ac + (rt * ksteps + i / CT) * 1024;
     }
 #pragma unroll
-    for (int c = 0; c < CT; ++c) xsb[c] = as + (tile.a * CT + c < mts ? tile.a * CT + c : mts - 1) * quads * 256;
+    for (int c = 0; c < CT; ++c) xsb[c] = as + ((int64_t)tile.a * CT + c < mts ? (int64_t)tile.a * CT + c : mts - 1) * quads * 256;
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-        int64_t rt = (tile.b * 4 + wave) * RT + i;
+        int64_t rt = ((int64_t)tile.b * 4 + wave) * RT + i;
         rt = rt < nts ? rt : nts - 1;
         qb[i] = bc + rt * ksteps * 1024;
         sb[i] = bs + rt * quads * 256;
@@ -836,7 +914,7 @@ __global__ __launch_bounds__(256, 2) void mx_matmul_tile_kernel(const unsigned c
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
             float o[4] = {acc[i][c][0], acc[i][c][1], acc[i][c][2], acc[i][c][3]};
-            mx_store<T, 4>(w, tile.z, (tile.a * CT + c) * 16 + l, ((tile.b * 4 + wave) * RT + i) * 16 + 4 * g, o);
+            mx_store<T, 4>(w, tile.z, ((int64_t)tile.a * CT + c) * 16 + l, (((int64_t)tile.b * 4 + wave) * RT + i) * 16 + 4 * g, o);
         }
 }
 

@@ -107,6 +107,12 @@ int         lcx_device_count(int* out_count);
  * operand along its preferred axis.  lcx_kernel_name(h, 0 | 1 | 2, ..) names the kernels in use; lcx_bytes_resident reports the bytes. */
 int lcx_create(lcx_ctx** out, int64_t n_samples, int64_t nv_local, int n_hidden,
                int dtype, int device);
+/* The same with a choice of how the shard is held: x_storage 0 = as lcx_create, 1 = in 4 bits per value (lcx_x_layout 3; the format of
+ * lcx_mx4_quantize below, blocks of 32 variables of a sample, and one float32 factor per variable that keeps its mean square 1 after the
+ * rounding): 4.25 bits instead of 32, so that 7.5 times larger shards fit and both X passes read that much less.  What is fitted is the
+ * rounded matrix (lcx_download_x returns it); with it every pass is exact up to float32 sums.  LCX_F32 and n_hidden <= 128 only.
+ * Everything else of the handle is the same; transform of new rows (lcx_project*) does not touch the shard. */
+int lcx_create_stored(lcx_ctx** out, int64_t n_samples, int64_t nv_local, int n_hidden, int dtype, int device, int x_storage);
 int lcx_destroy(lcx_ctx* h);
 /* stream all work is enqueued on (a hipStream_t); NULL = the handle's own stream. */
 int lcx_set_stream(lcx_ctx* h, void* hip_stream);
@@ -354,7 +360,8 @@ int lcx_bytes_resident(lcx_ctx* h, int64_t* total, int64_t* x_bytes);
  *   2  ONE panel-major copy [n_variables / P][n_samples][P], P = 64 bytes of a row: large shards, both X passes (:247, :259) on the
  *      stream-K kernels at full speed from the same bytes (LCX_X_LAYOUT=panel forces it, =rows forbids it);
  *   0  row-major + a transposed copy: small shards (each pass reads the copy whose contiguous axis it does not contract);
- *   1  row-major only: models with more than 256 factors, or LCX_SINGLE_COPY=1. */
+ *   1  row-major only: models with more than 256 factors, or LCX_SINGLE_COPY=1;
+ *   3  4 bits per value (lcx_create_stored). */
 int lcx_x_layout(lcx_ctx* h, int* layout);
 /* Arithmetic of the two X-streaming contractions (:247 / :210 x.dot(ws.T), :259 / :211 x.T.dot(y)) of a FLOAT32 shard in the
  * panel-major layout; switchable at any time between two launches, results of both modes within float32 rounding of each other:

@@ -33,6 +33,7 @@ SIGNATURES = {
     "lcx_last_error": [],
     "lcx_device_count": [C.POINTER(_i32)],
     "lcx_create": [C.POINTER(_vp), _i64, _i64, _i32, _i32, _i32],
+    "lcx_create_stored": [C.POINTER(_vp), _i64, _i64, _i32, _i32, _i32, _i32],
     "lcx_destroy": [_vp],
     "lcx_set_stream": [_vp, _vp],
     "lcx_synchronize": [_vp],

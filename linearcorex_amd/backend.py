@@ -27,15 +27,18 @@ MOMENT_KEYS = {
 
 
 class HipBackend:
-    def __init__(self, n_samples, nv_local, n_hidden, dtype=np.float32, device=0, lib=None):
+    X_STORAGE = {"dense": 0, "mx4": 1}
+
+    def __init__(self, n_samples, nv_local, n_hidden, dtype=np.float32, device=0, lib=None, x_storage="dense"):
         # lib: another build of the same ABI (tools/liblcx_probe.so, the lab: the engine plus kernel test hooks)
         self.lib = lib if lib is not None else _abi.load()
         self.dtype = np.dtype(dtype)
         self.n_samples, self.nv, self.m = int(n_samples), int(nv_local), int(n_hidden)
         self.device = int(device)
         h = C.c_void_p()
-        _abi.check(self.lib.lcx_create(C.byref(h), self.n_samples, self.nv, self.m,
-                                       _abi.dtype_code(self.dtype), self.device))
+        _abi.check(self.lib.lcx_create_stored(C.byref(h), self.n_samples, self.nv, self.m, _abi.dtype_code(self.dtype), self.device,
+                                              self.X_STORAGE[x_storage]))
+        self.x_storage = x_storage
         self.h = h
         self._ex = None            # torch exchange tensors when sharded
         self.torch_stream = None
@@ -446,7 +449,8 @@ class HipBackend:
         lay = C.c_int()
         _abi.check(self.lib.lcx_x_layout(self.h, C.byref(lay)))
         return {"total": tot.value, "x": xb.value,
-                "x_layout": {0: "row-major + transposed copy", 1: "row-major", 2: "panel-major (one copy)"}[lay.value]}
+                "x_layout": {0: "row-major + transposed copy", 1: "row-major", 2: "panel-major (one copy)",
+                             3: "4 bits per value"}[lay.value]}
 
     def predict(self, y, xz=None, syn=False, gaussianize=None, theta=None):
         """predict (linearcorex.py:440-441) for this shard: invert(y . X_i Z_j^T), (n_rows, nv_local).  xz: X_i Z_j

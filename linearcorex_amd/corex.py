@@ -301,6 +301,11 @@ class Corex(object):
               into three bf16 numbers, 6 of the 9 partial products on the bf16 matrix pipe with float32 accumulation: results
               within float32 rounding of "mfma", passes 1.3-1.5 x faster on large shards.  Taken only where the shard supports
               it (panel-major layout, 32 / 64 / 128 padded factors); `self.f32_gemm` tells which one the fit ran.
+      x_storage  how the data of a fit are held on the device: "dense" (the default) = in the working precision; "mx4" = in 4 bits per
+              value (`linearcorex_amd.mx4`; include/lcx.h, lcx_create_stored): 7.5 times less memory and traffic than float32, for
+              matrices that would not fit, or passes that would take too long.  The model is then fitted to the rounded data (about one
+              per cent of a variable's variance is rounding noise, so correlations come out that much weaker); products and sums are as
+              exact as those of a float32 fit.  float32 and n_hidden <= 128 only.  `transform` of new data is not affected.
     """
 
     # defaults for models pickled by an earlier build
@@ -308,11 +313,12 @@ class Corex(object):
     _engine_exchange = None
     _f32_gemm_asked = None
     f32_gemm = "mfma"
+    x_storage = "dense"
 
     def __init__(self, n_hidden=10, max_iter=10000, tol=1e-5, anneal=True, missing_values=None,
                  discourage_overlap=True, gaussianize='standard', gpu=False,
                  verbose=False, seed=None, *, dtype=np.float32, device=None, comm=None,
-                 eliminate_synergy=None, line_search=None, refresh_every=16, f32_gemm=None, _backend_factory=None):
+                 eliminate_synergy=None, line_search=None, refresh_every=16, f32_gemm=None, x_storage="dense", _backend_factory=None):
         if eliminate_synergy is not None:
             discourage_overlap = bool(eliminate_synergy)
         self.m = n_hidden
@@ -360,6 +366,13 @@ class Corex(object):
             raise ValueError("f32_gemm must be None, 'mfma' or 'split'")
         self._f32_gemm_asked = f32_gemm         # None: the library's default (float32 MFMA unless LCX_F32_GEMM=split)
         self.f32_gemm = "mfma"                  # what the fit ran, settled in _make_backend
+        if x_storage not in ("dense", "mx4"):
+            raise ValueError("x_storage must be 'dense' or 'mx4'")
+        if x_storage == "mx4" and (self.dtype != np.float32 or n_hidden is None or n_hidden > 128):
+            raise ValueError("x_storage='mx4' needs dtype float32 and n_hidden <= 128")
+        if x_storage == "mx4" and _backend_factory is not None:
+            raise ValueError("x_storage='mx4' is a form of the device's shard: not with _backend_factory")
+        self.x_storage = x_storage
         self.refresh_every = int(refresh_every)
         self._since_exact = 0
         self.stats = {"iterations": 0, "moment_evals": 0, "trials": 0, "invalid_trials": 0}
@@ -390,7 +403,7 @@ class Corex(object):
     # ------------------------------------------------------------------------------------------
     # backend plumbing
     # ------------------------------------------------------------------------------------------
-    def _make_backend(self, n_samples, nv_local, temporary=False):
+    def _make_backend(self, n_samples, nv_local, temporary=False, fit=True):
         """temporary: a short-lived handle beside the fit's own (transform(details=True) of a new batch): same transport, whose
         first-contact self-test the fit's handle has already passed"""
         if self._backend is not None:
@@ -403,7 +416,9 @@ class Corex(object):
             if dev is None:
                 import os
                 dev = int(os.environ.get("LOCAL_RANK", "0"))
-            be = HipBackend(n_samples, nv_local, self.m, self.dtype, dev)
+            # (a temporary handle holds a batch to be evaluated, a restored model no data at all: both dense)
+            storage = "dense" if temporary or not fit else self.x_storage
+            be = HipBackend(n_samples, nv_local, self.m, self.dtype, dev, x_storage=storage)
         self._backend = be
         exchange = getattr(self._comm, "exchange", self._comm.world > 1)
         be.set_world(self._comm.world)
@@ -513,9 +528,11 @@ class Corex(object):
         are not resident any more (a model restored from a pickle): call `transform(x)` then.
         details=True: `(y, moments)` as `transform(x_fit, details=True)` (:392-394) - the full moments of the fitted data under the
         final weights are what `fit` left in `self.moments` (:163), so nothing is evaluated and no second handle is built (at the size
-        of BASELINE configs[3] on one GPU a second resident copy of X would not fit)."""
+        of BASELINE configs[3] on one GPU a second resident copy of X would not fit).  None also with x_storage="mx4"."""
         be = self._backend
         if not getattr(self, "_x_resident", False) or be is None or not hasattr(be, "project_resident") or self.ws.size == 0:
+            return None
+        if self.x_storage != "dense":             # the resident data are rounded: not what `transform(x_fit)` returns
             return None
         if self.gaussianize == 'empirical':       # the reference's second preprocess of x says these again (:416-417, :425)
             print("Warning: correct inversion/transform of empirical gauss transform not implemented.")
@@ -1140,7 +1157,7 @@ class Corex(object):
             # resident any more, so the handle is created for a single (empty) sample: transform / get_covariance only
             # need W and the per-variable moments, not an n_samples x n_variables shard and its transposed copy
             self._cols = self._comm.shard(self.nv)
-            be = self._make_backend(1, self.nv)
+            be = self._make_backend(1, self.nv, fit=False)
             be.set_ws(np.asarray(self.ws, dtype=self.dtype))
             self._moments_restored = False
             self._x_resident = False

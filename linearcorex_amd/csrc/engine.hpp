@@ -11,6 +11,7 @@
 //                      (entry points; the typed work - most of the compile time - in lcx_levels_f32.hip / lcx_levels_f64.hip)
 //     lcx_data.hip     upload + preprocess, the on-device generator, download, transform of new rows
 //     lcx_outputs.hip  get_covariance, predict, invert
+//     lcx_mx4.hip      matrices in 4 bits per value: the lcx_mx4_* operators, and a shard that is resident in that form
 // (empirical.hip: gaussianize='empirical'.)  One object per unit, compiled side by side (__graft_entry__.py).
 #pragma once
 #include <hip/hip_runtime.h>
@@ -191,6 +192,12 @@ struct lcx_ctx {
                                 // off by default (LCX_F32_GEMM=split / lcx_set_f32_gemm)
     void* bsp;                  // the small operand of a pass in split form (split_b_kernel), 6 bytes per element
     size_t bsp_bytes;
+    // lcx_create_stored, x_storage 1: the shard in 4 bits per value (lcx_mx4.hip) instead of X / XT: codes, scales, one factor per variable
+    bool mx4;
+    void *xq, *xs, *xwork;
+    float* xunit;
+    size_t xq_bytes;
+    int64_t xwork_bytes;
     void* Wt[2];
     MomentSet set[2];
     void *grad, *update, *sgrad, *scratch;
@@ -969,6 +976,15 @@ static int wait_published(lcx_ctx* h, MomentSet& s) {
 
 // the launch geometry of a handle (lcx_create): lives with the kernels it sizes, in lcx_levels.hip
 __attribute__((visibility("hidden"))) int lcx_engine_geometry(lcx_ctx* h);
+
+// the shard in 4 bits per value (lcx_mx4.hip)
+#pragma GCC visibility push(hidden)
+int lcx_mx_shard_alloc(lcx_ctx* h);
+int lcx_mx_shard_fill(lcx_ctx* h, float* stage, int64_t ld, int64_t c0, int64_t cols);
+int lcx_mx_shard_read(lcx_ctx* h, float* stage, int64_t ld, int64_t c0, int64_t cols);
+int lcx_mx_shard_xbt(lcx_ctx* h, const float* B, float* out, const int* skip);
+int lcx_mx_shard_xty(lcx_ctx* h, const float* Y, float* out, const int* skip);
+#pragma GCC visibility pop
 
 // the member definitions of Impl<T, CT>, along the seams of the C ABI
 #include "impl_levels.hpp"

@@ -4,7 +4,7 @@
 
 template <typename T, int CT>
 int Impl<T, CT>::make_xt(lcx_ctx* h) {
-    if (h->single_copy || h->panel) { HIPCHECK(hipStreamSynchronize(h->stream)); return LCX_OK; }
+    if (h->single_copy || h->panel || h->mx4) { HIPCHECK(hipStreamSynchronize(h->stream)); return LCX_OK; }
     dim3 grid((unsigned)(h->ldx / 64), (unsigned)(h->Npad / 64));
     hipLaunchKernelGGL((transpose_kernel<T>), grid, dim3(256), 0, h->stream, P<T>(h->X), h->ldx, P<T>(h->XT), h->Npad);
     KCHECK();
@@ -167,10 +167,11 @@ int Impl<T, CT>::preprocess_view(lcx_ctx* h, T* X, const int64_t V, const int64_
 // ld, zeroed beforehand: that is the padding); the block is then scattered into its panels.  <= 2^28 staged elements.
 template <typename T, int CT>
 int64_t Impl<T, CT>::panel_block_cols(const lcx_ctx* h) {
-    int64_t w = (((int64_t)1 << 28) / h->Npad) / 64 * 64;
+    const int64_t unit = h->mx4 ? 512 : 64;                         // (4 bits: whole dwords of scales)
+    int64_t w = (((int64_t)1 << 28) / h->Npad) / unit * unit;
     const int forced = env_int("LCX_PANEL_BLOCK_COLS", 0);          // test hook: several blocks at small sizes
-    if (forced > 0) w = (int64_t)forced / 64 * 64;
-    if (w < 64) w = 64;
+    if (forced > 0) w = (int64_t)forced / unit * unit;
+    if (w < unit) w = unit;
     return w > h->ldx ? h->ldx : w;
 }
 
@@ -186,6 +187,10 @@ int Impl<T, CT>::panel_fill(lcx_ctx* h, F fill) {
         const int64_t wv = h->V - c0 < 0 ? 0 : (h->V - c0 < wp ? h->V - c0 : wp);
         HIPCHECK(hipMemsetAsync(stage, 0, sizeof(T) * (size_t)h->Npad * W, h->stream));
         if (wv > 0) LCXCHECK(fill(stage, W, c0, wv));
+        if (h->mx4) {
+            if constexpr (sizeof(T) == 4) LCXCHECK(lcx_mx_shard_fill(h, stage, W, c0, wp));
+            continue;
+        }
         hipLaunchKernelGGL((panel_block_kernel<T, true>), dim3(4096), dim3(256), 0, h->stream, stage, W, P<T>(h->X), h->Npad * PanelW<T>::v,
                            h->Npad, c0, wp);
         KCHECK();
@@ -196,7 +201,7 @@ int Impl<T, CT>::panel_fill(lcx_ctx* h, F fill) {
 
 template <typename T, int CT>
 int Impl<T, CT>::upload_x(lcx_ctx* h, const void* x, int64_t ld) {
-    if (!h->panel) {
+    if (!h->panel && !h->mx4) {
         HIPCHECK(hipMemcpy2DAsync(h->X, h->ldx * sizeof(T), x, ld * sizeof(T), h->V * sizeof(T), h->N, hipMemcpyHostToDevice, h->stream));
         HIPCHECK(hipStreamSynchronize(h->stream));
         return make_xt(h);
@@ -211,7 +216,7 @@ int Impl<T, CT>::upload_x(lcx_ctx* h, const void* x, int64_t ld) {
 
 template <typename T, int CT>
 int Impl<T, CT>::download_x(lcx_ctx* h, void* x, int64_t ld) {
-    if (!h->panel) {
+    if (!h->panel && !h->mx4) {
         HIPCHECK(hipMemcpy2DAsync(x, ld * sizeof(T), h->X, h->ldx * sizeof(T), h->V * sizeof(T), h->N, hipMemcpyDeviceToHost, h->stream));
         HIPCHECK(hipStreamSynchronize(h->stream));
         return LCX_OK;
@@ -223,9 +228,13 @@ int Impl<T, CT>::download_x(lcx_ctx* h, void* x, int64_t ld) {
     for (int64_t c0 = 0; c0 < h->V; c0 += W) {
         const int64_t wp = (h->ldx - c0) < W ? (h->ldx - c0) : W;
         const int64_t wv = h->V - c0 < wp ? h->V - c0 : wp;
-        hipLaunchKernelGGL((panel_block_kernel<T, false>), dim3(4096), dim3(256), 0, h->stream, stage, W, P<T>(h->X), h->Npad * PanelW<T>::v,
-                           h->Npad, c0, wp);
-        KCHECK();
+        if (h->mx4) {
+            if constexpr (sizeof(T) == 4) LCXCHECK(lcx_mx_shard_read(h, stage, W, c0, wp));
+        } else {
+            hipLaunchKernelGGL((panel_block_kernel<T, false>), dim3(4096), dim3(256), 0, h->stream, stage, W, P<T>(h->X), h->Npad * PanelW<T>::v,
+                               h->Npad, c0, wp);
+            KCHECK();
+        }
         HIPCHECK(hipMemcpy2DAsync(reinterpret_cast<T*>(x) + c0, ld * sizeof(T), stage, W * sizeof(T), wv * sizeof(T), h->N, hipMemcpyDeviceToHost,
                                   h->stream));
         HIPCHECK(hipStreamSynchronize(h->stream));
@@ -236,7 +245,7 @@ int Impl<T, CT>::download_x(lcx_ctx* h, void* x, int64_t ld) {
 template <typename T, int CT>
 int Impl<T, CT>::upload_preprocess(lcx_ctx* h, const void* x, int64_t ld, int kind, int has_missing, double sentinel, int fit,
     void* mean_io, void* std_io, int64_t* nobs_out, double* maxabs_out) {
-    if (!h->panel) {
+    if (!h->panel && !h->mx4) {
         HIPCHECK(hipMemcpy2DAsync(h->X, h->ldx * sizeof(T), x, ld * sizeof(T), h->V * sizeof(T), h->N, hipMemcpyHostToDevice, h->stream));
         LCXCHECK(preprocess_resident(h, kind, has_missing, sentinel, fit, mean_io, std_io, nobs_out, maxabs_out));
         return make_xt(h);
@@ -303,7 +312,7 @@ int Impl<T, CT>::project_raw(lcx_ctx* h, const void* x_host, int64_t n_rows, int
 
 template <typename T, int CT>
 int Impl<T, CT>::generate(lcx_ctx* h, uint64_t seed, int kind, int n_groups, int64_t col_offset) {
-    if (h->panel)          // the generator is keyed by (seed, row, global column): block by block gives the same matrix
+    if (h->panel || h->mx4)          // the generator is keyed by (seed, row, global column): block by block gives the same matrix
         return panel_fill(h, [&](T* stage, int64_t lds, int64_t c0, int64_t wv) -> int {
             hipLaunchKernelGGL((generate_kernel<T>), dim3(4096), dim3(256), 0, h->stream, stage, h->N, wv, lds, seed, kind,
                                n_groups < 1 ? 1 : n_groups, col_offset + c0);

@@ -211,6 +211,11 @@ int Impl<T, CT>::geometry_tuned(lcx_ctx* h) {
         h->gn_S = pick_split(Mp / (16 * Geo<T, CT>::G_RT), pick_kw(kgn), kgn, h->target_waves / (gdiv > 0 ? gdiv : 1), gcap);
         h->gv_S = pick_split(Mp / (16 * Geo<T, CT>::G_RT), pick_kw(kgv), kgv, h->target_waves / (gdiv > 0 ? gdiv : 1), gcap);
     }
+    if (h->mx4) {
+        // the 4-bit passes add their partial sums up themselves: one slot each, and none of the float32 kernels or layouts
+        h->nt_S = h->tn_S = 1;
+        h->nt_ct = h->tn_ct = h->panel = h->single_copy = h->merged_ok = h->f64_4x4 = false;
+    }
     int64_t groups = cdiv(h->V, VPB);
     h->pv_grid = (int)(groups < 1024 ? (groups < 1 ? 1 : groups) : 1024);
     // many slots (few column tiles): one wide reduction after the pass instead of a long serial sum per element in
@@ -255,7 +260,9 @@ int Impl<T, CT>::nt_pass(lcx_ctx* h, const T* B, const int* skip, T* dst, int64_
                                                                              dst + r0 * Mp, h->nt_S, h->nt_KW, skip, h->Npad)));
             return LCX_OK;
         }
-        if (h->panel)
+        if (h->mx4) {
+            if constexpr (sizeof(T) == 4) LCXCHECK(lcx_mx_shard_xbt(h, B, dst, skip));
+        } else if (h->panel)
             LCXCHECK((launch_cr<T, CT, true>(h->stream, P<T>(h->X), h->Npad * PanelW<T>::v, h->ldx, h->Npad, B, dst, h->nt_nb, h->nt_nsuper,
                                              h->nt_S, skip, h->split ? h->bsp : nullptr, h->n_cus)));
         else if (h->single_copy)
@@ -466,7 +473,9 @@ int Impl<T, CT>::tn_big(lcx_ctx* h, const int* skip) {
     if constexpr (WIDE) {
         LCXCHECK((wide_gemm<true, false>(h, P<T>(h->X), h->ldx, P<T>(h->ybuf), Mp, nullptr, P<T>(h->dpart), Mp, h->ldx, Mp, h->Npad, 1, skip)));
     } else {
-        if (h->panel)
+        if (h->mx4) {
+            if constexpr (sizeof(T) == 4) LCXCHECK(lcx_mx_shard_xty(h, P<T>(h->ybuf), P<T>(h->dpart), skip));
+        } else if (h->panel)
             LCXCHECK((launch_ct<T, CT, true>(h->stream, P<T>(h->X), h->Npad * PanelW<T>::v, h->Npad, h->ldx, P<T>(h->ybuf), P<T>(h->dpart),
                                              h->tn_nb, h->tn_nsuper, h->tn_S, skip, h->split ? h->bsp : nullptr, h->n_cus)));
         else if (h->tn_ct)
@@ -1278,6 +1287,12 @@ int Impl<T, CT>::kernel_name(lcx_ctx* h, int kind, char* buf, int64_t len) {
 
 template <typename T, int CT>
 int Impl<T, CT>::kernel_name_tuned(lcx_ctx* h, int kind, char* buf, int64_t len) {
+    if (h->mx4) {
+        if (kind == 2) buf[0] = 0;
+        else if (kind == 0) snprintf(buf, (size_t)len, "lcx::mx_linear_tile_kernel<float, %d, 4, %d>", CT > 4 ? 4 : CT, CT >= 4 ? 2 : 4);
+        else snprintf(buf, (size_t)len, "lcx::mx_grad_tile_kernel<float, %d, 1>", CT > 4 ? 4 : CT);
+        return LCX_OK;
+    }
     if (h->split) {
         if (kind == 2 && (!h->merged_ok || h->merged_agreed == 0)) { buf[0] = 0; return LCX_OK; }   // the group agreed not to take it
         const int ct = kind == 2 ? 2 * CT : CT;

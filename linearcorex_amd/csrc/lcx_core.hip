@@ -16,6 +16,13 @@ int lcx_device_count(int* out_count) {
 }
 
 int lcx_create(lcx_ctx** out, int64_t n_samples, int64_t nv_local, int n_hidden, int dtype, int device) {
+    return lcx_create_stored(out, n_samples, nv_local, n_hidden, dtype, device, 0);
+}
+
+int lcx_create_stored(lcx_ctx** out, int64_t n_samples, int64_t nv_local, int n_hidden, int dtype, int device, int x_storage) {
+    if (x_storage != 0 && x_storage != 1) return fail(LCX_ERR_ARG, "lcx_create_stored: x_storage must be 0 (dense) or 1 (4 bits per value)");
+    if (x_storage == 1 && (dtype != LCX_F32 || n_hidden > 128))
+        return fail(LCX_ERR_ARG, "lcx_create_stored: 4 bits per value need LCX_F32 and at most 128 factors");
     if (!out || n_samples < 1 || nv_local < 1 || n_hidden < 1) return fail(LCX_ERR_ARG, "lcx_create: bad sizes");
     if (dtype != LCX_F32 && dtype != LCX_F64) return fail(LCX_ERR_ARG, "lcx_create: dtype must be LCX_F32 or LCX_F64");
     const int ct = ct_for(n_hidden);
@@ -28,6 +35,9 @@ int lcx_create(lcx_ctx** out, int64_t n_samples, int64_t nv_local, int n_hidden,
     HIPCHECK(hipGetDeviceProperties(&prop, device));
 
     lcx_ctx* h = new lcx_ctx();
+    h->mx4 = x_storage == 1;
+    h->xq = h->xs = h->xwork = nullptr;
+    h->xunit = nullptr;
     h->split = false;
     h->bsp = nullptr;
     h->bsp_bytes = 0;
@@ -80,8 +90,13 @@ int lcx_create(lcx_ctx** out, int64_t n_samples, int64_t nv_local, int n_hidden,
     const int Mp = h->Mp;
     // a failed allocation releases everything allocated so far (lcx_destroy copes with a half-built handle)
 #define A_(ptr, bytes) do { const size_t b_ = (bytes); int r_ = dev_alloc((void**)&(ptr), b_, st); if (r_ != LCX_OK) { (void)lcx_destroy(h); return r_; } h->bytes_resident += b_ ? b_ : 16; } while (0)
-    A_(h->X, (size_t)h->Npad * h->ldx * es);
-    if (!h->single_copy && !h->panel) A_(h->XT, (size_t)h->Npad * h->ldx * es);
+    if (h->mx4) {
+        rc = lcx_mx_shard_alloc(h);
+        if (rc != LCX_OK) { (void)lcx_destroy(h); return rc; }
+    } else {
+        A_(h->X, (size_t)h->Npad * h->ldx * es);
+    }
+    if (!h->single_copy && !h->panel && !h->mx4) A_(h->XT, (size_t)h->Npad * h->ldx * es);
     for (int k = 0; k < 2; ++k) {
         A_(h->Wt[k], mv);
         A_(h->set[k].Y, (size_t)h->Npad * Mp * es);
@@ -157,6 +172,7 @@ int lcx_create(lcx_ctx** out, int64_t n_samples, int64_t nv_local, int n_hidden,
             h->ypipe_signal = signal && h->ypipe > 1;
             h->ypipe_poll = signal && f && !strcmp(f, ":poll");
         }
+        if (h->mx4) h->ypipe = 0;             // (row chunks exist for the dense passes only)
     }
 #undef A_
     h->set[0].st = h->states;
@@ -210,7 +226,7 @@ int lcx_destroy(lcx_ctx* h) {
         (void)hipFree(h->sig_counters);
         for (auto& f : h->sig_flag) if (f) (void)hipFree(f);
     }
-    void* ptrs[] = {h->X, h->XT, h->Wt[0], h->Wt[1], h->grad, h->update, h->sgrad, h->scratch, h->ydir, h->ddir, h->ybuf_own, h->sbuf_own,
+    void* ptrs[] = {h->X, h->XT, h->xq, h->xs, h->xwork, h->xunit, h->Wt[0], h->Wt[1], h->grad, h->update, h->sgrad, h->scratch, h->ydir, h->ddir, h->ybuf_own, h->sbuf_own,
                     h->gw, h->y2part, h->bjg, h->bsp,
                     h->ypart, h->dpart, h->gpart, h->gpartw, h->tcpart, h->bjpart, h->tanpart, h->detpart, h->ryinv, h->invwork,
                     h->states, h->order_dev, h->ticket};
@@ -528,7 +544,7 @@ int lcx_read_sbuf(lcx_ctx* h, int64_t offset, int64_t count, double* out) {
 int lcx_x_layout(lcx_ctx* h, int* layout) {
     NEED(h);
     if (!layout) return fail(LCX_ERR_ARG, "lcx_x_layout: null");
-    *layout = h->panel ? 2 : (h->single_copy ? 1 : 0);
+    *layout = h->mx4 ? 3 : h->panel ? 2 : (h->single_copy ? 1 : 0);
     return LCX_OK;
 }
 
@@ -542,7 +558,7 @@ int lcx_f32_gemm(lcx_ctx* h, int* mode) {
 int lcx_bytes_resident(lcx_ctx* h, int64_t* total, int64_t* x_bytes) {
     NEED(h);
     if (total) *total = (int64_t)h->bytes_resident;
-    if (x_bytes) *x_bytes = (int64_t)((h->single_copy || h->panel ? 1 : 2) * (size_t)h->Npad * h->ldx * h->es);
+    if (x_bytes) *x_bytes = h->mx4 ? (int64_t)h->xq_bytes : (int64_t)((h->single_copy || h->panel ? 1 : 2) * (size_t)h->Npad * h->ldx * h->es);
     return LCX_OK;
 }
 

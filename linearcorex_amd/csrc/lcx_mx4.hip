@@ -43,8 +43,10 @@ static int mx4_quantize(const void* x, int64_t rows, int64_t cols, int64_t rs, i
         hipLaunchKernelGGL((mx_quantize_across_kernel<T>), dim3(g), dim3(512), 0, st, (const T*)x, rows, cols, cs, qc, qs);
     } else {
         LCXCHECK(mx_grid(mx_row_tiles(rows), mx_quads(cols), &g));
-        if (cs == 1) hipLaunchKernelGGL((mx_quantize_kernel<T, true>), dim3(g), dim3(256), 0, st, (const T*)x, rows, cols, rs, cs, qc, qs);
-        else hipLaunchKernelGGL((mx_quantize_kernel<T, false>), dim3(g), dim3(256), 0, st, (const T*)x, rows, cols, rs, cs, qc, qs);
+        if (cs == 1) hipLaunchKernelGGL((mx_quantize_kernel<T, true>), dim3(g), dim3(256), 0, st, (const T*)x, rows, cols, rs, cs, qc, qs,
+                                        mx_steps(cols), mx_quads(cols), (int64_t)0, (unsigned)mx_quads(cols));
+        else hipLaunchKernelGGL((mx_quantize_kernel<T, false>), dim3(g), dim3(256), 0, st, (const T*)x, rows, cols, rs, cs, qc, qs, mx_steps(cols),
+                                mx_quads(cols), (int64_t)0, (unsigned)mx_quads(cols));
     }
     KCHECK();
     return LCX_OK;
@@ -59,8 +61,10 @@ static int mx4_dequantize(const void* codes, const void* scales, int64_t rows, i
         hipLaunchKernelGGL((mx_dequantize_across_kernel<T>), dim3(g), dim3(512), 0, st, qc, qs, rows, cols, (T*)out, cs);
     } else {
         LCXCHECK(mx_grid(mx_row_tiles(rows), mx_quads(cols), &g));
-        if (cs == 1) hipLaunchKernelGGL((mx_dequantize_kernel<T, true>), dim3(g), dim3(256), 0, st, qc, qs, rows, cols, (T*)out, rs, cs);
-        else hipLaunchKernelGGL((mx_dequantize_kernel<T, false>), dim3(g), dim3(256), 0, st, qc, qs, rows, cols, (T*)out, rs, cs);
+        if (cs == 1) hipLaunchKernelGGL((mx_dequantize_kernel<T, true>), dim3(g), dim3(256), 0, st, qc, qs, rows, cols, (T*)out, rs, cs, mx_steps(cols),
+                                        mx_quads(cols), (int64_t)0, (unsigned)mx_quads(cols));
+        else hipLaunchKernelGGL((mx_dequantize_kernel<T, false>), dim3(g), dim3(256), 0, st, qc, qs, rows, cols, (T*)out, rs, cs, mx_steps(cols),
+                                mx_quads(cols), (int64_t)0, (unsigned)mx_quads(cols));
     }
     KCHECK();
     return LCX_OK;
@@ -97,11 +101,19 @@ static int64_t split_for(int64_t tiles, int64_t steps, int64_t slots, double fix
     return best;
 }
 
+// what a fit adds to a product: a factor of every column of W (taken into x before it is split, or into the output), and the flag of a trial
+// that turned out invalid
+struct MxExtra {
+    const float *kscale = nullptr, *oscale = nullptr;
+    const int* skip = nullptr;
+    bool tiles = false;                // no row kernel
+};
+
 // M rows of x, C the contraction, O output columns; along: lcx_mx4_linear, else lcx_mx4_linear_grad
-template <typename T> static MxPlan mx_plan(bool along, int64_t M, int64_t C, int64_t O) {
+template <typename T> static MxPlan mx_plan(bool along, int64_t M, int64_t C, int64_t O, bool tiles = false) {
     constexpr int TERMS = MxTerms<T>::v;
     MxPlan p;
-    if (M <= 16 && along) {
+    if (M <= 16 && along && !tiles) {
         p.row = true;
         // 2 x 16 rows of W a wave halve the reads of x where there are enough rows to fill the chip; 16 waves split the contraction
         // where there are few
@@ -131,23 +143,30 @@ template <typename T> static int64_t mx_workspace(int op, int64_t M, int64_t N, 
 }
 
 template <typename T, bool ALONG>
-static int mx_fragments(const T* x, int64_t M, int64_t rs, int64_t cs, int64_t C, const MxPlan& p, unsigned short* frag, hipStream_t st) {
+static int mx_fragments(const T* x, int64_t M, int64_t rs, int64_t cs, int64_t C, const MxPlan& p, unsigned short* frag, const MxExtra& ex, hipStream_t st) {
     const int64_t tiles = p.mt * p.ct;
     unsigned g;
     LCXCHECK(mx_grid(tiles, cdiv(p.nfrag * 4, 16), &g));
     const int rows_first = (rs < 0 ? -rs : rs) < (cs < 0 ? -cs : cs);
     if (cs == 1)
-        hipLaunchKernelGGL((mx_fragments_kernel<T, ALONG, true>), dim3(g), dim3(256), 0, st, x, M, rs, cs, C, p.nfrag, tiles, frag, 0);
+        hipLaunchKernelGGL((mx_fragments_kernel<T, ALONG, true>), dim3(g), dim3(256), 0, st, x, M, rs, cs, C, p.nfrag, tiles, frag, 0, ex.kscale, ex.skip);
     else
-        hipLaunchKernelGGL((mx_fragments_kernel<T, ALONG, false>), dim3(g), dim3(256), 0, st, x, M, rs, cs, C, p.nfrag, tiles, frag, rows_first);
+        hipLaunchKernelGGL((mx_fragments_kernel<T, ALONG, false>), dim3(g), dim3(256), 0, st, x, M, rs, cs, C, p.nfrag, tiles, frag, rows_first,
+                           ex.kscale, ex.skip);
     KCHECK();
     return LCX_OK;
 }
 
 template <typename T> static int mx_join(int split, const MxOut<T>& w, hipStream_t st) {
     if (split == 1) return LCX_OK;
-    hipLaunchKernelGGL((mx_join_kernel<T>), dim3((unsigned)cdiv(w.O, 1024), (unsigned)(w.M < 32768 ? w.M : 32768)), dim3(256), 0, st, w.part, split, w.M, w.O,
-                       w.out, w.rs, w.cs);
+    // t_first: the partial sums lie transposed, and so does the output
+    const int64_t M = w.t_first ? w.O : w.M, O = w.t_first ? w.M : w.O;
+    int bx = 256;
+    while (bx > 4 && (int64_t)bx * 2 >= O) bx /= 2;
+    const int by = 256 / bx;
+    const int64_t gy = cdiv(M, by);
+    hipLaunchKernelGGL((mx_join_kernel<T>), dim3((unsigned)cdiv(O, bx * 4), (unsigned)(gy < 32768 ? gy : 32768)), dim3(bx, by), 0, st, w.part, split, M, O, w.out,
+                       w.t_first ? w.cs : w.rs, w.t_first ? w.rs : w.cs, w.oscale, w.skip);
     KCHECK();
     return LCX_OK;
 }
@@ -189,20 +208,22 @@ static int mx_linear_rows(const MxPlan& p, const T* x, int64_t rs, int64_t cs, c
 
 template <typename T>
 static int mx4_linear(const void* xv, int64_t M, int64_t xrs, int64_t xcs, const void* wcv, const void* wsv, int64_t N, int64_t K, void* out, int64_t rs,
-                      int64_t cs, void* space, int64_t space_bytes, hipStream_t st) {
+                      int64_t cs, void* space, int64_t space_bytes, hipStream_t st, const MxExtra& ex = MxExtra()) {
     constexpr int TERMS = MxTerms<T>::v;
     if (K == 0) return mx4_zero<T>(out, M, N, rs, cs, st);
-    const MxPlan p = mx_plan<T>(true, M, K, N);
+    const MxPlan p = mx_plan<T>(true, M, K, N, ex.tiles);
     if (space_bytes < mx_plan_bytes(p) || (mx_plan_bytes(p) && (!space || ((uintptr_t)space & 15)))) return fail(LCX_ERR_ARG, "lcx_mx4_linear: the work space is smaller than lcx_mx4_workspace says or not 16-byte aligned");
     const T* x = (const T*)xv;
     const unsigned char *wc = (const unsigned char*)wcv, *ws = (const unsigned char*)wsv;
     unsigned short* frag = (unsigned short*)space;
-    MxOut<T> w{(T*)out, rs, cs, p.split > 1 ? (float*)((char*)space + round_up(p.frag_bytes, 256)) : nullptr, M, N};
+    MxOut<T> w{(T*)out, rs, cs, p.split > 1 ? (float*)((char*)space + round_up(p.frag_bytes, 256)) : nullptr, M, N, rs == 1 && cs != 1, ex.oscale, ex.skip};
     if (p.row) return xcs == 1 ? mx_linear_rows<T, true>(p, x, xrs, xcs, wc, ws, N, K, w, st)
                                                 : mx_linear_rows<T, false>(p, x, xrs, xcs, wc, ws, N, K, w, st);
-    LCXCHECK((mx_fragments<T, true>(x, M, xrs, xcs, K, p, frag, st)));
+    LCXCHECK((mx_fragments<T, true>(x, M, xrs, xcs, K, p, frag, ex, st)));
     constexpr int JS = TERMS == 3 ? 2 : 4;
-    if (p.ct == 2) LCXCHECK((mx_linear_tiles<T, 2, 4>(p, frag, wc, ws, N, K, w, st)));
+    if (p.ct == 1) {
+        if constexpr (TERMS == 3) LCXCHECK((mx_linear_tiles<T, 1, 4>(p, frag, wc, ws, N, K, w, st)));
+    } else if (p.ct == 2) LCXCHECK((mx_linear_tiles<T, 2, 4>(p, frag, wc, ws, N, K, w, st)));
     else if (p.ct == 4) LCXCHECK((mx_linear_tiles<T, 4, JS>(p, frag, wc, ws, N, K, w, st)));
     else {
         if constexpr (TERMS == 1) LCXCHECK((mx_linear_tiles<T, 8, 4>(p, frag, wc, ws, N, K, w, st)));
@@ -212,16 +233,16 @@ static int mx4_linear(const void* xv, int64_t M, int64_t xrs, int64_t xcs, const
 
 template <typename T>
 static int mx4_linear_grad(const void* dyv, int64_t M, int64_t yrs, int64_t ycs, const void* wcv, const void* wsv, int64_t N, int64_t K, void* out, int64_t rs,
-                           int64_t cs, void* space, int64_t space_bytes, hipStream_t st) {
+                           int64_t cs, void* space, int64_t space_bytes, hipStream_t st, const MxExtra& ex = MxExtra()) {
     constexpr int TERMS = MxTerms<T>::v;
     if (N == 0) return mx4_zero<T>(out, M, K, rs, cs, st);
-    const MxPlan p = mx_plan<T>(false, M, N, K);
+    const MxPlan p = mx_plan<T>(false, M, N, K, ex.tiles);
     if (space_bytes < mx_plan_bytes(p) || (mx_plan_bytes(p) && (!space || ((uintptr_t)space & 15)))) return fail(LCX_ERR_ARG, "lcx_mx4_linear_grad: the work space is smaller than lcx_mx4_workspace says or not 16-byte aligned");
     const T* dy = (const T*)dyv;
     const unsigned char *wc = (const unsigned char*)wcv, *ws = (const unsigned char*)wsv;
     unsigned short* frag = (unsigned short*)space;
-    MxOut<T> w{(T*)out, rs, cs, p.split > 1 ? (float*)((char*)space + round_up(p.frag_bytes, 256)) : nullptr, M, K};
-    LCXCHECK((mx_fragments<T, false>(dy, M, yrs, ycs, N, p, frag, st)));
+    MxOut<T> w{(T*)out, rs, cs, p.split > 1 ? (float*)((char*)space + round_up(p.frag_bytes, 256)) : nullptr, M, K, rs == 1 && cs != 1, ex.oscale, ex.skip};
+    LCXCHECK((mx_fragments<T, false>(dy, M, yrs, ycs, N, p, frag, ex, st)));
     constexpr int JS = TERMS > 1 ? 1 : 2;
     if (p.ct == 1) LCXCHECK((mx_grad_tiles<T, 1, JS>(p, frag, wc, ws, N, K, w, st)));
     else if (p.ct == 2) LCXCHECK((mx_grad_tiles<T, 2, JS>(p, frag, wc, ws, N, K, w, st)));
@@ -272,7 +293,7 @@ static int mx4_matmul(const void* acv, const void* asv, int64_t M, const void* b
     const unsigned char *ac = (const unsigned char*)acv, *as = (const unsigned char*)asv, *bc = (const unsigned char*)bcv, *bs = (const unsigned char*)bsv;
     const MxMatmulPlan p = mx_matmul_plan(M, N, K);
     if (space_bytes < p.part_bytes || (p.part_bytes && (!space || ((uintptr_t)space & 15)))) return fail(LCX_ERR_ARG, "lcx_mx4_matmul: the work space is smaller than lcx_mx4_workspace says or not 16-byte aligned");
-    MxOut<T> w{(T*)out, rs, cs, p.split > 1 ? (float*)space : nullptr, M, N};
+    MxOut<T> w{(T*)out, rs, cs, p.split > 1 ? (float*)space : nullptr, M, N, rs == 1 && cs != 1, nullptr, nullptr};
     if (p.row) {
         unsigned g;
         LCXCHECK(mx_grid(1, cdiv(N, 16 * p.rt), &g));
@@ -290,6 +311,65 @@ static int mx4_matmul(const void* acv, const void* asv, int64_t M, const void* b
     else if (p.ct == 4) LCXCHECK((mx_matmul_tiles<T, 4, 4>(p, ac, as, bc, bs, N, K, w, st)));
     else LCXCHECK((mx_matmul_tiles<T, 2, 4>(p, ac, as, bc, bs, N, K, w, st)));
     return mx_join<T>(p.split, w, st);
+}
+
+// ---- the resident shard of a fit in 4 bits (engine.hpp) ----------------------------------------------------------------------------------
+// X~ (Npad samples x ldx variables, blocks along the variables).  The algorithm's moments assume variables of unit mean square; rounding to
+// 4 bits changes that by a per cent or so, hence one float32 factor per variable (xunit), which the passes apply to the small operand or to
+// the output: what is fitted is X~ = values of the 4 bits x factor.
+int lcx_mx_shard_alloc(lcx_ctx* h) {
+    const int64_t rt = mx_row_tiles(h->Npad);
+    const MxPlan a = mx_plan<float>(true, h->Mp, h->ldx, h->Npad, true), b = mx_plan<float>(false, h->Mp, h->Npad, h->ldx, true);
+    const int64_t wa = mx_plan_bytes(a), wb = mx_plan_bytes(b);
+    const size_t bytes[4] = {(size_t)(rt * mx_steps(h->ldx) * 1024), (size_t)(rt * mx_quads(h->ldx) * 256), (size_t)h->ldx * 4, (size_t)(wa > wb ? wa : wb)};
+    void** to[4] = {&h->xq, &h->xs, (void**)&h->xunit, &h->xwork};
+    for (int i = 0; i < 4; ++i) {
+        LCXCHECK(dev_alloc(to[i], bytes[i], h->stream));
+        h->bytes_resident += bytes[i];
+    }
+    h->xq_bytes = bytes[0] + bytes[1] + bytes[2];
+    h->xwork_bytes = (int64_t)bytes[3];
+    return LCX_OK;
+}
+// columns [c0, c0 + cols) from (and, rounded, back to) the row-major staging block; c0 is a multiple of 512
+static int mx_shard_block(lcx_ctx* h, float* stage, int64_t ld, int64_t c0, int64_t cols, bool fill) {
+    const int64_t nq = mx_quads(cols);
+    unsigned g;
+    LCXCHECK(mx_grid(mx_row_tiles(h->Npad), nq, &g));
+    unsigned char *qc = (unsigned char*)h->xq, *qs = (unsigned char*)h->xs;
+    if (fill) {
+        hipLaunchKernelGGL((mx_quantize_kernel<float, true>), dim3(g), dim3(256), 0, h->stream, stage, h->Npad, cols, ld, (int64_t)1, qc, qs, mx_steps(h->ldx),
+                           mx_quads(h->ldx), c0 / 512, (unsigned)nq);
+        KCHECK();
+    }
+    hipLaunchKernelGGL((mx_dequantize_kernel<float, true>), dim3(g), dim3(256), 0, h->stream, qc, qs, h->Npad, cols, stage, ld, (int64_t)1, mx_steps(h->ldx),
+                       mx_quads(h->ldx), c0 / 512, (unsigned)nq);
+    KCHECK();
+    if (fill) {
+        hipLaunchKernelGGL(mx_unit_columns_kernel, dim3((unsigned)cdiv(cols, 64)), dim3(1024), 0, h->stream, stage, h->N, cols, ld, (double)h->N, h->xunit + c0);
+    } else {
+        hipLaunchKernelGGL(mx_scale_columns_kernel, dim3(4096), dim3(256), 0, h->stream, stage, h->Npad, cols, ld, h->xunit + c0);
+    }
+    KCHECK();
+    return LCX_OK;
+}
+int lcx_mx_shard_fill(lcx_ctx* h, float* stage, int64_t ld, int64_t c0, int64_t cols) { return mx_shard_block(h, stage, ld, c0, cols, true); }
+int lcx_mx_shard_read(lcx_ctx* h, float* stage, int64_t ld, int64_t c0, int64_t cols) { return mx_shard_block(h, stage, ld, c0, cols, false); }
+// out [Npad][Mp] = X~ . B, B [ldx][Mp]
+int lcx_mx_shard_xbt(lcx_ctx* h, const float* B, float* out, const int* skip) {
+    MxExtra ex;
+    ex.kscale = h->xunit;
+    ex.skip = skip;
+    ex.tiles = true;
+    return mx4_linear<float>(B, h->Mp, 1, h->Mp, h->xq, h->xs, h->Npad, h->ldx, out, 1, h->Mp, h->xwork, h->xwork_bytes, h->stream, ex);
+}
+// out [ldx][Mp] = X~^T . Y, Y [Npad][Mp]
+int lcx_mx_shard_xty(lcx_ctx* h, const float* Y, float* out, const int* skip) {
+    MxExtra ex;
+    ex.oscale = h->xunit;
+    ex.skip = skip;
+    ex.tiles = true;
+    return mx4_linear_grad<float>(Y, h->Mp, 1, h->Mp, h->xq, h->xs, h->Npad, h->ldx, out, 1, h->Mp, h->xwork, h->xwork_bytes, h->stream, ex);
 }
 
 extern "C" {

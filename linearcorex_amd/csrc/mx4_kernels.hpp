@@ -132,19 +132,19 @@ __device__ __forceinline__ MxRaw8<T> mx_load8(const T* __restrict__ x, int64_t c
 
 // x[r * rs + c * cs] -> codes, scales.  Bound: reading x.  A block takes 16 rows x 512 columns: a thread 8 columns of each of four steps (16 bytes
 // of a 16-bit type each: VEC, where the columns are neighbours), so that it ends up with a whole dword of scales; four lanes share a
-// block of 32.  grid (row tile, quad of steps)
+// block of 32.  grid (row tile, quad of steps); x holds the columns from quad quad0 on of a matrix of `steps` steps
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t rs, int64_t cs,
-                                                          unsigned char* __restrict__ codes, unsigned char* __restrict__ scales) {
-    const int64_t steps = mx_steps(cols), quads = mx_quads(cols);
-    const unsigned int rt32 = blockIdx.x / (unsigned int)quads;
-    const int64_t rt = rt32, quad = blockIdx.x - rt32 * (unsigned int)quads;
+                                                          unsigned char* __restrict__ codes, unsigned char* __restrict__ scales, int64_t steps, int64_t quads,
+                                                          int64_t quad0, unsigned int nquads) {
+    const unsigned int rt32 = blockIdx.x / nquads;
+    const int64_t rt = rt32, here = blockIdx.x - rt32 * nquads, quad = quad0 + here;
     const int l = threadIdx.x >> 4, c = threadIdx.x & 15;                  // row of the tile, 8 columns of the step
     const int64_t r = rt * 16 + l;
     MxRaw8<T> raw[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-        if (r < rows) raw[u] = mx_load8<T, VEC>(x + r * rs, quad * 512 + u * 128 + c * 8, cols, cs);
+        if (r < rows) raw[u] = mx_load8<T, VEC>(x + r * rs, here * 512 + u * 128 + c * 8, cols, cs);
         else
 #pragma unroll
             for (int j = 0; j < 8; ++j) raw[u].v[j] = (T)0.0f;
@@ -224,10 +224,10 @@ __device__ __forceinline__ void mx_values8(unsigned int q, float s, float* v) {
 // codes, scales -> out[r * rs + c * cs].  Bound: writing out.  Threads as in mx_quantize_kernel; VEC: the columns of out are neighbours
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
-                                                            int64_t rows, int64_t cols, T* __restrict__ out, int64_t rs, int64_t cs) {
-    const int64_t steps = mx_steps(cols), quads = mx_quads(cols);
-    const unsigned int rt32 = blockIdx.x / (unsigned int)quads;
-    const int64_t rt = rt32, quad = blockIdx.x - rt32 * (unsigned int)quads;
+                                                            int64_t rows, int64_t cols, T* __restrict__ out, int64_t rs, int64_t cs, int64_t steps, int64_t quads,
+                                                            int64_t quad0, unsigned int nquads) {
+    const unsigned int rt32 = blockIdx.x / nquads;
+    const int64_t rt = rt32, here = blockIdx.x - rt32 * nquads, quad = quad0 + here;
     const int l = threadIdx.x >> 4, c = threadIdx.x & 15;
     const int64_t r = rt * 16 + l;
     if (r >= rows) return;
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned char*
         q[u] = quad * 4 + u < steps ? *reinterpret_cast<const unsigned int*>(codes + (rt * steps + quad * 4 + u) * 1024 + (c >> 2) * 256 + l * 16 + (c & 3) * 4) : 0u;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-        const int64_t c0 = quad * 512 + u * 128 + c * 8;
+        const int64_t c0 = here * 512 + u * 128 + c * 8;
         float v[8];
         mx_values8(q[u], __uint_as_float(((sd >> (8 * u)) & 255u) << 23), v);
         T* p = out + r * rs + c0 * cs;
@@ -310,35 +310,36 @@ template <typename T, int TERMS> __device__ __forceinline__ void mx_terms(const 
     }
 }
 
-// x[t * rs + k * cs], eight k from k0 on, as bf16 terms; zeros from nk on.  t must be a row.
-template <typename T, int TERMS, bool VEC>
-__device__ __forceinline__ void mx_load_terms(const T* __restrict__ x, int64_t t, int64_t rs, int64_t k0, int64_t nk, int64_t cs, mx_bf8* f) {
-    mx_terms<T, TERMS>(mx_load8<T, VEC>(x + t * rs, k0, nk, cs), f);
-}
-// where an output goes: split == 1 the result, else float32 partial sums [split][M][O] (mx_join_kernel adds them up in order)
+// where an output goes: split == 1 the result, else float32 partial sums [split][M][O] (t_first: [split][O][M], for an output whose rows are
+// neighbours in memory); mx_join_kernel adds them up in order.  oscale (may be null): a factor of every output column.  skip (may be null):
+// the whole product is left out if the word is not 0.
 template <typename T> struct MxOut {
     T* out;
     int64_t rs, cs;
     float* part;
     int64_t M, O;
+    bool t_first;
+    const float* oscale;
+    const int* skip;
 };
 // N consecutive columns o .. of row t
 template <typename T, int N>
 __device__ __forceinline__ void mx_store(const MxOut<T>& w, int64_t z, int64_t t, int64_t o, const float* v) {
     if (t >= w.M) return;
     if (w.part) {
-        float* p = w.part + (z * w.M + t) * w.O + o;
-        if (o + N <= w.O) {
+        float* p = w.part + z * w.M * w.O + (w.t_first ? o * w.M + t : t * w.O + o);
+        if (!w.t_first && o + N <= w.O) {
             mx_put<float, N>(p, v);
         } else {
+            const int64_t ps = w.t_first ? w.M : 1;
 #pragma unroll
             for (int j = 0; j < N; ++j)
-                if (o + j < w.O) p[j] = v[j];
+                if (o + j < w.O) p[j * ps] = v[j];
         }
         return;
     }
     T* p = w.out + t * w.rs + o * w.cs;
-    if (w.cs == 1 && o + N <= w.O) {
+    if (w.cs == 1 && o + N <= w.O && !w.oscale) {
         T r[N];
 #pragma unroll
         for (int j = 0; j < N; ++j) r[j] = mx_from_f32<T>(v[j]);
@@ -346,38 +347,58 @@ __device__ __forceinline__ void mx_store(const MxOut<T>& w, int64_t z, int64_t t
     } else {
 #pragma unroll
         for (int j = 0; j < N; ++j)
-            if (o + j < w.O) p[j * w.cs] = mx_from_f32<T>(v[j]);
+            if (o + j < w.O) p[j * w.cs] = mx_from_f32<T>(w.oscale ? v[j] * w.oscale[o + j] : v[j]);
     }
 }
-// out[t][o] = sum over the splits, in order; four columns a thread.  grid (columns, rows)
+// out[t][o] = sum over the splits, in order; four columns a thread, rscale (may be null) a factor of every row.  grid (columns, rows)
 template <typename T>
 __global__ __launch_bounds__(256) void mx_join_kernel(const float* __restrict__ part, int split, int64_t M, int64_t O, T* __restrict__ out, int64_t rs,
-                                                      int64_t cs) {
-    const int64_t o = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, n = M * O;
-    if (o >= O) return;
-    for (int64_t t = blockIdx.y; t < M; t += gridDim.y) {
+                                                      int64_t cs, const float* __restrict__ rscale, const int* __restrict__ skip) {
+    const int64_t o = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 4, n = M * O;
+    if (o >= O || (skip && *skip)) return;
+    for (int64_t t = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; t < M; t += (int64_t)gridDim.y * blockDim.y) {
         const float* p = part + t * O + o;
+        const float f = rscale ? rscale[t] : 1.0f;
         if (o + 4 <= O) {
             mx_f4 v = *reinterpret_cast<const mx_f4u*>(p);
             for (int z = 1; z < split; ++z) v += *reinterpret_cast<const mx_f4u*>(p + z * n);
             T* q = out + t * rs + o * cs;
-            if (cs == 1) {
-                T r[4];
+            T r[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) r[j] = mx_from_f32<T>(v[j]);
+            for (int j = 0; j < 4; ++j) r[j] = mx_from_f32<T>(v[j] * f);
+            if (cs == 1) {
                 mx_put<T, 4>(q, r);
             } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) q[j * cs] = mx_from_f32<T>(v[j]);
+                for (int j = 0; j < 4; ++j) q[j * cs] = r[j];
             }
         } else {
             for (int j = 0; o + j < O; ++j) {
                 float v = p[j];
                 for (int z = 1; z < split; ++z) v += p[z * n + j];
-                out[t * rs + (o + j) * cs] = mx_from_f32<T>(v);
+                out[t * rs + (o + j) * cs] = mx_from_f32<T>(v * f);
             }
         }
     }
+}
+
+// one factor per column that makes the mean square of the N rows 1 (1 for a column of zeros).  64 columns a block
+__global__ __launch_bounds__(1024) void mx_unit_columns_kernel(const float* __restrict__ x, int64_t N, int64_t cols, int64_t ld, double n, float* __restrict__ out) {
+    __shared__ double red[16][64];
+    const int c = threadIdx.x & 63, g = threadIdx.x >> 6;
+    const int64_t col = (int64_t)blockIdx.x * 64 + c;
+    double s = 0.0;
+    if (col < cols)
+        for (int64_t r = g; r < N; r += 16) { const double v = x[r * ld + col]; s += v * v; }
+    red[g][c] = s;
+    __syncthreads();
+    if (g == 0 && col < cols) {
+        for (int k = 1; k < 16; ++k) s += red[k][c];
+        out[col] = s > 0.0 ? (float)sqrt(n / s) : 1.0f;
+    }
+}
+__global__ __launch_bounds__(256) void mx_scale_columns_kernel(float* __restrict__ x, int64_t rows, int64_t cols, int64_t ld, const float* __restrict__ f) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * cols; i += (int64_t)gridDim.x * 256) x[(i / cols) * ld + i % cols] *= f[i % cols];
 }
 
 // ---- few rows of x (up to 16: tokens being decoded) -----------------------------------------------------------------------------
@@ -475,14 +496,17 @@ __device__ __forceinline__ void mx_unpack_across(const unsigned int* q, const fl
 //   along the blocks   128 (i / 4) + 32 g + 8 (i % 4)      (a lane of W owns one block of each 128 columns, 8 values an instruction)
 //   across the blocks  32 i + 8 g
 // mx_fragments_kernel lays x out that way once per call, split into its bf16 terms: frag[i][term][tile of 16 rows][lane][8].  A tile of the
-// products below is then a contiguous piece of memory, whatever x's type, strides or odd sizes.
+// products below is then a contiguous piece of memory, whatever x's type, strides or odd sizes.  kscale (may be null): a factor of every
+// column of W, taken into x here.
 template <bool ALONG> __device__ __forceinline__ int64_t mx_frag_k(int64_t i, int g) {
     return ALONG ? (i >> 2) * 128 + g * 32 + (i & 3) * 8 : i * 32 + g * 8;
 }
 template <typename T, bool ALONG, bool VEC>
 __global__ __launch_bounds__(256) void mx_fragments_kernel(const T* __restrict__ x, int64_t M, int64_t xrs, int64_t xcs, int64_t K, int64_t nfrag,
-                                                           int64_t tiles, unsigned short* __restrict__ frag, int rows_first) {
+                                                           int64_t tiles, unsigned short* __restrict__ frag, int rows_first,
+                                                           const float* __restrict__ kscale, const int* __restrict__ skip) {
     constexpr int TERMS = MxTerms<T>::v;
+    if (skip && *skip) return;
     // a block takes one tile of 16 rows and 16 groups of 8 values; neighbouring threads read neighbouring memory
     const unsigned int grp = blockIdx.x / (unsigned int)tiles;
     const int64_t tile = blockIdx.x - grp * (unsigned int)tiles, c0 = (int64_t)grp * 16;
@@ -493,7 +517,15 @@ __global__ __launch_bounds__(256) void mx_fragments_kernel(const T* __restrict__
     const int g = (int)(ALONG ? (c >> 2) & 3 : c & 3);
     const int64_t t = tile * 16 + l;
     mx_bf8 f[TERMS] = {};
-    if (t < M) mx_load_terms<T, TERMS, VEC>(x, t, xrs, c * 8, K, xcs, f);
+    if (t < M) {
+        MxRaw8<T> r = mx_load8<T, VEC>(x + t * xrs, c * 8, K, xcs);
+        if (kscale) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c * 8 + j < K) r.v[j] = (T)((float)r.v[j] * kscale[c * 8 + j]);
+        }
+        mx_terms<T, TERMS>(r, f);
+    }
 #pragma unroll
     for (int u = 0; u < TERMS; ++u) *reinterpret_cast<mx_bf8*>(frag + (((i * TERMS + u) * tiles + tile) * 64 + g * 16 + l) * 8) = f[u];
 }
@@ -546,6 +578,7 @@ __global__ __launch_bounds__(256, 2) void mx_linear_tile_kernel(const unsigned s
                                                              const unsigned char* __restrict__ ws, int64_t N, int64_t K, MxOut<T> w, int mt, int nt, int split) {
     constexpr int TERMS = MxTerms<T>::v, CH = JS * TERMS * CT;             // 1 KB pieces a stage
     const int64_t ksteps = mx_steps(K), quads = mx_quads(K), rts = mx_row_tiles(N);
+    if (w.skip && *w.skip) return;
     const MxTile tile = mx_tile(blockIdx.x, mt, nt, split);
     if (tile.a < 0) return;
     const int lane = threadIdx.x & 63, wave = mx_wave(), l = lane & 15, g = lane >> 4;
@@ -650,6 +683,7 @@ __global__ __launch_bounds__(256, 2) void mx_grad_tile_kernel(const unsigned sho
     constexpr bool AHEAD = TERMS == 1 && JS % 2 == 0;
     typedef MxGradLds<CT, JS, TERMS> L;
     const int64_t ksteps = mx_steps(K), quads = mx_quads(K), rts = mx_row_tiles(N);
+    if (w.skip && *w.skip) return;
     const MxTile tile = mx_tile(blockIdx.x, mt, nt, split);
     if (tile.a < 0) return;
     const int lane = threadIdx.x & 63, wave = mx_wave(), l = lane & 15, g = lane >> 4;

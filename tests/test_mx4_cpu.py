@@ -87,3 +87,15 @@ def test_reference_format():
     assert byte.tolist() == [[127, 125]]
     assert code[0, :9].tolist() == [6, 0, 2, 2, 4, 4, 6, 6, 15] and code[0, 32:35].tolist() == [6, 0, 9]
     assert R.values(code, byte)[0, [0, 8, 32, 34]].tolist() == [4.0, -6.0, 1.0, -0.125]
+
+
+def test_a_fit_refuses_4_bit_data_where_they_do_not_exist(lib):
+    from linearcorex_amd import Corex
+    for kw in (dict(x_storage="int8"), dict(x_storage="mx4", dtype=np.float64), dict(x_storage="mx4", n_hidden=129)):
+        with pytest.raises(ValueError, match="x_storage"):
+            Corex(**{"n_hidden": 4, **kw})
+    assert Corex(n_hidden=4).x_storage == "dense" and Corex(n_hidden=4, x_storage="mx4").x_storage == "mx4"
+    h = C.c_void_p()
+    for args in ((100, 20, 4, 1, 0, 1), (100, 20, 129, 0, 0, 1), (100, 20, 4, 0, 0, 2)):
+        assert lib.lcx_create_stored(C.byref(h), *args) == 1 and not h.value
+        assert b"lcx_create_stored" in lib.lcx_last_error()

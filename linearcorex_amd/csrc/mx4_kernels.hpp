@@ -350,6 +350,37 @@ __device__ __forceinline__ void mx_store(const MxOut<T>& w, int64_t z, int64_t t
             if (o + j < w.O) p[j * w.cs] = mx_from_f32<T>(w.oscale ? v[j] * w.oscale[o + j] : v[j]);
     }
 }
+// a wave's tiles: acc[i][c] holds rows 16 c + l of t0 and columns 16 i + 4 g .. of o0.  Whole tiles of an ordinary output take the short way:
+// one address a lane, the rest constant offsets
+template <typename T, int RT, int CT>
+__device__ __forceinline__ void mx_store_tile(const MxOut<T>& w, int64_t z, int64_t t0, int64_t o0, int l, int g, const mx_f4 (&acc)[RT][CT]) {
+    const bool whole = t0 + 16 * CT <= w.M && o0 + 16 * RT <= w.O && !w.t_first && !w.oscale;
+    if (whole && w.part) {
+        float* p = w.part + (z * w.M + t0 + l) * w.O + o0 + 4 * g;
+#pragma unroll
+        for (int c = 0; c < CT; ++c, p += 16 * w.O)
+#pragma unroll
+            for (int i = 0; i < RT; ++i) *reinterpret_cast<mx_f4u*>(p + 16 * i) = acc[i][c];
+    } else if (whole && w.cs == 1) {
+        T* p = w.out + (t0 + l) * w.rs + o0 + 4 * g;
+#pragma unroll
+        for (int c = 0; c < CT; ++c, p += 16 * w.rs)
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                const T r[4] = {mx_from_f32<T>(acc[i][c][0]), mx_from_f32<T>(acc[i][c][1]), mx_from_f32<T>(acc[i][c][2]), mx_from_f32<T>(acc[i][c][3])};
+                mx_put<T, 4>(p + 16 * i, r);
+            }
+    } else {
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                const float o[4] = {acc[i][c][0], acc[i][c][1], acc[i][c][2], acc[i][c][3]};
+                mx_store<T, 4>(w, z, t0 + 16 * c + l, o0 + 16 * i + 4 * g, o);
+            }
+    }
+}
+
 // out[t][o] = sum over the splits, in order; four columns a thread, rscale (may be null) a factor of every row.  grid (columns, rows)
 template <typename T>
 __global__ __launch_bounds__(256) void mx_join_kernel(const float* __restrict__ part, int split, int64_t M, int64_t O, T* __restrict__ out, int64_t rs,
@@ -530,24 +561,10 @@ __global__ __launch_bounds__(256) void mx_fragments_kernel(const T* __restrict__
     for (int u = 0; u < TERMS; ++u) *reinterpret_cast<mx_bf8*>(frag + (((i * TERMS + u) * tiles + tile) * 64 + g * 16 + l) * 8) = f[u];
 }
 
-// Order of the instructions around READS fragments from LDS of MFMA matrix instructions each.  Left alone, a wave reads a fragment, waits, uses
-// it, and unpacks in one piece; two waves of a SIMD then fall into step and neither pipe is fed while they do.  So: the fragments two ahead
-// (EXTRA reads of other data with the first of them), and VALU vector instructions behind every matrix instruction.
-template <int N, int VALU> __device__ __forceinline__ void mx_schedule_mfma() {
-    if constexpr (N > 0) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        if constexpr (VALU > 0) __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
-        mx_schedule_mfma<N - 1, VALU>();
-    }
-}
-template <int READS, int MFMA, int EXTRA, int VALU, bool FIRST = true> __device__ __forceinline__ void mx_schedule() {
-    constexpr int G = READS > 1 ? 2 : 1, REST = READS - G, NEXT = REST < 2 ? REST : 2;
-    if constexpr (FIRST) __builtin_amdgcn_sched_group_barrier(0x100, G + EXTRA, 0);
-    mx_schedule_mfma<1, VALU>();
-    if constexpr (NEXT > 0) __builtin_amdgcn_sched_group_barrier(0x100, NEXT, 0);
-    mx_schedule_mfma<G * MFMA - 1, VALU>();
-    if constexpr (NEXT > 0) mx_schedule<REST, MFMA, 0, VALU, false>();
-}
+// No instruction is moved across this by the compiler.  The tile kernels below run in slices: the fragments of the next slice are read from LDS
+// behind the first matrix instructions of this one, so that a wave never waits for a read it has just issued.  (Left alone, the compiler
+// reads each fragment right before its use, and two waves of a SIMD fall into step: neither pipe is fed while they wait.)
+__device__ __forceinline__ void mx_fence() { __builtin_amdgcn_sched_barrier(0); }
 
 typedef __attribute__((address_space(1))) const void* mx_gptr;
 typedef __attribute__((address_space(3))) void* mx_lptr;
@@ -596,20 +613,19 @@ __global__ __launch_bounds__(256, 2) void mx_linear_tile_kernel(const unsigned s
     // running address of the next stage: scalar, advanced by a constant
     const unsigned char* fp = (const unsigned char*)frag + (s0 * 4 * TERMS * tiles + (int64_t)tile.a * CT) * 1024;
     const int64_t fterm = tiles * 1024;
-    auto stage = [&](int b) {                                              // the next JS fragments of the contraction
-#pragma unroll
-        for (int c = 0; c < (CH + 3) / 4; ++c) {
-            const int i = c * 4 + wave;
-            if (CH % 4 == 0 || i < CH)
-                __builtin_amdgcn_global_load_lds((mx_gptr)(fp + (i / CT) * fterm + (i % CT) * 1024 + lane * 16), (mx_lptr)(&lds[b][i * 512]), 16, 0, 0);
-        }
-        fp += JS * TERMS * fterm;
+    // piece c of the wave's share of the next JS fragments of the contraction
+    constexpr int PIECES = (CH + 3) / 4;
+    auto stage = [&](int b, int c) {
+        const int i = c * 4 + wave;
+        if (CH % 4 == 0 || i < CH)
+            __builtin_amdgcn_global_load_lds((mx_gptr)(fp + (i / CT) * fterm + (i % CT) * 1024 + lane * 16), (mx_lptr)(&lds[b][i * 512]), 16, 0, 0);
     };
     mx_f4 acc[RT][CT] = {};
     mx_u4 q[RT];
     unsigned int sd[RT];
     if (s0 < s1) {
-        stage(0);
+#pragma unroll
+        for (int c = 0; c < PIECES; ++c) stage(0, c);
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
             q[i] = *reinterpret_cast<const mx_u4*>(pc[i] + s0 * 1024 + lane * 16);
@@ -621,49 +637,59 @@ __global__ __launch_bounds__(256, 2) void mx_linear_tile_kernel(const unsigned s
     for (int64_t s = s0; s < s1; ++s) {
         mx_u4 qn[RT];
         unsigned int sn[RT];
-#pragma unroll
-        for (int i = 0; i < RT; ++i) { qn[i] = q[i]; sn[i] = sd[i]; }
+        const int64_t sx = s + 1 < s1 ? s + 1 : s;
         float sc[RT];
 #pragma unroll
         for (int i = 0; i < RT; ++i) sc[i] = mx_scale_operand(sd[i], (int)(s & 3));
 #pragma unroll
         for (int h = 0; h < 4 / JS; ++h) {
-            if (h + 1 < 4 / JS || s + 1 < s1) stage(b ^ 1);
-            if (h == 0 && s + 1 < s1) {
+            if (h + 1 < 4 / JS || s + 1 < s1) fp += JS * TERMS * fterm;    // (behind the last stage: that one again, unused)
+            // slices of F fragments
+            constexpr int F = CT < 4 ? CT : 4, SL = CH / F;
+            mx_bf8 f[2][F], a[2][RT];
+            const unsigned short* at = &lds[b][lane * 8];
 #pragma unroll
-                for (int i = 0; i < RT; ++i) {
-                    qn[i] = *reinterpret_cast<const mx_u4*>(pc[i] + (s + 1) * 1024 + lane * 16);
-                    if (((s + 1) & 3) == 0) sn[i] = *reinterpret_cast<const unsigned int*>(ps[i] + ((s + 1) >> 2) * 256 + lane * 4);
-                }
-            }
+            for (int c = 0; c < F; ++c) f[0][c] = *reinterpret_cast<const mx_bf8*>(at + c * 512);
 #pragma unroll
-            for (int jj = 0; jj < JS; ++jj) {
-                mx_bf8 a[RT];
+            for (int i = 0; i < RT; ++i) a[0][i] = mx_unpack8(q[i][h * JS], sc[i]);
 #pragma unroll
-                for (int i = 0; i < RT; ++i) a[i] = mx_unpack8(q[i][h * JS + jj], sc[i]);
+            for (int sl = 0; sl < SL; ++sl) {
+                const int jj = sl * F / (TERMS * CT), c0 = sl * F % CT;
 #pragma unroll
-                for (int u = 0; u < TERMS; ++u)
+                for (int c = 0; c < F; ++c) {
+                    if (c == 1 || F == 1) {
+                        mx_fence();
+                        // the loads of the next stage, a few a slice: all at once they would fill the address queue and hold the wave up
 #pragma unroll
-                    for (int c = 0; c < CT; ++c) {
-                        const mx_bf8 f = *reinterpret_cast<const mx_bf8*>(&lds[b][((jj * TERMS + u) * CT + c) * 512 + lane * 8]);
+                        for (int p = sl * PIECES / SL; p < (sl + 1) * PIECES / SL; ++p) stage(b ^ 1, p);
+                        if (h == 0) {
 #pragma unroll
-                        for (int i = 0; i < RT; ++i) acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], f, acc[i][c], 0, 0, 0);
+                            for (int i = sl * RT / SL; i < (sl + 1) * RT / SL; ++i) {
+                                qn[i] = *reinterpret_cast<const mx_u4*>(pc[i] + sx * 1024 + lane * 16);
+                                sn[i] = *reinterpret_cast<const unsigned int*>(ps[i] + (sx >> 2) * 256 + lane * 4);
+                            }
+                        }
+                        if (sl + 1 < SL) {
+#pragma unroll
+                            for (int n = 0; n < F; ++n) f[(sl + 1) & 1][n] = *reinterpret_cast<const mx_bf8*>(at + ((sl + 1) * F + n) * 512);
+                            if ((sl + 1) * F % (TERMS * CT) == 0) {
+#pragma unroll
+                                for (int i = 0; i < RT; ++i) a[(jj + 1) & 1][i] = mx_unpack8(q[i][h * JS + jj + 1], sc[i]);
+                            }
+                        }
                     }
+#pragma unroll
+                    for (int i = 0; i < RT; ++i) acc[i][c0 + c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[jj & 1][i], f[sl & 1][c], acc[i][c0 + c], 0, 0, 0);
+                }
+                mx_fence();
             }
-            mx_schedule<JS * TERMS * CT, RT, 0, 1>();
             __syncthreads();
             b ^= 1;
         }
 #pragma unroll
         for (int i = 0; i < RT; ++i) { q[i] = qn[i]; sd[i] = sn[i]; }
     }
-#pragma unroll
-    for (int c = 0; c < CT; ++c)
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-            float o[4] = {acc[i][c][0], acc[i][c][1], acc[i][c][2], acc[i][c][3]};
-            mx_store<T, 4>(w, tile.z, ((int64_t)tile.a * CT + c) * 16 + l, n0 + 16 * i + 4 * g, o);
-        }
+    mx_store_tile<T, RT, CT>(w, tile.z, (int64_t)tile.a * CT * 16, n0, l, g, acc);
 }
 
 // dx[t][k] = sum_n dy[t][n] W[n][k] for tiles of 16 CT rows of dy and 512 columns of W: the contraction runs ACROSS the blocks.  A lane reads the
@@ -701,26 +727,26 @@ __global__ __launch_bounds__(256, 2) void mx_grad_tile_kernel(const unsigned sho
     int64_t left = rts - s0 * 2;
     const unsigned char* zp = (const unsigned char*)frag + ((s0 + (wave >> 1)) * TERMS * tiles + (int64_t)tile.a * CT) * 1024 + (wave & 1) * 512;
     const int wlane[2] = {g * 256 + (l ^ g) * 16, g * 256 + (l ^ (g | 4)) * 16};
-    auto stage_frag = [&](int at) {
-#pragma unroll
-        for (int c = 0; c < (CH + 3) / 4; ++c) {
-            const int i = c * 4 + wave;
-            if (CH % 4 == 0 || i < CH)
-                __builtin_amdgcn_global_load_lds((mx_gptr)(fp + (i / CT) * fterm + (i % CT) * 1024 + lane * 16), (mx_lptr)(glds + at + i * 1024), 16, 0, 0);
-        }
-        fp += JS * TERMS * fterm;
+    constexpr int FP = (CH + 3) / 4, WP = JS * 2, PIECES = FP + WP + 1;    // loads of a wave: fragments, codes, scales
+    auto load_frag = [&](int at, int c) {
+        const int i = c * 4 + wave;
+        if (CH % 4 == 0 || i < CH)
+            __builtin_amdgcn_global_load_lds((mx_gptr)(fp + (i / CT) * fterm + (i % CT) * 1024 + lane * 16), (mx_lptr)(glds + at + i * 1024), 16, 0, 0);
     };
-    auto stage_w = [&](int at) {
-#pragma unroll
-        for (int p = 0; p < JS * 2; ++p)                       // the wave's step of each row tile
+    auto load_w = [&](int at, int p) {                         // the wave's step of row tile p; p == WP: the scales
+        if (p < WP)
             __builtin_amdgcn_global_load_lds((mx_gptr)(wp + (p < left ? p : left - 1) * wtile + wlane[p & 1]), (mx_lptr)(glds + at + (p * 4 + wave) * 1024), 16,
                                              0, 0);
-        if (wave < JS * 2 && lane < 16)
+        else if (wave < WP && lane < 16)
             __builtin_amdgcn_global_load_lds((mx_gptr)((wave < left ? sp : zp) + lane * 16), (mx_lptr)(glds + at + L::codes + wave * 256), 16, 0, 0);
-        wp += JS * 2 * wtile;
-        sp += JS * 2 * stile;
-        zp += JS * TERMS * fterm;
-        left -= JS * 2;
+    };
+    // (behind the last stage: that one again, unused - the addresses stay where they are)
+    auto next_frag = [&](bool more) { fp += more ? JS * TERMS * fterm : 0; };
+    auto next_w = [&](bool more) {
+        wp += more ? WP * wtile : 0;
+        sp += more ? WP * stile : 0;
+        zp += more ? JS * TERMS * fterm : 0;
+        left -= more ? WP : 0;
     };
     // row 8 g + j of a step is row 8 (g % 2) + j of row tile g / 2
     const int blk = l >> 2, mask = blk | 4 * (g >> 1);
@@ -744,36 +770,79 @@ __global__ __launch_bounds__(256, 2) void mx_grad_tile_kernel(const unsigned sho
         mx_unpack_across(q, sc, to);
     };
     if (s0 < s1) {
-        stage_frag(f0);
-        stage_w(w0);
-        if (left > 0) stage_w(w1);
+#pragma unroll
+        for (int c = 0; c < FP; ++c) load_frag(f0, c);
+        next_frag(s0 + JS < s1);
+#pragma unroll
+        for (int p = 0; p <= WP; ++p) load_w(w0, p);
+        next_w(s0 + JS < s1);
+#pragma unroll
+        for (int p = 0; p <= WP; ++p) load_w(w1, p);
+        next_w(s0 + 2 * JS < s1);
     }
     __syncthreads();
     if (AHEAD && s0 < s1) unpack_step(w0, 0, a[0]);
     for (int64_t s = s0; s < s1; s += JS) {
-        if (s + JS < s1) {
-            stage_frag(f1);
-            if (left > 0) stage_w(w2);
-        }
 #pragma unroll
         for (int jj = 0; jj < JS; ++jj) {                      // (a step behind the last one: the fragments of dy are zeros)
             const int cur = AHEAD ? jj & 1 : 0, nxt = cur ^ 1;
             if (!AHEAD) unpack_step(w0, jj, a[0]);
-            else if (jj + 1 < JS) unpack_step(w0, jj + 1, a[nxt]);
-            else unpack_step(w1, 0, a[nxt]);
+            // slices of F fragments; the first of the next step's unpacking rides behind the first of them
+            constexpr int F = CT < 2 ? CT : 2, SL = TERMS * CT / F;
+            mx_bf8 f[2][F];
+            const unsigned char* at = glds + f0 + jj * TERMS * CT * 1024 + lane * 16;
 #pragma unroll
-            for (int u = 0; u < TERMS; ++u)
+            for (int c = 0; c < F; ++c) f[0][c] = *reinterpret_cast<const mx_bf8*>(at + c * 1024);
 #pragma unroll
-                for (int c = 0; c < CT; ++c) {
-                    const mx_bf8 f = *reinterpret_cast<const mx_bf8*>(glds + f0 + ((jj * TERMS + u) * CT + c) * 1024 + lane * 16);
+            for (int sl = 0; sl < SL; ++sl) {
+                const int c0 = sl * F % CT;
 #pragma unroll
-                    for (int m = 0; m < 8; ++m) acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[cur][m], f, acc[m][c], 0, 0, 0);
+                for (int c = 0; c < F; ++c) {
+                    if (c == 1 || F == 1) {
+                        mx_fence();
+                        // the loads of the stages ahead, a few a slice
+#pragma unroll
+                        for (int p = (jj * SL + sl) * PIECES / (JS * SL); p < (jj * SL + sl + 1) * PIECES / (JS * SL); ++p) {
+                            if (p < FP) load_frag(f1, p);
+                            else load_w(w2, p - FP);
+                        }
+                        if (sl + 1 < SL) {
+#pragma unroll
+                            for (int n = 0; n < F; ++n) f[(sl + 1) & 1][n] = *reinterpret_cast<const mx_bf8*>(at + ((sl + 1) * F + n) * 1024);
+                        }
+                        if (AHEAD && sl == 0) {
+                            if (jj + 1 < JS) unpack_step(w0, jj + 1, a[nxt]);
+                            else unpack_step(w1, 0, a[nxt]);
+                        }
+                    }
+#pragma unroll
+                    for (int m = 0; m < 8; ++m) acc[m][c0 + c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[cur][m], f[sl & 1][c], acc[m][c0 + c], 0, 0, 0);
                 }
-            if (AHEAD) mx_schedule<TERMS * CT, 8, 10, (80 + TERMS * CT * 8 - 1) / (TERMS * CT * 8)>();
+                if (!AHEAD || sl > 0) mx_fence();              // (unpacking mixes with the matrix instructions of two slices)
+            }
         }
+        next_frag(s + 2 * JS < s1);
+        next_w(s + 3 * JS < s1);
         __syncthreads();
         { const int t = f0; f0 = f1; f1 = t; }
         { const int t = w0; w0 = w1; w1 = w2; w2 = t; }
+    }
+    // a lane ends up with 32 neighbours of a row: columns 32 g + 8 e + m
+    const int64_t t0 = (int64_t)tile.a * CT * 16;
+    if (t0 + 16 * CT <= w.M && k0 + 128 <= w.O && !w.t_first && !w.oscale && (w.part || w.cs == 1)) {
+        const int64_t at = (t0 + l) * (w.part ? w.O : w.rs) + k0 + 32 * g;
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float o[8];
+                T r[8];
+#pragma unroll
+                for (int m = 0; m < 8; ++m) { o[m] = acc[m][c][e]; r[m] = mx_from_f32<T>(o[m]); }
+                if (w.part) mx_put<float, 8>(w.part + tile.z * w.M * w.O + at + 16 * c * w.O + 8 * e, o);
+                else mx_put<T, 8>(w.out + at + 16 * c * w.rs + 8 * e, r);
+            }
+        return;
     }
 #pragma unroll
     for (int c = 0; c < CT; ++c)
@@ -879,16 +948,15 @@ __global__ __launch_bounds__(256, 2) void mx_matmul_tile_kernel(const unsigned c
         qb[i] = bc + rt * ksteps * 1024;
         sb[i] = bs + rt * quads * 256;
     }
-    auto stage = [&](int64_t s, int b) {
-#pragma unroll
-        for (int c = 0; c < CH; ++c)
-            __builtin_amdgcn_global_load_lds((mx_gptr)(xb[c] + s * 2048 + lane * 16), (mx_lptr)(&lds[b][(c * 4 + wave) * 1024]), 16, 0, 0);
+    auto load_a = [&](int64_t s, int b, int c) {                            // piece c of the wave's share of stage s
+        __builtin_amdgcn_global_load_lds((mx_gptr)(xb[c] + s * 2048 + lane * 16), (mx_lptr)(&lds[b][(c * 4 + wave) * 1024]), 16, 0, 0);
     };
     mx_f4 acc[RT][CT] = {};
     mx_u4 q[RT][2];
     int sd[RT], sx[CT];
     if (s0 < s1) {
-        stage(s0, 0);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) load_a(s0, 0, c);
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
             q[i][0] = *reinterpret_cast<const mx_u4*>(qb[i] + s0 * 2048 + lane * 16);
@@ -905,35 +973,52 @@ __global__ __launch_bounds__(256, 2) void mx_matmul_tile_kernel(const unsigned c
         const int64_t sn = s + 2 < s1 ? s + 2 : s;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            if (s + h >= s1) break;
-            const int64_t nx = s + h + 1 < s1 ? s + h + 1 : s;             // (the last stage loads something it does not use)
+            if (h == 1 && s + 1 >= s1) break;
+            const int64_t nx = s + h + 1 < s1 ? s + h + 1 : s + h;         // (the last stage loads something it does not use)
             mx_u4 qn[RT][2];
-            stage(nx, h ^ 1);
+            constexpr int F = 2, SL = 2 * CT / F;
+            mx_u4 f[2][F];
+            const unsigned char* at = &lds[h][lane * 16];
 #pragma unroll
-            for (int i = 0; i < RT; ++i) {
-                qn[i][0] = *reinterpret_cast<const mx_u4*>(qb[i] + nx * 2048 + lane * 16);
-                qn[i][1] = *reinterpret_cast<const mx_u4*>(qb[i] + nx * 2048 + 1024 + lane * 16);
-            }
-            if (h == 0) {
+            for (int c = 0; c < F; ++c) f[0][c] = *reinterpret_cast<const mx_u4*>(at + c * 1024);
 #pragma unroll
-                for (int i = 0; i < RT; ++i) sdn[i] = *reinterpret_cast<const int*>(sb[i] + (sn >> 1) * 256 + lane * 4);
+            for (int sl = 0; sl < SL; ++sl) {
+                const int j = sl * F / CT, c0 = sl * F % CT;
 #pragma unroll
-                for (int c = 0; c < CT; ++c) sxn[c] = *reinterpret_cast<const int*>(xsb[c] + (sn >> 1) * 256 + lane * 4);
-            }
+                for (int n = 0; n < F; ++n) {
+                    const int c = c0 + n;
+                    if (n == 1) {
+                        mx_fence();
+                        // the loads of the next stage, a few a slice: all at once they would fill the address queue and hold the wave up
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+                        for (int p = sl * CH / SL; p < (sl + 1) * CH / SL; ++p) load_a(nx, h ^ 1, p);
 #pragma unroll
-                for (int c = 0; c < CT; ++c) {
-                    const mx_u4 f = *reinterpret_cast<const mx_u4*>(&lds[h][(j * CT + c) * 1024 + lane * 16]);
+                        for (int p = sl * 2 * RT / SL; p < (sl + 1) * 2 * RT / SL; ++p)
+                            qn[p / 2][p & 1] = *reinterpret_cast<const mx_u4*>(qb[p / 2] + nx * 2048 + (p & 1) * 1024 + lane * 16);
+                        if (h == 1) {
+#pragma unroll
+                            for (int p = sl * (RT + CT) / SL; p < (sl + 1) * (RT + CT) / SL; ++p) {
+                                if (p < RT) sdn[p] = *reinterpret_cast<const int*>(sb[p < RT ? p : 0] + (sn >> 1) * 256 + lane * 4);
+                                else sxn[p - RT] = *reinterpret_cast<const int*>(xsb[p < RT ? 0 : p - RT] + (sn >> 1) * 256 + lane * 4);
+                            }
+                        }
+                        if (sl + 1 < SL) {
+#pragma unroll
+                            for (int e = 0; e < F; ++e) f[(sl + 1) & 1][e] = *reinterpret_cast<const mx_u4*>(at + ((sl + 1) * F + e) * 1024);
+                        }
+                    }
 #pragma unroll
                     for (int i = 0; i < RT; ++i) {
                         // (the byte of the scales is part of the instruction)
-                        if (h == 0 && j == 0) acc[i][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(q[i][j]), mx_operand(f), acc[i][c], 4, 4, 0, sd[i], 0, sx[c]);
-                        else if (h == 0) acc[i][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(q[i][j]), mx_operand(f), acc[i][c], 4, 4, 1, sd[i], 1, sx[c]);
-                        else if (j == 0) acc[i][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(q[i][j]), mx_operand(f), acc[i][c], 4, 4, 2, sd[i], 2, sx[c]);
-                        else acc[i][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(q[i][j]), mx_operand(f), acc[i][c], 4, 4, 3, sd[i], 3, sx[c]);
+                        const mx_i8 A = mx_operand(q[i][j]), B = mx_operand(f[sl & 1][n]);
+                        if (h == 0 && j == 0) acc[i][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, acc[i][c], 4, 4, 0, sd[i], 0, sx[c]);
+                        else if (h == 0) acc[i][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, acc[i][c], 4, 4, 1, sd[i], 1, sx[c]);
+                        else if (j == 0) acc[i][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, acc[i][c], 4, 4, 2, sd[i], 2, sx[c]);
+                        else acc[i][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, acc[i][c], 4, 4, 3, sd[i], 3, sx[c]);
                     }
                 }
+                mx_fence();
+            }
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < RT; ++i) { q[i][0] = qn[i][0]; q[i][1] = qn[i][1]; }
@@ -943,13 +1028,7 @@ __global__ __launch_bounds__(256, 2) void mx_matmul_tile_kernel(const unsigned c
 #pragma unroll
         for (int c = 0; c < CT; ++c) sx[c] = sxn[c];
     }
-#pragma unroll
-    for (int c = 0; c < CT; ++c)
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-            float o[4] = {acc[i][c][0], acc[i][c][1], acc[i][c][2], acc[i][c][3]};
-            mx_store<T, 4>(w, tile.z, ((int64_t)tile.a * CT + c) * 16 + l, (((int64_t)tile.b * 4 + wave) * RT + i) * 16 + 4 * g, o);
-        }
+    mx_store_tile<T, RT, CT>(w, tile.z, (int64_t)tile.a * CT * 16, ((int64_t)tile.b * 4 + wave) * RT * 16, l, g, acc);
 }
 
 template <typename T>

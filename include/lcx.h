@@ -442,7 +442,8 @@ int lcx_kernel_name(lcx_ctx* h, int kind, char* buf, int64_t len);
  * These entry points have no handle: every pointer is device memory of the current device, the work goes to `stream` (a hipStream_t of
  * that device, NULL = the default stream) and the call returns without waiting; nothing is kept from one call to the next, so calls on
  * different streams may overlap.  Codes, scales and work space must be 16-byte aligned.  Strides count elements.  rows, cols, M, N, K
- * may be 0: an empty output is left alone, an empty contraction gives zeros.  Outputs must not overlap inputs. */
+ * may be 0: an empty output is left alone, an empty contraction gives zeros.  Outputs must not overlap inputs.  Sizes from 2^31 on, and
+ * matrices of more pieces of 16 rows x 512 columns than a launch can count (2^24), are refused with LCX_ERR_ARG. */
 int lcx_mx4_layout(int64_t rows, int64_t cols, int64_t* code_bytes, int64_t* scale_bytes);
 /* x[r * row_stride + c * col_stride] (any lcx_dtype) -> codes, scales; blocks run along c */
 int lcx_mx4_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, int64_t col_stride, void* codes,

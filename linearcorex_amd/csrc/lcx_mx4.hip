@@ -28,8 +28,9 @@ constexpr int MX_CUS = 256;            // blocks are sized for a whole MI355X; t
 static int64_t dim_bad(int64_t a, int64_t b, int64_t c = 0) { return a < 0 || b < 0 || c < 0 || a >= MX_MAX_DIM || b >= MX_MAX_DIM || c >= MX_MAX_DIM; }
 static bool mx_misaligned(const void* codes, const void* scales) { return (((uintptr_t)codes | (uintptr_t)scales) & 15) != 0; }
 
-static int mx_grid(int64_t mtiles, int64_t ntiles, unsigned* g) {
-    if (mtiles * ntiles > 0x7fffffffll) return fail(LCX_ERR_ARG, "lcx_mx4: the output is too large for one call");
+// a launch counts its threads in 32 bits
+static int mx_grid(int64_t mtiles, int64_t ntiles, int threads, unsigned* g) {
+    if (mtiles * ntiles > 0xffffffffll / threads) return fail(LCX_ERR_ARG, "lcx_mx4: the matrix is too large for one call");
     *g = (unsigned)(mtiles * ntiles);
     return LCX_OK;
 }
@@ -39,10 +40,10 @@ static int mx4_quantize(const void* x, int64_t rows, int64_t cols, int64_t rs, i
     unsigned char *qc = (unsigned char*)codes, *qs = (unsigned char*)scales;
     unsigned g;
     if (rs == 1 && cs != 1) {
-        LCXCHECK(mx_grid(cdiv(rows, 64), mx_quads(cols), &g));
+        LCXCHECK(mx_grid(cdiv(rows, 64), mx_quads(cols), 512, &g));
         hipLaunchKernelGGL((mx_quantize_across_kernel<T>), dim3(g), dim3(512), 0, st, (const T*)x, rows, cols, cs, qc, qs);
     } else {
-        LCXCHECK(mx_grid(mx_row_tiles(rows), mx_quads(cols), &g));
+        LCXCHECK(mx_grid(mx_row_tiles(rows), mx_quads(cols), 256, &g));
         if (cs == 1) hipLaunchKernelGGL((mx_quantize_kernel<T, true>), dim3(g), dim3(256), 0, st, (const T*)x, rows, cols, rs, cs, qc, qs,
                                         mx_steps(cols), mx_quads(cols), (int64_t)0, (unsigned)mx_quads(cols));
         else hipLaunchKernelGGL((mx_quantize_kernel<T, false>), dim3(g), dim3(256), 0, st, (const T*)x, rows, cols, rs, cs, qc, qs, mx_steps(cols),
@@ -57,10 +58,10 @@ static int mx4_dequantize(const void* codes, const void* scales, int64_t rows, i
     const unsigned char *qc = (const unsigned char*)codes, *qs = (const unsigned char*)scales;
     unsigned g;
     if (rs == 1 && cs != 1) {
-        LCXCHECK(mx_grid(cdiv(rows, 64), mx_quads(cols), &g));
+        LCXCHECK(mx_grid(cdiv(rows, 64), mx_quads(cols), 512, &g));
         hipLaunchKernelGGL((mx_dequantize_across_kernel<T>), dim3(g), dim3(512), 0, st, qc, qs, rows, cols, (T*)out, cs);
     } else {
-        LCXCHECK(mx_grid(mx_row_tiles(rows), mx_quads(cols), &g));
+        LCXCHECK(mx_grid(mx_row_tiles(rows), mx_quads(cols), 256, &g));
         if (cs == 1) hipLaunchKernelGGL((mx_dequantize_kernel<T, true>), dim3(g), dim3(256), 0, st, qc, qs, rows, cols, (T*)out, rs, cs, mx_steps(cols),
                                         mx_quads(cols), (int64_t)0, (unsigned)mx_quads(cols));
         else hipLaunchKernelGGL((mx_dequantize_kernel<T, false>), dim3(g), dim3(256), 0, st, qc, qs, rows, cols, (T*)out, rs, cs, mx_steps(cols),
@@ -146,7 +147,7 @@ template <typename T, bool ALONG>
 static int mx_fragments(const T* x, int64_t M, int64_t rs, int64_t cs, int64_t C, const MxPlan& p, unsigned short* frag, const MxExtra& ex, hipStream_t st) {
     const int64_t tiles = p.mt * p.ct;
     unsigned g;
-    LCXCHECK(mx_grid(tiles, cdiv(p.nfrag * 4, 16), &g));
+    LCXCHECK(mx_grid(tiles, cdiv(p.nfrag * 4, 16), 256, &g));
     const int rows_first = (rs < 0 ? -rs : rs) < (cs < 0 ? -cs : cs);
     if (cs == 1)
         hipLaunchKernelGGL((mx_fragments_kernel<T, ALONG, true>), dim3(g), dim3(256), 0, st, x, M, rs, cs, C, p.nfrag, tiles, frag, 0, ex.kscale, ex.skip);
@@ -175,7 +176,7 @@ template <typename T, int CT, int JS>
 static int mx_linear_tiles(const MxPlan& p, const unsigned short* frag, const unsigned char* wc, const unsigned char* ws, int64_t N, int64_t K, const MxOut<T>& w,
                            hipStream_t st) {
     unsigned g;
-    LCXCHECK(mx_grid(8, cdiv(p.mt * p.nt * p.split, 8), &g));
+    LCXCHECK(mx_grid(8, cdiv(p.mt * p.nt * p.split, 8), 256, &g));
     hipLaunchKernelGGL((mx_linear_tile_kernel<T, CT, 4, JS>), dim3(g), dim3(256), 0, st, frag, p.mt * p.ct, wc, ws, N, K, w, (int)p.mt, (int)p.nt, p.split);
     KCHECK();
     return LCX_OK;
@@ -184,7 +185,7 @@ template <typename T, int CT, int JS>
 static int mx_grad_tiles(const MxPlan& p, const unsigned short* frag, const unsigned char* wc, const unsigned char* ws, int64_t N, int64_t K, const MxOut<T>& w,
                          hipStream_t st) {
     unsigned g;
-    LCXCHECK(mx_grid(8, cdiv(p.mt * p.nt * p.split, 8), &g));
+    LCXCHECK(mx_grid(8, cdiv(p.mt * p.nt * p.split, 8), 256, &g));
     constexpr size_t lds = MxGradLds<CT, JS, MxTerms<T>::v>::total;
     LCXCHECK(allow_lds(mx_grad_tile_kernel<T, CT, JS>, lds));
     hipLaunchKernelGGL((mx_grad_tile_kernel<T, CT, JS>), dim3(g), dim3(256), lds, st, frag, p.mt * p.ct, wc, ws, N, K, w, (int)p.mt, (int)p.nt, p.split);
@@ -196,7 +197,7 @@ template <typename T, bool VEC>
 static int mx_linear_rows(const MxPlan& p, const T* x, int64_t rs, int64_t cs, const unsigned char* wc, const unsigned char* ws, int64_t N, int64_t K,
                           const MxOut<T>& w, hipStream_t st) {
     unsigned g;
-    LCXCHECK(mx_grid(1, cdiv(N, 16 * p.rt), &g));
+    LCXCHECK(mx_grid(1, cdiv(N, 16 * p.rt), 64 * p.waves, &g));
 #define MX_ROWS(RT, WV) hipLaunchKernelGGL((mx_linear_row_kernel<T, RT, WV, VEC>), dim3(g), dim3(64 * WV), 0, st, x, w.M, rs, cs, wc, ws, N, K, w)
     if (p.rt == 2) MX_ROWS(2, 8);
     else if (p.waves == 8) MX_ROWS(1, 8);
@@ -280,7 +281,7 @@ template <typename T, int CT, int RT>
 static int mx_matmul_tiles(const MxMatmulPlan& p, const unsigned char* ac, const unsigned char* as, const unsigned char* bc, const unsigned char* bs, int64_t N,
                            int64_t K, const MxOut<T>& w, hipStream_t st) {
     unsigned g;
-    LCXCHECK(mx_grid(8, cdiv(p.mt * p.nt * p.split, 8), &g));
+    LCXCHECK(mx_grid(8, cdiv(p.mt * p.nt * p.split, 8), 256, &g));
     hipLaunchKernelGGL((mx_matmul_tile_kernel<T, CT, RT>), dim3(g), dim3(256), 0, st, ac, as, bc, bs, N, K, w, (int)p.mt, (int)p.nt, p.split);
     KCHECK();
     return LCX_OK;
@@ -296,7 +297,7 @@ static int mx4_matmul(const void* acv, const void* asv, int64_t M, const void* b
     MxOut<T> w{(T*)out, rs, cs, p.split > 1 ? (float*)space : nullptr, M, N, rs == 1 && cs != 1, nullptr, nullptr};
     if (p.row) {
         unsigned g;
-        LCXCHECK(mx_grid(1, cdiv(N, 16 * p.rt), &g));
+        LCXCHECK(mx_grid(1, cdiv(N, 16 * p.rt), 64 * p.waves, &g));
 #define MX_ROWS(RT, WV) hipLaunchKernelGGL((mx_matmul_row_kernel<T, RT, WV>), dim3(g), dim3(64 * WV), 0, st, ac, as, M, bc, bs, N, K, w)
         if (p.rt == 2) {
             if (p.waves == 8) MX_ROWS(2, 8); else MX_ROWS(2, 16);
@@ -335,7 +336,7 @@ int lcx_mx_shard_alloc(lcx_ctx* h) {
 static int mx_shard_block(lcx_ctx* h, float* stage, int64_t ld, int64_t c0, int64_t cols, bool fill) {
     const int64_t nq = mx_quads(cols);
     unsigned g;
-    LCXCHECK(mx_grid(mx_row_tiles(h->Npad), nq, &g));
+    LCXCHECK(mx_grid(mx_row_tiles(h->Npad), nq, 256, &g));
     unsigned char *qc = (unsigned char*)h->xq, *qs = (unsigned char*)h->xs;
     if (fill) {
         hipLaunchKernelGGL((mx_quantize_kernel<float, true>), dim3(g), dim3(256), 0, h->stream, stage, h->Npad, cols, ld, (int64_t)1, qc, qs, mx_steps(h->ldx),

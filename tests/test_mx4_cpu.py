@@ -99,3 +99,25 @@ def test_a_fit_refuses_4_bit_data_where_they_do_not_exist(lib):
     for args in ((100, 20, 4, 1, 0, 1), (100, 20, 129, 0, 0, 1), (100, 20, 4, 0, 0, 2)):
         assert lib.lcx_create_stored(C.byref(h), *args) == 1 and not h.value
         assert b"lcx_create_stored" in lib.lcx_last_error()
+
+
+def test_sizes_beyond_one_launch_are_refused(lib):
+    """a launch counts its threads in 32 bits; what needs more is turned down (before a launch: the pointers are not real)"""
+    p, big = 4096, (1 << 31) - 1
+    for name, args in (("lcx_mx4_quantize", (p, 0, big, 1, 1, 1, p, p, None)), ("lcx_mx4_quantize", (p, 2, big, 1024, 1, big, p, p, None)),
+                       ("lcx_mx4_quantize", (p, 3, (1 << 28) + 1, 16, 16, 1, p, p, None)), ("lcx_mx4_dequantize", (p, p, big, 1, p, 0, 1, 1, None)),
+                       ("lcx_mx4_dequantize", (p, p, big, 1024, p, 0, 1, big, None)), ("lcx_mx4_linear", (p, 0, 1, 8, 1, p, p, big, 8, p, big, 1, None, 0, None)),
+                       ("lcx_mx4_matmul", (p, p, 1, p, p, big, 8, p, 0, big, 1, None, 0, None))):
+        rc, msg = _call(lib, name, *args)
+        assert rc == 1 and "too large" in msg, (name, args, rc, msg)
+
+
+def test_work_space_that_does_not_do_is_refused(lib):
+    p, b = 4096, C.c_int64()
+    for op, name, args in ((0, "lcx_mx4_matmul", (p, p, 40, p, p, 500, 9000, p, 0, 500, 1)),
+                           (1, "lcx_mx4_linear", (p, 0, 40, 9000, 1, p, p, 500, 9000, p, 500, 1)),
+                           (2, "lcx_mx4_linear_grad", (p, 0, 40, 500, 1, p, p, 500, 9000, p, 9000, 1))):
+        assert lib.lcx_mx4_workspace(op, 0, 40, 500, 9000, C.byref(b)) == 0 and b.value > 0
+        for space, size in ((None, b.value), (None, 0), (p, b.value - 1), (p + 8, b.value)):
+            rc, msg = _call(lib, name, *args, space, size, None)
+            assert rc == 1 and msg.startswith(name) and "work space" in msg, (name, space, size, rc, msg)

@@ -42,13 +42,18 @@ class Mx4(object):
     shape   (rows, columns) of the matrix
     axis    the axis along which 32 neighbours share a scale: 1 = along a row, 0 = along a column
     codes, scales   its device buffers (uint8): of the matrix itself for axis 1, of its transpose for axis 0
-    `q.t()` is the transposed matrix on the same buffers.  Like any tensor, a matrix that is used on another stream than the one it was
-    made on must outlive that use."""
+    `q.t()` is the transposed matrix on the same buffers; `copy.deepcopy` and pickling copy them.  Like any tensor, a matrix that is used on
+    another stream than the one it was made on must outlive that use."""
 
     __slots__ = ("shape", "axis", "index", "_buf", "_codes", "_scales", "_cp", "_sp")
 
     def __init__(self, shape, axis, codes, scales):
-        self.shape, self.axis, self._buf, self._codes, self._scales = shape, axis, None, codes, scales
+        self.shape, self.axis, self._buf, self._codes, self._scales = tuple(shape), axis, None, codes, scales
+        if axis not in (0, 1) or len(self.shape) != 2:
+            raise ValueError("a matrix has two dimensions and its blocks run along axis 0 or 1")
+        for t, n, what in zip((codes, scales), _sizes(*self._stored()), ("codes", "scales")):
+            if t.dtype != torch.uint8 or t.numel() != n or not t.is_contiguous() or t.device != codes.device:
+                raise ValueError("%s of a matrix of shape %r must be %d contiguous bytes on one device" % (what, self.shape, n))
         self.index, self._cp, self._sp = codes.get_device(), codes.data_ptr(), scales.data_ptr()
 
     @classmethod
@@ -84,6 +89,10 @@ class Mx4(object):
         q._buf, q._codes, q._scales, q._cp, q._sp = self._buf, self._codes, self._scales, self._cp, self._sp
         return q
 
+    def __reduce__(self):
+        # (the addresses are the buffers' own: a copy takes its own)
+        return Mx4, (self.shape, self.axis, self.codes, self.scales)
+
     def _stored(self):
         """(rows, columns) of the buffers: blocks run along the columns"""
         return self.shape if self.axis == 1 else (self.shape[1], self.shape[0])
@@ -111,6 +120,8 @@ _entry = {}
 
 def _call(index, name, *args):
     """one entry point on the current stream of device `index`"""
+    if index < 0:
+        raise ValueError("the matrix must be on the GPU (there is no CPU fallback)")
     fn = _entry.get(name)
     if fn is None:
         fn = _entry[name] = getattr(_abi.load(), name)

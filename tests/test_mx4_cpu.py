@@ -101,6 +101,23 @@ def test_a_fit_refuses_4_bit_data_where_they_do_not_exist(lib):
         assert b"lcx_create_stored" in lib.lcx_last_error()
 
 
+def test_a_matrix_of_buffers_that_do_not_fit_is_refused():
+    import copy
+    cb, sb = mx4._sizes(20, 300)
+    c, s = torch.zeros(cb, dtype=torch.uint8), torch.zeros(sb, dtype=torch.uint8)
+    for shape, axis, codes, scales in (((20, 300), 1, c[1:], s), ((20, 300), 1, c, s[1:]), ((20, 300), 0, c, s), ((20, 300), 1, c.int(), s),
+                                       ((20, 300), 1, c, torch.zeros(2 * sb, dtype=torch.uint8)[::2]), ((20, 300), 2, c, s), ((20,), 1, c, s)):
+        with pytest.raises(ValueError):
+            mx4.Mx4(shape, axis, codes, scales)
+    # on the host: copies hold their own buffers, no operator takes them
+    q = mx4.Mx4((20, 300), 1, c, s)
+    d, e = copy.deepcopy(q), copy.copy(q)
+    assert d._cp == d.codes.data_ptr() != q._cp and d._sp == d.scales.data_ptr() != q._sp and e._cp == q._cp and e.shape == q.shape
+    for call in (lambda: mx4.dequantize(q), lambda: mx4.matmul(q, q)):
+        with pytest.raises(ValueError, match="must be on the GPU"):
+            call()
+
+
 def test_sizes_beyond_one_launch_are_refused(lib):
     """a launch counts its threads in 32 bits; what needs more is turned down (before a launch: the pointers are not real)"""
     p, big = 4096, (1 << 31) - 1

@@ -348,3 +348,41 @@ def test_offsets_beyond_32_bits(mx4):
     z = mx4.quantize(x)
     one = k // 128 * 1024
     assert torch.equal(z.codes[-one:], z.codes[:one]) and torch.equal(z.scales[-one // 16:], z.scales[:one // 16])
+
+
+def test_copies_of_a_matrix_hold_their_own_buffers(mx4):
+    import copy
+    import pickle
+    for axis in (0, 1):
+        w, x = ints((70, 300), 1, torch.float32, hi=2), ints((5, 300), 2, torch.bfloat16)
+        q = mx4.quantize(w, axis=axis)
+        want = mx4.linear(x, q)
+        copies = [copy.deepcopy(q), pickle.loads(pickle.dumps(q)), copy.deepcopy(q.t()).t()]
+        q.codes.zero_()
+        for c in copies:
+            assert c.codes.data_ptr() == c._cp != q._cp and c.scales.data_ptr() == c._sp
+            assert torch.equal(mx4.linear(x, c), want) and torch.equal(mx4.dequantize(c), w)
+        assert not mx4.linear(x, q).any()
+
+
+@pytest.mark.parametrize("dt", PRODUCT, ids=ids)
+def test_captured_gradient(mx4, dt):
+    """forward and backward of a leaf in one graph, replayed with new values"""
+    q = mx4.quantize(ints((90, 333), 1, torch.float32, hi=2))
+    xs, dys = [ints((2, 37, 333), 5 + i, dt) for i in range(3)], [ints((2, 37, 90), 9 + i, dt) for i in range(3)]
+    want = [(mx4.linear(a, q), mx4.linear_grad(b, q)) for a, b in zip(xs, dys)]
+    x, dy = xs[0].clone().requires_grad_(True), dys[0].clone()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = mx4.linear(x, q)
+        dx, = torch.autograd.grad(y, x, dy)
+    for i in (0, 1, 2, 0):
+        with torch.no_grad():
+            x.copy_(xs[i])
+        dy.copy_(dys[i])
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y.detach(), want[i][0]) and torch.equal(dx, want[i][1])
+        again = mx4.linear(xs[i], q)
+        assert torch.equal(again, want[i][0])

@@ -459,7 +459,8 @@ int lcx_mx4_workspace(int op, int dtype, int64_t M, int64_t N, int64_t K, int64_
 int lcx_mx4_matmul(const void* a_codes, const void* a_scales, int64_t M, const void* b_codes, const void* b_scales, int64_t N, int64_t K,
                    void* out, int dtype, int64_t row_stride, int64_t col_stride, void* workspace, int64_t workspace_bytes, void* stream);
 /* out[m * row_stride + n * col_stride] = sum_k x[m][k] W[n][k]: x (M x K, LCX_F32 / LCX_BF16 / LCX_F16, strides x_row / x_col) as it is, W an
- * mx4 matrix N x K; products exact (x is split into bf16 numbers without loss), sums in float32, out in x's type, rounded once */
+ * mx4 matrix N x K; products exact (x is split into bf16 numbers without loss, but for bits of a
+ * float32 number below 2^-133, bf16's last place), sums in float32, out in x's type, rounded once */
 int lcx_mx4_linear(const void* x, int dtype, int64_t M, int64_t x_row, int64_t x_col, const void* codes, const void* scales, int64_t N,
                    int64_t K, void* out, int64_t row_stride, int64_t col_stride, void* workspace, int64_t workspace_bytes, void* stream);
 /* out[m * row_stride + k * col_stride] = sum_n dy[m][n] W[n][k]: the gradient of lcx_mx4_linear with respect to x (dy M x N), and the product

@@ -39,7 +39,8 @@ template <> struct MxTerms<__bf16> { static constexpr int v = 1; };
 __device__ __forceinline__ float mx_trunc_bf16(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 // x = term 0 + term 1 + term 2, each a bf16 number: the leading 8 significant bits are cut off twice, what remains has at most 8.  Every
 // term takes part in the products below, so cutting (rather than rounding) leaves no bias.  An infinity stays in term 0 alone (its
-// remainder would be a NaN); a NaN leaves one in the remainder, whatever the cut makes of its payload.
+// remainder would be a NaN); a NaN leaves one in the remainder, whatever the cut makes of its payload.  Numbers below 2^-110 reach under
+// bf16's last place, 2^-133: the last term is rounded to it.
 template <int TERMS> __device__ __forceinline__ void mx_split(float x, float* t) {
     if constexpr (TERMS == 1) {
         t[0] = x;

@@ -155,6 +155,7 @@ def quantize(x, axis=1):
     if isinstance(axis, bool) or axis not in (0, 1, -1, -2):
         raise ValueError("axis must be 0 or 1")
     axis %= 2
+    x = x.resolve_neg()                  # (the imaginary part of a conjugated view)
     (rows, cols), (rs, cs) = x.shape, x.stride()
     shape = (rows, cols)
     if axis == 0:
@@ -209,6 +210,7 @@ def _product(x, q, along):
     n, k = q._stored()
     c, o = (k, n) if along else (n, k)
     lead = x.shape[:-1]
+    x = x.resolve_neg()
     if x.dim() == 2:
         m, x2 = lead[0], x
     else:
@@ -261,8 +263,8 @@ def _checked(x, q, what, contracted):
 def linear(x, q):
     """x (..., K) . q (N, K)^T -> (..., N) in x's type (float32, bfloat16, float16): x as it is, the matrix in 4 bits.
 
-    Every product is exact (x enters as a sum of bfloat16 numbers: three for float32, two for float16), the sums are float32, the
-    result is rounded once.  Any strides of x.  Differentiable with respect to x, any number of times; q is a constant.  Blocks of q
+    Every product is exact (x enters as a sum of bfloat16 numbers: three for float32, two for float16; what a float32 number holds below
+    bfloat16's last place, 2^-133, is rounded to it), the sums are float32, the result is rounded once.  Any strides of x.  Differentiable with respect to x, any number of times; q is a constant.  Blocks of q
     along either axis."""
     _checked(x, q, "x", 1)
     return _apply(x, q, q.axis == 1)

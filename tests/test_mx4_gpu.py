@@ -365,6 +365,16 @@ def test_copies_of_a_matrix_hold_their_own_buffers(mx4):
         assert not mx4.linear(x, q).any()
 
 
+def test_views_that_negate_lazily(mx4):
+    """the imaginary part of a conjugated view is stored with the other sign"""
+    z = torch.complex(ints((40, 96), 1, torch.float32), ints((40, 96), 2, torch.float32))
+    x = z.conj().imag
+    assert x.is_neg()
+    q = mx4.quantize(ints((24, 96), 3, torch.float32, hi=2))
+    assert torch.equal(mx4.dequantize(mx4.quantize(x)), mx4.dequantize(mx4.quantize(-z.imag)))
+    assert torch.equal(mx4.linear(x, q), -mx4.linear(z.imag, q)) and torch.equal(mx4.linear_grad(x[:, :24], q), -mx4.linear_grad(z.imag[:, :24], q))
+
+
 @pytest.mark.parametrize("dt", PRODUCT, ids=ids)
 def test_captured_gradient(mx4, dt):
     """forward and backward of a leaf in one graph, replayed with new values"""

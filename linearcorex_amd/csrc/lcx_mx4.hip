@@ -262,7 +262,7 @@ static MxMatmulPlan mx_matmul_plan(int64_t M, int64_t N, int64_t K) {
     if (M <= 16) {
         p.row = true;
         p.rt = N >= 64 * MX_CUS ? 2 : 1;
-        p.waves = cdiv(N, 16 * p.rt) >= 2 * MX_CUS ? 8 : 16;
+        p.waves = p.rt == 2 || cdiv(N, 16) >= 2 * MX_CUS ? 8 : 16;
         return p;
     }
     // tiles of 128 rows of A where there are so many, the contraction split while CUs are left over
@@ -299,11 +299,9 @@ static int mx4_matmul(const void* acv, const void* asv, int64_t M, const void* b
         unsigned g;
         LCXCHECK(mx_grid(1, cdiv(N, 16 * p.rt), 64 * p.waves, &g));
 #define MX_ROWS(RT, WV) hipLaunchKernelGGL((mx_matmul_row_kernel<T, RT, WV>), dim3(g), dim3(64 * WV), 0, st, ac, as, M, bc, bs, N, K, w)
-        if (p.rt == 2) {
-            if (p.waves == 8) MX_ROWS(2, 8); else MX_ROWS(2, 16);
-        } else {
-            if (p.waves == 8) MX_ROWS(1, 8); else MX_ROWS(1, 16);
-        }
+        if (p.rt == 2) MX_ROWS(2, 8);
+        else if (p.waves == 8) MX_ROWS(1, 8);
+        else MX_ROWS(1, 16);
 #undef MX_ROWS
         KCHECK();
         return LCX_OK;

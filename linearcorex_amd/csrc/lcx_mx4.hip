@@ -90,14 +90,33 @@ struct MxPlan {
     int64_t frag_bytes = 0, part_bytes = 0;
 };
 
-// Parts a contraction of `steps` is cut into for `tiles` output tiles on `slots` resident blocks: time of the rounds (a block's steps and,
-// worth `fixed` of them, its start and its outputs) and of writing and adding up the partial sums (`join` steps a part)
-static int64_t split_for(int64_t tiles, int64_t steps, int64_t slots, double fixed, double join) {
-    int64_t best = 1;
-    double best_t = 1e300;
-    for (int64_t s = 1; s <= 64 && s <= steps; ++s) {
-        const double t = (double)cdiv(tiles * s, slots) * ((double)cdiv(steps, s) + fixed) + (s > 1 ? join * (double)s + fixed : 0.0);
-        if (t < best_t * 0.98) { best_t = t; best = s; }
+// Time of a tile kernel's step on a CU that holds one block (t1 + u1 x its work) or two (t2 + u2 x), in us: the work is the 16-row tiles of x per
+// block, times the bf16 terms.  A step is 128 of the contraction (lcx_mx4_matmul: 512).  pair: what a second block a CU costs once.
+// (Fitted to products of 256, 512, 768 and 1024 tiles, contractions of 4096 and 8192.)
+struct MxStep { double t1, u1, t2, u2, pair; };
+
+// Tile height (16 ct rows of x) and parts of the contraction for M rows, `cols` tiles over the O outputs and `steps`: least time of
+//   steps of a part x step time at so many blocks a CU (a second block on some CUs only counts half and its share of the other half,
+//     a later one three quarters)
+//   + start and outputs of a block, 1 us and 1.2 more per 16 rows
+//   + writing the parts and adding them up: 7 TB/s, 3 us for the launch, 0.1 a part
+// Within 10 % of the best of all (ct, split) over 78 sizes from 24 x 4096 x 4096 to 2048 x 14336 x 4096, and 512 x 20000 x 20000.  What it weighs, us:
+// bf16 512 x 14336 x 4096 in tiles of ct 2 / 4 / 8: 70 / 59 / 64; float32 64 x 20000 x 20000 in 1 / 3 / 6 / 8 parts: 345 / 134 / 123 / 141
+static double mx_choose(int64_t M, int64_t O, int64_t cols, int64_t steps, int terms, int min_ct, int max_ct, const MxStep& c, int* ct_out, int* split_out) {
+    *ct_out = min_ct;
+    *split_out = 1;
+    double best = 1e300;
+    for (int ct = min_ct; ct <= max_ct && (ct == min_ct || 8 * ct < M); ct *= 2) {
+        const int64_t tiles = cdiv(M, 16 * ct) * cols;
+        const double one = c.t1 + c.u1 * ct * terms, two = c.t2 + c.u2 * ct * terms, fixed = 1.0 + 1.2 * ct;
+        for (int64_t s = 1; s <= 64 && s <= steps && (s == 1 || tiles * s <= 4 * MX_CUS); ++s) {
+            const int64_t full = tiles * s / MX_CUS, rest = tiles * s % MX_CUS;
+            const double b = full == 0 ? 1.0 : (double)full + (rest == 0 ? 0.0 : full == 1 ? 0.5 + 0.5 * (double)rest / MX_CUS : 0.75 + 0.25 * (double)rest / MX_CUS);
+            const double step = b <= 2.0 ? one + (two - one) * (b - 1.0) : two * 0.5 * b;
+            const double t = (double)cdiv(steps, s) * step + (b <= 2.0 ? fixed + c.pair * (b - 1.0) : (fixed + c.pair) * 0.5 * b) +
+                             (s > 1 ? (double)(s * M * O) * 8 / 7e6 + 3.0 + 0.1 * (double)s : 0.0);
+            if (t < best * 0.98) { best = t; *ct_out = ct; *split_out = (int)s; }
+        }
     }
     return best;
 }
@@ -114,23 +133,36 @@ struct MxExtra {
 template <typename T> static MxPlan mx_plan(bool along, int64_t M, int64_t C, int64_t O, bool tiles = false) {
     constexpr int TERMS = MxTerms<T>::v;
     MxPlan p;
+    p.rt = 4;
+    p.nt = along ? cdiv(O, 64 * p.rt) : cdiv(O, 512);
+    const MxStep step = along        ? MxStep{0.58, 0.145, 0.4, 0.33, 0.0}
+                        : TERMS == 1 ? MxStep{1.7, 0.21, 1.9, 0.48, 4.0}
+                                     : MxStep{2.7, 0.19, 2.1, 0.53, 4.0};
+    const double t = mx_choose(M, O, p.nt, cdiv(C, 128), TERMS, M <= 16 ? 1 : 2, along && TERMS == 1 ? 8 : 4, step, &p.ct, &p.split);
     if (M <= 16 && along && !tiles) {
-        p.row = true;
-        // 2 x 16 rows of W a wave halve the reads of x where there are enough rows to fill the chip; 16 waves split the contraction
-        // where there are few
-        p.rt = M <= 4 || O < 32 * MX_CUS ? 1 : 2;
-        p.waves = p.rt == 2 || cdiv(O, 16) >= 2 * MX_CUS ? 8 : 16;
-    } else {
-        p.ct = M <= 16 ? 1 : M <= 32 ? 2 : M <= 64 || TERMS > 1 || !along ? 4 : 8;
-        p.rt = 4;
-        p.mt = cdiv(M, 16 * p.ct);
-        p.nt = along ? cdiv(O, 64 * p.rt) : cdiv(O, 512);
-        p.nfrag = cdiv(C, 128) * 4;
-        // a step of 128 takes two blocks of a CU about 0.4 us per tile of 16 rows and bf16 term; partial sums move at about 4 TB/s
-        const double step_us = 0.4 * p.ct * TERMS;
-        p.split = (int)split_for(p.mt * p.nt, cdiv(C, 128), 2 * MX_CUS, 3.0 / step_us, (double)M * O * 8 / 4e6 / step_us);
-        p.frag_bytes = p.nfrag * TERMS * p.mt * p.ct * 1024;
+        // The row kernel or the tiles, whichever takes less time by these models (fitted for K and N from 512 to 28672; 10 %):
+        //   row    3.5 us + the steps a CU works through
+        //   tiles  mx_choose, or reading W; 8 us for the two launches more
+        // Measured, us, row / tiles: 1 x 4096 x 4096 bf16 4.7 / 11; 16 x 20000 x 20000 bf16 68 / 42, float32 135 / 49.
+        // 2 x 16 rows of W a wave halve the reads of x where there are enough rows to fill the chip (4 x 14336 x 4096 bf16 11.1 -> 8.7; 4 x 4096 x
+        // 4096 5.2 -> 5.9); 16 waves split the contraction where there are few
+        const int rt = O < 32 * MX_CUS ? 1 : 2;
+        const double blocks = (double)cdiv(O, 16 * rt) / MX_CUS;
+        const double row = 3.5 + (double)cdiv(C, 128) * (blocks < 1.0 ? 1.0 : blocks) *
+                                     ((rt == 2 ? 0.09 : 0.04) + (TERMS == 1 ? 0.0 : TERMS == 2 ? 0.075 : 0.09) +
+                                      (TERMS == 1 ? 0.0045 : TERMS == 2 ? 0.002 : 0.0075) * (double)M);
+        const double read = (double)O * (double)C * 0.53 / 6e6 + 5.0;
+        if (row <= (t > read ? t : read) + 8.0) {
+            p = MxPlan();
+            p.row = true;
+            p.rt = rt;
+            p.waves = rt == 2 || cdiv(O, 16) >= 2 * MX_CUS ? 8 : 16;
+            return p;
+        }
     }
+    p.mt = cdiv(M, 16 * p.ct);
+    p.nfrag = cdiv(C, 128) * 4;
+    p.frag_bytes = p.nfrag * TERMS * p.mt * p.ct * 1024;
     if (p.split > 1) p.part_bytes = (int64_t)p.split * M * O * 4;
     return p;
 }
@@ -222,9 +254,8 @@ static int mx4_linear(const void* xv, int64_t M, int64_t xrs, int64_t xcs, const
                                                 : mx_linear_rows<T, false>(p, x, xrs, xcs, wc, ws, N, K, w, st);
     LCXCHECK((mx_fragments<T, true>(x, M, xrs, xcs, K, p, frag, ex, st)));
     constexpr int JS = TERMS == 3 ? 2 : 4;
-    if (p.ct == 1) {
-        if constexpr (TERMS == 3) LCXCHECK((mx_linear_tiles<T, 1, 4>(p, frag, wc, ws, N, K, w, st)));
-    } else if (p.ct == 2) LCXCHECK((mx_linear_tiles<T, 2, 4>(p, frag, wc, ws, N, K, w, st)));
+    if (p.ct == 1) LCXCHECK((mx_linear_tiles<T, 1, 4>(p, frag, wc, ws, N, K, w, st)));
+    else if (p.ct == 2) LCXCHECK((mx_linear_tiles<T, 2, 4>(p, frag, wc, ws, N, K, w, st)));
     else if (p.ct == 4) LCXCHECK((mx_linear_tiles<T, 4, JS>(p, frag, wc, ws, N, K, w, st)));
     else {
         if constexpr (TERMS == 1) LCXCHECK((mx_linear_tiles<T, 8, 4>(p, frag, wc, ws, N, K, w, st)));
@@ -261,16 +292,14 @@ static MxMatmulPlan mx_matmul_plan(int64_t M, int64_t N, int64_t K) {
     MxMatmulPlan p;
     if (M <= 16) {
         p.row = true;
-        p.rt = N >= 64 * MX_CUS ? 2 : 1;
+        // (8 x 14336 x 4096, one / two row tiles a wave: 7.0 / 6.3 us; x 4096: 4.2 / 4.5; 28672 x 8192: 19.7 / 20.2)
+        p.rt = N >= 32 * MX_CUS && N < 64 * MX_CUS ? 2 : 1;
         p.waves = p.rt == 2 || cdiv(N, 16) >= 2 * MX_CUS ? 8 : 16;
         return p;
     }
-    // tiles of 128 rows of A where there are so many, the contraction split while CUs are left over
-    p.ct = M <= 32 ? 2 : M <= 64 ? 4 : 8;
-    p.mt = cdiv(M, 16 * p.ct);
     p.nt = cdiv(N, 256);
-    const double quad_us = 0.25 * p.ct;
-    p.split = (int)split_for(p.mt * p.nt, cdiv(K, 512), 2 * MX_CUS, 3.0 / quad_us, (double)M * N * 8 / 4e6 / quad_us);
+    mx_choose(M, N, p.nt, cdiv(K, 512), 1, 2, 8, MxStep{1.5, 0.06, 0.9, 0.34, 5.0}, &p.ct, &p.split);
+    p.mt = cdiv(M, 16 * p.ct);
     if (p.split > 1) p.part_bytes = (int64_t)p.split * M * N * 4;
     return p;
 }

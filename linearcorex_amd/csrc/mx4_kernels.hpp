@@ -393,6 +393,7 @@ __global__ __launch_bounds__(256) void mx_join_kernel(const float* __restrict__ 
         const float f = rscale ? rscale[t] : 1.0f;
         if (o + 4 <= O) {
             mx_f4 v = *reinterpret_cast<const mx_f4u*>(p);
+#pragma unroll 4
             for (int z = 1; z < split; ++z) v += *reinterpret_cast<const mx_f4u*>(p + z * n);
             T* q = out + t * rs + o * cs;
             T r[4];

@@ -83,7 +83,7 @@ template <typename T> static int mx4_zero(void* out, int64_t rows, int64_t cols,
 // What one call does: sizes of its tiles, its splits of the contraction and its work space [fragments of x | partial sums].
 struct MxPlan {
     bool row = false;                  // up to 16 rows of x: the row kernels
-    int ct = 1, rt = 1, waves = 8;     // 16-row tiles of x, of W (linear); waves of a row kernel's block
+    int ct = 1, rt = 1;                // 16-row tiles of x, of W (linear)
     int64_t mt = 1, nt = 1;            // tiles over the rows of x / over the output columns
     int64_t nfrag = 0;                 // fragments of the contraction
     int split = 1;
@@ -145,7 +145,7 @@ template <typename T> static MxPlan mx_plan(bool along, int64_t M, int64_t C, in
         //   tiles  mx_choose, or reading W; 8 us for the two launches more
         // Measured, us, row / tiles: 1 x 4096 x 4096 bf16 4.7 / 11; 16 x 20000 x 20000 bf16 68 / 42, float32 135 / 49.
         // 2 x 16 rows of W a wave halve the reads of x where there are enough rows to fill the chip (4 x 14336 x 4096 bf16 11.1 -> 8.7; 4 x 4096 x
-        // 4096 5.2 -> 5.9); 16 waves split the contraction where there are few
+        // 4096 5.2 -> 5.9)
         const int rt = O < 32 * MX_CUS ? 1 : 2;
         const double blocks = (double)cdiv(O, 16 * rt) / MX_CUS;
         const double row = 3.5 + (double)cdiv(C, 128) * (blocks < 1.0 ? 1.0 : blocks) *
@@ -156,7 +156,6 @@ template <typename T> static MxPlan mx_plan(bool along, int64_t M, int64_t C, in
             p = MxPlan();
             p.row = true;
             p.rt = rt;
-            p.waves = rt == 2 || cdiv(O, 16) >= 2 * MX_CUS ? 8 : 16;
             return p;
         }
     }
@@ -229,11 +228,10 @@ template <typename T, bool VEC>
 static int mx_linear_rows(const MxPlan& p, const T* x, int64_t rs, int64_t cs, const unsigned char* wc, const unsigned char* ws, int64_t N, int64_t K,
                           const MxOut<T>& w, hipStream_t st) {
     unsigned g;
-    LCXCHECK(mx_grid(1, cdiv(N, 16 * p.rt), 64 * p.waves, &g));
-#define MX_ROWS(RT, WV) hipLaunchKernelGGL((mx_linear_row_kernel<T, RT, WV, VEC>), dim3(g), dim3(64 * WV), 0, st, x, w.M, rs, cs, wc, ws, N, K, w)
-    if (p.rt == 2) MX_ROWS(2, 8);
-    else if (p.waves == 8) MX_ROWS(1, 8);
-    else MX_ROWS(1, 16);
+    LCXCHECK(mx_grid(1, cdiv(N, 16 * p.rt), 64 * MX_ROW_WAVES, &g));
+#define MX_ROWS(RT) hipLaunchKernelGGL((mx_linear_row_kernel<T, RT, VEC>), dim3(g), dim3(64 * MX_ROW_WAVES), 0, st, x, w.M, rs, cs, wc, ws, N, K, w)
+    if (p.rt == 2) MX_ROWS(2);
+    else MX_ROWS(1);
 #undef MX_ROWS
     KCHECK();
     return LCX_OK;
@@ -285,7 +283,7 @@ static int mx4_linear_grad(const void* dyv, int64_t M, int64_t yrs, int64_t ycs,
 // ---- 4 bits x 4 bits --------------------------------------------------------------------------------------------------------------------
 struct MxMatmulPlan {
     bool row = false;
-    int ct = 1, rt = 1, waves = 8, split = 1;
+    int ct = 1, rt = 1, split = 1;
     int64_t mt = 1, nt = 1, part_bytes = 0;
 };
 static MxMatmulPlan mx_matmul_plan(int64_t M, int64_t N, int64_t K) {
@@ -294,7 +292,6 @@ static MxMatmulPlan mx_matmul_plan(int64_t M, int64_t N, int64_t K) {
         p.row = true;
         // (8 x 14336 x 4096, one / two row tiles a wave: 7.0 / 6.3 us; x 4096: 4.2 / 4.5; 28672 x 8192: 19.7 / 20.2)
         p.rt = N >= 32 * MX_CUS && N < 64 * MX_CUS ? 2 : 1;
-        p.waves = p.rt == 2 || cdiv(N, 16) >= 2 * MX_CUS ? 8 : 16;
         return p;
     }
     p.nt = cdiv(N, 256);
@@ -326,11 +323,10 @@ static int mx4_matmul(const void* acv, const void* asv, int64_t M, const void* b
     MxOut<T> w{(T*)out, rs, cs, p.split > 1 ? (float*)space : nullptr, M, N, rs == 1 && cs != 1, nullptr, nullptr};
     if (p.row) {
         unsigned g;
-        LCXCHECK(mx_grid(1, cdiv(N, 16 * p.rt), 64 * p.waves, &g));
-#define MX_ROWS(RT, WV) hipLaunchKernelGGL((mx_matmul_row_kernel<T, RT, WV>), dim3(g), dim3(64 * WV), 0, st, ac, as, M, bc, bs, N, K, w)
-        if (p.rt == 2) MX_ROWS(2, 8);
-        else if (p.waves == 8) MX_ROWS(1, 8);
-        else MX_ROWS(1, 16);
+        LCXCHECK(mx_grid(1, cdiv(N, 16 * p.rt), 64 * MX_ROW_WAVES, &g));
+#define MX_ROWS(RT) hipLaunchKernelGGL((mx_matmul_row_kernel<T, RT>), dim3(g), dim3(64 * MX_ROW_WAVES), 0, st, ac, as, M, bc, bs, N, K, w)
+        if (p.rt == 2) MX_ROWS(2);
+        else MX_ROWS(1);
 #undef MX_ROWS
         KCHECK();
         return LCX_OK;

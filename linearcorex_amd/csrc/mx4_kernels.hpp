@@ -438,11 +438,15 @@ __global__ __launch_bounds__(256) void mx_scale_columns_kernel(float* __restrict
 // out[t][n] = sum_k x[t][k] W[n][k], W in 4 bits with its blocks along k: the codes become bf16 in registers, x is split into bf16 terms
 // (MxTerms), every product is exact, float32 sums.  Bound: reading W (4.25 bits a value).  The waves of a block share 16 RT rows of W and
 // split the contraction (128 columns a step), so that a single token still puts every load of W in flight at once; partial sums meet in LDS.
-template <typename T, int RT, int WAVES, bool VEC>
-__global__ __launch_bounds__(64 * WAVES) void mx_linear_row_kernel(const T* __restrict__ x, int64_t M, int64_t xrs, int64_t xcs,
+// Eight waves: sixteen gain where 512 rows meet 20000 columns (11.6 -> 10.9 us) and lose elsewhere (4-bit 8 x 7000 x 4096 4.8 -> 5.6).
+// 1 x 4096 x 4096 bf16 takes 4.7 us (of which a launch is 3.5), 1 x 28672 x 8192 24.8 us, 5.0 TB/s.  Four rows of x cost as much; sixteen read
+// x in scattered 16-byte pieces and take 12.5 us at 14336 x 4096 (2.5 TB/s) where one takes 8.8.  (x through LDS in whole lines: 9 % slower.)
+constexpr int MX_ROW_WAVES = 8;
+template <typename T, int RT, bool VEC>
+__global__ __launch_bounds__(64 * MX_ROW_WAVES) void mx_linear_row_kernel(const T* __restrict__ x, int64_t M, int64_t xrs, int64_t xcs,
                                                                    const unsigned char* __restrict__ wc, const unsigned char* __restrict__ ws, int64_t N,
                                                                    int64_t K, MxOut<T> w) {
-    constexpr int TERMS = MxTerms<T>::v, U = 4;
+    constexpr int TERMS = MxTerms<T>::v, U = 4, WAVES = MX_ROW_WAVES;
     const int64_t ksteps = mx_steps(K), quads = mx_quads(K), rts = mx_row_tiles(N);
     const int64_t n0 = (int64_t)blockIdx.x * 16 * RT;
     const int lane = threadIdx.x & 63, wave = mx_wave(), l = lane & 15, g = lane >> 4;
@@ -863,11 +867,11 @@ __global__ __launch_bounds__(256, 2) void mx_grad_tile_kernel(const unsigned sho
 __device__ __forceinline__ mx_i8 mx_operand(mx_u4 q) { return mx_i8{(int)q[0], (int)q[1], (int)q[2], (int)q[3], 0, 0, 0, 0}; }
 
 // up to 16 rows of A: as mx_linear_row_kernel, bound by reading B
-template <typename T, int RT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void mx_matmul_row_kernel(const unsigned char* __restrict__ ac, const unsigned char* __restrict__ as, int64_t M,
+template <typename T, int RT>
+__global__ __launch_bounds__(64 * MX_ROW_WAVES) void mx_matmul_row_kernel(const unsigned char* __restrict__ ac, const unsigned char* __restrict__ as, int64_t M,
                                                                    const unsigned char* __restrict__ bc, const unsigned char* __restrict__ bs, int64_t N,
                                                                    int64_t K, MxOut<T> w) {
-    constexpr int U = 4;
+    constexpr int U = 4, WAVES = MX_ROW_WAVES;
     const int64_t ksteps = mx_steps(K), quads = mx_quads(K), rts = mx_row_tiles(N);
     const int64_t n0 = (int64_t)blockIdx.x * 16 * RT;
     const int lane = threadIdx.x & 63, wave = mx_wave(), l = lane & 15, g = lane >> 4;

@@ -189,6 +189,11 @@ static int mx_fragments(const T* x, int64_t M, int64_t rs, int64_t cs, int64_t C
     return LCX_OK;
 }
 
+// rows that the tile kernels take as they are (MxDirect; the offsets inside a tile are 32-bit)
+template <typename T> static bool mx_direct(const T* x, int64_t rs, int64_t cs) {
+    return cs == 1 && rs >= 0 && rs < (1 << 23) && rs % 8 == 0 && ((uintptr_t)x & 15) == 0;
+}
+
 template <typename T> static int mx_join(int split, const MxOut<T>& w, hipStream_t st) {
     if (split == 1) return LCX_OK;
     // t_first: the partial sums lie transposed, and so does the output
@@ -203,23 +208,23 @@ template <typename T> static int mx_join(int split, const MxOut<T>& w, hipStream
     return LCX_OK;
 }
 
-template <typename T, int CT, int JS>
-static int mx_linear_tiles(const MxPlan& p, const unsigned short* frag, const unsigned char* wc, const unsigned char* ws, int64_t N, int64_t K, const MxOut<T>& w,
+template <typename T, int CT, int JS, bool DIRECT = false>
+static int mx_linear_tiles(const MxPlan& p, const unsigned short* frag, int64_t tiles, const unsigned char* wc, const unsigned char* ws, int64_t N, int64_t K, const MxOut<T>& w,
                            hipStream_t st) {
     unsigned g;
     LCXCHECK(mx_grid(8, cdiv(p.mt * p.nt * p.split, 8), 256, &g));
-    hipLaunchKernelGGL((mx_linear_tile_kernel<T, CT, 4, JS>), dim3(g), dim3(256), 0, st, frag, p.mt * p.ct, wc, ws, N, K, w, (int)p.mt, (int)p.nt, p.split);
+    hipLaunchKernelGGL((mx_linear_tile_kernel<T, CT, 4, JS, DIRECT>), dim3(g), dim3(256), 0, st, frag, tiles, wc, ws, N, K, w, (int)p.mt, (int)p.nt, p.split);
     KCHECK();
     return LCX_OK;
 }
-template <typename T, int CT, int JS>
-static int mx_grad_tiles(const MxPlan& p, const unsigned short* frag, const unsigned char* wc, const unsigned char* ws, int64_t N, int64_t K, const MxOut<T>& w,
+template <typename T, int CT, int JS, bool DIRECT = false>
+static int mx_grad_tiles(const MxPlan& p, const unsigned short* frag, int64_t tiles, const unsigned char* wc, const unsigned char* ws, int64_t N, int64_t K, const MxOut<T>& w,
                          hipStream_t st) {
     unsigned g;
     LCXCHECK(mx_grid(8, cdiv(p.mt * p.nt * p.split, 8), 256, &g));
     constexpr size_t lds = MxGradLds<CT, JS, MxTerms<T>::v>::total;
-    LCXCHECK(allow_lds(mx_grad_tile_kernel<T, CT, JS>, lds));
-    hipLaunchKernelGGL((mx_grad_tile_kernel<T, CT, JS>), dim3(g), dim3(256), lds, st, frag, p.mt * p.ct, wc, ws, N, K, w, (int)p.mt, (int)p.nt, p.split);
+    LCXCHECK(allow_lds(mx_grad_tile_kernel<T, CT, JS, DIRECT>, lds));
+    hipLaunchKernelGGL((mx_grad_tile_kernel<T, CT, JS, DIRECT>), dim3(g), dim3(256), lds, st, frag, tiles, wc, ws, N, K, w, (int)p.mt, (int)p.nt, p.split);
     KCHECK();
     return LCX_OK;
 }
@@ -250,13 +255,24 @@ static int mx4_linear(const void* xv, int64_t M, int64_t xrs, int64_t xcs, const
     MxOut<T> w{(T*)out, rs, cs, p.split > 1 ? (float*)((char*)space + round_up(p.frag_bytes, 256)) : nullptr, M, N, rs == 1 && cs != 1, ex.oscale, ex.skip};
     if (p.row) return xcs == 1 ? mx_linear_rows<T, true>(p, x, xrs, xcs, wc, ws, N, K, w, st)
                                                 : mx_linear_rows<T, false>(p, x, xrs, xcs, wc, ws, N, K, w, st);
+    if constexpr (TERMS == 1) {
+        if (K % 128 == 0 && mx_direct(x, xrs, xcs)) {
+            const unsigned short* xb = (const unsigned short*)xv;
+            if (p.ct == 1) LCXCHECK((mx_linear_tiles<T, 1, 4, true>(p, xb, xrs, wc, ws, N, K, w, st)));
+            else if (p.ct == 2) LCXCHECK((mx_linear_tiles<T, 2, 4, true>(p, xb, xrs, wc, ws, N, K, w, st)));
+            else if (p.ct == 4) LCXCHECK((mx_linear_tiles<T, 4, 4, true>(p, xb, xrs, wc, ws, N, K, w, st)));
+            else LCXCHECK((mx_linear_tiles<T, 8, 4, true>(p, xb, xrs, wc, ws, N, K, w, st)));
+            return mx_join<T>(p.split, w, st);
+        }
+    }
     LCXCHECK((mx_fragments<T, true>(x, M, xrs, xcs, K, p, frag, ex, st)));
+    const int64_t tiles = p.mt * p.ct;
     constexpr int JS = TERMS == 3 ? 2 : 4;
-    if (p.ct == 1) LCXCHECK((mx_linear_tiles<T, 1, 4>(p, frag, wc, ws, N, K, w, st)));
-    else if (p.ct == 2) LCXCHECK((mx_linear_tiles<T, 2, 4>(p, frag, wc, ws, N, K, w, st)));
-    else if (p.ct == 4) LCXCHECK((mx_linear_tiles<T, 4, JS>(p, frag, wc, ws, N, K, w, st)));
+    if (p.ct == 1) LCXCHECK((mx_linear_tiles<T, 1, 4>(p, frag, tiles, wc, ws, N, K, w, st)));
+    else if (p.ct == 2) LCXCHECK((mx_linear_tiles<T, 2, 4>(p, frag, tiles, wc, ws, N, K, w, st)));
+    else if (p.ct == 4) LCXCHECK((mx_linear_tiles<T, 4, JS>(p, frag, tiles, wc, ws, N, K, w, st)));
     else {
-        if constexpr (TERMS == 1) LCXCHECK((mx_linear_tiles<T, 8, 4>(p, frag, wc, ws, N, K, w, st)));
+        if constexpr (TERMS == 1) LCXCHECK((mx_linear_tiles<T, 8, 4>(p, frag, tiles, wc, ws, N, K, w, st)));
     }
     return mx_join<T>(p.split, w, st);
 }
@@ -272,11 +288,21 @@ static int mx4_linear_grad(const void* dyv, int64_t M, int64_t yrs, int64_t ycs,
     const unsigned char *wc = (const unsigned char*)wcv, *ws = (const unsigned char*)wsv;
     unsigned short* frag = (unsigned short*)space;
     MxOut<T> w{(T*)out, rs, cs, p.split > 1 ? (float*)((char*)space + round_up(p.frag_bytes, 256)) : nullptr, M, K, rs == 1 && cs != 1, ex.oscale, ex.skip};
+    if constexpr (TERMS == 1) {
+        if (N % 64 == 0 && mx_direct(dy, yrs, ycs)) {
+            const unsigned short* yb = (const unsigned short*)dyv;
+            if (p.ct == 1) LCXCHECK((mx_grad_tiles<T, 1, 2, true>(p, yb, yrs, wc, ws, N, K, w, st)));
+            else if (p.ct == 2) LCXCHECK((mx_grad_tiles<T, 2, 2, true>(p, yb, yrs, wc, ws, N, K, w, st)));
+            else LCXCHECK((mx_grad_tiles<T, 4, 2, true>(p, yb, yrs, wc, ws, N, K, w, st)));
+            return mx_join<T>(p.split, w, st);
+        }
+    }
     LCXCHECK((mx_fragments<T, false>(dy, M, yrs, ycs, N, p, frag, ex, st)));
+    const int64_t tiles = p.mt * p.ct;
     constexpr int JS = TERMS > 1 ? 1 : 2;
-    if (p.ct == 1) LCXCHECK((mx_grad_tiles<T, 1, JS>(p, frag, wc, ws, N, K, w, st)));
-    else if (p.ct == 2) LCXCHECK((mx_grad_tiles<T, 2, JS>(p, frag, wc, ws, N, K, w, st)));
-    else LCXCHECK((mx_grad_tiles<T, 4, JS>(p, frag, wc, ws, N, K, w, st)));
+    if (p.ct == 1) LCXCHECK((mx_grad_tiles<T, 1, JS>(p, frag, tiles, wc, ws, N, K, w, st)));
+    else if (p.ct == 2) LCXCHECK((mx_grad_tiles<T, 2, JS>(p, frag, tiles, wc, ws, N, K, w, st)));
+    else LCXCHECK((mx_grad_tiles<T, 4, JS>(p, frag, tiles, wc, ws, N, K, w, st)));
     return mx_join<T>(p.split, w, st);
 }
 

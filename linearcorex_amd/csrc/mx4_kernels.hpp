@@ -575,6 +575,23 @@ __device__ __forceinline__ void mx_fence() { __builtin_amdgcn_sched_barrier(0); 
 typedef __attribute__((address_space(1))) const void* mx_gptr;
 typedef __attribute__((address_space(3))) void* mx_lptr;
 
+// bf16 whose rows are whole lines (neighbouring columns, 16-byte aligned, whole stages of the contraction) goes to LDS without being laid out first:
+// that saves a launch and its pass over x (8 us of 206 at 4096 x 8192 x 4096, 26 of 282 forward and backward at 2048 x 8192 x 4096).  A stage is P
+// pieces of 16 bytes of each row; a load takes 64 / P rows, the lane's piece exchanged with a power-of-two pattern of its row such that the 16
+// lanes that read a fragment's column of pieces together touch every bank once: piece p of row r lies at p ^ r (P = 16: a row is all banks)
+// or p ^ (r / 2) (P = 8: two rows are).  Rows behind the last repeat it and are not stored.
+template <int P> struct MxDirect {
+    unsigned int at, end, next;                                // the lane's place in its first load, in the last row; bytes from load to load
+    __device__ __forceinline__ MxDirect(int lane, int wave, int64_t stride, int64_t rows) {
+        const int r = (wave * 64 + lane) / P, piece = (lane % P) ^ (P == 16 ? r % 16 : (r / 2) % 8);
+        at = (unsigned int)(r * stride * 2) + piece * 16;
+        const int64_t last = rows - 1 < 127 ? rows - 1 : 127;
+        end = (unsigned int)(last * stride * 2) + piece * 16;
+        next = (unsigned int)(256 / P * stride * 2);
+    }
+    __device__ __forceinline__ unsigned int from(int c) const { return at + c * next < end ? at + c * next : end; }
+};
+
 // block -> (row tile, column tile, split): consecutive blocks go to the 8 XCDs in turn, so each XCD gets a contiguous piece of an order in which
 // eight row tiles share a column tile of W
 struct MxTile { int a, b, z; };
@@ -596,9 +613,11 @@ __device__ __forceinline__ MxTile mx_tile(unsigned int id, unsigned int na, unsi
 // out[t][n] = sum_k x[t][k] W[n][k] for tiles of 16 CT rows of x and 64 RT rows of W.  Bound: the bf16 matrix pipe (TERMS instructions per
 // product).  The four waves own 16 RT rows of W each - codes go from memory to registers and become bf16 there, no LDS - and share the fragments
 // of x through LDS (JS of them a stage, double buffered).
-template <typename T, int CT, int RT, int JS>
+// DIRECT: frag is x itself (rows `tiles` elements apart), see MxDirect.
+template <typename T, int CT, int RT, int JS, bool DIRECT>
 __global__ __launch_bounds__(256, 2) void mx_linear_tile_kernel(const unsigned short* __restrict__ frag, int64_t tiles, const unsigned char* __restrict__ wc,
                                                              const unsigned char* __restrict__ ws, int64_t N, int64_t K, MxOut<T> w, int mt, int nt, int split) {
+    static_assert(!DIRECT || (MxTerms<T>::v == 1 && JS == 4), "");
     constexpr int TERMS = MxTerms<T>::v, CH = JS * TERMS * CT;             // 1 KB pieces a stage
     const int64_t ksteps = mx_steps(K), quads = mx_quads(K), rts = mx_row_tiles(N);
     if (w.skip && *w.skip) return;
@@ -617,14 +636,21 @@ __global__ __launch_bounds__(256, 2) void mx_linear_tile_kernel(const unsigned s
         ps[i] = ws + rt * quads * 256;
     }
     // running address of the next stage: scalar, advanced by a constant
-    const unsigned char* fp = (const unsigned char*)frag + (s0 * 4 * TERMS * tiles + (int64_t)tile.a * CT) * 1024;
-    const int64_t fterm = tiles * 1024;
+    const unsigned char* fp = (const unsigned char*)frag + (DIRECT ? (int64_t)tile.a * CT * 16 * tiles * 2 + s0 * 256 : (s0 * 4 * TERMS * tiles + (int64_t)tile.a * CT) * 1024);
+    const int64_t fstage = DIRECT ? 256 : JS * TERMS * tiles * 1024, fterm = tiles * 1024;
+    const MxDirect<16> dx(lane, wave, tiles, w.M - (int64_t)tile.a * CT * 16);
     // piece c of the wave's share of the next JS fragments of the contraction
     constexpr int PIECES = (CH + 3) / 4;
     auto stage = [&](int b, int c) {
         const int i = c * 4 + wave;
         if (CH % 4 == 0 || i < CH)
-            __builtin_amdgcn_global_load_lds((mx_gptr)(fp + (i / CT) * fterm + (i % CT) * 1024 + lane * 16), (mx_lptr)(&lds[b][i * 512]), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((mx_gptr)(DIRECT ? fp + dx.from(c) : fp + (i / CT) * fterm + (i % CT) * 1024 + lane * 16), (mx_lptr)(&lds[b][i * 512]),
+                                             16, 0, 0);
+    };
+    // fragment i of a stage (step i / CT, tile i % CT)
+    const int dlane = l * 256 + ((4 * g) ^ l) * 16;
+    auto fragment = [&](int b, int i) {
+        return *reinterpret_cast<const mx_bf8*>((const unsigned char*)lds[b] + (DIRECT ? (i % CT) * 4096 + (dlane ^ (i / CT * 16)) : i * 1024 + lane * 16));
     };
     mx_f4 acc[RT][CT] = {};
     mx_u4 q[RT];
@@ -649,13 +675,12 @@ __global__ __launch_bounds__(256, 2) void mx_linear_tile_kernel(const unsigned s
         for (int i = 0; i < RT; ++i) sc[i] = mx_scale_operand(sd[i], (int)(s & 3));
 #pragma unroll
         for (int h = 0; h < 4 / JS; ++h) {
-            if (h + 1 < 4 / JS || s + 1 < s1) fp += JS * TERMS * fterm;    // (behind the last stage: that one again, unused)
+            if (h + 1 < 4 / JS || s + 1 < s1) fp += fstage;    // (behind the last stage: that one again, unused)
             // slices of F fragments
             constexpr int F = CT < 4 ? CT : 4, SL = CH / F;
             mx_bf8 f[2][F], a[2][RT];
-            const unsigned short* at = &lds[b][lane * 8];
 #pragma unroll
-            for (int c = 0; c < F; ++c) f[0][c] = *reinterpret_cast<const mx_bf8*>(at + c * 512);
+            for (int c = 0; c < F; ++c) f[0][c] = fragment(b, c);
 #pragma unroll
             for (int i = 0; i < RT; ++i) a[0][i] = mx_unpack8(q[i][h * JS], sc[i]);
 #pragma unroll
@@ -677,7 +702,7 @@ __global__ __launch_bounds__(256, 2) void mx_linear_tile_kernel(const unsigned s
                         }
                         if (sl + 1 < SL) {
 #pragma unroll
-                            for (int n = 0; n < F; ++n) f[(sl + 1) & 1][n] = *reinterpret_cast<const mx_bf8*>(at + ((sl + 1) * F + n) * 512);
+                            for (int n = 0; n < F; ++n) f[(sl + 1) & 1][n] = fragment(b, (sl + 1) * F + n);
                             if ((sl + 1) * F % (TERMS * CT) == 0) {
 #pragma unroll
                                 for (int i = 0; i < RT; ++i) a[(jj + 1) & 1][i] = mx_unpack8(q[i][h * JS + jj + 1], sc[i]);
@@ -708,9 +733,11 @@ __global__ __launch_bounds__(256, 2) void mx_linear_tile_kernel(const unsigned s
 template <int CT, int JS, int TERMS> struct MxGradLds {
     static constexpr int frag = JS * TERMS * CT * 1024, codes = JS * 8 * 1024, scales = JS * 2 * 256, wstage = codes + scales, total = 2 * frag + 3 * wstage;
 };
-template <typename T, int CT, int JS>
+// DIRECT: frag is dy itself (rows `tiles` elements apart), see MxDirect.
+template <typename T, int CT, int JS, bool DIRECT>
 __global__ __launch_bounds__(256, 2) void mx_grad_tile_kernel(const unsigned short* __restrict__ frag, int64_t tiles, const unsigned char* __restrict__ wc,
                                                              const unsigned char* __restrict__ ws, int64_t N, int64_t K, MxOut<T> w, int mt, int nt, int split) {
+    static_assert(!DIRECT || (MxTerms<T>::v == 1 && JS == 2), "");
     constexpr int TERMS = MxTerms<T>::v, CH = JS * TERMS * CT;
     constexpr bool AHEAD = TERMS == 1 && JS % 2 == 0;
     typedef MxGradLds<CT, JS, TERMS> L;
@@ -724,8 +751,9 @@ __global__ __launch_bounds__(256, 2) void mx_grad_tile_kernel(const unsigned sho
     const int64_t s0 = per * tile.z, s1 = s0 + per < steps ? s0 + per : steps;
     extern __shared__ __attribute__((aligned(16))) unsigned char glds[];
     // running addresses of the next stage: scalar, advanced by a constant
-    const unsigned char* fp = (const unsigned char*)frag + (s0 * TERMS * tiles + (int64_t)tile.a * CT) * 1024;
-    const int64_t fterm = tiles * 1024, wtile = ksteps * 1024, stile = quads * 256;
+    const unsigned char* fp = (const unsigned char*)frag + (DIRECT ? (int64_t)tile.a * CT * 16 * tiles * 2 + s0 * 64 : (s0 * TERMS * tiles + (int64_t)tile.a * CT) * 1024);
+    const MxDirect<8> dx(lane, wave, tiles, w.M - (int64_t)tile.a * CT * 16);
+    const int64_t fterm = tiles * 1024, fstage = DIRECT ? 128 : JS * TERMS * fterm, wtile = ksteps * 1024, stile = quads * 256;
     const unsigned char* wp = wc + (s0 * 2 * ksteps + ((int64_t)tile.b * 4 + wave < ksteps ? (int64_t)tile.b * 4 + wave : ksteps - 1)) * 1024;
     const unsigned char* sp = ws + ((s0 * 2 + (wave < JS * 2 ? wave : 0)) * quads + tile.b) * 256;
     // row tiles from the next stage on.  Those behind the last one: its codes again, whose factors in dy are zero; their scales must not be a
@@ -737,17 +765,23 @@ __global__ __launch_bounds__(256, 2) void mx_grad_tile_kernel(const unsigned sho
     auto load_frag = [&](int at, int c) {
         const int i = c * 4 + wave;
         if (CH % 4 == 0 || i < CH)
-            __builtin_amdgcn_global_load_lds((mx_gptr)(fp + (i / CT) * fterm + (i % CT) * 1024 + lane * 16), (mx_lptr)(glds + at + i * 1024), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((mx_gptr)(DIRECT ? fp + dx.from(c) : fp + (i / CT) * fterm + (i % CT) * 1024 + lane * 16), (mx_lptr)(glds + at + i * 1024),
+                                             16, 0, 0);
+    };
+    // fragment i of step jj of the stage at LDS offset at
+    const int dlane = l * 128 + (g ^ (l >> 1)) * 16;
+    auto fragment = [&](int at, int jj, int i) {
+        return *reinterpret_cast<const mx_bf8*>(glds + at + (DIRECT ? i * 2048 + (dlane ^ (jj * 64)) : (jj * TERMS * CT + i) * 1024 + lane * 16));
     };
     auto load_w = [&](int at, int p) {                         // the wave's step of row tile p; p == WP: the scales
         if (p < WP)
             __builtin_amdgcn_global_load_lds((mx_gptr)(wp + (p < left ? p : left - 1) * wtile + wlane[p & 1]), (mx_lptr)(glds + at + (p * 4 + wave) * 1024), 16,
                                              0, 0);
         else if (wave < WP && lane < 16)
-            __builtin_amdgcn_global_load_lds((mx_gptr)((wave < left ? sp : zp) + lane * 16), (mx_lptr)(glds + at + L::codes + wave * 256), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((mx_gptr)((DIRECT || wave < left ? sp : zp) + lane * 16), (mx_lptr)(glds + at + L::codes + wave * 256), 16, 0, 0);
     };
     // (behind the last stage: that one again, unused - the addresses stay where they are)
-    auto next_frag = [&](bool more) { fp += more ? JS * TERMS * fterm : 0; };
+    auto next_frag = [&](bool more) { fp += more ? fstage : 0; };
     auto next_w = [&](bool more) {
         wp += more ? WP * wtile : 0;
         sp += more ? WP * stile : 0;
@@ -796,9 +830,8 @@ __global__ __launch_bounds__(256, 2) void mx_grad_tile_kernel(const unsigned sho
             // slices of F fragments; the first of the next step's unpacking rides behind the first of them
             constexpr int F = CT < 2 ? CT : 2, SL = TERMS * CT / F;
             mx_bf8 f[2][F];
-            const unsigned char* at = glds + f0 + jj * TERMS * CT * 1024 + lane * 16;
 #pragma unroll
-            for (int c = 0; c < F; ++c) f[0][c] = *reinterpret_cast<const mx_bf8*>(at + c * 1024);
+            for (int c = 0; c < F; ++c) f[0][c] = fragment(f0, jj, c);
 #pragma unroll
             for (int sl = 0; sl < SL; ++sl) {
                 const int c0 = sl * F % CT;
@@ -814,7 +847,7 @@ __global__ __launch_bounds__(256, 2) void mx_grad_tile_kernel(const unsigned sho
                         }
                         if (sl + 1 < SL) {
 #pragma unroll
-                            for (int n = 0; n < F; ++n) f[(sl + 1) & 1][n] = *reinterpret_cast<const mx_bf8*>(at + ((sl + 1) * F + n) * 1024);
+                            for (int n = 0; n < F; ++n) f[(sl + 1) & 1][n] = fragment(f0, jj, (sl + 1) * F + n);
                         }
                         if (AHEAD && sl == 0) {
                             if (jj + 1 < JS) unpack_step(w0, jj + 1, a[nxt]);

@@ -194,6 +194,28 @@ def test_activations_of_any_strides(mx4, dt, m):
     assert torch.equal(mx4.linear(base[0, :300], q), mx4.linear(base[:1, :300], q)[0])
 
 
+@pytest.mark.parametrize("m", [3, 17, 40, 100, 129, 300])
+@pytest.mark.parametrize("n,k", [(64, 128), (192, 384), (640, 1280), (20032, 4096)])
+def test_whole_lines_of_bfloat16_take_the_short_way(mx4, m, n, k):
+    """rows of whole lines are read in place, others are laid out first: the same sums in the same order, to the bit"""
+    q = mx4.quantize(torch.randn(n, k, generator=gen(1)).cuda())
+    base, top = torch.randn(2 * m, k + 8, generator=gen(2)).bfloat16().cuda(), torch.randn(2 * m, n + 8, generator=gen(3)).bfloat16().cuda()
+    for rows in (slice(0, m), slice(m - 1, 2 * m - 1), slice(0, 2 * m, 2)):
+        for f, b, c in ((mx4.linear, base, k), (mx4.linear_grad, top, n)):
+            x = b[rows, :c]
+            want = f(x, q)
+            odd = torch.empty(m, c + 1, dtype=x.dtype, device="cuda")[:, :c].copy_(x)
+            col = torch.empty(c, m, dtype=x.dtype, device="cuda").t().copy_(x)
+            behind = b[rows, 8:c + 8].clone()[:, :c]
+            assert torch.equal(f(odd, q), want) and torch.equal(f(col, q), want) and torch.equal(f(b[rows, 8:], q), f(behind, q))
+    one = base[:1, :k].expand(m, k)
+    assert torch.equal(mx4.linear(one, q), mx4.linear(one.contiguous(), q))
+    # rows and columns behind a matrix are not read into the result
+    x = torch.full((2 * m, k + 8), float("nan"), dtype=torch.bfloat16, device="cuda")
+    x[:m, :k] = base[:m, :k]
+    assert torch.equal(mx4.linear(x[:m, :k], q), mx4.linear(base[:m, :k], q))
+
+
 @pytest.mark.parametrize("dt", PRODUCT, ids=ids)
 @pytest.mark.parametrize("m", [1, 20, 150])
 def test_non_finite_values_stay_in_their_rows(mx4, dt, m):

@@ -96,11 +96,11 @@ struct MxPlan {
 struct MxStep { double t1, u1, t2, u2, pair; };
 
 // Tile height (16 ct rows of x) and parts of the contraction for M rows, `cols` tiles over the O outputs and `steps`: least time of
-//   steps of a part x step time at so many blocks a CU (a second block on some CUs only counts half and its share of the other half,
-//     a later one three quarters)
-//   + start and outputs of a block, 1 us and 1.2 more per 16 rows
+//   steps of a part x step time at so many blocks a CU (a second block on some CUs only counts 0.3 and its share of the rest,
+//     a later one three quarters; where CUs are left over, a block takes down to 0.85 of the time)
+//   + start and outputs of a block, 1 us and 1.3 more per 16 rows
 //   + writing the parts and adding them up: 7 TB/s, 3 us for the launch, 0.1 a part
-// Within 10 % of the best of all (ct, split) over 78 sizes from 24 x 4096 x 4096 to 2048 x 14336 x 4096, and 512 x 20000 x 20000.  What it weighs, us:
+// Within 2 % of the best (ct, split) on average, 15 % at worst, over 78 sizes from 1 x 4096 x 4096 to 512 x 20000 x 20000.  What it weighs, us:
 // bf16 512 x 14336 x 4096 in tiles of ct 2 / 4 / 8: 70 / 59 / 64; float32 64 x 20000 x 20000 in 1 / 3 / 6 / 8 parts: 345 / 134 / 123 / 141
 static double mx_choose(int64_t M, int64_t O, int64_t cols, int64_t steps, int terms, int min_ct, int max_ct, const MxStep& c, int* ct_out, int* split_out) {
     *ct_out = min_ct;
@@ -108,11 +108,11 @@ static double mx_choose(int64_t M, int64_t O, int64_t cols, int64_t steps, int t
     double best = 1e300;
     for (int ct = min_ct; ct <= max_ct && (ct == min_ct || 8 * ct < M); ct *= 2) {
         const int64_t tiles = cdiv(M, 16 * ct) * cols;
-        const double one = c.t1 + c.u1 * ct * terms, two = c.t2 + c.u2 * ct * terms, fixed = 1.0 + 1.2 * ct;
+        const double one = c.t1 + c.u1 * ct * terms, two = c.t2 + c.u2 * ct * terms, fixed = 1.0 + 1.3 * ct;
         for (int64_t s = 1; s <= 64 && s <= steps && (s == 1 || tiles * s <= 4 * MX_CUS); ++s) {
             const int64_t full = tiles * s / MX_CUS, rest = tiles * s % MX_CUS;
-            const double b = full == 0 ? 1.0 : (double)full + (rest == 0 ? 0.0 : full == 1 ? 0.5 + 0.5 * (double)rest / MX_CUS : 0.75 + 0.25 * (double)rest / MX_CUS);
-            const double step = b <= 2.0 ? one + (two - one) * (b - 1.0) : two * 0.5 * b;
+            const double b = full == 0 ? 1.0 : (double)full + (rest == 0 ? 0.0 : full == 1 ? 0.3 + 0.7 * (double)rest / MX_CUS : 0.75 + 0.25 * (double)rest / MX_CUS);
+            const double step = full == 0 ? one * (0.85 + 0.15 * (double)rest / MX_CUS) : b <= 2.0 ? one + (two - one) * (b - 1.0) : two * 0.5 * b;
             const double t = (double)cdiv(steps, s) * step + (b <= 2.0 ? fixed + c.pair * (b - 1.0) : (fixed + c.pair) * 0.5 * b) +
                              (s > 1 ? (double)(s * M * O) * 8 / 7e6 + 3.0 + 0.1 * (double)s : 0.0);
             if (t < best * 0.98) { best = t; *ct_out = ct; *split_out = (int)s; }
@@ -135,7 +135,7 @@ template <typename T> static MxPlan mx_plan(bool along, int64_t M, int64_t C, in
     MxPlan p;
     p.rt = 4;
     p.nt = along ? cdiv(O, 64 * p.rt) : cdiv(O, 512);
-    const MxStep step = along        ? MxStep{0.58, 0.145, 0.4, 0.33, 0.0}
+    const MxStep step = along        ? TERMS == 1 ? MxStep{0.52, 0.13, 0.42, 0.33, 1.5} : MxStep{0.58, 0.145, 0.4, 0.33, 0.0}
                         : TERMS == 1 ? MxStep{1.7, 0.21, 1.9, 0.48, 4.0}
                                      : MxStep{2.7, 0.19, 2.1, 0.53, 4.0};
     const double t = mx_choose(M, O, p.nt, cdiv(C, 128), TERMS, M <= 16 ? 1 : 2, along && TERMS == 1 ? 8 : 4, step, &p.ct, &p.split);

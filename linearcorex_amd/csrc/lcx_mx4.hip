@@ -39,15 +39,21 @@ template <typename T>
 static int mx4_quantize(const void* x, int64_t rows, int64_t cols, int64_t rs, int64_t cs, void* codes, void* scales, hipStream_t st) {
     unsigned char *qc = (unsigned char*)codes, *qs = (unsigned char*)scales;
     unsigned g;
+    const bool once = rows * cols * (int64_t)sizeof(T) >= MX_ONCE_BYTES;
+    const int64_t steps = mx_steps(cols), quads = mx_quads(cols);
     if (rs == 1 && cs != 1) {
-        LCXCHECK(mx_grid(cdiv(rows, 64), mx_quads(cols), 512, &g));
-        hipLaunchKernelGGL((mx_quantize_across_kernel<T>), dim3(g), dim3(512), 0, st, (const T*)x, rows, cols, cs, qc, qs);
+        LCXCHECK(mx_grid(cdiv(rows, 64), quads, 512, &g));
+        if (once) hipLaunchKernelGGL((mx_quantize_across_kernel<T, true>), dim3(g), dim3(512), 0, st, (const T*)x, rows, cols, cs, qc, qs);
+        else hipLaunchKernelGGL((mx_quantize_across_kernel<T, false>), dim3(g), dim3(512), 0, st, (const T*)x, rows, cols, cs, qc, qs);
     } else {
-        LCXCHECK(mx_grid(mx_row_tiles(rows), mx_quads(cols), 256, &g));
-        if (cs == 1) hipLaunchKernelGGL((mx_quantize_kernel<T, true>), dim3(g), dim3(256), 0, st, (const T*)x, rows, cols, rs, cs, qc, qs,
-                                        mx_steps(cols), mx_quads(cols), (int64_t)0, (unsigned)mx_quads(cols));
-        else hipLaunchKernelGGL((mx_quantize_kernel<T, false>), dim3(g), dim3(256), 0, st, (const T*)x, rows, cols, rs, cs, qc, qs, mx_steps(cols),
-                                mx_quads(cols), (int64_t)0, (unsigned)mx_quads(cols));
+        LCXCHECK(mx_grid(mx_row_tiles(rows), quads, 256, &g));
+#define MX_QUANTIZE(VEC, ONCE)                                                                                                                              \
+    hipLaunchKernelGGL((mx_quantize_kernel<T, VEC, ONCE>), dim3(g), dim3(256), 0, st, (const T*)x, rows, cols, rs, cs, qc, qs, steps, quads, (int64_t)0, \
+                       (unsigned)quads)
+        if (cs != 1) MX_QUANTIZE(false, false);
+        else if (once) MX_QUANTIZE(true, true);
+        else MX_QUANTIZE(true, false);
+#undef MX_QUANTIZE
     }
     KCHECK();
     return LCX_OK;
@@ -388,7 +394,7 @@ static int mx_shard_block(lcx_ctx* h, float* stage, int64_t ld, int64_t c0, int6
     LCXCHECK(mx_grid(mx_row_tiles(h->Npad), nq, 256, &g));
     unsigned char *qc = (unsigned char*)h->xq, *qs = (unsigned char*)h->xs;
     if (fill) {
-        hipLaunchKernelGGL((mx_quantize_kernel<float, true>), dim3(g), dim3(256), 0, h->stream, stage, h->Npad, cols, ld, (int64_t)1, qc, qs, mx_steps(h->ldx),
+        hipLaunchKernelGGL((mx_quantize_kernel<float, true, true>), dim3(g), dim3(256), 0, h->stream, stage, h->Npad, cols, ld, (int64_t)1, qc, qs, mx_steps(h->ldx),
                            mx_quads(h->ldx), c0 / 512, (unsigned)nq);
         KCHECK();
     }

@@ -116,13 +116,13 @@ template <typename T, int N> __device__ __forceinline__ void mx_put(T* p, const 
 // eight neighbours of a row, read or written 16 bytes at a time from any address the element type allows (global memory takes it)
 template <typename T> struct MxRaw8 { T v[8]; };
 // zeros behind the last column; VEC: the columns are neighbours (cs == 1)
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool ONCE = false>
 __device__ __forceinline__ MxRaw8<T> mx_load8(const T* __restrict__ x, int64_t c0, int64_t cols, int64_t cs) {
     MxRaw8<T> r;
     if (VEC && c0 + 8 <= cols) {
         mx_u4 t[sizeof(T) / 2];
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) t[i] = reinterpret_cast<const mx_u4u*>(x + c0)[i];
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) t[i] = ONCE ? __builtin_nontemporal_load(reinterpret_cast<const mx_u4u*>(x + c0) + i) : reinterpret_cast<const mx_u4u*>(x + c0)[i];
         __builtin_memcpy(&r, t, sizeof(r));
     } else {
 #pragma unroll
@@ -131,10 +131,16 @@ __device__ __forceinline__ MxRaw8<T> mx_load8(const T* __restrict__ x, int64_t c
     return r;
 }
 
+// From this size on x is read past the caches: it does not fit what earlier kernels have left there to be written back, and loads that would take
+// its place wait for that.  Measured (us; through / past the caches; x just written by another kernel, then after others' writes):
+// 64 MB of bf16 16.3 / 17.1, 24 / 18; 128 MB 29.2 / 29.9, 44 / 32; 256 MB 65 / 47, 81 / 61; 20 MB of bf16 8.6 / 10.4, 9.2 / 6.6
+constexpr int64_t MX_ONCE_BYTES = 128 << 20;
+
 // x[r * rs + c * cs] -> codes, scales.  Bound: reading x.  A block takes 16 rows x 512 columns: a thread 8 columns of each of four steps (16 bytes
 // of a 16-bit type each: VEC, where the columns are neighbours), so that it ends up with a whole dword of scales; four lanes share a
-// block of 32.  grid (row tile, quad of steps); x holds the columns from quad quad0 on of a matrix of `steps` steps
-template <typename T, bool VEC>
+// block of 32.  grid (row tile, quad of steps); x holds the columns from quad quad0 on of a matrix of `steps` steps.
+// ONCE: x is read past the caches (MX_ONCE_BYTES).  16384 x 8192 bf16 (340 MB read and written): 57 us, 5.9 TB/s; 32 x 4096: 3.4 us.
+template <typename T, bool VEC, bool ONCE>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t rs, int64_t cs,
                                                           unsigned char* __restrict__ codes, unsigned char* __restrict__ scales, int64_t steps, int64_t quads,
                                                           int64_t quad0, unsigned int nquads) {
@@ -145,7 +151,7 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ 
     MxRaw8<T> raw[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-        if (r < rows) raw[u] = mx_load8<T, VEC>(x + r * rs, here * 512 + u * 128 + c * 8, cols, cs);
+        if (r < rows) raw[u] = mx_load8<T, VEC, ONCE>(x + r * rs, here * 512 + u * 128 + c * 8, cols, cs);
         else
 #pragma unroll
             for (int j = 0; j < 8; ++j) raw[u].v[j] = (T)0.0f;
@@ -171,14 +177,15 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ 
 
 // the same for a matrix whose ROWS are neighbours in memory (rs == 1: a transposed view).  A block of 8 waves takes 64 rows x 512 columns; lane =
 // row, so that every load of a wave is contiguous; a thread holds whole blocks of 32 columns and writes its 16 bytes of the fragment.
-template <typename T>
+// 5000 x 10000 float32 (226 MB): 54 us, 4.2 TB/s; mx_quantize_kernel, element by element, takes twice as long (x in the caches: 45 / 91 us).
+template <typename T, bool ONCE>
 __global__ __launch_bounds__(512) void mx_quantize_across_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t cs,
                                                                  unsigned char* __restrict__ codes, unsigned char* __restrict__ scales) {
     const int64_t steps = mx_steps(cols), quads = mx_quads(cols);
     __shared__ __attribute__((aligned(16))) unsigned char ls[4][256];      // [row tile][lane][step]
     const int lane = threadIdx.x & 63, wave = mx_wave(), tile = lane >> 4, l = lane & 15;
-    const unsigned int rt32 = blockIdx.x / (unsigned int)quads;
-    const int64_t quad = blockIdx.x - rt32 * (unsigned int)quads, rt = (int64_t)rt32 * 4 + tile, r = rt * 16 + l, rts = mx_row_tiles(rows);
+    const unsigned int groups = (unsigned int)((rows + 63) / 64), q32 = blockIdx.x / groups, rt32 = blockIdx.x - q32 * groups;
+    const int64_t quad = q32, rt = (int64_t)rt32 * 4 + tile, r = rt * 16 + l, rts = mx_row_tiles(rows);
     const T* p = x + (r < rows ? r : rows - 1);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -187,7 +194,7 @@ __global__ __launch_bounds__(512) void mx_quantize_across_kernel(const T* __rest
         T raw[32];
         if (c + 32 <= cols) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) raw[j] = p[(c + j) * cs];
+            for (int j = 0; j < 32; ++j) raw[j] = ONCE ? __builtin_nontemporal_load(&p[(c + j) * cs]) : p[(c + j) * cs];
         } else {
 #pragma unroll
             for (int j = 0; j < 32; ++j) raw[j] = c + j < cols ? p[(c + j) * cs] : (T)0.0f;
@@ -222,7 +229,8 @@ __device__ __forceinline__ void mx_values8(unsigned int q, float s, float* v) {
     p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, s, 3); v[6] = p[0]; v[7] = p[1];
 }
 
-// codes, scales -> out[r * rs + c * cs].  Bound: writing out.  Threads as in mx_quantize_kernel; VEC: the columns of out are neighbours
+// codes, scales -> out[r * rs + c * cs].  Bound: writing out.  Threads as in mx_quantize_kernel; VEC: the columns of out are neighbours.
+// 16384 x 8192 bf16: 51 us, 6.6 TB/s.  (Stores past the caches: 5000 x 10000 float32 transposed 38 -> 83 us.)
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
                                                             int64_t rows, int64_t cols, T* __restrict__ out, int64_t rs, int64_t cs, int64_t steps, int64_t quads,
@@ -256,7 +264,8 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned char*
     }
 }
 
-// the same into a matrix whose rows are neighbours in memory (rs == 1): the mirror image of mx_quantize_across_kernel
+// the same into a matrix whose rows are neighbours in memory (rs == 1): the mirror image of mx_quantize_across_kernel.  5000 x 10000 float32:
+// 38 us, 6.0 TB/s (element by element 103)
 template <typename T>
 __global__ __launch_bounds__(512) void mx_dequantize_across_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
                                                                    int64_t rows, int64_t cols, T* __restrict__ out, int64_t cs) {

@@ -273,7 +273,7 @@ static int mx4_linear(const void* xv, int64_t M, int64_t xrs, int64_t xcs, const
     }
     LCXCHECK((mx_fragments<T, true>(x, M, xrs, xcs, K, p, frag, ex, st)));
     const int64_t tiles = p.mt * p.ct;
-    constexpr int JS = TERMS == 3 ? 2 : 4;
+    constexpr int JS = TERMS == 3 ? 2 : 4;                  // (three terms of four fragments would be 96 KB of LDS: one block a CU)
     if (p.ct == 1) LCXCHECK((mx_linear_tiles<T, 1, 4>(p, frag, tiles, wc, ws, N, K, w, st)));
     else if (p.ct == 2) LCXCHECK((mx_linear_tiles<T, 2, 4>(p, frag, tiles, wc, ws, N, K, w, st)));
     else if (p.ct == 4) LCXCHECK((mx_linear_tiles<T, 4, JS>(p, frag, tiles, wc, ws, N, K, w, st)));
@@ -305,7 +305,7 @@ static int mx4_linear_grad(const void* dyv, int64_t M, int64_t yrs, int64_t ycs,
     }
     LCXCHECK((mx_fragments<T, false>(dy, M, yrs, ycs, N, p, frag, ex, st)));
     const int64_t tiles = p.mt * p.ct;
-    constexpr int JS = TERMS > 1 ? 1 : 2;
+    constexpr int JS = TERMS > 1 ? 1 : 2;                   // (a second step would be 83 KB of LDS with two terms: one block a CU)
     if (p.ct == 1) LCXCHECK((mx_grad_tiles<T, 1, JS>(p, frag, tiles, wc, ws, N, K, w, st)));
     else if (p.ct == 2) LCXCHECK((mx_grad_tiles<T, 2, JS>(p, frag, tiles, wc, ws, N, K, w, st)));
     else LCXCHECK((mx_grad_tiles<T, 4, JS>(p, frag, tiles, wc, ws, N, K, w, st)));

@@ -391,7 +391,8 @@ __device__ __forceinline__ void mx_store_tile(const MxOut<T>& w, int64_t z, int6
     }
 }
 
-// out[t][o] = sum over the splits, in order; four columns a thread, rscale (may be null) a factor of every row.  grid (columns, rows)
+// out[t][o] = sum over the splits, in order; four columns a thread, rscale (may be null) a factor of every row.  grid (columns, rows).  Bound:
+// reading the parts; two of 2048 x 4096 (84 MB read and written): 13 us, 6.4 TB/s
 template <typename T>
 __global__ __launch_bounds__(256) void mx_join_kernel(const float* __restrict__ part, int split, int64_t M, int64_t O, T* __restrict__ out, int64_t rs,
                                                       int64_t cs, const float* __restrict__ rscale, const int* __restrict__ skip) {
@@ -424,7 +425,8 @@ __global__ __launch_bounds__(256) void mx_join_kernel(const float* __restrict__ 
     }
 }
 
-// one factor per column that makes the mean square of the N rows 1 (1 for a column of zeros).  64 columns a block
+// one factor per column that makes the mean square of the N rows 1 (1 for a column of zeros).  64 columns a block; sums in 64 bits.  Once per filled
+// block of a shard, as the next kernel: reading the block bounds both
 __global__ __launch_bounds__(1024) void mx_unit_columns_kernel(const float* __restrict__ x, int64_t N, int64_t cols, int64_t ld, double n, float* __restrict__ out) {
     __shared__ double red[16][64];
     const int c = threadIdx.x & 63, g = threadIdx.x >> 6;
@@ -543,7 +545,7 @@ __device__ __forceinline__ void mx_unpack_across(const unsigned int* q, const fl
 //   across the blocks  32 i + 8 g
 // mx_fragments_kernel lays x out that way once per call, split into its bf16 terms: frag[i][term][tile of 16 rows][lane][8].  A tile of the
 // products below is then a contiguous piece of memory, whatever x's type, strides or odd sizes.  kscale (may be null): a factor of every
-// column of W, taken into x here.
+// column of W, taken into x here.  Bound: the fragments' stores; 64 x 20000 float32 5.4 us, 2048 x 8192 bf16 (67 MB) 17 us, 3.9 TB/s.
 template <bool ALONG> __device__ __forceinline__ int64_t mx_frag_k(int64_t i, int g) {
     return ALONG ? (i >> 2) * 128 + g * 32 + (i & 3) * 8 : i * 32 + g * 8;
 }
@@ -585,7 +587,8 @@ typedef __attribute__((address_space(1))) const void* mx_gptr;
 typedef __attribute__((address_space(3))) void* mx_lptr;
 
 // bf16 whose rows are whole lines (neighbouring columns, 16-byte aligned, whole stages of the contraction) goes to LDS without being laid out first:
-// that saves a launch and its pass over x (8 us of 206 at 4096 x 8192 x 4096, 26 of 282 forward and backward at 2048 x 8192 x 4096).  A stage is P
+// that saves a launch and its pass over x (4096 x 8192 x 4096 207 -> 195 us; forward and backward of 2048 x 8192 x 4096 282 -> 252; 24 x 4096 x
+// 4096 14.3 -> 11.1).  A stage is P
 // pieces of 16 bytes of each row; a load takes 64 / P rows, the lane's piece exchanged with a power-of-two pattern of its row such that the 16
 // lanes that read a fragment's column of pieces together touch every bank once: piece p of row r lies at p ^ r (P = 16: a row is all banks)
 // or p ^ (r / 2) (P = 8: two rows are).  Rows behind the last repeat it and are not stored.
@@ -621,7 +624,10 @@ __device__ __forceinline__ MxTile mx_tile(unsigned int id, unsigned int na, unsi
 
 // out[t][n] = sum_k x[t][k] W[n][k] for tiles of 16 CT rows of x and 64 RT rows of W.  Bound: the bf16 matrix pipe (TERMS instructions per
 // product).  The four waves own 16 RT rows of W each - codes go from memory to registers and become bf16 there, no LDS - and share the fragments
-// of x through LDS (JS of them a stage, double buffered).
+// of x through LDS (JS of them a stage, double buffered: as many as leave room for two blocks a CU).  4096 x 8192 x 4096 bf16: 188 us, 1.46
+// PFLOP/s, where the instructions alone reach 2.17 on operands that stay in registers; 64 x 20000 x 20000 float32: 121 us, 1.27 (three terms).  Of
+// 218 us of an earlier form the kernel took 195 without its loads of x, 202 without those of W, 156 without reading LDS.  Tried: tiles of 8 x 8 a
+// wave (the accumulators spill), one block a CU (140 against 126 us, float32), eight pieces in flight instead of one a slice (slower).
 // DIRECT: frag is x itself (rows `tiles` elements apart), see MxDirect.
 template <typename T, int CT, int RT, int JS, bool DIRECT>
 __global__ __launch_bounds__(256, 2) void mx_linear_tile_kernel(const unsigned short* __restrict__ frag, int64_t tiles, const unsigned char* __restrict__ wc,
@@ -737,7 +743,9 @@ __global__ __launch_bounds__(256, 2) void mx_linear_tile_kernel(const unsigned s
 // (lane % 16) + m, eight n.  So a wave owns 128 columns as 8 tiles and no value crosses lanes.  Bound: the bf16 matrix pipe; unpacking
 // costs three vector instructions per matrix instruction at CT 4, one step ahead and in between them.  32 JS rows of W (codes, scales) and
 // their fragments of dy a stage, all of them to LDS without passing registers: the fragments double buffered, W in three buffers, since it is
-// unpacked a step early.  Row r of block b in row tile p is stored at row r ^ (b | 4 (p % 2)) of its block: the sixteen (block, lane group)
+// unpacked a step early (AHEAD; with two or three terms the fragments need its registers: 219 against 183 us).  2048 x 8192 x 4096 bf16 in two
+// parts: 148 us, 0.93 PFLOP/s (8192 rows: 1.15); 64 x 20000 x 20000 float32: 155 us, 0.99.  Of 155 us it took 98 without reading W from LDS, 118
+// without unpacking, 130 without loads.  Row r of block b in row tile p is stored at row r ^ (b | 4 (p % 2)) of its block: the sixteen (block, lane group)
 // that a wave reads at once lie in different banks.
 template <int CT, int JS, int TERMS> struct MxGradLds {
     static constexpr int frag = JS * TERMS * CT * 1024, codes = JS * 8 * 1024, scales = JS * 2 * 256, wstage = codes + scales, total = 2 * frag + 3 * wstage;
@@ -908,7 +916,7 @@ __global__ __launch_bounds__(256, 2) void mx_grad_tile_kernel(const unsigned sho
 // scale; the instruction multiplies codes and scales, float32 sums.  Rows behind the last one repeat it and are not stored.
 __device__ __forceinline__ mx_i8 mx_operand(mx_u4 q) { return mx_i8{(int)q[0], (int)q[1], (int)q[2], (int)q[3], 0, 0, 0, 0}; }
 
-// up to 16 rows of A: as mx_linear_row_kernel, bound by reading B
+// up to 16 rows of A: as mx_linear_row_kernel, bound by reading B.  8 x 8192 x 8192: 6.7 us, 5.3 TB/s (its tiles: 13)
 template <typename T, int RT>
 __global__ __launch_bounds__(64 * MX_ROW_WAVES) void mx_matmul_row_kernel(const unsigned char* __restrict__ ac, const unsigned char* __restrict__ as, int64_t M,
                                                                    const unsigned char* __restrict__ bc, const unsigned char* __restrict__ bs, int64_t N,
@@ -966,7 +974,8 @@ __global__ __launch_bounds__(64 * MX_ROW_WAVES) void mx_matmul_row_kernel(const 
 // Tiles of 16 CT rows of A by 64 RT rows of B.  Bound: the 4-bit matrix pipe (16 cycles an instruction of 64 Kflop) and what feeds it: as in
 // mx_linear_tile_kernel the four waves own 16 RT rows of B each, whose fragments and scales go from memory to registers (an instruction's
 // operands are 2 KB, and both through LDS would take all of its bandwidth), and share the fragments of A through LDS, two steps a stage,
-// double buffered.  A dword of scales serves four steps.
+// double buffered.  A dword of scales serves four steps.  8192 x 8192 x 8192: 268 us, 4.1 PFLOP/s (the instructions alone: 7.5); 1000 x 5003 x 10007: 46
+// us, 2.2.  Tried: four stages in flight (spills, 388 us), A's codes row-major in 64-byte pieces (557 against 423 us).
 template <typename T, int CT, int RT>
 __global__ __launch_bounds__(256, 2) void mx_matmul_tile_kernel(const unsigned char* __restrict__ ac, const unsigned char* __restrict__ as,
                                                                const unsigned char* __restrict__ bc, const unsigned char* __restrict__ bs, int64_t N,

@@ -115,7 +115,8 @@ static double mx_choose(int64_t M, int64_t O, int64_t cols, int64_t steps, int t
     for (int ct = min_ct; ct <= max_ct && (ct == min_ct || 8 * ct < M); ct *= 2) {
         const int64_t tiles = cdiv(M, 16 * ct) * cols;
         const double one = c.t1 + c.u1 * ct * terms, two = c.t2 + c.u2 * ct * terms, fixed = 1.0 + 1.3 * ct;
-        for (int64_t s = 1; s <= 64 && s <= steps && (s == 1 || tiles * s <= 4 * MX_CUS); ++s) {
+        // (more than four blocks a CU only pay where the last round's waste is long: products of some 300 us)
+        for (int64_t s = 1; s <= 64 && s <= steps && (s == 1 || tiles * s <= (best > 300.0 ? 16 : 4) * MX_CUS); ++s) {
             const int64_t full = tiles * s / MX_CUS, rest = tiles * s % MX_CUS;
             const double b = full == 0 ? 1.0 : (double)full + (rest == 0 ? 0.0 : full == 1 ? 0.3 + 0.7 * (double)rest / MX_CUS : 0.75 + 0.25 * (double)rest / MX_CUS);
             const double step = full == 0 ? one * (0.85 + 0.15 * (double)rest / MX_CUS) : b <= 2.0 ? one + (two - one) * (b - 1.0) : two * 0.5 * b;

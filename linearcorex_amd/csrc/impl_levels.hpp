@@ -1289,8 +1289,7 @@ template <typename T, int CT>
 int Impl<T, CT>::kernel_name_tuned(lcx_ctx* h, int kind, char* buf, int64_t len) {
     if (h->mx4) {
         if (kind == 2) buf[0] = 0;
-        else if (kind == 0) snprintf(buf, (size_t)len, "lcx::mx_linear_tile_kernel<float, %d, 4, %d>", CT > 4 ? 4 : CT, CT >= 4 ? 2 : 4);
-        else snprintf(buf, (size_t)len, "lcx::mx_grad_tile_kernel<float, %d, 1>", CT > 4 ? 4 : CT);
+        else lcx_mx_shard_kernel(h, kind, buf, len);
         return LCX_OK;
     }
     if (h->split) {

@@ -428,6 +428,12 @@ int lcx_mx_shard_xty(lcx_ctx* h, const float* Y, float* out, const int* skip) {
     ex.tiles = true;
     return mx4_linear_grad<float>(Y, h->Mp, 1, h->Mp, h->xq, h->xs, h->Npad, h->ldx, out, 1, h->Mp, h->xwork, h->xwork_bytes, h->stream, ex);
 }
+// name of the kernel of a pass (kind 0: X~ . B, else X~^T . Y), as a profiler shows it
+void lcx_mx_shard_kernel(const lcx_ctx* h, int kind, char* buf, int64_t len) {
+    const MxPlan p = kind == 0 ? mx_plan<float>(true, h->Mp, h->ldx, h->Npad, true) : mx_plan<float>(false, h->Mp, h->Npad, h->ldx, true);
+    if (kind == 0) snprintf(buf, (size_t)len, "lcx::mx_linear_tile_kernel<float, %d, 4, %d, false>", p.ct, p.ct == 4 ? 2 : 4);
+    else snprintf(buf, (size_t)len, "lcx::mx_grad_tile_kernel<float, %d, 1, false>", p.ct);
+}
 
 extern "C" {
 

@@ -140,3 +140,18 @@ def test_other_paths_run_on_it():
         assert a.f32_gemm == "mfma" and np.isfinite(a.tc) and abs(a.tc - b.tc) <= 2e-3 * max(1.0, abs(b.tc)), kw
     g = Corex(n_hidden=4, seed=0, x_storage="mx4", max_iter=5).fit_generated(500, 700, seed=3, kind=1, n_groups=4)
     assert np.isfinite(g.tc)
+
+
+@pytest.mark.parametrize("n,v,m", [(300, 200, 3), (4000, 3000, 30), (2000, 9000, 64), (700, 2000, 128)])
+def test_kernel_names_are_those_that_run(n, v, m):
+    """what a profiler shows of the passes, templates included"""
+    import re
+    be = HipBackend(n, v, m, np.float32, 0, x_storage="mx4")
+    try:
+        a, b = re.fullmatch(r"lcx::mx_linear_tile_kernel<float, ([124]), 4, ([24]), false>", be.kernel_name(0)), \
+            re.fullmatch(r"lcx::mx_grad_tile_kernel<float, ([124]), 1, false>", be.kernel_name(1))
+        assert a and b and be.kernel_name(2) == "" and int(a[2]) == (2 if a[1] == "4" else 4)
+        rows = max(16, 1 << (m - 1).bit_length())                        # factors, padded
+        assert int(a[1]) * 16 <= rows and int(b[1]) * 16 <= rows
+    finally:
+        be.close()

@@ -145,7 +145,7 @@ template <typename T> static MxPlan mx_plan(bool along, int64_t M, int64_t C, in
     const MxStep step = along        ? TERMS == 1 ? MxStep{0.52, 0.13, 0.42, 0.33, 1.5} : MxStep{0.58, 0.145, 0.4, 0.33, 0.0}
                         : TERMS == 1 ? MxStep{1.7, 0.21, 1.9, 0.48, 4.0}
                                      : MxStep{2.7, 0.19, 2.1, 0.53, 4.0};
-    const double t = mx_choose(M, O, p.nt, cdiv(C, 128), TERMS, M <= 16 ? 1 : 2, along && TERMS == 1 ? 8 : 4, step, &p.ct, &p.split);
+    const auto choose = [&] { return mx_choose(M, O, p.nt, cdiv(C, 128), TERMS, M <= 16 ? 1 : 2, along && TERMS == 1 ? 8 : 4, step, &p.ct, &p.split); };
     if (M <= 16 && along && !tiles) {
         // The row kernel or the tiles, whichever takes less time by these models (fitted for K and N from 512 to 28672; 10 %):
         //   row    3.5 us + the steps a CU works through
@@ -159,12 +159,15 @@ template <typename T> static MxPlan mx_plan(bool along, int64_t M, int64_t C, in
                                      ((rt == 2 ? 0.09 : 0.04) + (TERMS == 1 ? 0.0 : TERMS == 2 ? 0.075 : 0.09) +
                                       (TERMS == 1 ? 0.0045 : TERMS == 2 ? 0.002 : 0.0075) * (double)M);
         const double read = (double)O * (double)C * 0.53 / 6e6 + 5.0;
-        if (row <= (t > read ? t : read) + 8.0) {
+        // (nearly always the row kernel: a microsecond of the call is saved by not looking at the tiles then)
+        if (row <= read + 8.0 || row <= choose() + 8.0) {
             p = MxPlan();
             p.row = true;
             p.rt = rt;
             return p;
         }
+    } else {
+        (void)choose();
     }
     p.mt = cdiv(M, 16 * p.ct);
     p.nfrag = cdiv(C, 128) * 4;

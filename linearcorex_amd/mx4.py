@@ -125,7 +125,7 @@ def _call(index, name, *args):
     fn = _entry.get(name)
     if fn is None:
         fn = _entry[name] = getattr(_abi.load(), name)
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:        # (a matrix on the GPU exists: torch has been initialised)
         status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
@@ -155,7 +155,8 @@ def quantize(x, axis=1):
     if isinstance(axis, bool) or axis not in (0, 1, -1, -2):
         raise ValueError("axis must be 0 or 1")
     axis %= 2
-    x = x.resolve_neg()                  # (the imaginary part of a conjugated view)
+    if x.is_neg():                       # (the imaginary part of a conjugated view)
+        x = x.resolve_neg()
     (rows, cols), (rs, cs) = x.shape, x.stride()
     shape = (rows, cols)
     if axis == 0:
@@ -209,12 +210,13 @@ def _product(x, q, along):
     """x (..., C) . q: along the blocks (contraction over the stored columns) or across them (over the stored rows)"""
     n, k = q._stored()
     c, o = (k, n) if along else (n, k)
-    lead = x.shape[:-1]
-    x = x.resolve_neg()
+    if x.is_neg():
+        x = x.resolve_neg()
+    lead = None
     if x.dim() == 2:
-        m, x2 = lead[0], x
+        m, x2 = x.size(0), x
     else:
-        m = 1
+        lead, m = x.shape[:-1], 1
         for d in lead:
             m *= d
         x2 = x.reshape(m, c)
@@ -226,7 +228,7 @@ def _product(x, q, along):
         rs, cs = x2.stride()
         _call(q.index, "lcx_mx4_linear" if along else "lcx_mx4_linear_grad", x2.data_ptr(), dt, m, rs, cs, q._cp, q._sp, n, k,
               out.data_ptr(), o, 1, w.data_ptr() if wb else None, wb)
-    return out if x.dim() == 2 else out.reshape(lead + (o,))
+    return out if lead is None else out.reshape(lead + (o,))
 
 
 class _Product(torch.autograd.Function):
@@ -254,8 +256,8 @@ def _checked(x, q, what, contracted):
         raise TypeError("%s must be float32, bfloat16 or float16, not %s" % (what, x.dtype))
     if x.dim() < 1:
         raise ValueError("%s must have a dimension to contract" % what)
-    if x.shape[-1] != q.shape[contracted]:
-        raise ValueError("%s has %d values to contract, q has shape %r" % (what, x.shape[-1], q.shape))
+    if x.size(-1) != q.shape[contracted]:
+        raise ValueError("%s has %d values to contract, q has shape %r" % (what, x.size(-1), q.shape))
     if x.get_device() != q.index:
         raise ValueError("%s is on %s, q on %s" % (what, x.device, q.device))
 

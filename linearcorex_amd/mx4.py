@@ -220,7 +220,7 @@ def _product(x, q, along):
         for d in lead:
             m *= d
         x2 = x.reshape(m, c)
-    out = torch.empty((m, o), dtype=x.dtype, device=x.device)
+    out = x.new_empty((m, o))
     if m and o:
         dt = _DTYPES[x.dtype]
         wb = _workspace_bytes(1 if along else 2, dt, m, n, k)

@@ -296,7 +296,12 @@ def supervise_rank(args, argv=None):
                 reason = "ok" if rc == 0 else "rank %d's worker exited with rc %d" % (rank, rc)
                 break
             if os.path.exists(f_fail):
-                reason = "another rank's worker failed"
+                # (what ended the other worker may be ending this one too, a moment later: its own exit code says more)
+                try:
+                    rc = p.wait(timeout=3.0) or None
+                except subprocess.TimeoutExpired:
+                    pass
+                reason = "rank %d's worker exited with rc %d" % (rank, rc) if rc else "another rank's worker failed"
                 break
             if time.time() - t0 > budget:
                 reason = "rank %d's worker killed after the attempt's wall-clock budget of %.0f s" % (rank, budget)

@@ -398,6 +398,7 @@ static int mx_shard_block(lcx_ctx* h, float* stage, int64_t ld, int64_t c0, int6
     LCXCHECK(mx_grid(mx_row_tiles(h->Npad), nq, 256, &g));
     unsigned char *qc = (unsigned char*)h->xq, *qs = (unsigned char*)h->xs;
     if (fill) {
+        // (a staging block is up to 1 GB, just written: MX_ONCE_BYTES)
         hipLaunchKernelGGL((mx_quantize_kernel<float, true, true>), dim3(g), dim3(256), 0, h->stream, stage, h->Npad, cols, ld, (int64_t)1, qc, qs, mx_steps(h->ldx),
                            mx_quads(h->ldx), c0 / 512, (unsigned)nq);
         KCHECK();

@@ -633,7 +633,7 @@ __device__ __forceinline__ MxTile mx_tile(unsigned int id, unsigned int na, unsi
 // of x through LDS (JS of them a stage, double buffered: as many as leave room for two blocks a CU).  4096 x 8192 x 4096 bf16: 188 us, 1.46
 // PFLOP/s, where the instructions alone reach 2.17 on operands that stay in registers; 64 x 20000 x 20000 float32: 121 us, 1.27 (three terms).  Of
 // 218 us of an earlier form the kernel took 195 without its loads of x, 202 without those of W, 156 without reading LDS.  Tried: tiles of 8 x 8 a
-// wave (the accumulators spill), one block a CU (140 against 126 us, float32), eight pieces in flight instead of one a slice (slower).
+// wave (the accumulators spill), three waves a SIMD (140 against 126 us, float32), all loads of a stage at once (the same here, 10 % slower in the 4-bit tiles).
 // DIRECT: frag is x itself (rows `tiles` elements apart), see MxDirect.
 template <typename T, int CT, int RT, int JS, bool DIRECT>
 __global__ __launch_bounds__(256, 2) void mx_linear_tile_kernel(const unsigned short* __restrict__ frag, int64_t tiles, const unsigned char* __restrict__ wc,

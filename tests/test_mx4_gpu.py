@@ -418,3 +418,19 @@ def test_captured_gradient(mx4, dt):
         assert torch.equal(y.detach(), want[i][0]) and torch.equal(dx, want[i][1])
         again = mx4.linear(xs[i], q)
         assert torch.equal(again, want[i][0])
+
+
+@pytest.mark.parametrize("dt,low", [(torch.float32, -133), (torch.bfloat16, -133), (torch.float16, -24)], ids=["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("m", [1, 40])
+def test_subnormal_activations_count(mx4, dt, low, m):
+    """down to bfloat16's last place (all of float16): one product by 4 an output, so nothing is rounded"""
+    w = torch.zeros(64, 64)
+    w[torch.arange(64), torch.arange(64)] = 4.0
+    q = mx4.quantize(w.cuda())
+    x = torch.exp2(torch.arange(low, low + 64, dtype=torch.float64).clamp(max=8)).expand(m, 64).to(dt).cuda()
+    assert (x != 0).all()
+    assert torch.equal(f64_t(mx4.linear(x, q)), 4 * f64_t(x)) and torch.equal(f64_t(mx4.linear_grad(x, q)), 4 * f64_t(x))
+
+
+def f64_t(t):
+    return t.detach().cpu().double()

@@ -305,7 +305,8 @@ class Corex(object):
               value (`linearcorex_amd.mx4`; include/lcx.h, lcx_create_stored): 7.5 times less memory and traffic than float32, for
               matrices that would not fit, or passes that would take too long.  The model is then fitted to the rounded data (about one
               per cent of a variable's variance is rounding noise, so correlations come out that much weaker); products and sums are as
-              exact as those of a float32 fit.  float32 and n_hidden <= 128 only.  `transform` of new data is not affected.
+              exact as those of a float32 fit.  Every variable keeps its mean square; 32 neighbours share a scale, so with
+              gaussianize="none" neighbours should be of similar size.  float32 and n_hidden <= 128 only.  `transform` of new data is not affected.
     """
 
     # defaults for models pickled by an earlier build

@@ -1,6 +1,7 @@
 // lcx_mx4.hip - matrices in 4 bits per value: quantisation and products on device memory (include/lcx.h, lcx_mx4_*)
 #include "engine.hpp"
 #include "mx4_kernels.hpp"
+#include <algorithm>
 
 // sizes of the operators: offsets inside the kernels are 64-bit, tile counts must fit a grid
 static constexpr int64_t MX_MAX_DIM = (int64_t)1 << 31;
@@ -374,14 +375,16 @@ static int mx4_matmul(const void* acv, const void* asv, int64_t M, const void* b
 }
 
 // ---- the resident shard of a fit in 4 bits (engine.hpp) ----------------------------------------------------------------------------------
-// X~ (Npad samples x ldx variables, blocks along the variables).  The algorithm's moments assume variables of unit mean square; rounding to
-// 4 bits changes that by a per cent or so, hence one float32 factor per variable (xunit), which the passes apply to the small operand or to
-// the output: what is fitted is X~ = values of the 4 bits x factor.
+// X~ (Npad samples x ldx variables, blocks along the variables).  Rounding to 4 bits changes a variable's mean square by a per cent or so, and
+// the algorithm's moments are relative to it (preprocessed data have 1 where nothing is missing or transformed, other values elsewhere): hence one
+// float32 factor per variable (xunit) that gives it back the mean square it had, which the passes apply to the small operand or to the
+// output.  What is fitted is X~ = values of the 4 bits x factor.
 int lcx_mx_shard_alloc(lcx_ctx* h) {
     const int64_t rt = mx_row_tiles(h->Npad);
     const MxPlan a = mx_plan<float>(true, h->Mp, h->ldx, h->Npad, true), b = mx_plan<float>(false, h->Mp, h->Npad, h->ldx, true);
     const int64_t wa = mx_plan_bytes(a), wb = mx_plan_bytes(b);
-    const size_t bytes[4] = {(size_t)(rt * mx_steps(h->ldx) * 1024), (size_t)(rt * mx_quads(h->ldx) * 256), (size_t)h->ldx * 4, (size_t)(wa > wb ? wa : wb)};
+    const size_t bytes[4] = {(size_t)(rt * mx_steps(h->ldx) * 1024), (size_t)(rt * mx_quads(h->ldx) * 256), (size_t)h->ldx * 4,
+                             (size_t)std::max({wa, wb, h->ldx * 8})};             // (ldx doubles: the sums of a block being filled)
     void** to[4] = {&h->xq, &h->xs, (void**)&h->xunit, &h->xwork};
     for (int i = 0; i < 4; ++i) {
         LCXCHECK(dev_alloc(to[i], bytes[i], h->stream));
@@ -397,7 +400,10 @@ static int mx_shard_block(lcx_ctx* h, float* stage, int64_t ld, int64_t c0, int6
     unsigned g;
     LCXCHECK(mx_grid(mx_row_tiles(h->Npad), nq, 256, &g));
     unsigned char *qc = (unsigned char*)h->xq, *qs = (unsigned char*)h->xs;
+    double* sum = (double*)h->xwork;
     if (fill) {
+        hipLaunchKernelGGL((mx_square_columns_kernel<false>), dim3((unsigned)cdiv(cols, 64)), dim3(1024), 0, h->stream, stage, h->N, cols, ld, sum, h->xunit + c0);
+        KCHECK();
         // (a staging block is up to 1 GB, just written: MX_ONCE_BYTES)
         hipLaunchKernelGGL((mx_quantize_kernel<float, true, true>), dim3(g), dim3(256), 0, h->stream, stage, h->Npad, cols, ld, (int64_t)1, qc, qs, mx_steps(h->ldx),
                            mx_quads(h->ldx), c0 / 512, (unsigned)nq);
@@ -407,7 +413,7 @@ static int mx_shard_block(lcx_ctx* h, float* stage, int64_t ld, int64_t c0, int6
                        mx_quads(h->ldx), c0 / 512, (unsigned)nq);
     KCHECK();
     if (fill) {
-        hipLaunchKernelGGL(mx_unit_columns_kernel, dim3((unsigned)cdiv(cols, 64)), dim3(1024), 0, h->stream, stage, h->N, cols, ld, (double)h->N, h->xunit + c0);
+        hipLaunchKernelGGL((mx_square_columns_kernel<true>), dim3((unsigned)cdiv(cols, 64)), dim3(1024), 0, h->stream, stage, h->N, cols, ld, sum, h->xunit + c0);
     } else {
         hipLaunchKernelGGL(mx_scale_columns_kernel, dim3(4096), dim3(256), 0, h->stream, stage, h->Npad, cols, ld, h->xunit + c0);
     }

@@ -425,9 +425,12 @@ __global__ __launch_bounds__(256) void mx_join_kernel(const float* __restrict__ 
     }
 }
 
-// one factor per column that makes the mean square of the N rows 1 (1 for a column of zeros).  64 columns a block; sums in 64 bits.  Once per filled
-// block of a shard, as the next kernel: reading the block bounds both
-__global__ __launch_bounds__(1024) void mx_unit_columns_kernel(const float* __restrict__ x, int64_t N, int64_t cols, int64_t ld, double n, float* __restrict__ out) {
+// The factor per column that gives a rounded block back the mean square it had: !FACTOR sums the squares of the N rows before the rounding, FACTOR
+// after it and takes the root of the ratio (1 where either sum is 0 or not a number).  64 columns a block; sums in 64 bits.  Once per filled
+// block of a shard, as the next kernel: reading the block bounds all three
+template <bool FACTOR>
+__global__ __launch_bounds__(1024) void mx_square_columns_kernel(const float* __restrict__ x, int64_t N, int64_t cols, int64_t ld, double* __restrict__ sum,
+                                                                 float* __restrict__ out) {
     __shared__ double red[16][64];
     const int c = threadIdx.x & 63, g = threadIdx.x >> 6;
     const int64_t col = (int64_t)blockIdx.x * 64 + c;
@@ -438,7 +441,8 @@ __global__ __launch_bounds__(1024) void mx_unit_columns_kernel(const float* __re
     __syncthreads();
     if (g == 0 && col < cols) {
         for (int k = 1; k < 16; ++k) s += red[k][c];
-        out[col] = s > 0.0 ? (float)sqrt(n / s) : 1.0f;
+        if (!FACTOR) sum[col] = s;
+        else out[col] = s > 0.0 && sum[col] > 0.0 ? (float)sqrt(sum[col] / s) : 1.0f;
     }
 }
 __global__ __launch_bounds__(256) void mx_scale_columns_kernel(float* __restrict__ x, int64_t rows, int64_t cols, int64_t ld, const float* __restrict__ f) {

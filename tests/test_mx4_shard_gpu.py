@@ -1,0 +1,87 @@
+"""The shard of a fit with Corex(x_storage="mx4") where preprocessed variables do not have mean square 1: missing cells (the standard deviation is
+that of the observed ones, the others are 0), squashed outliers, ranks, no scaling at all.  X~ is the 4-bit rounding times one float32 factor
+per variable, sqrt(sum x^2 / sum rounded^2): every variable keeps the mean square it had."""
+import numpy as np
+import pytest
+
+from linearcorex_amd import Corex
+from linearcorex_amd.backend import HipBackend
+from oracle import corex_oracle as O
+from tests import mx4_reference as R
+
+pytestmark = pytest.mark.gpu
+
+
+def kept(x):
+    """X~ of preprocessed data, in float64"""
+    x = x.astype(np.float64)
+    v = R.round4(x)
+    a, b = (x ** 2).sum(axis=0), (v ** 2).sum(axis=0)
+    return v * np.sqrt(np.where((a > 0) & (b > 0), a, 1) / np.where((a > 0) & (b > 0), b, 1))
+
+
+def data(kind, n, v, k):
+    """data whose preprocessed variables have a mean square of their own"""
+    x, _ = O.gen_planted(n, v, k, seed=5)
+    r = np.random.RandomState(2)
+    kw = dict(gaussianize="standard", missing_values=None)
+    if kind == "missing":
+        x[r.rand(*x.shape) < 0.3] = -999.0
+        kw["missing_values"] = -999.0
+    elif kind == "none":
+        x *= np.linspace(0.3, 0.7, v)
+        kw["gaussianize"] = "none"
+    elif kind == "outliers":
+        x *= np.exp(0.8 * r.randn(n, 1))
+        kw["gaussianize"] = "outliers"
+    elif kind == "empirical":
+        kw["gaussianize"] = "empirical"
+    return np.asarray(x, np.float32), kw
+
+
+KINDS = ["standard", "missing", "none", "outliers", "empirical"]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n,v", [(400, 60), (130, 1200)])
+def test_every_variable_keeps_its_mean_square(kind, n, v, monkeypatch):
+    if v > 1000:
+        monkeypatch.setenv("LCX_PANEL_BLOCK_COLS", "512")                # several staging blocks
+    x, kw = data(kind, n, v, 3)
+    a, b = (Corex(n_hidden=3, seed=0, max_iter=2, x_storage=s, **kw).fit(x) for s in ("mx4", "dense"))
+    dense = b._backend.download_x()
+    got, want = a._backend.download_x().astype(np.float64), kept(dense)
+    # the factor is rounded once and the product once; the 64-bit sums behind the factor count next to nothing
+    assert (np.abs(got - want) <= 2.01 * 2.0 ** -24 * np.abs(want)).all()
+    ms = (dense.astype(np.float64) ** 2).mean(axis=0)
+    assert kind == "standard" or np.abs(ms - 1).max() > 1e-3             # what the factor has to keep
+    # every value of a column has at most those two roundings, so its root mean square does
+    assert (np.abs(np.sqrt((got ** 2).mean(axis=0)) - np.sqrt(ms)) <= 2.01 * 2.0 ** -24 * np.sqrt(ms)).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_fit_is_that_of_the_original_data_but_for_rounding_noise(kind):
+    """the bars of the clean data's fit (test_mx4_fit_gpu.py): 5e-5 against a dense fit of X~, 15 % against one of the data themselves"""
+    x, kw = data(kind, 400, 60, 3)
+    a, b = (Corex(n_hidden=3, seed=0, x_storage=s, **kw).fit(x) for s in ("mx4", "dense"))
+    c = Corex(n_hidden=3, seed=0, gaussianize="none").fit(kept(b._backend.download_x()).astype(np.float32))
+    assert abs(a.tc - c.tc) <= 5e-5 * abs(c.tc), (a.tc, c.tc)
+    assert abs(a.tc - b.tc) <= 0.15 * abs(b.tc), (a.tc, b.tc)
+    # new rows are projected as they are: weights of a rescaled matrix would be off by the scale
+    y, yd = a.transform(x), Corex.transform(c, b._backend.download_x())
+    assert np.abs(y - yd).max() <= 0.02 * np.abs(yd).max()
+
+
+def test_columns_without_a_value_and_columns_rounded_away():
+    """a variable of zeros, one that is far below the others of its block (all of it rounds to zero), one huge"""
+    x = np.random.RandomState(0).randn(90, 70).astype(np.float32)
+    x[:, 3], x[:, 40] = 0.0, x[:, 40] * 1e-4
+    x[:, 66] *= 2.0 ** 60
+    be = HipBackend(90, 70, 2, np.float32, x_storage="mx4")
+    try:
+        be.upload_x(x)
+        got, want = be.download_x().astype(np.float64), kept(x)
+        assert not got[:, 3].any() and not got[:, 40].any() and got[:, 66].any() and not got[:, 64:66].any() and not got[:, 67:].any()
+        assert (np.abs(got - want) <= 2.01 * 2.0 ** -24 * np.abs(want)).all()
+    finally:
+        be.close()

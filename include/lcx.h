@@ -110,7 +110,8 @@ int lcx_create(lcx_ctx** out, int64_t n_samples, int64_t nv_local, int n_hidden,
 /* The same with a choice of how the shard is held: x_storage 0 = as lcx_create, 1 = in 4 bits per value (lcx_x_layout 3; the format of
  * lcx_mx4_quantize below, blocks of 32 variables of a sample, and one float32 factor per variable that gives it back the mean
  * square it had before the rounding): 4.25 bits instead of 32, so that 7.5 times larger shards fit and both X passes read that much less.  What is fitted is the
- * rounded matrix (lcx_download_x returns it); with it every pass is exact up to float32 sums.  LCX_F32 and n_hidden <= 128 only.
+ * rounded matrix (lcx_download_x returns it), the same for any number of ranks if their shards begin at multiples of 32 variables; with it
+ * every pass is exact up to float32 sums.  LCX_F32 and n_hidden <= 128 only.
  * Everything else of the handle is the same; transform of new rows (lcx_project*) does not touch the shard. */
 int lcx_create_stored(lcx_ctx** out, int64_t n_samples, int64_t nv_local, int n_hidden, int dtype, int device, int x_storage);
 int lcx_destroy(lcx_ctx* h);

@@ -102,13 +102,20 @@ class Comm:
         elif err:
             raise ValueError(err)
 
-    # contiguous column ranges: balanced, or the caller's boundaries
-    def shard(self, nv, rank=None):
+    # contiguous column ranges: balanced, or the caller's boundaries.  unit: shards begin at multiples of it (variables that must stay together)
+    def shard(self, nv, rank=None, unit=1):
         r = self.rank if rank is None else rank
         if self.bounds is not None:
             if self.bounds[-1] != nv:
                 raise ValueError("shard boundaries end at %d, the data have %d variables" % (self.bounds[-1], nv))
+            if any(b % unit for b in self.bounds[:-1]):
+                raise ValueError("shard boundaries %r: %d neighbouring variables must stay together" % (self.bounds, unit))
             return self.bounds[r], self.bounds[r + 1]
+        if unit > 1 and self.world > 1:
+            blocks = -(-nv // unit)
+            if blocks < self.world:
+                raise ValueError("%d variables in blocks of %d do not give each of %d ranks one" % (nv, unit, self.world))
+            return blocks * r // self.world * unit, min(nv, blocks * (r + 1) // self.world * unit)
         return (nv * r) // self.world, (nv * (r + 1)) // self.world
 
     def allreduce(self, tensor):
@@ -270,13 +277,13 @@ class Comm:
                                % (self.rank, err or "on another rank"))
         return "hook"
 
-    def gather_columns(self, local, nv, like):
-        """All-gather per-rank column blocks (last axis) into the full array on every rank.
+    def gather_columns(self, local, nv, like, unit=1):
+        """All-gather per-rank column blocks (last axis, cut by `shard` with this unit) into the full array on every rank.
         `like` is a tensor on the device the group communicates on."""
         import torch
         if self.world == 1:
             return local
-        widths = [self.shard(nv, r)[1] - self.shard(nv, r)[0] for r in range(self.world)]
+        widths = [b - a for a, b in (self.shard(nv, r, unit) for r in range(self.world))]
         wmax = max(widths)
         lead = local.shape[:-1]
         pad = np.zeros(lead + (wmax,), dtype=local.dtype)
@@ -293,7 +300,7 @@ class SingleComm:
     """world size 1: no torch import, no collectives."""
     rank, world, exchange = 0, 1, False
 
-    def shard(self, nv, rank=None):
+    def shard(self, nv, rank=None, unit=1):
         return 0, nv
 
     def allreduce(self, tensor):
@@ -308,5 +315,5 @@ class SingleComm:
     def bind_engine(self, backend, first_contact=True):
         return None
 
-    def gather_columns(self, local, nv, like=None):
+    def gather_columns(self, local, nv, like=None, unit=1):
         return local

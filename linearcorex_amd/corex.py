@@ -306,7 +306,8 @@ class Corex(object):
               matrices that would not fit, or passes that would take too long.  The model is then fitted to the rounded data (about one
               per cent of a variable's variance is rounding noise, so correlations come out that much weaker); products and sums are as
               exact as those of a float32 fit.  Every variable keeps its mean square; 32 neighbours share a scale, so with
-              gaussianize="none" neighbours should be of similar size.  float32 and n_hidden <= 128 only.  `transform` of new data is not affected.
+              gaussianize="none" neighbours should be of similar size.  Several ranks: shards begin at multiples of 32
+              variables, so the rounded data are the same for any number of them.  float32 and n_hidden <= 128 only.  `transform` of new data is not affected.
     """
 
     # defaults for models pickled by an earlier build
@@ -509,8 +510,16 @@ class Corex(object):
         if self._comm.world == 1:
             return local
         if key == "X_i Z_j":
-            return self._comm.gather_columns(np.ascontiguousarray(local.T), self.nv, self._ex[1]).T
-        return self._comm.gather_columns(local, self.nv, self._ex[1])
+            return self._comm.gather_columns(np.ascontiguousarray(local.T), self.nv, self._ex[1], **self._unit()).T
+        return self._comm.gather_columns(local, self.nv, self._ex[1], **self._unit())
+
+    def _unit(self):
+        """32 variables of a 4-bit shard share a scale: the blocks stay together, so that the rounded matrix is the same for any number of ranks"""
+        return {} if self.x_storage == "dense" else {"unit": 32}
+
+    def _shard(self):
+        """columns [c0, c1) of this rank"""
+        return self._comm.shard(self.nv, **self._unit())
 
     # ------------------------------------------------------------------------------------------
     # public API
@@ -553,7 +562,7 @@ class Corex(object):
             raise NotImplementedError("n_hidden=None (pick_n_hidden) is broken in the reference (SURVEY.md §2 #14)")
         x = np.asarray(x, dtype=self.dtype)                    # reference casts to float32 (:108)
         self.n_samples, self.nv = x.shape
-        c0, c1 = self._comm.shard(self.nv)
+        c0, c1 = self._shard()
         self._cols = (c0, c1)
         be = self._make_backend(self.n_samples, c1 - c0)
         self._x_resident = True
@@ -583,7 +592,7 @@ class Corex(object):
         """Fit on synthetic data generated and standardised on the device (sizes that cannot be
         staged on the host).  kind 0 = iid N(0,1), 1 = planted groups."""
         self.n_samples, self.nv = int(n_samples), int(n_variables)
-        c0, c1 = self._comm.shard(self.nv)
+        c0, c1 = self._shard()
         self._cols = (c0, c1)
         be = self._make_backend(self.n_samples, c1 - c0)
         self._x_resident = True
@@ -594,9 +603,9 @@ class Corex(object):
 
     def _attach_shard(self, x_local, nv_total):
         """Make an already preprocessed column block resident as this rank's shard (bench / tests):
-        x_local is n_samples x (c1-c0) for (c0, c1) = comm.shard(nv_total)."""
+        x_local is n_samples x (c1-c0) for (c0, c1) = comm.shard(nv_total) (data in 4 bits: with unit=32)."""
         self.n_samples, self.nv = int(x_local.shape[0]), int(nv_total)
-        self._cols = self._comm.shard(self.nv)
+        self._cols = self._shard()
         assert x_local.shape[1] == self._cols[1] - self._cols[0]
         be = self._make_backend(self.n_samples, x_local.shape[1])
         self._x_resident = True
@@ -1157,7 +1166,7 @@ class Corex(object):
             # restored from a pickle: bring W (and what get_covariance needs) back to the device.  The data are NOT
             # resident any more, so the handle is created for a single (empty) sample: transform / get_covariance only
             # need W and the per-variable moments, not an n_samples x n_variables shard and its transposed copy
-            self._cols = self._comm.shard(self.nv)
+            self._cols = self._shard()
             be = self._make_backend(1, self.nv, fit=False)
             be.set_ws(np.asarray(self.ws, dtype=self.dtype))
             self._moments_restored = False

@@ -1,13 +1,18 @@
 """The shard of a fit with Corex(x_storage="mx4") where preprocessed variables do not have mean square 1: missing cells (the standard deviation is
 that of the observed ones, the others are 0), squashed outliers, ranks, no scaling at all.  X~ is the 4-bit rounding times one float32 factor
 per variable, sqrt(sum x^2 / sum rounded^2): every variable keeps the mean square it had."""
+import threading
+
 import numpy as np
 import pytest
 
-from linearcorex_amd import Corex
-from linearcorex_amd.backend import HipBackend
-from oracle import corex_oracle as O
-from tests import mx4_reference as R
+torch = pytest.importorskip("torch")          # before the library, which must resolve against the HIP runtime of torch's wheel
+from linearcorex_amd import Corex                                       # noqa: E402
+from linearcorex_amd.backend import HipBackend                          # noqa: E402
+from linearcorex_amd.comm import Comm                                   # noqa: E402
+from oracle import corex_oracle as O                                    # noqa: E402
+from tests import mx4_reference as R                                    # noqa: E402
+from tests.test_thread_ranks_gpu import TIMEOUT, ThreadComm, _run_loop, _Shared       # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -85,3 +90,64 @@ def test_columns_without_a_value_and_columns_rounded_away():
         assert (np.abs(got - want) <= 2.01 * 2.0 ** -24 * np.abs(want)).all()
     finally:
         be.close()
+
+
+class BlockComm(ThreadComm):
+    """ranks that are threads, cut as `linearcorex_amd.comm.Comm` cuts them"""
+
+    def __init__(self, shared, rank, nv):
+        c = Comm.__new__(Comm)
+        c.world, c.bounds = shared.world, None
+        self.cut = c
+        super().__init__(shared, rank, [0] + [c.shard(nv, r, 32)[1] for r in range(shared.world)])
+
+    def shard(self, nv, rank=None, unit=1):
+        return self.cut.shard(nv, self.rank if rank is None else rank, unit)
+
+    def gather_columns(self, local, nv, like, unit=1):
+        assert local.shape[-1] == self.shard(nv, unit=unit)[1] - self.shard(nv, unit=unit)[0]
+        return super().gather_columns(local, nv, like)
+
+
+def _ranked(x, w0, iters, comm, out):
+    n, v = x.shape
+    model = Corex(n_hidden=len(w0), seed=None, tol=0.0, device=0, comm=comm, x_storage="mx4")
+    c0, c1 = (0, v) if comm is None else comm.shard(v, unit=32)
+    be = model._attach_shard(np.ascontiguousarray(x[:, c0:c1]), v)
+    model.ws = w0
+    out["x"] = be.download_x()
+    out["history"] = _run_loop(model, iters)
+    out["ws"] = model._gather(be.get_ws(0))
+    be.close()
+
+
+@pytest.mark.parametrize("world", [2, 3, 8])
+@pytest.mark.parametrize("n,v,m", [(400, 260, 3), (900, 1111, 40)])
+def test_the_fitted_matrix_does_not_depend_on_the_number_of_ranks(world, n, v, m):
+    iters = 8
+    x = O.preprocess(O.gen_planted(n, v, 3, seed=4)[0])[0].astype(np.float32)
+    w0 = (np.random.RandomState(3).randn(m, v) * 0.004).astype(np.float32)
+    one = {}
+    _ranked(x, w0, iters, None, one)
+    shared, results, errors = _Shared(world), [{} for _ in range(world)], []
+
+    def main(r):
+        try:
+            torch.cuda.set_device(0)
+            _ranked(x, w0, iters, BlockComm(shared, r, v), results[r])
+        except BaseException as e:          # noqa: BLE001 - the others fail on the broken barrier
+            errors.append(e)
+            shared.barrier.abort()
+
+    threads = [threading.Thread(target=main, args=(r,), daemon=True) for r in range(world)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(TIMEOUT)
+    assert not errors, errors
+    # X~ to the bit; the trajectory to float32 rounding (the bar of test_thread_ranks_gpu.py)
+    assert np.array_equal(np.concatenate([r["x"] for r in results], axis=1), one["x"])
+    for r in results:
+        assert np.array_equal(r["history"], results[0]["history"]) and len(r["history"]) == len(one["history"]) == iters
+        assert np.max(np.abs(r["history"] - one["history"]) / np.maximum(1.0, np.abs(one["history"]))) < 5e-5
+        assert np.max(np.abs(r["ws"] - one["ws"])) < 1e-3 * np.max(np.abs(one["ws"]))

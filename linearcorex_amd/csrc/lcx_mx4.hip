@@ -219,20 +219,25 @@ template <typename T> static int mx_join(int split, const MxOut<T>& w, hipStream
     return LCX_OK;
 }
 
-template <typename T, int CT, int JS, bool DIRECT = false>
+// fragments of the contraction (linear) and steps (linear_grad) a stage holds, by the height of a tile
+template <typename T> constexpr int mx_linear_js(int ct) { return MxTerms<T>::v == 3 && ct == 4 ? 2 : 4; }      // (three terms of four: 96 KB of LDS, one block a CU)
+template <typename T> constexpr int mx_grad_js() { return MxTerms<T>::v > 1 ? 1 : 2; }         // (a second step would be 83 KB with two terms: one block a CU)
+
+template <typename T, int CT, bool DIRECT = false>
 static int mx_linear_tiles(const MxPlan& p, const unsigned short* frag, int64_t tiles, const unsigned char* wc, const unsigned char* ws, int64_t N, int64_t K, const MxOut<T>& w,
                            hipStream_t st) {
     unsigned g;
     LCXCHECK(mx_grid(8, cdiv(p.mt * p.nt * p.split, 8), 256, &g));
-    hipLaunchKernelGGL((mx_linear_tile_kernel<T, CT, 4, JS, DIRECT>), dim3(g), dim3(256), 0, st, frag, tiles, wc, ws, N, K, w, (int)p.mt, (int)p.nt, p.split);
+    hipLaunchKernelGGL((mx_linear_tile_kernel<T, CT, 4, mx_linear_js<T>(CT), DIRECT>), dim3(g), dim3(256), 0, st, frag, tiles, wc, ws, N, K, w, (int)p.mt, (int)p.nt, p.split);
     KCHECK();
     return LCX_OK;
 }
-template <typename T, int CT, int JS, bool DIRECT = false>
+template <typename T, int CT, bool DIRECT = false>
 static int mx_grad_tiles(const MxPlan& p, const unsigned short* frag, int64_t tiles, const unsigned char* wc, const unsigned char* ws, int64_t N, int64_t K, const MxOut<T>& w,
                          hipStream_t st) {
     unsigned g;
     LCXCHECK(mx_grid(8, cdiv(p.mt * p.nt * p.split, 8), 256, &g));
+    constexpr int JS = mx_grad_js<T>();
     constexpr size_t lds = MxGradLds<CT, JS, MxTerms<T>::v>::total;
     LCXCHECK(allow_lds(mx_grad_tile_kernel<T, CT, JS, DIRECT>, lds));
     hipLaunchKernelGGL((mx_grad_tile_kernel<T, CT, JS, DIRECT>), dim3(g), dim3(256), lds, st, frag, tiles, wc, ws, N, K, w, (int)p.mt, (int)p.nt, p.split);
@@ -269,21 +274,20 @@ static int mx4_linear(const void* xv, int64_t M, int64_t xrs, int64_t xcs, const
     if constexpr (TERMS == 1) {
         if (K % 128 == 0 && mx_direct(x, xrs, xcs)) {
             const unsigned short* xb = (const unsigned short*)xv;
-            if (p.ct == 1) LCXCHECK((mx_linear_tiles<T, 1, 4, true>(p, xb, xrs, wc, ws, N, K, w, st)));
-            else if (p.ct == 2) LCXCHECK((mx_linear_tiles<T, 2, 4, true>(p, xb, xrs, wc, ws, N, K, w, st)));
-            else if (p.ct == 4) LCXCHECK((mx_linear_tiles<T, 4, 4, true>(p, xb, xrs, wc, ws, N, K, w, st)));
-            else LCXCHECK((mx_linear_tiles<T, 8, 4, true>(p, xb, xrs, wc, ws, N, K, w, st)));
+            if (p.ct == 1) LCXCHECK((mx_linear_tiles<T, 1, true>(p, xb, xrs, wc, ws, N, K, w, st)));
+            else if (p.ct == 2) LCXCHECK((mx_linear_tiles<T, 2, true>(p, xb, xrs, wc, ws, N, K, w, st)));
+            else if (p.ct == 4) LCXCHECK((mx_linear_tiles<T, 4, true>(p, xb, xrs, wc, ws, N, K, w, st)));
+            else LCXCHECK((mx_linear_tiles<T, 8, true>(p, xb, xrs, wc, ws, N, K, w, st)));
             return mx_join<T>(p.split, w, st);
         }
     }
     LCXCHECK((mx_fragments<T, true>(x, M, xrs, xcs, K, p, frag, ex, st)));
     const int64_t tiles = p.mt * p.ct;
-    constexpr int JS = TERMS == 3 ? 2 : 4;                  // (three terms of four fragments would be 96 KB of LDS: one block a CU)
-    if (p.ct == 1) LCXCHECK((mx_linear_tiles<T, 1, 4>(p, frag, tiles, wc, ws, N, K, w, st)));
-    else if (p.ct == 2) LCXCHECK((mx_linear_tiles<T, 2, 4>(p, frag, tiles, wc, ws, N, K, w, st)));
-    else if (p.ct == 4) LCXCHECK((mx_linear_tiles<T, 4, JS>(p, frag, tiles, wc, ws, N, K, w, st)));
+    if (p.ct == 1) LCXCHECK((mx_linear_tiles<T, 1>(p, frag, tiles, wc, ws, N, K, w, st)));
+    else if (p.ct == 2) LCXCHECK((mx_linear_tiles<T, 2>(p, frag, tiles, wc, ws, N, K, w, st)));
+    else if (p.ct == 4) LCXCHECK((mx_linear_tiles<T, 4>(p, frag, tiles, wc, ws, N, K, w, st)));
     else {
-        if constexpr (TERMS == 1) LCXCHECK((mx_linear_tiles<T, 8, 4>(p, frag, tiles, wc, ws, N, K, w, st)));
+        if constexpr (TERMS == 1) LCXCHECK((mx_linear_tiles<T, 8>(p, frag, tiles, wc, ws, N, K, w, st)));
     }
     return mx_join<T>(p.split, w, st);
 }
@@ -302,18 +306,17 @@ static int mx4_linear_grad(const void* dyv, int64_t M, int64_t yrs, int64_t ycs,
     if constexpr (TERMS == 1) {
         if (N % 64 == 0 && mx_direct(dy, yrs, ycs)) {
             const unsigned short* yb = (const unsigned short*)dyv;
-            if (p.ct == 1) LCXCHECK((mx_grad_tiles<T, 1, 2, true>(p, yb, yrs, wc, ws, N, K, w, st)));
-            else if (p.ct == 2) LCXCHECK((mx_grad_tiles<T, 2, 2, true>(p, yb, yrs, wc, ws, N, K, w, st)));
-            else LCXCHECK((mx_grad_tiles<T, 4, 2, true>(p, yb, yrs, wc, ws, N, K, w, st)));
+            if (p.ct == 1) LCXCHECK((mx_grad_tiles<T, 1, true>(p, yb, yrs, wc, ws, N, K, w, st)));
+            else if (p.ct == 2) LCXCHECK((mx_grad_tiles<T, 2, true>(p, yb, yrs, wc, ws, N, K, w, st)));
+            else LCXCHECK((mx_grad_tiles<T, 4, true>(p, yb, yrs, wc, ws, N, K, w, st)));
             return mx_join<T>(p.split, w, st);
         }
     }
     LCXCHECK((mx_fragments<T, false>(dy, M, yrs, ycs, N, p, frag, ex, st)));
     const int64_t tiles = p.mt * p.ct;
-    constexpr int JS = TERMS > 1 ? 1 : 2;                   // (a second step would be 83 KB of LDS with two terms: one block a CU)
-    if (p.ct == 1) LCXCHECK((mx_grad_tiles<T, 1, JS>(p, frag, tiles, wc, ws, N, K, w, st)));
-    else if (p.ct == 2) LCXCHECK((mx_grad_tiles<T, 2, JS>(p, frag, tiles, wc, ws, N, K, w, st)));
-    else LCXCHECK((mx_grad_tiles<T, 4, JS>(p, frag, tiles, wc, ws, N, K, w, st)));
+    if (p.ct == 1) LCXCHECK((mx_grad_tiles<T, 1>(p, frag, tiles, wc, ws, N, K, w, st)));
+    else if (p.ct == 2) LCXCHECK((mx_grad_tiles<T, 2>(p, frag, tiles, wc, ws, N, K, w, st)));
+    else LCXCHECK((mx_grad_tiles<T, 4>(p, frag, tiles, wc, ws, N, K, w, st)));
     return mx_join<T>(p.split, w, st);
 }
 
@@ -441,8 +444,8 @@ int lcx_mx_shard_xty(lcx_ctx* h, const float* Y, float* out, const int* skip) {
 // name of the kernel of a pass (kind 0: X~ . B, else X~^T . Y), as a profiler shows it
 void lcx_mx_shard_kernel(const lcx_ctx* h, int kind, char* buf, int64_t len) {
     const MxPlan p = kind == 0 ? mx_plan<float>(true, h->Mp, h->ldx, h->Npad, true) : mx_plan<float>(false, h->Mp, h->Npad, h->ldx, true);
-    if (kind == 0) snprintf(buf, (size_t)len, "lcx::mx_linear_tile_kernel<float, %d, 4, %d, false>", p.ct, p.ct == 4 ? 2 : 4);
-    else snprintf(buf, (size_t)len, "lcx::mx_grad_tile_kernel<float, %d, 1, false>", p.ct);
+    if (kind == 0) snprintf(buf, (size_t)len, "lcx::mx_linear_tile_kernel<float, %d, 4, %d, false>", p.ct, mx_linear_js<float>(p.ct));
+    else snprintf(buf, (size_t)len, "lcx::mx_grad_tile_kernel<float, %d, %d, false>", p.ct, mx_grad_js<float>());
 }
 
 extern "C" {

@@ -1,6 +1,9 @@
 """The shard of a fit with Corex(x_storage="mx4") where preprocessed variables do not have mean square 1: missing cells (the standard deviation is
 that of the observed ones, the others are 0), squashed outliers, ranks, no scaling at all.  X~ is the 4-bit rounding times one float32 factor
 per variable, sqrt(sum x^2 / sum rounded^2): every variable keeps the mean square it had."""
+import os
+import subprocess
+import sys
 import threading
 
 import numpy as np
@@ -151,3 +154,33 @@ def test_the_fitted_matrix_does_not_depend_on_the_number_of_ranks(world, n, v, m
         assert np.array_equal(r["history"], results[0]["history"]) and len(r["history"]) == len(one["history"]) == iters
         assert np.max(np.abs(r["history"] - one["history"]) / np.maximum(1.0, np.abs(one["history"]))) < 5e-5
         assert np.max(np.abs(r["ws"] - one["ws"])) < 1e-3 * np.max(np.abs(one["ws"]))
+
+
+def test_kernel_names_are_in_the_trace_of_a_run():
+    """`kernel_name` against the kernels that a profiler saw (a child process: the profiler stays attached to the one it ran in)"""
+    code = r'''
+import sys
+sys.path.insert(0, %r)
+import numpy as np
+import torch
+from torch.profiler import ProfilerActivity, profile
+from linearcorex_amd.backend import HipBackend
+for n, v, m in ((300, 200, 3), (2000, 3000, 30), (2000, 9000, 64), (700, 2000, 128), (20000, 2000, 64)):
+    r = np.random.RandomState(0)
+    be = HipBackend(n, v, m, np.float32, 0, x_storage="mx4")
+    be.upload_x(r.randn(n, v).astype(np.float32))
+    be.set_ws((r.randn(m, v) * 0.004).astype(np.float32))
+    torch.cuda.synchronize()
+    with profile(activities=[ProfilerActivity.CUDA]) as p:
+        be.moments_a(0)
+        be.moments_b(0, 0.3, False)
+        be.moments_c(0)
+        torch.cuda.synchronize()
+    ran = {e.name.split("(")[0].replace("void ", "") for e in p.events()}
+    for kind in (0, 1):
+        assert be.kernel_name(kind) in ran, (n, v, m, be.kernel_name(kind), sorted(ran))
+    be.close()
+print("NAMES_OK")
+''' % os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    p = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=110)
+    assert p.returncode == 0 and "NAMES_OK" in p.stdout, (p.stdout[-500:], p.stderr[-2000:])

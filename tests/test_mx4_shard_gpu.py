@@ -184,3 +184,20 @@ print("NAMES_OK")
 ''' % os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     p = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=110)
     assert p.returncode == 0 and "NAMES_OK" in p.stdout, (p.stdout[-500:], p.stderr[-2000:])
+
+
+def test_fit_transform_is_fit_and_transform():
+    """of the data as they are, not of the rounded ones"""
+    x, kw = data("missing", 300, 100, 3)
+    # (the seed is NumPy's global one, set when a model is made)
+    a = Corex(n_hidden=3, seed=0, x_storage="mx4", **kw)
+    y = a.fit_transform(x)
+    b = Corex(n_hidden=3, seed=0, x_storage="mx4", **kw)
+    yt = b.fit(x).transform(x)
+    assert np.array_equal(a.ws, b.ws) and np.array_equal(y, yt)          # one process, one seed: the same launches
+    want = O.preprocess(x.astype(np.float64), None, "standard", -999.0)[0] @ a.ws.T.astype(np.float64)
+    s = np.abs(O.preprocess(x.astype(np.float64), None, "standard", -999.0)[0]) @ np.abs(a.ws.T.astype(np.float64))
+    # float32: preprocessing (mean, scale, difference, quotient: 4 roundings of values up to |x - mean| + |mean|, |mean| < 1), 100 products and sums
+    assert (np.abs(y - want) <= (100 + 8) * 2.0 ** -24 * s + 4 * 2.0 ** -24 * np.abs(a.ws).sum(axis=1)).all()
+    rounded = kept(O.preprocess(x.astype(np.float64), None, "standard", -999.0)[0]) @ a.ws.T.astype(np.float64)
+    assert np.abs(y - want).max() < 1e-3 * np.abs(rounded - want).max()

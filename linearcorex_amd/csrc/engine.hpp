@@ -985,6 +985,7 @@ int lcx_mx_shard_read(lcx_ctx* h, float* stage, int64_t ld, int64_t c0, int64_t 
 int lcx_mx_shard_xbt(lcx_ctx* h, const float* B, float* out, const int* skip);
 int lcx_mx_shard_xty(lcx_ctx* h, const float* Y, float* out, const int* skip);
 void lcx_mx_shard_kernel(const lcx_ctx* h, int kind, char* buf, int64_t len);
+void lcx_mx_plan(int op, int dtype, int64_t M, int64_t N, int64_t K, int* v);
 #pragma GCC visibility pop
 
 // the member definitions of Impl<T, CT>, along the seams of the C ABI

@@ -343,6 +343,22 @@ static MxMatmulPlan mx_matmul_plan(int64_t M, int64_t N, int64_t K) {
 
 static int64_t mx_matmul_bytes(int64_t M, int64_t N, int64_t K) { return mx_matmul_plan(M, N, K).part_bytes; }
 
+// what a product of these sizes is made of (tools/lcx_probe.h, lcx_test_mx4_plan): {row kernel, 16-row tiles of x, of W, parts}
+template <typename T> static void mx_plan_of(int op, int64_t M, int64_t N, int64_t K, int* v) {
+    if (op == 0) {
+        const MxMatmulPlan p = mx_matmul_plan(M, N, K);
+        v[0] = p.row, v[1] = p.ct, v[2] = p.row ? p.rt : 4, v[3] = p.split;
+    } else {
+        const MxPlan p = op == 1 ? mx_plan<T>(true, M, K, N) : mx_plan<T>(false, M, N, K);
+        v[0] = p.row, v[1] = p.ct, v[2] = p.rt, v[3] = p.split;
+    }
+}
+void lcx_mx_plan(int op, int dtype, int64_t M, int64_t N, int64_t K, int* v) {
+    if (dtype == LCX_F32) mx_plan_of<float>(op, M, N, K, v);
+    else if (dtype == LCX_BF16) mx_plan_of<__bf16>(op, M, N, K, v);
+    else mx_plan_of<_Float16>(op, M, N, K, v);
+}
+
 template <typename T, int CT, int RT>
 static int mx_matmul_tiles(const MxMatmulPlan& p, const unsigned char* ac, const unsigned char* as, const unsigned char* bc, const unsigned char* bs, int64_t N,
                            int64_t K, const MxOut<T>& w, hipStream_t st) {

@@ -16,6 +16,7 @@ PROBE_SIGNATURES = {
     "lcx_bench_graph": [_vp, _dbl, _i32, C.POINTER(_dbl), C.POINTER(_dbl)],
     "lcx_test_gemm_nt": [_i32, _i32, _vp, _i64, _i64, _i64, _vp, _i32, _vp, _i32, _i32],
     "lcx_test_gemm_tn": [_i32, _i32, _vp, _i64, _i64, _i64, _vp, _i32, _vp, _vp, _i32, _i32],
+    "lcx_test_mx4_plan": [_i32, _i32, _i64, _i64, _i64, C.POINTER(_i32)],
 }
 _lib = None
 
@@ -55,6 +56,13 @@ class ProbeBackend(HipBackend):
         ms = C.c_double()
         check(self.lib.lcx_bench_gemm(self.h, int(kind), int(iters), C.byref(ms)))
         return ms.value
+
+
+def mx4_plan(op, dtype, m, n, k):
+    """(row kernel, 16-row tiles of x, of W, parts of the contraction) of a product of 4-bit matrices; no GPU needed"""
+    v = (C.c_int * 4)()
+    check(load().lcx_test_mx4_plan(op, dtype, m, n, k, v))
+    return bool(v[0]), v[1], v[2], v[3]
 
 
 def gemm_nt_check(a, b_km, m_pad, dtype, device=0, split=1, waves=4):

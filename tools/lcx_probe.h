@@ -30,6 +30,10 @@ int lcx_test_gemm_tn(int dtype, int device, const void* a_host, int64_t k, int64
                      const void* b_host, int m_pad, const void* rowscale_host, void* out_host,
                      int force_split, int force_kw);
 
+/* ---- which kernels a product of 4-bit matrices takes (host only): op and dtype as lcx_mx4_workspace; out {row kernel, 16-row tiles of x and of W
+ * a wave holds, parts of the contraction} */
+int lcx_test_mx4_plan(int op, int dtype, int64_t M, int64_t N, int64_t K, int* out);
+
 #ifdef __cplusplus
 }
 #endif

@@ -196,5 +196,11 @@ int lcx_test_gemm_tn(int dtype, int device, const void* a, int64_t k, int64_t v,
     return fail(LCX_ERR_ARG, "m_pad must be 16, 32, 64 or 128");
 }
 
+int lcx_test_mx4_plan(int op, int dtype, int64_t M, int64_t N, int64_t K, int* out) {
+    if (!out || op < 0 || op > 2 || M < 1 || N < 1 || K < 1 || dtype < LCX_F32 || dtype > LCX_F16 || dtype == LCX_F64)
+        return fail(LCX_ERR_ARG, "lcx_test_mx4_plan: bad argument");
+    lcx_mx_plan(op, dtype, M, N, K, out);
+    return LCX_OK;
+}
 
 }  // extern "C"

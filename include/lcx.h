@@ -443,8 +443,11 @@ int lcx_kernel_name(lcx_ctx* h, int kind, char* buf, int64_t len);
  * These entry points have no handle: every pointer is device memory of the current device, the work goes to `stream` (a hipStream_t of
  * that device, NULL = the default stream) and the call returns without waiting; nothing is kept from one call to the next, so calls on
  * different streams may overlap.  Codes, scales and work space must be 16-byte aligned.  Strides count elements.  rows, cols, M, N, K
- * may be 0: an empty output is left alone, an empty contraction gives zeros.  Outputs must not overlap inputs.  Sizes from 2^31 on, and
- * matrices of more pieces of 16 rows x 512 columns than a launch can count (2^24), are refused with LCX_ERR_ARG. */
+ * may be 0: an empty output is left alone, an empty contraction gives zeros.  Outputs must not overlap inputs.  Sizes from 2^31 on are
+ * refused with LCX_ERR_ARG, and so is what one launch cannot count: quantising and reading back from 2^24 pieces of 16 rows x 512 columns on (2^23 of
+ * 64 x 512 where rows are neighbours); products from 2^24 pieces of 16 rows x 128 of the contraction of x on,
+ * from 2^24 tiles of output times parts of the contraction on (a tile is 16 to 128 rows x 256 columns, lcx_mx4_linear_grad: 512), and with up
+ * to 16 rows of x from 2^23 pieces of 16 (lcx_mx4_linear: 32) rows of W on. */
 int lcx_mx4_layout(int64_t rows, int64_t cols, int64_t* code_bytes, int64_t* scale_bytes);
 /* x[r * row_stride + c * col_stride] (any lcx_dtype) -> codes, scales; blocks run along c */
 int lcx_mx4_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, int64_t col_stride, void* codes,

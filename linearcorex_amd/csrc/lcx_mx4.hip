@@ -24,6 +24,8 @@ static constexpr int64_t MX_MAX_DIM = (int64_t)1 << 31;
         default: return fail(LCX_ERR_ARG, std::string(#fn) + ": dtype must be LCX_F32, LCX_BF16 or LCX_F16"); \
     }
 
+constexpr int64_t MX_MAX_PIECES = (int64_t)1 << 24;             // blocks of 256 threads that a launch can count
+
 constexpr int MX_CUS = 256;            // blocks are sized for a whole MI355X; the choices below only shift speed
 
 static int64_t dim_bad(int64_t a, int64_t b, int64_t c = 0) { return a < 0 || b < 0 || c < 0 || a >= MX_MAX_DIM || b >= MX_MAX_DIM || c >= MX_MAX_DIM; }
@@ -40,11 +42,11 @@ template <typename T>
 static int mx4_quantize(const void* x, int64_t rows, int64_t cols, int64_t rs, int64_t cs, void* codes, void* scales, hipStream_t st) {
     unsigned char *qc = (unsigned char*)codes, *qs = (unsigned char*)scales;
     unsigned g;
-    const bool once = rows * cols * (int64_t)sizeof(T) >= MX_ONCE_BYTES;
     const int64_t steps = mx_steps(cols), quads = mx_quads(cols);
+    const auto once = [&] { return rows * cols * (int64_t)sizeof(T) >= MX_ONCE_BYTES; };          // (of sizes that a launch can count)
     if (rs == 1 && cs != 1) {
         LCXCHECK(mx_grid(cdiv(rows, 64), quads, 512, &g));
-        if (once) hipLaunchKernelGGL((mx_quantize_across_kernel<T, true>), dim3(g), dim3(512), 0, st, (const T*)x, rows, cols, cs, qc, qs);
+        if (once()) hipLaunchKernelGGL((mx_quantize_across_kernel<T, true>), dim3(g), dim3(512), 0, st, (const T*)x, rows, cols, cs, qc, qs);
         else hipLaunchKernelGGL((mx_quantize_across_kernel<T, false>), dim3(g), dim3(512), 0, st, (const T*)x, rows, cols, cs, qc, qs);
     } else {
         LCXCHECK(mx_grid(mx_row_tiles(rows), quads, 256, &g));
@@ -52,7 +54,7 @@ static int mx4_quantize(const void* x, int64_t rows, int64_t cols, int64_t rs, i
     hipLaunchKernelGGL((mx_quantize_kernel<T, VEC, ONCE>), dim3(g), dim3(256), 0, st, (const T*)x, rows, cols, rs, cs, qc, qs, steps, quads, (int64_t)0, \
                        (unsigned)quads)
         if (cs != 1) MX_QUANTIZE(false, false);
-        else if (once) MX_QUANTIZE(true, true);
+        else if (once()) MX_QUANTIZE(true, true);
         else MX_QUANTIZE(true, false);
 #undef MX_QUANTIZE
     }
@@ -172,7 +174,8 @@ template <typename T> static MxPlan mx_plan(bool along, int64_t M, int64_t C, in
     }
     p.mt = cdiv(M, 16 * p.ct);
     p.nfrag = cdiv(C, 128) * 4;
-    p.frag_bytes = p.nfrag * TERMS * p.mt * p.ct * 1024;
+    const int64_t pieces = p.mt * p.ct * cdiv(C, 128);         // (a block of mx_fragments_kernel each)
+    p.frag_bytes = pieces < MX_MAX_PIECES ? pieces * 4 * TERMS * 1024 : -1;
     if (p.split > 1) p.part_bytes = (int64_t)p.split * M * O * 4;
     return p;
 }
@@ -182,7 +185,8 @@ static int64_t mx_matmul_bytes(int64_t M, int64_t N, int64_t K);
 template <typename T> static int64_t mx_workspace(int op, int64_t M, int64_t N, int64_t K) {
     if (M == 0 || N == 0 || K == 0) return 0;
     if (op == 0) return mx_matmul_bytes(M, N, K);
-    return op == 1 ? mx_plan_bytes(mx_plan<T>(true, M, K, N)) : mx_plan_bytes(mx_plan<T>(false, M, N, K));
+    const MxPlan p = op == 1 ? mx_plan<T>(true, M, K, N) : mx_plan<T>(false, M, N, K);
+    return p.frag_bytes < 0 ? -1 : mx_plan_bytes(p);
 }
 
 template <typename T, bool ALONG>
@@ -200,9 +204,21 @@ static int mx_fragments(const T* x, int64_t M, int64_t rs, int64_t cs, int64_t C
     return LCX_OK;
 }
 
-// rows that the tile kernels take as they are (MxDirect; the offsets inside a tile are 32-bit)
-template <typename T> static bool mx_direct(const T* x, int64_t rs, int64_t cs) {
-    return cs == 1 && rs >= 0 && rs < (1 << 23) && rs % 8 == 0 && ((uintptr_t)x & 15) == 0;
+// rows that the tile kernels take as they are (MxDirect; the offsets inside a tile are 32-bit): C of the contraction, whole stages of it
+template <typename T> static bool mx_direct(const MxPlan& p, const T* x, int64_t rs, int64_t cs, int64_t C, int stage) {
+    return MxTerms<T>::v == 1 && !p.row && C % stage == 0 && cs == 1 && rs >= 0 && rs < (1 << 23) && rs % 8 == 0 && ((uintptr_t)x & 15) == 0;
+}
+
+// the work space as the plan wants it
+static int mx_space(const char* name, MxPlan& p, bool direct, const void* space, int64_t bytes) {
+    if (p.frag_bytes < 0) {
+        if (!direct) return fail(LCX_ERR_ARG, std::string(name) + ": x is too large for one call");
+        p.frag_bytes = 0;
+    }
+    const int64_t want = mx_plan_bytes(p);
+    if (bytes < want || (want && (!space || ((uintptr_t)space & 15))))
+        return fail(LCX_ERR_ARG, std::string(name) + ": the work space is smaller than lcx_mx4_workspace says or not 16-byte aligned");
+    return LCX_OK;
 }
 
 template <typename T> static int mx_join(int split, const MxOut<T>& w, hipStream_t st) {
@@ -263,16 +279,17 @@ static int mx4_linear(const void* xv, int64_t M, int64_t xrs, int64_t xcs, const
                       int64_t cs, void* space, int64_t space_bytes, hipStream_t st, const MxExtra& ex = MxExtra()) {
     constexpr int TERMS = MxTerms<T>::v;
     if (K == 0) return mx4_zero<T>(out, M, N, rs, cs, st);
-    const MxPlan p = mx_plan<T>(true, M, K, N, ex.tiles);
-    if (space_bytes < mx_plan_bytes(p) || (mx_plan_bytes(p) && (!space || ((uintptr_t)space & 15)))) return fail(LCX_ERR_ARG, "lcx_mx4_linear: the work space is smaller than lcx_mx4_workspace says or not 16-byte aligned");
+    MxPlan p = mx_plan<T>(true, M, K, N, ex.tiles);
     const T* x = (const T*)xv;
+    const bool direct = mx_direct(p, x, xrs, xcs, K, 128);
+    LCXCHECK(mx_space("lcx_mx4_linear", p, direct, space, space_bytes));
     const unsigned char *wc = (const unsigned char*)wcv, *ws = (const unsigned char*)wsv;
     unsigned short* frag = (unsigned short*)space;
     MxOut<T> w{(T*)out, rs, cs, p.split > 1 ? (float*)((char*)space + round_up(p.frag_bytes, 256)) : nullptr, M, N, rs == 1 && cs != 1, ex.oscale, ex.skip};
     if (p.row) return xcs == 1 ? mx_linear_rows<T, true>(p, x, xrs, xcs, wc, ws, N, K, w, st)
                                                 : mx_linear_rows<T, false>(p, x, xrs, xcs, wc, ws, N, K, w, st);
     if constexpr (TERMS == 1) {
-        if (K % 128 == 0 && mx_direct(x, xrs, xcs)) {
+        if (direct) {
             const unsigned short* xb = (const unsigned short*)xv;
             if (p.ct == 1) LCXCHECK((mx_linear_tiles<T, 1, true>(p, xb, xrs, wc, ws, N, K, w, st)));
             else if (p.ct == 2) LCXCHECK((mx_linear_tiles<T, 2, true>(p, xb, xrs, wc, ws, N, K, w, st)));
@@ -297,14 +314,15 @@ static int mx4_linear_grad(const void* dyv, int64_t M, int64_t yrs, int64_t ycs,
                            int64_t cs, void* space, int64_t space_bytes, hipStream_t st, const MxExtra& ex = MxExtra()) {
     constexpr int TERMS = MxTerms<T>::v;
     if (N == 0) return mx4_zero<T>(out, M, K, rs, cs, st);
-    const MxPlan p = mx_plan<T>(false, M, N, K, ex.tiles);
-    if (space_bytes < mx_plan_bytes(p) || (mx_plan_bytes(p) && (!space || ((uintptr_t)space & 15)))) return fail(LCX_ERR_ARG, "lcx_mx4_linear_grad: the work space is smaller than lcx_mx4_workspace says or not 16-byte aligned");
+    MxPlan p = mx_plan<T>(false, M, N, K, ex.tiles);
     const T* dy = (const T*)dyv;
+    const bool direct = mx_direct(p, dy, yrs, ycs, N, 64);
+    LCXCHECK(mx_space("lcx_mx4_linear_grad", p, direct, space, space_bytes));
     const unsigned char *wc = (const unsigned char*)wcv, *ws = (const unsigned char*)wsv;
     unsigned short* frag = (unsigned short*)space;
     MxOut<T> w{(T*)out, rs, cs, p.split > 1 ? (float*)((char*)space + round_up(p.frag_bytes, 256)) : nullptr, M, K, rs == 1 && cs != 1, ex.oscale, ex.skip};
     if constexpr (TERMS == 1) {
-        if (N % 64 == 0 && mx_direct(dy, yrs, ycs)) {
+        if (direct) {
             const unsigned short* yb = (const unsigned short*)dyv;
             if (p.ct == 1) LCXCHECK((mx_grad_tiles<T, 1, true>(p, yb, yrs, wc, ws, N, K, w, st)));
             else if (p.ct == 2) LCXCHECK((mx_grad_tiles<T, 2, true>(p, yb, yrs, wc, ws, N, K, w, st)));
@@ -506,7 +524,9 @@ int lcx_mx4_workspace(int op, int dtype, int64_t M, int64_t N, int64_t K, int64_
     MX_ENTRY({
         if (!bytes || op < 0 || op > 2 || dim_bad(M, N, K)) return fail(LCX_ERR_ARG, "lcx_mx4_workspace: bad argument");
         if (dtype != LCX_F32 && dtype != LCX_BF16 && dtype != LCX_F16) return fail(LCX_ERR_ARG, "lcx_mx4_workspace: bad dtype");
-        *bytes = dtype == LCX_F32 ? mx_workspace<float>(op, M, N, K) : dtype == LCX_BF16 ? mx_workspace<__bf16>(op, M, N, K) : mx_workspace<_Float16>(op, M, N, K);
+        const int64_t b = dtype == LCX_F32 ? mx_workspace<float>(op, M, N, K) : dtype == LCX_BF16 ? mx_workspace<__bf16>(op, M, N, K) : mx_workspace<_Float16>(op, M, N, K);
+        if (b < 0) return fail(LCX_ERR_ARG, "lcx_mx4_workspace: x is too large for one call");
+        *bytes = b;
         return LCX_OK;
     })
 }

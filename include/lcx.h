@@ -445,7 +445,7 @@ int lcx_kernel_name(lcx_ctx* h, int kind, char* buf, int64_t len);
  * different streams may overlap.  Codes, scales and work space must be 16-byte aligned.  Strides count elements.  rows, cols, M, N, K
  * may be 0: an empty output is left alone, an empty contraction gives zeros.  Outputs must not overlap inputs.  Sizes from 2^31 on are
  * refused with LCX_ERR_ARG, and so is what one launch cannot count: quantising and reading back from 2^24 pieces of 16 rows x 512 columns on (2^23 of
- * 64 x 512 where rows are neighbours); products from 2^24 pieces of 16 rows x 128 of the contraction of x on,
+ * 64 x 512 where rows are neighbours); products from 2^24 pieces of 16 rows x 128 of the contraction of x on (unless it is read in place),
  * from 2^24 tiles of output times parts of the contraction on (a tile is 16 to 128 rows x 256 columns, lcx_mx4_linear_grad: 512), and with up
  * to 16 rows of x from 2^23 pieces of 16 (lcx_mx4_linear: 32) rows of W on. */
 int lcx_mx4_layout(int64_t rows, int64_t cols, int64_t* code_bytes, int64_t* scale_bytes);
@@ -456,7 +456,8 @@ int lcx_mx4_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64
 int lcx_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, void* out, int dtype, int64_t row_stride,
                        int64_t col_stride, void* stream);
 /* Bytes of device memory that the product of the given sizes wants as work space: op 0 lcx_mx4_matmul, 1 lcx_mx4_linear,
- * 2 lcx_mx4_linear_grad; dtype as in the call (op 0: of the output).  The same space may serve any number of calls on ONE stream. */
+ * 2 lcx_mx4_linear_grad; dtype as in the call (op 0: of the output).  3, 4: as 1, 2 for LCX_BF16 x that is read in place, which takes less: neighbouring
+ * columns, rows a multiple of 8 (0 included) below 2^23 apart, 16-byte aligned, K a multiple of 128 (linear_grad: N of 64).  The same space may serve any number of calls on ONE stream. */
 int lcx_mx4_workspace(int op, int dtype, int64_t M, int64_t N, int64_t K, int64_t* bytes);
 /* out[m * row_stride + n * col_stride] = sum_k A[m][k] B[n][k] of two mx4 matrices (M x K, N x K): products exact, sums in float32, out in
  * LCX_F32 / LCX_BF16 / LCX_F16, rounded once */

@@ -185,8 +185,8 @@ static int64_t mx_matmul_bytes(int64_t M, int64_t N, int64_t K);
 template <typename T> static int64_t mx_workspace(int op, int64_t M, int64_t N, int64_t K) {
     if (M == 0 || N == 0 || K == 0) return 0;
     if (op == 0) return mx_matmul_bytes(M, N, K);
-    const MxPlan p = op == 1 ? mx_plan<T>(true, M, K, N) : mx_plan<T>(false, M, N, K);
-    return p.frag_bytes < 0 ? -1 : mx_plan_bytes(p);
+    const MxPlan p = op & 1 ? mx_plan<T>(true, M, K, N) : mx_plan<T>(false, M, N, K);
+    return op > 2 ? p.part_bytes : p.frag_bytes < 0 ? -1 : mx_plan_bytes(p);
 }
 
 template <typename T, bool ALONG>
@@ -209,12 +209,10 @@ template <typename T> static bool mx_direct(const MxPlan& p, const T* x, int64_t
     return MxTerms<T>::v == 1 && !p.row && C % stage == 0 && cs == 1 && rs >= 0 && rs < (1 << 23) && rs % 8 == 0 && ((uintptr_t)x & 15) == 0;
 }
 
-// the work space as the plan wants it
+// the plan without the fragments' space where x is taken as it is; the work space as the plan wants it
 static int mx_space(const char* name, MxPlan& p, bool direct, const void* space, int64_t bytes) {
-    if (p.frag_bytes < 0) {
-        if (!direct) return fail(LCX_ERR_ARG, std::string(name) + ": x is too large for one call");
-        p.frag_bytes = 0;
-    }
+    if (direct) p.frag_bytes = 0;
+    if (p.frag_bytes < 0) return fail(LCX_ERR_ARG, std::string(name) + ": x is too large for one call");
     const int64_t want = mx_plan_bytes(p);
     if (bytes < want || (want && (!space || ((uintptr_t)space & 15))))
         return fail(LCX_ERR_ARG, std::string(name) + ": the work space is smaller than lcx_mx4_workspace says or not 16-byte aligned");
@@ -522,7 +520,8 @@ int lcx_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int6
 
 int lcx_mx4_workspace(int op, int dtype, int64_t M, int64_t N, int64_t K, int64_t* bytes) {
     MX_ENTRY({
-        if (!bytes || op < 0 || op > 2 || dim_bad(M, N, K)) return fail(LCX_ERR_ARG, "lcx_mx4_workspace: bad argument");
+        if (!bytes || op < 0 || op > 4 || dim_bad(M, N, K)) return fail(LCX_ERR_ARG, "lcx_mx4_workspace: bad argument");
+        if (op > 2 && dtype != LCX_BF16) return fail(LCX_ERR_ARG, "lcx_mx4_workspace: only LCX_BF16 is read in place");
         if (dtype != LCX_F32 && dtype != LCX_BF16 && dtype != LCX_F16) return fail(LCX_ERR_ARG, "lcx_mx4_workspace: bad dtype");
         const int64_t b = dtype == LCX_F32 ? mx_workspace<float>(op, M, N, K) : dtype == LCX_BF16 ? mx_workspace<__bf16>(op, M, N, K) : mx_workspace<_Float16>(op, M, N, K);
         if (b < 0) return fail(LCX_ERR_ARG, "lcx_mx4_workspace: x is too large for one call");

@@ -244,11 +244,12 @@ def _product(x, shape, index, cp, sp, n, k, along):
         x2 = x.reshape(m, c)
     out = x.new_empty((m, o))
     if m and o:
-        dt = _DTYPES[x.dtype]
-        wb = _workspace_bytes(1 if along else 2, dt, m, n, k)
-        w = torch.empty(wb, dtype=torch.uint8, device=x.device) if wb else None
-        rs, cs = x2.stride()
-        _call(index, "lcx_mx4_linear" if along else "lcx_mx4_linear_grad", x2.data_ptr(), dt, m, rs, cs, cp, sp, n, k,
+        dt, (rs, cs), xp, op = _DTYPES[x.dtype], x2.stride(), x2.data_ptr(), 1 if along else 2
+        if m > 16 and dt == 2 and cs == 1 and not (rs | xp >> 1) & 7 and rs < 1 << 23 and not c & (127 if along else 63):
+            op += 2                      # read in place (include/lcx.h, lcx_mx4_workspace)
+        wb = _workspace_bytes(op, dt, m, n, k)
+        w = x.new_empty(wb, dtype=torch.uint8) if wb else None
+        _call(index, "lcx_mx4_linear" if along else "lcx_mx4_linear_grad", xp, dt, m, rs, cs, cp, sp, n, k,
               out.data_ptr(), o, 1, w.data_ptr() if wb else None, wb)
     return out if lead is None else out.reshape(lead + (o,))
 

@@ -110,3 +110,26 @@ def test_large_matrices_are_quantised_as_small_ones(t):
     for v in (x, xt):
         for q in (mx4.quantize(v), mx4.quantize(v.t(), axis=0)):
             assert torch.equal(q.codes, codes) and torch.equal(q.scales, scales)
+
+
+@pytest.mark.parametrize("m,n,k", [(2000, 4096, 8192), (40, 512, 8960)])
+def test_bfloat16_read_in_place_takes_no_copy(m, n, k):
+    from linearcorex_amd import mx4
+    q = mx4.quantize(ints((n, k), 1, 2))
+    for f, c, o in ((mx4.linear, k, n), (mx4.linear_grad, n, k)):
+        x = ints((m, c), 3, 4).bfloat16()
+        want = f(x, q)
+        torch.cuda.synchronize()
+        parts = taken((1 if f is mx4.linear else 2, BF16, m, n, k))[1]
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        assert torch.equal(f(x, q), want)
+        # the result, its comparison, the partial sums (blocks of 2 MB at most beside them)
+        assert torch.cuda.max_memory_allocated() - before <= m * o * (2 + 1) + (parts * m * o * 4 if parts > 1 else 0) + 4 * (2 << 20)
+        # the space that the C entry asks for does, to the byte
+        wb = mx4._workspace_bytes(3 if f is mx4.linear else 4, BF16, m, n, k)
+        space = torch.full((wb + 64,), 77, dtype=torch.uint8, device="cuda")
+        out = torch.empty(m, o, dtype=torch.bfloat16, device="cuda")
+        mx4._call(0, "lcx_mx4_linear" if f is mx4.linear else "lcx_mx4_linear_grad", x.data_ptr(), BF16, m, c, 1, q._cp, q._sp, n, k, out.data_ptr(), o, 1,
+                  space.data_ptr(), wb)
+        assert torch.equal(out, want) and (space[wb:] == 77).all()

@@ -154,8 +154,12 @@ template <typename T> static MxPlan mx_plan(bool along, int64_t M, int64_t C, in
         //   row    3.5 us + the steps a CU works through
         //   tiles  mx_choose, or reading W; 8 us for the two launches more
         // Measured, us, row / tiles: 1 x 4096 x 4096 bf16 4.7 / 11; 16 x 20000 x 20000 bf16 68 / 42, float32 135 / 49.
-        // 2 x 16 rows of W a wave halve the reads of x where there are enough rows to fill the chip (4 x 14336 x 4096 bf16 11.1 -> 8.7; 4 x 4096 x
-        // 4096 5.2 -> 5.9)
+        // 2 x 16 rows of W a wave halve the reads of x where there are enough rows to fill the chip.  One / two, us, bf16, W out of HBM:
+        //   rows of W x 4096   2048       4096       5120       6144       8192       12288      16384      28672
+        //   1 row of x         4.8/5.8    5.3/6.1    6.8/6.2    7.0/6.5    7.4/7.1    10.0/9.9   12.6/11.1  20.0/18.2
+        //   13                 6.3/7.1    7.0/7.5    10.9/7.6   11.0/7.9   11.3/8.4   15.5/13.2  19.6/14.0  32.0/23.7
+        // (Two are faster from 4097 rows on, but the model of the row kernel then comes out too low for long contractions: float16
+        // 16 x 7942 x 8833 would take it, 36 us, instead of the tiles, 24.)
         const int rt = O < 32 * MX_CUS ? 1 : 2;
         const double blocks = (double)cdiv(O, 16 * rt) / MX_CUS;
         const double row = 3.5 + (double)cdiv(C, 128) * (blocks < 1.0 ? 1.0 : blocks) *
@@ -346,8 +350,11 @@ static MxMatmulPlan mx_matmul_plan(int64_t M, int64_t N, int64_t K) {
     MxMatmulPlan p;
     if (M <= 16) {
         p.row = true;
-        // (8 x 14336 x 4096, one / two row tiles a wave: 7.0 / 6.3 us; x 4096: 4.2 / 4.5; 28672 x 8192: 19.7 / 20.2)
-        p.rt = N >= 32 * MX_CUS && N < 64 * MX_CUS ? 2 : 1;
+        // Two row tiles a block, which halve the reads of A, once one would leave more blocks than CUs.  One / two, us, 8 rows, B out of HBM:
+        //   n x 4096   2048 4.3/5.1   4096 4.5/5.3   5120 5.9/5.4   8192 6.8/6.1   12288 8.7/8.7    16384 10.5/9.3   28672 16.7/15.0
+        //   n x 8192   2048 6.0/7.6   4096 6.4/8.2   5120 9.7/9.1   8192 11.1/10.2 12288 15.4/15.1  16384 19.4/16.7  28672 31.8/28.7
+        // (B in the caches: up to 10 % slower at 10240 and 12288, 5 % from 16384 on)
+        p.rt = N <= 16 * MX_CUS ? 1 : 2;
         return p;
     }
     p.nt = cdiv(N, 256);

@@ -32,3 +32,10 @@ def test_every_variant_has_a_case():
     for op, edge in ((1, 128), (2, 64)):
         for ct in ((2, 4, 8) if op == 1 else (1, 2, 4)):
             assert any(c[:2] == (op, V.BF16) and w[0] == ct and (c[4] if op == 1 else c[3]) % edge == 0 for c, w in V.CASES), (op, ct)
+
+
+def test_two_row_tiles_where_one_would_leave_more_blocks_than_cus():
+    from tests import probe
+    for dt, m in ((V.BF16, 8), (V.F32, 16), (V.F16, 1)):
+        for n, rt in ((1, 1), (4096, 1), (4097, 2), (8191, 2), (8192, 2), (16384, 2), (100000, 2)):
+            assert probe.mx4_plan(0, dt, m, n, 4096)[:3] == (True, 1, rt), (dt, m, n)

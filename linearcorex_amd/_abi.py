@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import sys
 
 import numpy as np
 
@@ -108,6 +109,7 @@ SIGNATURES = {
 }
 
 _lib = None
+torch_first = True            # whether torch was imported when the library was loaded (until it is loaded: nothing is lost yet)
 
 
 class LcxError(RuntimeError):
@@ -116,13 +118,14 @@ class LcxError(RuntimeError):
 
 def load():
     """Load liblcx_hip.so (built by __graft_entry__.build()).  Raises if it is missing."""
-    global _lib
+    global _lib, torch_first
     if _lib is not None:
         return _lib
     if not os.path.exists(LIB_PATH):
         raise LcxError(
             "linearcorex_amd: HIP library %s is missing - build it with "
             "`python -c 'import __graft_entry__ as g; g.build()'` (there is no CPU fallback)" % LIB_PATH)
+    torch_first = "torch" in sys.modules
     lib = C.CDLL(LIB_PATH)
     for name, args in SIGNATURES.items():
         fn = getattr(lib, name)           # AttributeError here == header/library mismatch

@@ -14,18 +14,26 @@ waiting, on the device of the tensors.  Traced, compiled and under dispatch mode
 `linear_grad` have derivatives in both modes and work inside torch.func's transforms.  Wrong arguments raise ValueError or TypeError before anything is launched, a failing call
 `LcxError`; there is no CPU fallback.
 
+Import torch, or this module, before the first fit of a process: the library then shares the HIP runtime that torch brings along.  Loaded the other way
+round there are two of them, and torch finds no GPU (a warning says so here).
+
 `Corex(x_storage="mx4")` keeps the data of a fit in this form.
 """
 from __future__ import annotations
 
 import ctypes as C
 import functools
+import warnings
 
 import torch
 from torch.autograd import forward_ad as _forward_ad
 
 from . import _abi
 from ._abi import LcxError          # noqa: F401  (what a failing call raises)
+
+if not _abi.torch_first:
+    warnings.warn("linearcorex_amd was used before torch was imported: torch brings a HIP runtime of its own and may find no GPU now; import torch (or "
+                  "linearcorex_amd.mx4) first", RuntimeWarning, stacklevel=2)
 
 _DTYPES = {torch.float32: _abi.LCX_F32, torch.float64: _abi.LCX_F64, torch.bfloat16: _abi.LCX_BF16, torch.float16: _abi.LCX_F16}
 _PRODUCT_DTYPES = (torch.float32, torch.bfloat16, torch.float16)

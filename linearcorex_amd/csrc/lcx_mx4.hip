@@ -109,8 +109,9 @@ struct MxStep { double t1, u1, t2, u2, pair; };
 //     a later one three quarters; where CUs are left over, a block takes down to 0.85 of the time)
 //   + start and outputs of a block, 1 us and 1.3 more per 16 rows
 //   + writing the parts and adding them up: 7 TB/s, 3 us for the launch, 0.1 a part
-// Within 2 % of the best (ct, split) on average, 15 % at worst, over 78 sizes from 1 x 4096 x 4096 to 512 x 20000 x 20000.  What it weighs, us:
-// bf16 512 x 14336 x 4096 in tiles of ct 2 / 4 / 8: 70 / 59 / 64; float32 64 x 20000 x 20000 in 1 / 3 / 6 / 8 parts: 345 / 134 / 123 / 141
+// Within 2.5 % of the best (ct, split) on average, 0.9 % at the median, 26 % at worst (float32 1000 x 5003 x 10007), over 175 sizes from 24 x 4096 x 4096 to
+// 512 x 20000 x 20000.  What it weighs, us: bf16 512 x 14336 x 4096 in tiles of ct 2 / 4 / 8: 59 / 51 / 56; float32 64 x 20000 x 20000 in
+// 1 / 2 / 3 / 4 / 6 parts: 201 / 155 / 125 / 133 / 130
 static double mx_choose(int64_t M, int64_t O, int64_t cols, int64_t steps, int terms, int min_ct, int max_ct, const MxStep& c, int* ct_out, int* split_out) {
     *ct_out = min_ct;
     *split_out = 1;
@@ -153,7 +154,8 @@ template <typename T> static MxPlan mx_plan(bool along, int64_t M, int64_t C, in
         // The row kernel or the tiles, whichever takes less time by these models (fitted for K and N from 512 to 28672; 10 %):
         //   row    3.5 us + the steps a CU works through
         //   tiles  mx_choose, or reading W; 8 us for the two launches more
-        // Measured, us, row / tiles: 1 x 4096 x 4096 bf16 4.7 / 11; 16 x 20000 x 20000 bf16 68 / 42, float32 135 / 49.
+        // Measured, us, row / tiles, W out of HBM (in the caches): 1 x 4096 x 4096 bf16 5.3 / 10.3 (4.9 / 8.6); 16 x 20000 x 20000 bf16
+        // 100 / 58 (70 / 42), float32 174 / 67 (135 / 47); 8 x 28672 x 8192 float16 48 / 40 (42 / 29); 1 x 28672 x 8192 bf16 34 / 34 (25 / 25).
         // 2 x 16 rows of W a wave halve the reads of x where there are enough rows to fill the chip.  One / two, us, bf16, W out of HBM:
         //   rows of W x 4096   2048       4096       5120       6144       8192       12288      16384      28672
         //   1 row of x         4.8/5.8    5.3/6.1    6.8/6.2    7.0/6.5    7.4/7.1    10.0/9.9   12.6/11.1  20.0/18.2

@@ -230,7 +230,7 @@ __device__ __forceinline__ void mx_values8(unsigned int q, float s, float* v) {
 }
 
 // codes, scales -> out[r * rs + c * cs].  Bound: writing out.  Threads as in mx_quantize_kernel; VEC: the columns of out are neighbours.
-// 16384 x 8192 bf16: 51 us, 6.6 TB/s.  (Stores past the caches: 5000 x 10000 float32 transposed 38 -> 83 us.)
+// 16384 x 8192 bf16: 51-52 us, 6.5 TB/s.  (Stores past the caches: 5000 x 10000 float32 transposed 38 -> 83 us.)
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
                                                             int64_t rows, int64_t cols, T* __restrict__ out, int64_t rs, int64_t cs, int64_t steps, int64_t quads,
@@ -454,8 +454,9 @@ __global__ __launch_bounds__(256) void mx_scale_columns_kernel(float* __restrict
 // (MxTerms), every product is exact, float32 sums.  Bound: reading W (4.25 bits a value).  The waves of a block share 16 RT rows of W and
 // split the contraction (128 columns a step), so that a single token still puts every load of W in flight at once; partial sums meet in LDS.
 // Eight waves: sixteen gain where 512 rows meet 20000 columns (11.6 -> 10.9 us) and lose elsewhere (4-bit 8 x 7000 x 4096 4.8 -> 5.6).
-// 1 x 4096 x 4096 bf16 takes 4.7 us (of which a launch is 3.5), 1 x 28672 x 8192 24.8 us, 5.0 TB/s.  Four rows of x cost as much; sixteen read
-// x in scattered 16-byte pieces and take 12.5 us at 14336 x 4096 (2.5 TB/s) where one takes 8.8.  (x through LDS in whole lines: 9 % slower.)
+// W out of HBM: 1 x 4096 x 4096 bf16 takes 5.5 us (of which a launch is 3.5), 1 x 28672 x 8192 31 us, 4.0 TB/s (in the caches 5 and 25 us).  Four rows of x
+// cost a tenth more; sixteen read x in scattered 16-byte pieces and take 15 us at 14336 x 4096 (2.1 TB/s) where one takes 11.  (x through LDS in
+// whole lines: 9 % slower.)
 constexpr int MX_ROW_WAVES = 8;
 template <typename T, int RT, bool VEC>
 __global__ __launch_bounds__(64 * MX_ROW_WAVES) void mx_linear_row_kernel(const T* __restrict__ x, int64_t M, int64_t xrs, int64_t xcs,
@@ -549,7 +550,7 @@ __device__ __forceinline__ void mx_unpack_across(const unsigned int* q, const fl
 //   across the blocks  32 i + 8 g
 // mx_fragments_kernel lays x out that way once per call, split into its bf16 terms: frag[i][term][tile of 16 rows][lane][8].  A tile of the
 // products below is then a contiguous piece of memory, whatever x's type, strides or odd sizes.  kscale (may be null): a factor of every
-// column of W, taken into x here.  Bound: the fragments' stores; 64 x 20000 float32 5.4 us, 2048 x 8192 bf16 (67 MB) 17 us, 3.9 TB/s.
+// column of W, taken into x here.  Bound: the fragments' stores; 64 x 20000 float32 5.5 us, 2048 x 8192 bf16 (67 MB) 12 us, 5.5 TB/s.
 template <bool ALONG> __device__ __forceinline__ int64_t mx_frag_k(int64_t i, int g) {
     return ALONG ? (i >> 2) * 128 + g * 32 + (i & 3) * 8 : i * 32 + g * 8;
 }
@@ -634,8 +635,8 @@ __device__ __forceinline__ MxTile mx_tile(unsigned int id, unsigned int na, unsi
 
 // out[t][n] = sum_k x[t][k] W[n][k] for tiles of 16 CT rows of x and 64 RT rows of W.  Bound: the bf16 matrix pipe (TERMS instructions per
 // product).  The four waves own 16 RT rows of W each - codes go from memory to registers and become bf16 there, no LDS - and share the fragments
-// of x through LDS (JS of them a stage, double buffered: as many as leave room for two blocks a CU).  4096 x 8192 x 4096 bf16: 188 us, 1.46
-// PFLOP/s, where the instructions alone reach 2.17 on operands that stay in registers; 64 x 20000 x 20000 float32: 121 us, 1.27 (three terms).  Of
+// of x through LDS (JS of them a stage, double buffered: as many as leave room for two blocks a CU).  4096 x 8192 x 4096 bf16: 192-195 us, 1.42
+// PFLOP/s, where the instructions alone reach 2.17 on operands that stay in registers; 64 x 20000 x 20000 float32: 115-118 us, 1.32 (three terms).  Of
 // 218 us of an earlier form the kernel took 195 without its loads of x, 202 without those of W, 156 without reading LDS.  Tried: tiles of 8 x 8 a
 // wave (the accumulators spill), three waves a SIMD (140 against 126 us, float32), all loads of a stage at once (the same here, 10 % slower in the 4-bit tiles).
 // DIRECT: frag is x itself (rows `tiles` elements apart), see MxDirect.
@@ -756,8 +757,8 @@ __global__ __launch_bounds__(256, 2) void mx_linear_tile_kernel(const unsigned s
 // costs three vector instructions per matrix instruction at CT 4, one step ahead and in between them.  32 JS rows of W (codes, scales) and
 // their fragments of dy a stage, all of them to LDS without passing registers: the fragments double buffered, W in three buffers, since it is
 // unpacked a step early (AHEAD; with two or three terms the fragments need its registers: 219 against 183 us).  2048 x 8192 x 4096 bf16 in two
-// parts: 148 us, 0.93 PFLOP/s (8192 rows: 1.15); 64 x 20000 x 20000 float32: 155 us, 0.99.  Of 155 us it took 98 without reading W from LDS, 118
-// without unpacking, 130 without loads.  Row r of block b in row tile p is stored at row r ^ (b | 4 (p % 2)) of its block: the sixteen (block, lane group)
+// parts: 136-142 us, 0.99 PFLOP/s (154 behind the forward product; 8192 rows: 1.1 PFLOP/s); 64 x 20000 x 20000 float32: 157-163 us, 0.96.  Of 155 us of an earlier form the bf16 kernel took 98 without
+// reading W from LDS, 118 without unpacking, 130 without loads.  Row r of block b in row tile p is stored at row r ^ (b | 4 (p % 2)) of its block: the sixteen (block, lane group)
 // that a wave reads at once lie in different banks.
 template <int CT, int JS, int TERMS> struct MxGradLds {
     static constexpr int frag = JS * TERMS * CT * 1024, codes = JS * 8 * 1024, scales = JS * 2 * 256, wstage = codes + scales, total = 2 * frag + 3 * wstage;
@@ -930,7 +931,8 @@ __global__ __launch_bounds__(256, 2) void mx_grad_tile_kernel(const unsigned sho
 // scale; the instruction multiplies codes and scales, float32 sums.  Rows behind the last one repeat it and are not stored.
 __device__ __forceinline__ mx_i8 mx_operand(mx_u4 q) { return mx_i8{(int)q[0], (int)q[1], (int)q[2], (int)q[3], 0, 0, 0, 0}; }
 
-// up to 16 rows of A: as mx_linear_row_kernel, bound by reading B.  8 x 8192 x 8192: 6.7 us, 5.3 TB/s (its tiles: 13)
+// up to 16 rows of A: as mx_linear_row_kernel, bound by reading B.  8 x 8192 x 8192: 10 us out of HBM, 3.5 TB/s; 6.6
+// with B in the caches (its tiles: 13)
 template <typename T, int RT>
 __global__ __launch_bounds__(64 * MX_ROW_WAVES) void mx_matmul_row_kernel(const unsigned char* __restrict__ ac, const unsigned char* __restrict__ as, int64_t M,
                                                                    const unsigned char* __restrict__ bc, const unsigned char* __restrict__ bs, int64_t N,
@@ -988,8 +990,8 @@ __global__ __launch_bounds__(64 * MX_ROW_WAVES) void mx_matmul_row_kernel(const 
 // Tiles of 16 CT rows of A by 64 RT rows of B.  Bound: the 4-bit matrix pipe (16 cycles an instruction of 64 Kflop) and what feeds it: as in
 // mx_linear_tile_kernel the four waves own 16 RT rows of B each, whose fragments and scales go from memory to registers (an instruction's
 // operands are 2 KB, and both through LDS would take all of its bandwidth), and share the fragments of A through LDS, two steps a stage,
-// double buffered.  A dword of scales serves four steps.  8192 x 8192 x 8192: 268 us, 4.1 PFLOP/s (the instructions alone: 7.5); 1000 x 5003 x 10007: 46
-// us, 2.2.  Tried: four stages in flight (spills, 388 us), A's codes row-major in 64-byte pieces (557 against 423 us).
+// double buffered.  A dword of scales serves four steps.  8192 x 8192 x 8192: 267-290 us, 253 at best, 3.8-4.3 PFLOP/s (the instructions alone: 7.5); 1000 x 5003 x 10007: 47
+// us, 2.1.  Tried: four stages in flight (spills, 388 us), A's codes row-major in 64-byte pieces (557 against 423 us).
 template <typename T, int CT, int RT>
 __global__ __launch_bounds__(256, 2) void mx_matmul_tile_kernel(const unsigned char* __restrict__ ac, const unsigned char* __restrict__ as,
                                                                const unsigned char* __restrict__ bc, const unsigned char* __restrict__ bs, int64_t N,

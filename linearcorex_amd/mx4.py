@@ -42,6 +42,9 @@ BLOCK = 32
 # who may be looking at the operations (each a tenth of a microsecond a call): torch.compile, dispatch modes, torch.jit.trace, torch.func
 _compiling, _watching, _tracing = torch.compiler.is_compiling, torch._C._len_torch_dispatch_stack, torch._C._is_tracing
 _transforming, _PLAIN = torch._C._are_functorch_transforms_active, (torch.Tensor, torch.nn.Parameter)
+# (looked up once: a call of a few microseconds notices)
+_Tensor, _strided, _uint8 = torch.Tensor, torch.strided, torch.uint8
+_current, _raw_stream = getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _sizes(rows, cols):
@@ -113,9 +116,9 @@ class Mx4(object):
 
 
 def _on_gpu(t, what):
-    if not isinstance(t, torch.Tensor):
+    if not isinstance(t, _Tensor):
         raise TypeError("%s must be a torch tensor, not %s" % (what, type(t).__name__))
-    if t.layout is not torch.strided:
+    if t.layout is not _strided:
         raise TypeError("%s must be a dense tensor" % what)
     if not t.is_cuda:
         raise ValueError("%s must be on the GPU, it is on %s (there is no CPU fallback)" % (what, t.device))
@@ -136,11 +139,11 @@ def _call(index, name, *args):
     fn = _entry.get(name)
     if fn is None:
         fn = _entry[name] = getattr(_abi.load(), name)
-    if torch._C._cuda_getDevice() == index:        # (a matrix on the GPU exists: torch has been initialised)
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if _current() == index:                        # (a matrix on the GPU exists: torch has been initialised)
+        status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+            status = fn(*args, _raw_stream(index))
     if status != 0:
         _abi.check(status)
 
@@ -180,7 +183,7 @@ def _quantize(x, shape, axis):
     if axis == 0:
         rows, cols, rs, cs = cols, rows, cs, rs
     cb, sb = _sizes(rows, cols)
-    buf = x.new_empty(cb + sb, dtype=torch.uint8)
+    buf = x.new_empty(cb + sb, dtype=_uint8)
     index, cp = x.get_device(), buf.data_ptr()
     sp = cp + cb
     if rows and cols:
@@ -232,7 +235,7 @@ def _matmul(like, index, ac, asc, m, bc, bsc, n, k, dtype):
     if m and n:
         dt = _DTYPES[dtype]
         wb = _workspace_bytes(0, dt, m, n, k)
-        w = like.new_empty(wb, dtype=torch.uint8) if wb else None
+        w = like.new_empty(wb, dtype=_uint8) if wb else None
         _call(index, "lcx_mx4_matmul", ac, asc, m, bc, bsc, n, k, out.data_ptr(), dt, n, 1, w.data_ptr() if wb else None, wb)
     return out
 
@@ -256,7 +259,7 @@ def _product(x, shape, index, cp, sp, n, k, along):
         if m > 16 and dt == 2 and cs == 1 and not (rs | xp >> 1) & 7 and rs < 1 << 23 and not c & (127 if along else 63):
             op += 2                      # read in place (include/lcx.h, lcx_mx4_workspace)
         wb = _workspace_bytes(op, dt, m, n, k)
-        w = x.new_empty(wb, dtype=torch.uint8) if wb else None
+        w = x.new_empty(wb, dtype=_uint8) if wb else None
         _call(index, "lcx_mx4_linear" if along else "lcx_mx4_linear_grad", xp, dt, m, rs, cs, cp, sp, n, k,
               out.data_ptr(), o, 1, w.data_ptr() if wb else None, wb)
     return out if lead is None else out.reshape(lead + (o,))
@@ -398,7 +401,7 @@ def _call_product(x, q, what, contracted):
     if x.get_device() != q.index:
         raise ValueError("%s is on %s, q on %s" % (what, x.device, q.device))
     along = q.axis == contracted
-    if _compiling() or _watching() or _tracing() or _transforming() or _forward_ad._current_level >= 0 or x.requires_grad or type(x) is not torch.Tensor \
+    if _compiling() or _watching() or _tracing() or _transforming() or _forward_ad._current_level >= 0 or x.requires_grad or type(x) is not _Tensor \
             or q._cp is None:
         return _apply(x, q, along)
     n, k = q._stored()
